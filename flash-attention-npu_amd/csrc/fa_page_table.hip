@@ -1,0 +1,132 @@
+// fa_page_table.hip -- the page table of a paged cache, brought from one step's
+// request lengths to the next on the GPU: fa_update_page_table.
+//
+// Request b holds have = ceil(before / P) pages and needs need = ceil(after / P).
+// With rel and take the two differences (each at least 0), and prefix sums over the
+// requests in their order, released page r goes to place n0 + r of the free stack
+// (n0 ids on it) and needed page t comes from place top - 1 - t, top = n0 + all
+// released. Token i of request b has slot table[(before + i) / P] * P + (before +
+// i) % P. Nothing below n0 is written and no entry of the table that the step
+// still uses, so a step taken twice gives the same.
+#include "fa_common.h"
+#include "fa_quant_args.h"
+
+namespace fa {
+
+namespace {
+
+constexpr int NT = 1024;
+
+// exclusive prefix over the workgroup of v, total in `sum`
+__device__ __forceinline__ int block_scan(int v, int* s_w, int& sum) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int incl = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(incl, o);
+        if (lane >= o) incl += u;
+    }
+    __syncthreads();
+    if (lane == 63) s_w[wave] = incl;
+    __syncthreads();
+    int pre = 0;
+    sum = 0;
+    for (int w = 0; w < NT / 64; ++w) {
+        pre += w < wave ? s_w[w] : 0;
+        sum += s_w[w];
+    }
+    return pre + incl - v;
+}
+
+struct Req {
+    int row;           // of the table, -1: none
+    int have, need;    // pages
+    int fresh;         // new tokens
+};
+
+__device__ __forceinline__ Req request(const PageTableArgs& a, int b) {
+    Req r{-1, 0, 0, 0};
+    if (b >= a.B) return r;
+    const int before = max(a.before[b], 0), after = max(a.after[b], 0);
+    r.fresh = max(after - before, 0);
+    r.row = a.batch_idx ? a.batch_idx[b] : b;
+    if (r.row < 0 || r.row >= a.table_rows) {
+        r.row = -1;
+        return r;
+    }
+    r.have = min((int)udiv(a.page, (uint32_t)before) + (before % a.page_size ? 1 : 0), a.max_pages);
+    r.need = min((int)udiv(a.page, (uint32_t)after) + (after % a.page_size ? 1 : 0), a.max_pages);
+    return r;
+}
+
+// One workgroup: the stack, the table, the prefix of the new tokens.
+__global__ void __launch_bounds__(NT) fa_page_table_kernel(PageTableArgs a) {
+    __shared__ int s_w[NT / 64];
+    const int n0 = min(max(a.num_free[0], 0), a.free_cap);
+    int released = 0;
+    for (int b0 = 0; b0 < a.B; b0 += NT) {
+        const Req r = request(a, b0 + threadIdx.x);
+        const int* row = a.table + (int64_t)max(r.row, 0) * a.t_stride;
+        int n = 0, sum;
+        for (int j = r.need; j < r.have; ++j) n += row[j] >= 0;
+        int64_t at = (int64_t)n0 + released + block_scan(n, s_w, sum);
+        for (int j = r.need; j < r.have; ++j) {
+            const int id = row[j];
+            if (id < 0) continue;
+            if (at < a.free_cap) a.free_pages[at] = id;
+            ++at;
+        }
+        released += sum;
+    }
+    const int top = (int)min((int64_t)n0 + released, (int64_t)a.free_cap);
+    __syncthreads();  // the stack is whole
+    int taken = 0, fresh = 0;
+    for (int b0 = 0; b0 < a.B; b0 += NT) {
+        const int b = b0 + threadIdx.x;
+        const Req r = request(a, b);
+        int sum;
+        const int t0 = taken + block_scan(max(r.need - r.have, 0), s_w, sum);
+        taken += sum;
+        int* row = a.table + (int64_t)max(r.row, 0) * a.t_stride;
+        for (int j = r.have; j < r.need; ++j) {
+            const int at = top - 1 - (t0 + j - r.have);
+            row[j] = at >= 0 ? a.free_pages[at] : -1;
+        }
+        const int f0 = fresh + block_scan(r.fresh, s_w, sum);
+        fresh += sum;
+        if (b < a.B) a.cu_new[b] = f0;
+    }
+    if (threadIdx.x == 0) {
+        a.cu_new[a.B] = fresh;
+        a.num_free_out[0] = top - taken;
+    }
+}
+
+// The slots, one thread each, from the table and prefix that the kernel above left.
+__global__ void __launch_bounds__(256) fa_slot_kernel(PageTableArgs a) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= a.total_new) return;
+    int64_t slot = -1;
+    if (i < a.cu_new[a.B]) {
+        const int b = seq_of(a.cu_new, a.B, (int)i);
+        const int row = a.batch_idx ? a.batch_idx[b] : b;
+        const int64_t at = (int64_t)max(a.before[b], 0) + (i - a.cu_new[b]);
+        if (row >= 0 && row < a.table_rows && at < (int64_t)a.max_pages * a.page_size) {
+            const int j = (int)udiv(a.page, (uint32_t)at);
+            const int id = a.table[(int64_t)row * a.t_stride + j];
+            if (id >= 0) slot = (int64_t)id * a.page_size + (at - (int64_t)j * a.page_size);
+        }
+    }
+    a.slots[i] = slot;
+}
+
+}  // namespace
+
+hipError_t launch_page_table(const PageTableArgs& a, hipStream_t stream) {
+    hipLaunchKernelGGL(fa_page_table_kernel, dim3(1), dim3(NT), 0, stream, a);
+    if (a.total_new > 0)
+        hipLaunchKernelGGL(fa_slot_kernel, dim3((unsigned)((a.total_new + 255) / 256)), dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace fa

@@ -1,7 +1,7 @@
 // fa_torch_ops.cpp -- PyTorch-ROCm operators over the C ABI (libfa_mi355x.so).
 //
 // Registers torch.ops.fa_mi355x.{fwd_kvcache, fwd_kvcache_v3, fwd, varlen_fwd, fwd_combine,
-// fwd_combine_out, bwd, varlen_bwd}.
+// fwd_combine_out, bwd, varlen_bwd, update_page_table, quant_append, quant_fwd}.
 // Argument order and meaning follow the reference pybind entry points
 // (csrc/arch22/flash_attn_npu_v2/flash_api.cpp: mha_fwd_kvcache :356-377,
 // mha_fwd :628-640, mha_varlen_fwd :828-850, bound at :1301-1309). Unlike the
@@ -700,9 +700,229 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> varlen_bwd(const Tensor& dout, const 
     return {dq, dk, dv, sd};
 }
 
+// ---- the quantised cache: page table, append, attention ----------------------------------------
+const int32_t* i32_vec(const Tensor& t, const Tensor& on, int64_t n, const char* name) {
+    check_dev(t, on, name);
+    TORCH_CHECK(t.scalar_type() == at::kInt, name, " must have dtype int32");
+    TORCH_CHECK(t.dim() == 1 && t.is_contiguous(), name, " must be a contiguous vector");
+    TORCH_CHECK(t.size(0) == n, name, " must have ", n, " entries, got ", t.size(0));
+    return t.data_ptr<int32_t>();
+}
+
+std::tuple<Tensor, Tensor, Tensor> update_page_table(Tensor& page_table, const Tensor& cache_seqlens,
+                                                     const Tensor& new_seqlens, Tensor& free_pages,
+                                                     const Tensor& num_free, int64_t page_size, int64_t total_new,
+                                                     const OptT& cache_batch_idx) {
+    c10::DeviceGuard guard(page_table.device());
+    TORCH_CHECK(page_table.is_cuda(), "page_table must be on a GPU device");
+    TORCH_CHECK(page_table.scalar_type() == at::kInt && page_table.dim() == 2 && page_table.stride(1) == 1,
+                "page_table must be an int32 matrix with contiguous rows");
+    TORCH_CHECK(cache_seqlens.dim() == 1, "cache_seqlens must be a vector");
+    TORCH_CHECK(page_size >= 1 && page_size <= INT32_MAX, "page_size must be positive");
+    TORCH_CHECK(total_new >= 0, "total_new must be >= 0");
+    const int64_t B = cache_seqlens.size(0);
+    TORCH_CHECK(B >= 1, "batch size must be positive");
+    fa_page_table_params p{};
+    p.abi_version = FA_MI355X_ABI_VERSION;
+    p.batch = (int32_t)B;
+    p.page_size = (int32_t)page_size;
+    p.table_rows = (int32_t)page_table.size(0);
+    p.max_pages = (int32_t)page_table.size(1);
+    p.page_table = page_table.data_ptr<int32_t>();
+    p.page_table_row_stride = page_table.stride(0);
+    if (cache_batch_idx.has_value()) p.cache_batch_idx = i32_vec(*cache_batch_idx, page_table, B, "cache_batch_idx");
+    p.cache_seqlens = i32_vec(cache_seqlens, page_table, B, "cache_seqlens");
+    p.new_seqlens = i32_vec(new_seqlens, page_table, B, "new_seqlens");
+    p.free_pages = const_cast<int32_t*>(i32_vec(free_pages, page_table, free_pages.numel(), "free_pages"));
+    p.free_capacity = (int32_t)free_pages.size(0);
+    p.num_free = i32_vec(num_free, page_table, 1, "num_free");
+    Tensor slots = at::empty({total_new}, page_table.options().dtype(at::kLong));
+    Tensor cu = at::empty({B + 1}, page_table.options());
+    Tensor left = at::empty({1}, page_table.options());
+    p.num_free_out = left.data_ptr<int32_t>();
+    p.cu_seqlens_new = cu.data_ptr<int32_t>();
+    p.slot_mapping = slots.data_ptr<int64_t>();
+    p.total_new = total_new;
+    check_status(fa_update_page_table(&p, cur_stream()));
+    return {slots, cu, left};
+}
+
+int32_t cache_code(const Tensor& t, const char* name) {
+    if (t.scalar_type() == at::kChar) return FA_DTYPE_INT8;
+    if (t.scalar_type() == at::kFloat8_e4m3fn) return FA_DTYPE_FP8_E4M3;
+    TORCH_CHECK(false, name, " must hold int8 or float8_e4m3fn");
+}
+
+// The caches and their scales, in the fields that the append and the attention share.
+template <typename P>
+void set_quant_cache(P& p, const Tensor& kcache, const Tensor& vcache, const Tensor& kscale, const Tensor& vscale,
+                     const Tensor& q, int64_t headdim) {
+    check_dev(kcache, q, "k_cache");
+    check_dev(vcache, q, "v_cache");
+    check_dev(kscale, q, "k_scale");
+    check_dev(vscale, q, "v_scale");
+    TORCH_CHECK(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16,
+                "FlashAttention only support fp16 and bf16 data type");
+    TORCH_CHECK(kcache.dim() == 4 && vcache.sizes() == kcache.sizes(),
+                "k_cache and v_cache must have shape (num_pages, page_size, num_heads_k, head_size)");
+    TORCH_CHECK(kcache.scalar_type() == vcache.scalar_type(), "k_cache and v_cache must have the same dtype");
+    TORCH_CHECK(kcache.stride(3) == 1 && vcache.stride(3) == 1, "the caches must have contiguous last dimension");
+    TORCH_CHECK(kcache.size(3) == headdim, "head size of the caches must match");
+    TORCH_CHECK(kscale.scalar_type() == at::kFloat && vscale.scalar_type() == at::kFloat,
+                "k_scale and v_scale must have dtype fp32");
+    const int64_t page = kcache.size(1);
+    TORCH_CHECK(kscale.dim() == 3 && vscale.sizes() == kscale.sizes() && kscale.size(0) == kcache.size(0) &&
+                    kscale.size(2) == kcache.size(2),
+                "k_scale and v_scale must have shape (num_pages, blocks of a page, num_heads_k)");
+    TORCH_CHECK(kscale.size(1) >= 1 && page % kscale.size(1) == 0, "page_size ", page,
+                " must be a multiple of the blocks of a page, ", kscale.size(1));
+    p.abi_version = FA_MI355X_ABI_VERSION;
+    p.dtype = dtype_code(q);
+    p.cache_dtype = cache_code(kcache, "k_cache");
+    p.nheads_k = (int32_t)kcache.size(2);
+    p.headdim = (int32_t)headdim;
+    p.num_pages = (int32_t)kcache.size(0);
+    p.page_size = (int32_t)page;
+    p.scale_block = (int32_t)(page / kscale.size(1));
+    p.k_page_stride = kcache.stride(0);
+    p.k_row_stride = kcache.stride(1);
+    p.k_head_stride = kcache.stride(2);
+    p.v_page_stride = vcache.stride(0);
+    p.v_row_stride = vcache.stride(1);
+    p.v_head_stride = vcache.stride(2);
+    p.k = kcache.data_ptr();
+    p.v = vcache.data_ptr();
+    p.k_scale = kscale.data_ptr<float>();
+    p.k_scale_page_stride = kscale.stride(0);
+    p.k_scale_block_stride = kscale.stride(1);
+    p.k_scale_head_stride = kscale.stride(2);
+    p.v_scale = vscale.data_ptr<float>();
+    p.v_scale_page_stride = vscale.stride(0);
+    p.v_scale_block_stride = vscale.stride(1);
+    p.v_scale_head_stride = vscale.stride(2);
+}
+
+void quant_append(const Tensor& k, const Tensor& v, Tensor& kcache, Tensor& vcache, Tensor& kscale, Tensor& vscale,
+                  const Tensor& slot_mapping) {
+    c10::DeviceGuard guard(kcache.device());
+    TORCH_CHECK(k.is_cuda(), "k must be on a GPU device");
+    TORCH_CHECK(k.dim() == 3 && v.sizes() == k.sizes(), "k and v must have shape (total_new, num_heads_k, head_size)");
+    check_dev(v, k, "v");
+    TORCH_CHECK(v.scalar_type() == k.scalar_type(), "k and v must have the same dtype");
+    fa_quant_append_params p{};
+    set_quant_cache(p, kcache, vcache, kscale, vscale, k, k.size(2));
+    TORCH_CHECK(k.size(1) == p.nheads_k, "k must have the key/value heads of the cache");
+    check_dev(slot_mapping, k, "slot_mapping");
+    TORCH_CHECK(slot_mapping.scalar_type() == at::kLong && slot_mapping.dim() == 1 && slot_mapping.is_contiguous(),
+                "slot_mapping must be a contiguous int64 vector");
+    TORCH_CHECK(slot_mapping.size(0) == k.size(0), "slot_mapping must have an entry per row of k");
+    // rows that a 16-byte load cannot take are copied, as elsewhere
+    auto rows = [](const Tensor& t) {
+        return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && ((uintptr_t)t.data_ptr() & 15) == 0
+                   ? t
+                   : t.contiguous();
+    };
+    const Tensor kn = rows(k), vn = rows(v);
+    p.total_new = k.size(0);
+    p.k_new = kn.data_ptr();
+    p.knew_row_stride = kn.stride(0);
+    p.knew_head_stride = kn.stride(1);
+    p.v_new = vn.data_ptr();
+    p.vnew_row_stride = vn.stride(0);
+    p.vnew_head_stride = vn.stride(1);
+    p.slot_mapping = slot_mapping.data_ptr<int64_t>();
+    check_status(fa_quant_append(&p, cur_stream()));
+}
+
+std::tuple<Tensor, Tensor> quant_fwd(const Tensor& q, const Tensor& kcache, const Tensor& vcache, const Tensor& kscale,
+                                     const Tensor& vscale, const Tensor& cache_seqlens, const OptT& page_table,
+                                     const OptT& cache_batch_idx, const OptT& cu_seqlens_q, int64_t max_seqlen_q,
+                                     double softmax_scale, bool is_causal, int64_t window_size_left,
+                                     int64_t window_size_right, double softcap) {
+    c10::DeviceGuard guard(q.device());
+    TORCH_CHECK(q.is_cuda(), "q must be on a GPU device");
+    const bool ragged = cu_seqlens_q.has_value();
+    if (ragged) {
+        TORCH_CHECK(q.dim() == 3, "q must have shape (total_q, num_heads, head_size) with cu_seqlens_q");
+    } else {
+        TORCH_CHECK(q.dim() == 4, "q must have shape (batch_size, seqlen_q, num_heads, head_size)");
+    }
+    TORCH_CHECK(max_seqlen_q >= 0 && max_seqlen_q <= INT32_MAX, "max_seqlen_q must be >= 0");
+    fa_quant_fwd_params p{};
+    set_quant_cache(p, kcache, vcache, kscale, vscale, q, q.size(-1));
+    const Tensor qc = q.stride(-1) == 1 && q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 && q.stride(-2) % 8 == 0 &&
+                              ((uintptr_t)q.data_ptr() & 15) == 0
+                          ? q
+                          : q.contiguous();
+    const int64_t B = ragged ? cu_seqlens_q->numel() - 1 : q.size(0);
+    TORCH_CHECK(B >= 1, "batch size must be positive");
+    p.batch = (int32_t)B;
+    p.nheads = (int32_t)q.size(-2);
+    Tensor out = at::empty(q.sizes(), q.options());
+    Tensor lse = ragged ? at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat))
+                        : at::empty({B, q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+    p.q = qc.data_ptr();
+    p.out = out.data_ptr();
+    p.softmax_lse = lse.data_ptr<float>();
+    if (ragged) {
+        p.cu_seqlens_q = i32_vec(*cu_seqlens_q, q, B + 1, "cu_seqlens_q");
+        p.seqlen_q = (int32_t)max_seqlen_q;
+        p.total_q = (int32_t)q.size(0);
+        p.q_row_stride = qc.stride(0);
+        p.q_head_stride = qc.stride(1);
+        p.out_row_stride = out.stride(0);
+        p.out_head_stride = out.stride(1);
+    } else {
+        p.seqlen_q = (int32_t)q.size(1);
+        p.q_batch_stride = qc.stride(0);
+        p.q_row_stride = qc.stride(1);
+        p.q_head_stride = qc.stride(2);
+        p.out_batch_stride = out.stride(0);
+        p.out_row_stride = out.stride(1);
+        p.out_head_stride = out.stride(2);
+    }
+    p.cache_seqlens = i32_vec(cache_seqlens, q, B, "cache_seqlens");
+    if (page_table.has_value()) {
+        check_dev(*page_table, q, "page_table");
+        TORCH_CHECK(page_table->scalar_type() == at::kInt && page_table->dim() == 2 && page_table->stride(1) == 1,
+                    "page_table must be an int32 matrix with contiguous rows");
+        p.page_table = page_table->data_ptr<int32_t>();
+        p.page_table_row_stride = page_table->stride(0);
+        p.table_rows = (int32_t)page_table->size(0);
+        p.max_pages = (int32_t)page_table->size(1);
+        TORCH_CHECK(p.table_rows >= 1 && p.max_pages >= 1, "page_table must have rows and columns");
+    }
+    if (cache_batch_idx.has_value()) p.cache_batch_idx = i32_vec(*cache_batch_idx, q, B, "cache_batch_idx");
+    p.softmax_scale = (float)softmax_scale;
+    p.softcap = (float)softcap;
+    p.is_causal = is_causal ? 1 : 0;
+    p.window_size_left = (int32_t)std::min<int64_t>(window_size_left, INT32_MAX);
+    p.window_size_right = (int32_t)std::min<int64_t>(window_size_right, INT32_MAX);
+    size_t bytes = 0;
+    check_status(fa_quant_fwd_workspace_size(&p, &bytes));
+    Tensor ws;
+    if (bytes) {
+        ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+        p.workspace = ws.data_ptr();
+        p.workspace_bytes = bytes;
+    }
+    check_status(fa_quant_fwd(&p, cur_stream()));
+    return {out, lse};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(fa_mi355x, m) {
+    m.def(
+        "update_page_table(Tensor(a!) page_table, Tensor cache_seqlens, Tensor new_seqlens, Tensor(b!) free_pages, "
+        "Tensor num_free, int page_size, int total_new, Tensor? cache_batch_idx=None) -> (Tensor, Tensor, Tensor)");
+    m.def(
+        "quant_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, "
+        "Tensor(d!) v_scale, Tensor slot_mapping) -> ()");
+    m.def(
+        "quant_fwd(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor cache_seqlens, "
+        "Tensor? page_table, Tensor? cache_batch_idx, Tensor? cu_seqlens_q, int max_seqlen_q, float softmax_scale, "
+        "bool is_causal, int window_size_left, int window_size_right, float softcap) -> (Tensor, Tensor)");
     m.def(
         "fwd_kvcache(Tensor q, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor? k, Tensor? v, Tensor? seqlens_k, "
         "Tensor? rotary_cos, Tensor? rotary_sin, Tensor? cache_batch_idx, Tensor? leftpad_k, Tensor? block_table, "
@@ -750,4 +970,7 @@ TORCH_LIBRARY_IMPL(fa_mi355x, CUDA, m) {
     m.impl("fwd_combine_out", &fwd_combine_out);
     m.impl("bwd", &bwd);
     m.impl("varlen_bwd", &varlen_bwd);
+    m.impl("update_page_table", &update_page_table);
+    m.impl("quant_append", &quant_append);
+    m.impl("quant_fwd", &quant_fwd);
 }

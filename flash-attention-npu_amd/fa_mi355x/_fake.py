@@ -76,3 +76,22 @@ def _varlen_bwd_fake(dout, q, k, v, out, softmax_lse, cu_seqlens_q, cu_seqlens_k
     t, h, _ = q.shape
     return (torch.empty_like(q), torch.empty_like(k), torch.empty_like(v),
             q.new_empty((h, t), dtype=torch.float32))
+
+
+@torch.library.register_fake("fa_mi355x::update_page_table")
+def _update_page_table_fake(page_table, cache_seqlens, new_seqlens, free_pages, num_free, page_size, total_new,
+                            cache_batch_idx=None):
+    return (page_table.new_empty((total_new,), dtype=torch.int64), page_table.new_empty((cache_seqlens.shape[0] + 1,)),
+            page_table.new_empty((1,)))
+
+
+@torch.library.register_fake("fa_mi355x::quant_append")
+def _quant_append_fake(k, v, k_cache, v_cache, k_scale, v_scale, slot_mapping):
+    return None
+
+
+@torch.library.register_fake("fa_mi355x::quant_fwd")
+def _quant_fwd_fake(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, page_table, cache_batch_idx, cu_seqlens_q,
+                    max_seqlen_q, softmax_scale, is_causal, window_size_left, window_size_right, softcap):
+    lse = (q.shape[1], q.shape[0]) if cu_seqlens_q is not None else (q.shape[0], q.shape[2], q.shape[1])
+    return q.new_empty(q.shape), q.new_empty(lse, dtype=torch.float32)

@@ -13,12 +13,13 @@ CORE_LIB = os.path.join(_HERE, "lib", "libfa_mi355x.so")
 
 ABI_VERSION = 4
 FA_OK, FA_EINVAL, FA_EUNSUPPORTED, FA_EHIP, FA_EWORKSPACE = 0, 1, 2, 3, 4
-FA_DTYPE_FP16, FA_DTYPE_BF16, FA_DTYPE_FP32, FA_DTYPE_FP8_E4M3 = 0, 1, 2, 3
+FA_DTYPE_FP16, FA_DTYPE_BF16, FA_DTYPE_FP32, FA_DTYPE_FP8_E4M3, FA_DTYPE_INT8 = 0, 1, 2, 3, 4
 FA_KIND_KVCACHE, FA_KIND_DENSE, FA_KIND_VARLEN = 0, 1, 2
 
 EXPORTED = ["fa_abi_version", "fa_validate", "fa_fwd_workspace_size", "fa_mha_fwd_kvcache", "fa_mha_fwd",
             "fa_mha_varlen_fwd", "fa_mha_fwd_kvcache_noalloc", "fa_combine", "fa_last_error", "fa_validate_bwd",
-            "fa_bwd_workspace_size", "fa_mha_bwd", "fa_mha_varlen_bwd"]
+            "fa_bwd_workspace_size", "fa_mha_bwd", "fa_mha_varlen_bwd", "fa_update_page_table", "fa_quant_append",
+            "fa_quant_fwd_workspace_size", "fa_quant_fwd"]
 NOALLOC_SCRATCH_BYTES = 32 << 20  # FA_NOALLOC_SCRATCH_BYTES
 
 _i32 = ctypes.c_int32
@@ -82,6 +83,50 @@ class BwdParams(ctypes.Structure):
     ]
 
 
+class PageTableParams(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32), ("batch", _i32), ("page_size", _i32), ("table_rows", _i32), ("max_pages", _i32),
+        ("page_table", _vp), ("page_table_row_stride", _i64),
+        ("cache_batch_idx", _vp), ("cache_seqlens", _vp), ("new_seqlens", _vp),
+        ("free_pages", _vp), ("free_capacity", _i32), ("num_free", _vp), ("num_free_out", _vp),
+        ("cu_seqlens_new", _vp), ("slot_mapping", _vp), ("total_new", _i64),
+    ]
+
+
+def _cache_fields():
+    """The caches and scales of QuantAppendParams and QuantFwdParams."""
+    f = []
+    for n in ("k", "v"):
+        f += [(n, _vp), (n + "_page_stride", _i64), (n + "_row_stride", _i64), (n + "_head_stride", _i64)]
+    for n in ("k_scale", "v_scale"):
+        f += [(n, _vp), (n + "_page_stride", _i64), (n + "_block_stride", _i64), (n + "_head_stride", _i64)]
+    return f
+
+
+class QuantAppendParams(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32), ("dtype", _i32), ("cache_dtype", _i32), ("nheads_k", _i32), ("headdim", _i32),
+        ("num_pages", _i32), ("page_size", _i32), ("scale_block", _i32), ("total_new", _i64),
+        ("k_new", _vp), ("knew_row_stride", _i64), ("knew_head_stride", _i64),
+        ("v_new", _vp), ("vnew_row_stride", _i64), ("vnew_head_stride", _i64),
+    ] + _cache_fields() + [("slot_mapping", _vp)]
+
+
+class QuantFwdParams(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32), ("dtype", _i32), ("cache_dtype", _i32), ("batch", _i32), ("seqlen_q", _i32),
+        ("nheads", _i32), ("nheads_k", _i32), ("headdim", _i32),
+        ("num_pages", _i32), ("page_size", _i32), ("scale_block", _i32),
+        ("q", _vp), ("q_batch_stride", _i64), ("q_row_stride", _i64), ("q_head_stride", _i64),
+    ] + _cache_fields() + [
+        ("out", _vp), ("out_batch_stride", _i64), ("out_row_stride", _i64), ("out_head_stride", _i64),
+        ("softmax_lse", _vp), ("cache_seqlens", _vp), ("cu_seqlens_q", _vp), ("total_q", _i32),
+        ("page_table", _vp), ("page_table_row_stride", _i64), ("table_rows", _i32), ("max_pages", _i32),
+        ("cache_batch_idx", _vp), ("softmax_scale", ctypes.c_float), ("softcap", ctypes.c_float), ("is_causal", _i32),
+        ("window_size_left", _i32), ("window_size_right", _i32), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 _lib = None
 
 
@@ -110,6 +155,12 @@ def lib():
         for fn in ("fa_mha_bwd", "fa_mha_varlen_bwd"):
             getattr(L, fn).argtypes = [PB, _vp]
             getattr(L, fn).restype = ctypes.c_int
+        for fn, params in (("fa_update_page_table", PageTableParams), ("fa_quant_append", QuantAppendParams),
+                           ("fa_quant_fwd", QuantFwdParams)):
+            getattr(L, fn).argtypes = [ctypes.POINTER(params), _vp]
+            getattr(L, fn).restype = ctypes.c_int
+        L.fa_quant_fwd_workspace_size.argtypes = [ctypes.POINTER(QuantFwdParams), ctypes.POINTER(ctypes.c_size_t)]
+        L.fa_quant_fwd_workspace_size.restype = ctypes.c_int
         _lib = L
     return _lib
 
@@ -167,3 +218,27 @@ def validate_bwd(p, kind):
 def backward(p, kind, stream=0):
     fn = lib().fa_mha_varlen_bwd if kind == FA_KIND_VARLEN else lib().fa_mha_bwd
     return fn(ctypes.byref(p), stream)
+
+
+def update_page_table(stream=0, **kw):
+    """fa_update_page_table with the given fields (zero elsewhere)."""
+    return lib().fa_update_page_table(ctypes.byref(PageTableParams(abi_version=ABI_VERSION, **kw)), stream)
+
+
+def quant_append(stream=0, **kw):
+    """fa_quant_append with the given fields (zero elsewhere)."""
+    return lib().fa_quant_append(ctypes.byref(QuantAppendParams(abi_version=ABI_VERSION, **kw)), stream)
+
+
+def new_quant_fwd_params(**kw):
+    return QuantFwdParams(**dict(dict(abi_version=ABI_VERSION, window_size_left=-1, window_size_right=-1), **kw))
+
+
+def quant_fwd_workspace_size(p):
+    n = ctypes.c_size_t(0)
+    st = lib().fa_quant_fwd_workspace_size(ctypes.byref(p), ctypes.byref(n))
+    return st, n.value
+
+
+def quant_fwd(p, stream=0):
+    return lib().fa_quant_fwd(ctypes.byref(p), stream)

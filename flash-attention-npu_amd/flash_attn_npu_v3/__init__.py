@@ -13,3 +13,8 @@ from .interface import (  # noqa: F401
     flash_attn_with_kvcache,
     get_scheduler_metadata,
 )
+from .quantized import (  # noqa: F401
+    append_quantized_kvcache,
+    flash_attn_with_quantized_kvcache,
+    update_page_table,
+)

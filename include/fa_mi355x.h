@@ -59,8 +59,9 @@ typedef enum {
     FA_DTYPE_FP16 = 0,
     FA_DTYPE_BF16 = 1,
     FA_DTYPE_FP32 = 2,     /* fa_combine output only */
-    FA_DTYPE_FP8_E4M3 = 3  /* forward only: q, k, v, k_new, v_new in OCP float8 e4m3fn (torch.float8_e4m3fn),
-                              out in bf16; see q_descale below */
+    FA_DTYPE_FP8_E4M3 = 3, /* forward only: q, k, v, k_new, v_new in OCP float8 e4m3fn (torch.float8_e4m3fn),
+                              out in bf16; see q_descale below. Also a cache type of the quantised cache */
+    FA_DTYPE_INT8 = 4      /* cache type of the quantised cache only */
 } fa_dtype_t;
 
 typedef enum {
@@ -296,6 +297,121 @@ fa_status_t fa_bwd_workspace_size(const fa_bwd_params* p, int32_t kind, size_t* 
  * Deterministic: no atomics, every output element is written by one thread. */
 fa_status_t fa_mha_bwd(const fa_bwd_params* p, void* stream);
 fa_status_t fa_mha_varlen_bwd(const fa_bwd_params* p, void* stream);
+
+/* ---- serving over a quantised cache -------------------------------------------
+ * A cache of 8-bit codes with a scale for each block of tokens and kv head, the
+ * page table that leads to it and the append that fills it. The reference has no
+ * counterpart: its caches hold the type of q.
+ *
+ * Cache: k and v are (num_pages, page_size, Hk, D) codes, int8 or e4m3; the
+ * scales are fp32 (num_pages, page_size / scale_block, Hk); a code c of a row
+ * stands for c * scale of its block and head. page_size is a multiple of
+ * scale_block, scale_block a multiple of 16. A contiguous cache is one page per
+ * sequence (page_table NULL). Slot s is row s % page_size of page s / page_size. */
+typedef struct fa_page_table_params {
+    int32_t abi_version;
+    int32_t batch;
+    int32_t page_size;
+    int32_t table_rows, max_pages;   /* of page_table */
+    int32_t* page_table;             /* (table_rows, max_pages), written in place */
+    int64_t page_table_row_stride;
+    const int32_t* cache_batch_idx;  /* (batch,) row of each request, distinct; NULL: request b has row b.
+                                        A request whose row is not in the table gets no pages */
+    const int32_t* cache_seqlens;    /* (batch,) tokens of each request before the step */
+    const int32_t* new_seqlens;      /* (batch,) and after it: more (new tokens), fewer (taken back) or 0 (ended) */
+    int32_t* free_pages;             /* (free_capacity,) stack of free page ids, written in place */
+    int32_t free_capacity;
+    const int32_t* num_free;         /* (1,) ids on the stack; taken as within [0, free_capacity] */
+    int32_t* num_free_out;           /* (1,) ids on it after the step, negative by the pages that were missing */
+    int32_t* cu_seqlens_new;         /* (batch + 1,) prefix of the new tokens of the requests */
+    int64_t* slot_mapping;           /* (total_new,) slot of each new token, -1 where there is none */
+    int64_t total_new;
+} fa_page_table_params;
+
+/* Takes the step in this order. Pages that requests no longer need go onto the
+ * stack, request by request (ids below 0 and ids that the stack has no room for
+ * are dropped). Pages that requests need come off its top, request by request; an
+ * empty stack gives -1. Tokens past max_pages * page_size have no page. Entries
+ * of num_free_out, cu_seqlens_new and slot_mapping may not overlap the inputs. */
+fa_status_t fa_update_page_table(const fa_page_table_params* p, void* stream);
+
+typedef struct fa_quant_append_params {
+    int32_t abi_version;
+    int32_t dtype;                   /* of k_new, v_new: FP16 or BF16 */
+    int32_t cache_dtype;             /* INT8 or FP8_E4M3 */
+    int32_t nheads_k, headdim;       /* headdim: a multiple of 16, at most 256 */
+    int32_t num_pages, page_size, scale_block;
+    int64_t total_new;
+    const void* k_new;               /* (total_new, Hk, D) */
+    int64_t knew_row_stride, knew_head_stride;
+    const void* v_new;
+    int64_t vnew_row_stride, vnew_head_stride;
+    void* k;                         /* written in place, as v and the scales */
+    int64_t k_page_stride, k_row_stride, k_head_stride;
+    void* v;
+    int64_t v_page_stride, v_row_stride, v_head_stride;
+    float* k_scale;
+    int64_t k_scale_page_stride, k_scale_block_stride, k_scale_head_stride;
+    float* v_scale;
+    int64_t v_scale_page_stride, v_scale_block_stride, v_scale_head_stride;
+    const int64_t* slot_mapping;     /* (total_new,) slot of each row; rows with a slot outside the cache are skipped */
+} fa_quant_append_params;
+
+/* Quantises the new rows into their slots. Rows whose slots lie in one block
+ * stand together in slot_mapping (a run); their slots differ. The scale of a
+ * run's block and head is the smallest power of two s with max |x| <= s * m over
+ * the run (m = 127 for int8, 448 for e4m3; s >= 2^-100, +-inf counts as the largest finite
+ * value of dtype, NaN is left out), or the block's old scale where that is larger and the run does
+ * not begin the block. Where the scale of a begun block grows, the codes before
+ * the run's first row are rounded to the new scale. Codes are x / s rounded to
+ * nearest even; NaN becomes 0 in int8 and NaN in e4m3. */
+fa_status_t fa_quant_append(const fa_quant_append_params* p, void* stream);
+
+typedef struct fa_quant_fwd_params {
+    int32_t abi_version;
+    int32_t dtype;                   /* of q and out: FP16 or BF16 */
+    int32_t cache_dtype;             /* INT8 or FP8_E4M3 */
+    int32_t batch;
+    int32_t seqlen_q;                /* query rows of a sequence, the most of any with cu_seqlens_q */
+    int32_t nheads, nheads_k, headdim; /* headdim: a multiple of 16, at most 256 */
+    int32_t num_pages, page_size, scale_block;
+    const void* q;                   /* (B, Sq, H, D), with cu_seqlens_q (total_q, H, D) */
+    int64_t q_batch_stride, q_row_stride, q_head_stride;
+    const void* k;
+    int64_t k_page_stride, k_row_stride, k_head_stride;
+    const void* v;
+    int64_t v_page_stride, v_row_stride, v_head_stride;
+    const float* k_scale;
+    int64_t k_scale_page_stride, k_scale_block_stride, k_scale_head_stride;
+    const float* v_scale;
+    int64_t v_scale_page_stride, v_scale_block_stride, v_scale_head_stride;
+    void* out;                       /* like q */
+    int64_t out_batch_stride, out_row_stride, out_head_stride;
+    float* softmax_lse;              /* (B, H, Sq), with cu_seqlens_q (H, total_q) */
+    const int32_t* cache_seqlens;    /* (B,) keys of each sequence, the step's own among them */
+    const int32_t* cu_seqlens_q;     /* (B + 1,) or NULL */
+    int32_t total_q;                 /* with cu_seqlens_q */
+    const int32_t* page_table;       /* (table_rows, max_pages) or NULL: contiguous */
+    int64_t page_table_row_stride;
+    int32_t table_rows, max_pages;
+    const int32_t* cache_batch_idx;  /* (B,) row of the page table (of the cache when contiguous), or NULL: row b */
+    float softmax_scale;
+    float softcap;                   /* 0 = off */
+    int32_t is_causal;
+    int32_t window_size_left, window_size_right; /* -1 = unbounded */
+    void* workspace;                 /* fa_quant_fwd_workspace_size() bytes, 256-byte aligned */
+    size_t workspace_bytes;
+} fa_quant_fwd_params;
+
+/* Attention over the cache: with c the codes,
+ *   scores[i, j] = softmax_scale * k_scale[block of j] * (q_i . ck_j)   (soft cap as in fa_mha_fwd)
+ *   out[i]       = sum_j softmax(scores)[i, j] * v_scale[block of j] * cv_j
+ * with the masks of fa_mha_fwd_kvcache (bottom-right causal, local window). Keys
+ * on a page whose id is not in [0, num_pages) are not visible. A row that sees no
+ * key gets out 0, lse +inf; rows of out behind the last sequence of cu_seqlens_q
+ * are left as they are. */
+fa_status_t fa_quant_fwd_workspace_size(const fa_quant_fwd_params* p, size_t* bytes);
+fa_status_t fa_quant_fwd(const fa_quant_fwd_params* p, void* stream);
 
 /* Thread-local message describing the last non-FA_OK status on this thread. */
 const char* fa_last_error(void);
