@@ -875,6 +875,7 @@ fa_status_t forward_kvcache_on(const fa_fwd_params* p, void* stream, void* scrat
     return run_forward_ws(p, FA_KIND_KVCACHE, stream, scratch, bytes);
 }
 fa_status_t report_error(fa_status_t st, const char* msg) { return fail(st, "%s", msg); }
+int compute_units() { return cu_count(); }
 }  // namespace fa
 
 extern "C" {

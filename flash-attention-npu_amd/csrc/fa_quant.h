@@ -1,0 +1,91 @@
+// fa_quant.h -- device code that the attention kernels over 8-bit codes share:
+// codes to fp16 operands, and the sequences of a call.
+//
+// Every code is an fp16 value (int8: |c| <= 128; e4m3: steps of 2^-9 up to 448), so
+// both products run as fp16 MFMAs on the codes themselves and the scales meet the
+// results: K's on the scores, V's on the weights.
+#pragma once
+#include "fa_common.h"
+#include "fa_quant_args.h"
+
+namespace fa {
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ uint32_t byte_perm(uint32_t hi, uint32_t lo, uint32_t sel) {
+    return __builtin_amdgcn_perm(hi, lo, sel);  // sel bytes 0..3: of lo, 4..7: of hi
+}
+
+// Four codes (the bytes of w, lowest first) as four fp16 values, exactly.
+// int8: the byte plus 128 under the exponent of 1024 is 1152 + c.
+template <int CT>
+__device__ __forceinline__ u32x2 widen4(uint32_t w) {
+    if constexpr (CT == CT_INT8) {
+        const uint32_t u = w ^ 0x80808080u;
+        const f16x2 off = {(_Float16)1152.f, (_Float16)1152.f};
+        const f16x2 a = __builtin_bit_cast(f16x2, byte_perm(0x64646464u, u, 0x04010400u)) - off;
+        const f16x2 b = __builtin_bit_cast(f16x2, byte_perm(0x64646464u, u, 0x04030402u)) - off;
+        return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+    } else {
+        return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, false)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, true))};
+    }
+}
+
+__device__ __forceinline__ f32x4 mfma_f16(u32x4 a, u32x4 b, f32x4 c) { return mfma16x16x32<DT_FP16>(a, b, c); }
+
+// 2^k for k in [-126, 127]
+__device__ __forceinline__ float exp2i(int k) { return __builtin_bit_cast(float, (uint32_t)(k + 127) << 23); }
+
+// A query row enters its products as fp16, times the power of two that puts its
+// largest value in [2^14, 2^15): a bf16 value keeps its 8 bits down to 2^-28 of
+// the largest and what is lost below is less than 2^-38 of it, under the rounding of the
+// fp32 sums. The exponent for a row whose largest |q| is `most`:
+__device__ __forceinline__ int q_shift(float most) {
+    const int e = (int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127;
+    return most > 0.f ? min(14 - e, 126) : 0;
+}
+
+// Keys and query rows of a sequence; [lo, hi) holds the keys that some row sees.
+struct QuantSeq {
+    int lo, hi, sk, sq, crow;
+};
+
+__device__ __forceinline__ QuantSeq quant_seq(const QuantFwdArgs& a, int b) {
+    QuantSeq s;
+    const int sq = a.cu_q ? a.cu_q[b + 1] - a.cu_q[b] : a.Sq;
+    s.sq = min(max(sq, 0), a.Sq);
+    s.sk = min(max(a.seqlens[b], 0), a.capacity);
+    s.lo = max(0, key_lo(s.sk - s.sq, a.wl, 0));
+    s.hi = min(s.sk, key_hi(s.sk - 1, a.wr, 0) + 1);
+    s.crow = a.batch_idx ? min(max(a.batch_idx[b], 0), a.rows - 1) : a.row0 + b;
+    if (s.sq == 0) s.hi = s.lo;
+    return s;
+}
+
+// Rows of q and out, and the lse, of query position i of sequence b
+__device__ __forceinline__ int64_t q_row(const QuantFwdArgs& a, int b, int i, int64_t sb, int64_t si) {
+    return a.cu_q ? ((int64_t)a.cu_q[b] + i) * si : (int64_t)b * sb + (int64_t)i * si;
+}
+__device__ __forceinline__ int64_t lse_at(const QuantFwdArgs& a, int b, int h, int i) {
+    return a.cu_q ? (int64_t)h * a.lse_sh + a.cu_q[b] + i : (int64_t)b * a.lse_sb + (int64_t)h * a.lse_sh + i;
+}
+
+// eight 16-bit values of either type as fp32
+__device__ __forceinline__ f32x8 load8(const void* base, int64_t off, bool bf16) {
+    const u32x4 r = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(base) + off);
+    f32x8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint16_t h = (uint16_t)(r[e >> 1] >> (16 * (e & 1)));
+        y[e] = bf16 ? f16_to_32<DT_BF16>(h) : f16_to_32<DT_FP16>(h);
+    }
+    return y;
+}
+__device__ __forceinline__ uint32_t pack2(float x, float y, bool bf16) {
+    const uint32_t b = (uint32_t)f32_to_16<DT_BF16>(x) | (uint32_t)f32_to_16<DT_BF16>(y) << 16;
+    const uint32_t h = (uint32_t)f32_to_16<DT_FP16>(x) | (uint32_t)f32_to_16<DT_FP16>(y) << 16;
+    return bf16 ? b : h;
+}
+
+}  // namespace fa

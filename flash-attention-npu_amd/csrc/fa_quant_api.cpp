@@ -17,6 +17,9 @@ fa_status_t report_error(fa_status_t st, const char* msg);
 hipError_t launch_page_table(const PageTableArgs& a, hipStream_t stream);
 hipError_t launch_quant_append(const QuantAppendArgs& a, int dtype, int ct, hipStream_t stream);
 hipError_t launch_quant_fwd(const QuantFwdArgs& a, int dtype, int ct, hipStream_t stream);
+int quant_decode_workers(int grid);
+hipError_t launch_quant_decode(const QuantFwdArgs& a, int ct, int kd, int nr, int grid, hipStream_t stream);
+int compute_units();
 }  // namespace fa
 
 namespace {
@@ -126,7 +129,44 @@ fa_status_t check_fwd(const fa_quant_fwd_params* p) {
     FA_CHECK(multiples(16, p->k_page_stride, p->k_row_stride, p->k_head_stride) &&
                  multiples(16, p->v_page_stride, p->v_row_stride, p->v_head_stride),
              "strides of the caches must be multiples of 16");
+    // the rows of 16 keys are addressed in 32 bits
+    FA_CHECK(p->k_row_stride >= 0 && p->k_row_stride < (1 << 27) && p->v_row_stride >= 0 && p->v_row_stride < (1 << 27),
+             "row strides of the caches must be in [0, 2^27)");
     return FA_OK;
+}
+
+constexpr int kMaxBatch = 2048;  // sequences of one launch (their list lives in LDS)
+constexpr int kDecodeRows = 64;  // packed rows of a kv head that the decode kernel takes
+
+struct Plan {
+    int kd;          // kernel head dim
+    int g;
+    int dec_rows;    // sequences of at most so many packed rows run on the decode kernel
+    bool prefill;    // some may have more
+    int nr;          // decode: 16-row tiles
+    int grid;        // decode: workgroups
+    size_t off_lse, off_o, total;
+};
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+Plan make_plan(const fa_quant_fwd_params* p) {
+    Plan pl{};
+    pl.kd = p->headdim <= 64 ? 64 : p->headdim <= 128 ? 128 : 256;
+    pl.g = p->nheads / p->nheads_k;
+    const int64_t rows = (int64_t)p->seqlen_q * pl.g;
+    pl.prefill = rows > kDecodeRows;
+    // of a ragged batch with longer sequences the ones at their next token or two
+    pl.dec_rows = !pl.prefill ? (int)rows : p->cu_seqlens_q ? 16 : 0;
+    pl.nr = pl.dec_rows <= 16 ? 1 : pl.dec_rows <= 32 ? 2 : 4;
+    pl.grid = fa::compute_units();
+    if (pl.dec_rows) {
+        const size_t parts = (size_t)fa::quant_decode_workers(pl.grid) * 2 * 16 * pl.nr;
+        pl.off_lse = align256(sizeof(int) * ((size_t)std::min(p->batch, kMaxBatch) + 1));
+        pl.off_o = align256(pl.off_lse + sizeof(float) * parts);
+        pl.total = align256(pl.off_o + sizeof(float) * parts * pl.kd);
+    }
+    return pl;
 }
 
 int window_bound(int32_t w) { return w < 0 ? -1 : std::min(w, 1 << 30); }
@@ -204,7 +244,7 @@ fa_status_t fa_quant_fwd_workspace_size(const fa_quant_fwd_params* p, size_t* by
     if (!bytes) return fail(FA_EINVAL, "bytes must not be null");
     fa_status_t st = check_fwd(p);
     if (st != FA_OK) return st;
-    *bytes = 0;
+    *bytes = p->seqlen_q > 0 ? make_plan(p).total : 0;
     return FA_OK;
 }
 
@@ -213,6 +253,12 @@ fa_status_t fa_quant_fwd(const fa_quant_fwd_params* p, void* stream) {
     if (st != FA_OK) return st;
     const int64_t rows = p->cu_seqlens_q ? (int64_t)p->total_q : (int64_t)p->batch * p->seqlen_q;
     if (rows == 0 || p->seqlen_q == 0) return FA_OK;
+    const Plan pl = make_plan(p);
+    if (pl.total > 0) {
+        if (!p->workspace || p->workspace_bytes < pl.total)
+            return fail(FA_EWORKSPACE, "workspace of %zu bytes required, %zu given", pl.total, p->workspace ? p->workspace_bytes : (size_t)0);
+        if (reinterpret_cast<uintptr_t>(p->workspace) & 255u) return fail(FA_EWORKSPACE, "workspace must be 256-byte aligned");
+    }
     fa::QuantFwdArgs a{};
     a.q = p->q;
     a.q_sb = p->q_batch_stride;
@@ -255,17 +301,40 @@ fa_status_t fa_quant_fwd(const fa_quant_fwd_params* p, void* stream) {
     a.capacity = (int)((int64_t)a.max_pages * p->page_size);
     a.scale = p->softmax_scale;
     a.softcap = p->softcap;
-    a.B = p->batch;
     a.Sq = p->seqlen_q;
     a.H = p->nheads;
     a.Hk = p->nheads_k;
-    a.g = p->nheads / p->nheads_k;
+    a.g = pl.g;
     a.hd = p->headdim;
     a.total_q = p->total_q;
     a.wl = window_bound(p->window_size_left);
     a.wr = p->is_causal ? 0 : window_bound(p->window_size_right);
-    hipError_t e = fa::launch_quant_fwd(a, p->dtype, p->cache_dtype, static_cast<hipStream_t>(stream));
-    if (e != hipSuccess) return fail(FA_EHIP, "attention launch failed: %s", hipGetErrorString(e));
+    a.bf16 = p->dtype == FA_DTYPE_BF16;
+    a.dec_rows = pl.dec_rows;
+    char* ws = static_cast<char*>(p->workspace);
+    a.sched = reinterpret_cast<int*>(ws);
+    a.part_lse = reinterpret_cast<float*>(ws + pl.off_lse);
+    a.part_o = reinterpret_cast<float*>(ws + pl.off_o);
+    // a batch of more sequences than a launch lists runs in parts, one after another
+    // on the stream and on the same scratch
+    for (int b0 = 0; b0 < p->batch; b0 += kMaxBatch) {
+        fa::QuantFwdArgs c = a;
+        c.B = std::min(p->batch - b0, kMaxBatch);
+        c.row0 = b0;
+        c.seqlens = a.seqlens + b0;
+        if (a.cu_q) {
+            c.cu_q = a.cu_q + b0;
+        } else {
+            c.q = static_cast<const uint16_t*>(a.q) + (int64_t)b0 * a.q_sb;
+            c.out = static_cast<uint16_t*>(a.out) + (int64_t)b0 * a.o_sb;
+            c.lse = a.lse + (int64_t)b0 * a.lse_sb;
+        }
+        if (a.batch_idx) c.batch_idx = a.batch_idx + b0;
+        hipError_t e = hipSuccess;
+        if (pl.dec_rows) e = fa::launch_quant_decode(c, p->cache_dtype, pl.kd, pl.nr, pl.grid, static_cast<hipStream_t>(stream));
+        if (e == hipSuccess && pl.prefill) e = fa::launch_quant_fwd(c, p->dtype, p->cache_dtype, static_cast<hipStream_t>(stream));
+        if (e != hipSuccess) return fail(FA_EHIP, "attention launch failed: %s", hipGetErrorString(e));
+    }
     return FA_OK;
 }
 

@@ -68,7 +68,14 @@ struct QuantFwdArgs {
     float scale;                   // softmax_scale
     float softcap;                 // 0 = off
     int B, Sq, H, Hk, g, hd, total_q;
+    int row0;                      // row of sequence 0 without batch_idx
     int wl, wr;                    // normalised window, -1 = unbounded, causal => wr = 0
+    int bf16;                      // q and out: 0 = fp16, 1 = bf16
+    int dec_rows;                  // sequences of at most as many packed rows take the decode kernel
+    // scratch of the decode kernel
+    int* sched;                    // [0..B]: tile prefix
+    float* part_lse;               // [worker][2][16 * row tiles]
+    float* part_o;                 // [worker][2][16 * row tiles][kernel head dim]
 };
 
 }  // namespace fa

@@ -48,11 +48,12 @@ __global__ void __launch_bounds__(NT) fa_quant_fwd_kernel(QuantFwdArgs a) {
         i = (int)(T % a.Sq);
         sq = a.Sq;
     }
+    if (sq * a.g <= a.dec_rows) return;
     const uint16_t* q = static_cast<const uint16_t*>(a.q) + (a.cu_q ? T * a.q_si : (int64_t)b * a.q_sb + (int64_t)i * a.q_si) +
                         (int64_t)h * a.q_sh;
     if (tid < a.hd) s_q[tid] = f16_to_32<DT>(q[tid]);
     const int sk = min(max(a.seqlens[b], 0), a.capacity);
-    const int row = a.batch_idx ? min(max(a.batch_idx[b], 0), a.rows - 1) : b;
+    const int row = a.batch_idx ? min(max(a.batch_idx[b], 0), a.rows - 1) : a.row0 + b;
     const int d = i + sk - sq;
     const int lo = max(0, key_lo(d, a.wl, 0)), hi = min(sk, key_hi(d, a.wr, 0) + 1);
     float m = -INFINITY, l = 0.f, acc = 0.f;

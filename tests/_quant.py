@@ -51,7 +51,8 @@ class Cache:
         return [t.to(dev) for t in (*self.codes, *self.scales)]
 
     def rows(self, b):
-        """k, v in 64 bits and whether their page is in the cache, of sequence b."""
+        """k, v in 64 bits, whether their page is in the cache, and the largest value that its v could hold, of
+        sequence b."""
         n = self.lens[b]
         if self.table is None:
             pages = [b]
@@ -59,18 +60,24 @@ class Cache:
             pages = self.table[b].tolist()
         k, ok = qo.rows_of(self.codes[0], self.scales[0], pages, n)
         v, _ = qo.rows_of(self.codes[1], self.scales[1], pages, n)
-        return k, v, ok
+        return k, v, ok, largest(self.codes[1], self.scales[1])
 
 
-def check_attend(out, lse, q, k, v, ok, dtype, scale=None, softcap=0.0, **how):
+def largest(codes, scale):
+    return scale.nan_to_num(0.0).abs().max().item() * qo.CODE_MAX[codes.dtype]
+
+
+def check_attend(out, lse, q, k, v, ok, top, dtype, scale=None, softcap=0.0, **how):
     """out (n, H, D) and lse (H, n) of one sequence against the definition.
 
     The bounds count: the 16-bit codes of q, K and V enter their products exactly;
     a score is an fp32 sum of D products and a handful of roundings, so off by
     less than d = (D + 16) 2^-24 X, X the sum of the products' sizes (a soft cap
     adds the 2^-21 of its tanh, times the cap); e^x moves by d, sums of n of them
-    by n 2^-24; the weights are rounded to 16 bits before they meet V (fp16 half a
-    step, 2^-11); the result is rounded once more."""
+    by n 2^-24; the weights p t of the V scales t are rounded to fp16 before they
+    meet V: half a step, 2^-11, or 2^-25 of the unit they are kept in, which is at
+    most 2 max t 2^-14, so 2^-38 max t for each of L keys and `top`, max t times the
+    largest code, for what they multiply; the result is rounded once more."""
     n, H, D = q.shape
     L, g = k.shape[0], H // k.shape[1]
     if scale is None:
@@ -86,6 +93,7 @@ def check_attend(out, lse, q, k, v, ok, dtype, scale=None, softcap=0.0, **how):
     assert not torch.isnan(got).any(), "NaN in out"
     half = torch.finfo(dtype).eps / 2
     bound = size * (2.0 ** -11 + 2 * d + (L + 16) * 2.0 ** -24) + half * ref.abs() + torch.finfo(dtype).smallest_normal * half * 2
+    bound = bound + L * 2.0 ** -38 * top
     worst = ((got - ref).abs() / bound.clamp(min=1e-300)).max().item() if got.numel() else 0.0
     assert worst <= 1, f"out {worst:.2f} times its bound"
     got = lse.detach().cpu().double()

@@ -8,7 +8,7 @@ import torch
 
 import flash_attn_npu_v3 as fa
 from oracle import fa_quant_oracle as qo
-from tests._quant import CACHES, TYPES, check_attend
+from tests._quant import CACHES, TYPES, check_attend, largest
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -419,5 +419,6 @@ def test_serving_steps(cache, page, block):
             if m:
                 kk, ok = qo.rows_of(st[0], st[2], table[i], y)
                 vv, _ = qo.rows_of(st[1], st[3], table[i], y)
-                check_attend(out[at:at + m], lse[:, at:at + m], q[at:at + m], kk, vv, ok, torch.bfloat16, causal=True)
+                check_attend(out[at:at + m], lse[:, at:at + m], q[at:at + m], kk, vv, ok, largest(st[1], st[3]),
+                             torch.bfloat16, causal=True)
             at += m

@@ -63,7 +63,8 @@ def test_fwd_accepts():
     (dict(v_scale=None), "required"), (dict(softmax_lse=None), "required"), (dict(q=PTR + 8), "aligned"), (dict(k=PTR + 4), "aligned"),
     (dict(q_row_stride=1028), "multiples of 8"), (dict(out_head_stride=4), "multiples of 8"),
     (dict(k_row_stride=264), "multiples of 16"), (dict(v_head_stride=8), "multiples of 16"),
-    (dict(seqlen_q=1 << 30), "too many query rows")])
+    (dict(seqlen_q=1 << 30), "too many query rows"), (dict(k_row_stride=1 << 27), "row strides"),
+    (dict(v_row_stride=-256), "row strides")])
 def test_fwd_refuses(more, says):
     p = capi.new_quant_fwd_params(**dict(FWD, **more))
     assert capi.quant_fwd(p) == capi.FA_EINVAL and says in capi.last_error(), capi.last_error()
