@@ -30,7 +30,7 @@ ARCH = os.environ.get("FA_MI355X_ARCH", "gfx950")
 HIP_SOURCES = ["fa_fwd.hip", "fa_fwd_pipe64.hip", "fa_fwd_pipe128.hip", "fa_fwd_pipe256.hip",
                "fa_fwd_pipe_fp8.hip", "fa_decode.hip", "fa_kv_prep.hip", "fa_bwd.hip", "fa_bwd_kv.hip",
                "fa_bwd_dq.hip", "fa_api.cpp", "fa_noalloc.hip", "fa_page_table.hip", "fa_quant_append.hip",
-               "fa_quant_fwd.hip", "fa_quant_decode.hip", "fa_quant_api.cpp"]
+               "fa_quant_decode.hip", "fa_quant_prefill.hip", "fa_quant_api.cpp"]
 HIPFLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
     # no packed fp32 ops (v_pk_*_f32) in any generated code

@@ -16,9 +16,11 @@ namespace fa {
 fa_status_t report_error(fa_status_t st, const char* msg);
 hipError_t launch_page_table(const PageTableArgs& a, hipStream_t stream);
 hipError_t launch_quant_append(const QuantAppendArgs& a, int dtype, int ct, hipStream_t stream);
-hipError_t launch_quant_fwd(const QuantFwdArgs& a, int dtype, int ct, hipStream_t stream);
 int quant_decode_workers(int grid);
 hipError_t launch_quant_decode(const QuantFwdArgs& a, int ct, int kd, int nr, int grid, hipStream_t stream);
+int quant_prefill_rows(int kd);
+int quant_prefill_keys(int kd);
+hipError_t launch_quant_prefill(const QuantFwdArgs& a, int ct, int kd, int grid, int mt_max, hipStream_t stream);
 int compute_units();
 }  // namespace fa
 
@@ -143,9 +145,11 @@ struct Plan {
     int g;
     int dec_rows;    // sequences of at most so many packed rows run on the decode kernel
     bool prefill;    // some may have more
-    int nr;          // decode: 16-row tiles
-    int grid;        // decode: workgroups
-    size_t off_lse, off_o, total;
+    int nr, grid;    // decode: 16-row tiles, workgroups
+    int pf_grid, mt_max;
+    bool allow_split;
+    int target_items, min_chunk;
+    size_t off_lse, off_o, off_psched, off_plse, off_po, total;
 };
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -159,13 +163,36 @@ Plan make_plan(const fa_quant_fwd_params* p) {
     // of a ragged batch with longer sequences the ones at their next token or two
     pl.dec_rows = !pl.prefill ? (int)rows : p->cu_seqlens_q ? 16 : 0;
     pl.nr = pl.dec_rows <= 16 ? 1 : pl.dec_rows <= 32 ? 2 : 4;
-    pl.grid = fa::compute_units();
+    const int cus = fa::compute_units();
+    const size_t nb = std::min(p->batch, kMaxBatch);
+    pl.grid = cus;
+    size_t off = 0;
     if (pl.dec_rows) {
         const size_t parts = (size_t)fa::quant_decode_workers(pl.grid) * 2 * 16 * pl.nr;
-        pl.off_lse = align256(sizeof(int) * ((size_t)std::min(p->batch, kMaxBatch) + 1));
-        pl.off_o = align256(pl.off_lse + sizeof(float) * parts);
-        pl.total = align256(pl.off_o + sizeof(float) * parts * pl.kd);
+        pl.off_lse = off = align256(sizeof(int) * (nb + 1));
+        pl.off_o = off = align256(off + sizeof(float) * parts);
+        off = align256(off + sizeof(float) * parts * pl.kd);
     }
+    if (pl.prefill) {
+        const int bm = fa::quant_prefill_rows(pl.kd);
+        pl.mt_max = (int)((rows + bm - 1) / bm);
+        int64_t items = (int64_t)nb * pl.mt_max * p->nheads_k;
+        // ragged: a part tile more per sequence than the rows fill
+        if (p->cu_seqlens_q) items = std::min(items, ((int64_t)p->total_q * pl.g / bm + (int64_t)nb) * p->nheads_k);
+        pl.allow_split = items < cus;
+        pl.target_items = cus;
+        pl.min_chunk = 4 * fa::quant_prefill_keys(pl.kd);
+        // pieces: each item's keys in chunks of at least the mean work, so at most one part chunk more each
+        const int64_t pieces = pl.allow_split ? items + pl.target_items : items;
+        pl.pf_grid = (int)std::min<int64_t>(pieces, pl.allow_split ? 2 * cus : cus);
+        if (pl.allow_split) {
+            pl.off_psched = off;
+            pl.off_plse = off = align256(off + sizeof(int) * (2 * nb + 1));
+            pl.off_po = off = align256(off + sizeof(float) * pieces * bm);
+            off = align256(off + sizeof(float) * pieces * bm * pl.kd);
+        }
+    }
+    pl.total = off;
     return pl;
 }
 
@@ -315,6 +342,12 @@ fa_status_t fa_quant_fwd(const fa_quant_fwd_params* p, void* stream) {
     a.sched = reinterpret_cast<int*>(ws);
     a.part_lse = reinterpret_cast<float*>(ws + pl.off_lse);
     a.part_o = reinterpret_cast<float*>(ws + pl.off_o);
+    a.allow_split = pl.allow_split;
+    a.target_items = pl.target_items;
+    a.min_chunk = pl.min_chunk;
+    a.pf_sched = reinterpret_cast<int*>(ws + pl.off_psched);
+    a.pf_lse = reinterpret_cast<float*>(ws + pl.off_plse);
+    a.pf_o = reinterpret_cast<float*>(ws + pl.off_po);
     // a batch of more sequences than a launch lists runs in parts, one after another
     // on the stream and on the same scratch
     for (int b0 = 0; b0 < p->batch; b0 += kMaxBatch) {
@@ -332,7 +365,7 @@ fa_status_t fa_quant_fwd(const fa_quant_fwd_params* p, void* stream) {
         if (a.batch_idx) c.batch_idx = a.batch_idx + b0;
         hipError_t e = hipSuccess;
         if (pl.dec_rows) e = fa::launch_quant_decode(c, p->cache_dtype, pl.kd, pl.nr, pl.grid, static_cast<hipStream_t>(stream));
-        if (e == hipSuccess && pl.prefill) e = fa::launch_quant_fwd(c, p->dtype, p->cache_dtype, static_cast<hipStream_t>(stream));
+        if (e == hipSuccess && pl.prefill) e = fa::launch_quant_prefill(c, p->cache_dtype, pl.kd, pl.pf_grid, pl.mt_max, static_cast<hipStream_t>(stream));
         if (e != hipSuccess) return fail(FA_EHIP, "attention launch failed: %s", hipGetErrorString(e));
     }
     return FA_OK;

@@ -76,6 +76,12 @@ struct QuantFwdArgs {
     int* sched;                    // [0..B]: tile prefix
     float* part_lse;               // [worker][2][16 * row tiles]
     float* part_o;                 // [worker][2][16 * row tiles][kernel head dim]
+    // prefill kernel: items may be cut over the keys into about target_items
+    // pieces of at least min_chunk keys; their scratch
+    int allow_split, target_items, min_chunk;
+    int* pf_sched;                 // [0..B]: item prefix, [B+1..2B]: pieces of each sequence's items
+    float* pf_lse;                 // [item][rows of an item]
+    float* pf_o;                   // [item][rows of an item][kernel head dim]
 };
 
 }  // namespace fa
