@@ -8,6 +8,12 @@
 // released. Token i of request b has slot table[(before + i) / P] * P + (before +
 // i) % P. Nothing below n0 is written and no entry of the table that the step
 // still uses, so a step taken twice gives the same.
+//
+// What bounds it is latency: a few dependent reads, one launch. Every workgroup
+// makes the prefix sums for itself in LDS (lengths and released ids are a few KB,
+// read from L2) and then writes its share of stack, table and slots; an id that
+// this step both releases and takes is found in the table, where its owner's row
+// is not written, so no workgroup waits for another.
 #include "fa_common.h"
 #include "fa_quant_args.h"
 
@@ -59,8 +65,113 @@ __device__ __forceinline__ Req request(const PageTableArgs& a, int b) {
     return r;
 }
 
-// One workgroup: the stack, the table, the prefix of the new tokens.
+constexpr int MAXB = 4096;  // requests whose sums fit in LDS
+
+// Inclusive prefix of s[1..n] over the workgroup, in place (s[0] = 0); `carry` is
+// scratch.
+__device__ __forceinline__ void scan_lds(int* s, int n, int* s_w) {
+    int carry = 0;
+    for (int b0 = 0; b0 < n; b0 += NT) {
+        const int b = b0 + threadIdx.x, v = b < n ? s[b + 1] : 0;
+        int sum;
+        const int pre = carry + block_scan(v, s_w, sum);
+        carry += sum;
+        if (b < n) s[b + 1] = pre + v;
+    }
+    if (threadIdx.x == 0) s[0] = 0;
+    __syncthreads();
+}
+
 __global__ void __launch_bounds__(NT) fa_page_table_kernel(PageTableArgs a) {
+    __shared__ int s_rel[MAXB + 1], s_val[MAXB + 1], s_take[MAXB + 1], s_fresh[MAXB + 1], s_w[NT / 64];
+    const int tid = threadIdx.x, B = a.B;
+    const int64_t first = (int64_t)blockIdx.x * NT + tid, stride = (int64_t)gridDim.x * NT;
+    const int n0 = min(max(a.num_free[0], 0), a.free_cap);
+    for (int b = tid; b < B; b += NT) {
+        const Req r = request(a, b);
+        s_rel[b + 1] = max(r.have - r.need, 0);
+        s_take[b + 1] = max(r.need - r.have, 0);
+        s_fresh[b + 1] = r.fresh;
+        s_val[b + 1] = 0;
+    }
+    scan_lds(s_rel, B, s_w);
+    scan_lds(s_take, B, s_w);
+    scan_lds(s_fresh, B, s_w);
+    const int raw = s_rel[B], taken = s_take[B], fresh = s_fresh[B];
+    // released entry f of the requests in turn: its request and id
+    auto entry = [&](int f, int& b, int& j) -> int {
+        b = seq_of(s_rel, B, f);
+        const Req r = request(a, b);
+        j = f - s_rel[b];
+        return a.table[(int64_t)r.row * a.t_stride + r.need + j];
+    };
+    if (raw > 0) {  // how many of each request's are ids
+        for (int f = tid; f < raw; f += NT) {
+            int b, j;
+            if (entry(f, b, j) >= 0) atomicAdd(&s_val[b + 1], 1);
+        }
+        __syncthreads();
+        scan_lds(s_val, B, s_w);
+        for (int64_t f = first; f < raw; f += stride) {
+            int b, j;
+            const int id = entry((int)f, b, j);
+            if (id < 0) continue;
+            int rank = j;
+            if (s_val[b + 1] - s_val[b] != s_rel[b + 1] - s_rel[b]) {  // -1 among them
+                rank = 0;
+                for (int u = 0; u < j; ++u) {
+                    int bb, jj;
+                    rank += entry(s_rel[b] + u, bb, jj) >= 0;
+                }
+            }
+            const int64_t at = (int64_t)n0 + s_val[b] + rank;
+            if (at < a.free_cap) a.free_pages[at] = id;
+        }
+    }
+    const int released = raw > 0 ? s_val[B] : 0;
+    const int top = (int)min((int64_t)n0 + released, (int64_t)a.free_cap);
+    // the id that needed page t comes to
+    auto page_at = [&](int t) -> int {
+        const int at = top - 1 - t;
+        if (at < 0) return -1;
+        if (at < n0) return a.free_pages[at];
+        const int b = seq_of(s_val, B, at - n0);
+        int k = at - n0 - s_val[b], bb, jj;
+        if (s_val[b + 1] - s_val[b] == s_rel[b + 1] - s_rel[b]) return entry(s_rel[b] + k, bb, jj);
+        for (int u = s_rel[b]; u < s_rel[b + 1]; ++u) {
+            const int id = entry(u, bb, jj);
+            if (id >= 0 && k-- == 0) return id;
+        }
+        return -1;
+    };
+    for (int64_t t = first; t < taken; t += stride) {
+        const int b = seq_of(s_take, B, (int)t);
+        const Req r = request(a, b);
+        a.table[(int64_t)r.row * a.t_stride + r.have + ((int)t - s_take[b])] = page_at((int)t);
+    }
+    for (int64_t i = first; i < a.total_new; i += stride) {
+        int64_t slot = -1;
+        if (i < fresh) {
+            const int b = seq_of(s_fresh, B, (int)i);
+            const Req r = request(a, b);
+            const int64_t at = (int64_t)max(a.before[b], 0) + (i - s_fresh[b]);
+            if (r.row >= 0 && at < (int64_t)a.max_pages * a.page_size) {
+                const int j = (int)udiv(a.page, (uint32_t)at);
+                const int id = j < r.have ? a.table[(int64_t)r.row * a.t_stride + j] : page_at(s_take[b] + j - r.have);
+                if (id >= 0) slot = (int64_t)id * a.page_size + (at - (int64_t)j * a.page_size);
+            }
+        }
+        a.slots[i] = slot;
+    }
+    if (blockIdx.x == 0) {
+        for (int b = tid; b <= B; b += NT) a.cu_new[b] = s_fresh[b];
+        if (tid == 0) a.num_free_out[0] = top - taken;
+    }
+}
+
+// For more requests: one workgroup writes the stack, the table and the prefix of
+// the new tokens, ...
+__global__ void __launch_bounds__(NT) fa_page_table_large_kernel(PageTableArgs a) {
     __shared__ int s_w[NT / 64];
     const int n0 = min(max(a.num_free[0], 0), a.free_cap);
     int released = 0;
@@ -102,7 +213,7 @@ __global__ void __launch_bounds__(NT) fa_page_table_kernel(PageTableArgs a) {
     }
 }
 
-// The slots, one thread each, from the table and prefix that the kernel above left.
+// ... and a second launch the slots, from what the first left.
 __global__ void __launch_bounds__(256) fa_slot_kernel(PageTableArgs a) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= a.total_new) return;
@@ -123,7 +234,13 @@ __global__ void __launch_bounds__(256) fa_slot_kernel(PageTableArgs a) {
 }  // namespace
 
 hipError_t launch_page_table(const PageTableArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL(fa_page_table_kernel, dim3(1), dim3(NT), 0, stream, a);
+    if (a.B <= MAXB) {
+        // two slots a thread: few enough workgroups that their common work stays small
+        const int grid = (int)((a.total_new + 2 * NT - 1) / (2 * NT));
+        hipLaunchKernelGGL(fa_page_table_kernel, dim3(grid < 1 ? 1 : grid > 256 ? 256 : grid), dim3(NT), 0, stream, a);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL(fa_page_table_large_kernel, dim3(1), dim3(NT), 0, stream, a);
     if (a.total_new > 0)
         hipLaunchKernelGGL(fa_slot_kernel, dim3((unsigned)((a.total_new + 255) / 256)), dim3(256), 0, stream, a);
     return hipGetLastError();

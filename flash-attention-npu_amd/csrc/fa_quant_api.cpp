@@ -15,7 +15,7 @@
 namespace fa {
 fa_status_t report_error(fa_status_t st, const char* msg);
 hipError_t launch_page_table(const PageTableArgs& a, hipStream_t stream);
-hipError_t launch_quant_append(const QuantAppendArgs& a, int dtype, int ct, hipStream_t stream);
+hipError_t launch_quant_append(QuantAppendArgs a, int dtype, int ct, hipStream_t stream);
 int quant_decode_workers(int grid);
 hipError_t launch_quant_decode(const QuantFwdArgs& a, int ct, int kd, int nr, int grid, hipStream_t stream);
 int quant_prefill_rows(int kd);
@@ -93,6 +93,9 @@ fa_status_t check_append(const fa_quant_append_params* p) {
              "k, v and the caches must be 16-byte aligned");
     FA_CHECK(multiples(8, p->knew_row_stride, p->knew_head_stride, 0) && multiples(8, p->vnew_row_stride, p->vnew_head_stride, 0),
              "strides of k and v must be multiples of 8 elements");
+    // a pass of the kernel addresses up to 128 rows in 32 bits
+    FA_CHECK(p->knew_row_stride >= 0 && p->knew_row_stride < (1 << 24) && p->vnew_row_stride >= 0 && p->vnew_row_stride < (1 << 24),
+             "row strides of k and v must be in [0, 2^24)");
     FA_CHECK(multiples(16, p->k_page_stride, p->k_row_stride, p->k_head_stride) &&
                  multiples(16, p->v_page_stride, p->v_row_stride, p->v_head_stride),
              "strides of the caches must be multiples of 16");

@@ -38,6 +38,8 @@ struct QuantAppendArgs {
     const int64_t* slots;
     int64_t total_new, num_slots;  // num_slots: num_pages * page_size
     int Hk, hd, page_size, scale_block;
+    int rows_per_unit;             // rows among which a unit looks for the beginning of a run
+    UDiv block, page, chunks;      // division by scale_block, page_size and hd / 8
 };
 
 // Strides are in elements; cache elements are bytes.

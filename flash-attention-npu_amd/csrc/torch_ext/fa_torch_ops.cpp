@@ -818,7 +818,7 @@ void quant_append(const Tensor& k, const Tensor& v, Tensor& kcache, Tensor& vcac
     TORCH_CHECK(slot_mapping.size(0) == k.size(0), "slot_mapping must have an entry per row of k");
     // rows that a 16-byte load cannot take are copied, as elsewhere
     auto rows = [](const Tensor& t) {
-        return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && ((uintptr_t)t.data_ptr() & 15) == 0
+        return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(0) < (1 << 24) && t.stride(1) % 8 == 0 && ((uintptr_t)t.data_ptr() & 15) == 0
                    ? t
                    : t.contiguous();
     };

@@ -48,7 +48,7 @@ def server(r, B, width, page, spare, done=0.2, extra_rows=0):
     return table, before, after, free, len(ids), page, total, idx
 
 
-@pytest.mark.parametrize("B", [1, 2, 63, 64, 65, 300, 1024, 1025, 3000])
+@pytest.mark.parametrize("B", [1, 2, 63, 64, 65, 300, 1024, 1025, 3000, 4096, 4097])
 @pytest.mark.parametrize("page", [1, 16, 48, 256])
 def test_steps_of_a_server(B, page):
     print(f"case table {B} {page}", flush=True)

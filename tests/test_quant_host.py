@@ -83,7 +83,7 @@ def test_append_of_nothing():
     (dict(dtype=3), "fp16 and bf16"), (dict(cache_dtype=0), "int8 or float8_e4m3fn"), (dict(headdim=8), "multiple of 16"),
     (dict(page_size=40), "multiple of the 16 tokens"), (dict(scale_block=0), "multiple of 16 tokens"), (dict(nheads_k=70000), "key/value heads"),
     (dict(total_new=-1), "new rows"), (dict(total_new=1 << 31), "new rows"), (dict(k_new=None), "required"), (dict(slot_mapping=None), "required"),
-    (dict(v_new=PTR + 2), "aligned"), (dict(knew_row_stride=260), "multiples of 8"), (dict(v_page_stride=8), "multiples of 16")])
+    (dict(v_new=PTR + 2), "aligned"), (dict(knew_row_stride=1 << 24), "row strides"), (dict(knew_row_stride=260), "multiples of 8"), (dict(v_page_stride=8), "multiples of 16")])
 def test_append_refuses(more, says):
     assert capi.quant_append(**dict(APPEND, **more)) == capi.FA_EINVAL and says in capi.last_error(), capi.last_error()
 
