@@ -17,6 +17,8 @@
 #include "fa_common.h"
 #include "fa_quant_args.h"
 
+#include <algorithm>
+
 namespace fa {
 
 namespace {
@@ -83,32 +85,38 @@ __device__ __forceinline__ void scan_lds(int* s, int n, int* s_w) {
 }
 
 __global__ void __launch_bounds__(NT) fa_page_table_kernel(PageTableArgs a) {
-    __shared__ int s_rel[MAXB + 1], s_val[MAXB + 1], s_take[MAXB + 1], s_fresh[MAXB + 1], s_w[NT / 64];
+    // prefixes of released entries, ids among them, needed pages and new tokens;
+    // row (-1: none) and the smaller of have and need of each request
+    __shared__ int s_rel[MAXB + 1], s_val[MAXB + 1], s_take[MAXB + 1], s_fresh[MAXB + 1], s_row[MAXB], s_min[MAXB], s_w[NT / 64];
     const int tid = threadIdx.x, B = a.B;
     const int64_t first = (int64_t)blockIdx.x * NT + tid, stride = (int64_t)gridDim.x * NT;
     const int n0 = min(max(a.num_free[0], 0), a.free_cap);
     for (int b = tid; b < B; b += NT) {
         const Req r = request(a, b);
-        s_rel[b + 1] = max(r.have - r.need, 0);
+        s_rel[b + 1] = s_val[b + 1] = max(r.have - r.need, 0);
         s_take[b + 1] = max(r.need - r.have, 0);
         s_fresh[b + 1] = r.fresh;
-        s_val[b + 1] = 0;
+        s_row[b] = r.row;
+        s_min[b] = min(r.have, r.need);
     }
     scan_lds(s_rel, B, s_w);
     scan_lds(s_take, B, s_w);
     scan_lds(s_fresh, B, s_w);
     const int raw = s_rel[B], taken = s_take[B], fresh = s_fresh[B];
-    // released entry f of the requests in turn: its request and id
+    // released entry f of the requests in turn: its request, place among the request's, id
     auto entry = [&](int f, int& b, int& j) -> int {
         b = seq_of(s_rel, B, f);
-        const Req r = request(a, b);
         j = f - s_rel[b];
-        return a.table[(int64_t)r.row * a.t_stride + r.need + j];
+        return a.table[(int64_t)s_row[b] * a.t_stride + s_min[b] + j];
     };
-    if (raw > 0) {  // how many of each request's are ids
-        for (int f = tid; f < raw; f += NT) {
-            int b, j;
-            if (entry(f, b, j) >= 0) atomicAdd(&s_val[b + 1], 1);
+    if (raw > 0) {
+        for (int f = tid; f < raw; f += 4 * NT) {  // four reads at once
+            int id[4], b[4], j;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) id[u] = f + u * NT < raw ? entry(f + u * NT, b[u], j) : 0;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (id[u] < 0) atomicSub(&s_val[b[u] + 1], 1);
         }
         __syncthreads();
         scan_lds(s_val, B, s_w);
@@ -146,18 +154,16 @@ __global__ void __launch_bounds__(NT) fa_page_table_kernel(PageTableArgs a) {
     };
     for (int64_t t = first; t < taken; t += stride) {
         const int b = seq_of(s_take, B, (int)t);
-        const Req r = request(a, b);
-        a.table[(int64_t)r.row * a.t_stride + r.have + ((int)t - s_take[b])] = page_at((int)t);
+        a.table[(int64_t)s_row[b] * a.t_stride + s_min[b] + ((int)t - s_take[b])] = page_at((int)t);
     }
     for (int64_t i = first; i < a.total_new; i += stride) {
         int64_t slot = -1;
         if (i < fresh) {
             const int b = seq_of(s_fresh, B, (int)i);
-            const Req r = request(a, b);
             const int64_t at = (int64_t)max(a.before[b], 0) + (i - s_fresh[b]);
-            if (r.row >= 0 && at < (int64_t)a.max_pages * a.page_size) {
-                const int j = (int)udiv(a.page, (uint32_t)at);
-                const int id = j < r.have ? a.table[(int64_t)r.row * a.t_stride + j] : page_at(s_take[b] + j - r.have);
+            if (s_row[b] >= 0 && at < (int64_t)a.max_pages * a.page_size) {
+                const int j = (int)udiv(a.page, (uint32_t)at), have = s_min[b];  // the request grows
+                const int id = j < have ? a.table[(int64_t)s_row[b] * a.t_stride + j] : page_at(s_take[b] + j - have);
                 if (id >= 0) slot = (int64_t)id * a.page_size + (at - (int64_t)j * a.page_size);
             }
         }
@@ -235,9 +241,10 @@ __global__ void __launch_bounds__(256) fa_slot_kernel(PageTableArgs a) {
 
 hipError_t launch_page_table(const PageTableArgs& a, hipStream_t stream) {
     if (a.B <= MAXB) {
-        // two slots a thread: few enough workgroups that their common work stays small
-        const int grid = (int)((a.total_new + 2 * NT - 1) / (2 * NT));
-        hipLaunchKernelGGL(fa_page_table_kernel, dim3(grid < 1 ? 1 : grid > 256 ? 256 : grid), dim3(NT), 0, stream, a);
+        // two slots a thread, pages of 128 requests a workgroup: few enough that
+        // what they all do stays small
+        const int64_t grid = std::max<int64_t>((a.total_new + 2 * NT - 1) / (2 * NT), (a.B + 127) / 128);
+        hipLaunchKernelGGL(fa_page_table_kernel, dim3((unsigned)std::min<int64_t>(grid, 256)), dim3(NT), 0, stream, a);
         return hipGetLastError();
     }
     hipLaunchKernelGGL(fa_page_table_large_kernel, dim3(1), dim3(NT), 0, stream, a);

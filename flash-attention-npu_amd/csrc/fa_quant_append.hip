@@ -74,7 +74,7 @@ __device__ __forceinline__ int64_t lane_value(int64_t x, int l) {
 // hd / 8 lanes take a row, 16 bytes each, so a lane's columns stay the same.
 // KEEP: passes of rows that stay in registers between the two readings.
 template <int DT, int CT, int WPU, int KEEP>
-__global__ void __launch_bounds__(256, 4) fa_quant_append_kernel(QuantAppendArgs a) {
+__global__ void __launch_bounds__(256, KEEP > 4 ? 3 : 4) fa_quant_append_kernel(QuantAppendArgs a) {
     __shared__ uint32_t s_most[4];
     constexpr int UNITS = 4 / WPU, LANES = 64 * WPU;
     constexpr uint32_t kInf = DT == DT_FP16 ? 0x7c00u : 0x7f80u;

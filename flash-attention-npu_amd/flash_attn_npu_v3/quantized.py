@@ -22,6 +22,8 @@ from fa_mi355x import ops
 
 from .interface import maybe_contiguous
 
+_update_page_table, _append, _fwd = (op.default for op in (ops.update_page_table, ops.quant_append, ops.quant_fwd))
+
 
 def update_page_table(page_table, cache_seqlens, new_seqlens, free_pages, num_free, page_size, total_new,
                       cache_batch_idx: Optional[torch.Tensor] = None):
@@ -49,8 +51,8 @@ def update_page_table(page_table, cache_seqlens, new_seqlens, free_pages, num_fr
 
     No new token is dropped if total_new is at least the sum of
     max(new_seqlens - cache_seqlens, 0). Nothing is read back to the host."""
-    return ops.update_page_table(page_table, maybe_contiguous(cache_seqlens), maybe_contiguous(new_seqlens), free_pages,
-                                 num_free, int(page_size), int(total_new), maybe_contiguous(cache_batch_idx))
+    return _update_page_table(page_table, maybe_contiguous(cache_seqlens), maybe_contiguous(new_seqlens), free_pages,
+                              num_free, int(page_size), int(total_new), maybe_contiguous(cache_batch_idx))
 
 
 def append_quantized_kvcache(k, v, k_cache, v_cache, k_scale, v_scale, slot_mapping):
@@ -68,7 +70,7 @@ def append_quantized_kvcache(k, v, k_cache, v_cache, k_scale, v_scale, slot_mapp
     are rounded to the new scale. Codes are x / s rounded to the nearest, ties
     to even. +-inf counts as the type's largest finite value; NaN becomes 0 in
     int8 and NaN in e4m3."""
-    ops.quant_append(k, v, k_cache, v_cache, k_scale, v_scale, maybe_contiguous(slot_mapping))
+    _append(k, v, k_cache, v_cache, k_scale, v_scale, maybe_contiguous(slot_mapping))
 
 
 def flash_attn_with_quantized_kvcache(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens,
@@ -98,8 +100,8 @@ def flash_attn_with_quantized_kvcache(q, k_cache, v_cache, k_scale, v_scale, cac
         softmax_scale = q.shape[-1] ** (-0.5)
     if cu_seqlens_q is not None and max_seqlen_q is None:
         raise RuntimeError("max_seqlen_q is required with cu_seqlens_q")
-    out, softmax_lse = ops.quant_fwd(q, k_cache, v_cache, k_scale, v_scale, maybe_contiguous(cache_seqlens),
-                                     maybe_contiguous(page_table), maybe_contiguous(cache_batch_idx),
-                                     maybe_contiguous(cu_seqlens_q), int(max_seqlen_q or 0), float(softmax_scale),
-                                     bool(causal), int(window_size[0]), int(window_size[1]), float(softcap))
+    out, softmax_lse = _fwd(q, k_cache, v_cache, k_scale, v_scale, maybe_contiguous(cache_seqlens),
+                            maybe_contiguous(page_table), maybe_contiguous(cache_batch_idx),
+                            maybe_contiguous(cu_seqlens_q), int(max_seqlen_q or 0), float(softmax_scale), bool(causal),
+                            int(window_size[0]), int(window_size[1]), float(softcap))
     return (out, softmax_lse) if return_softmax_lse else out
