@@ -61,6 +61,7 @@ SRC_FLAGS = {
     **{f"fa_fwd_pipe{d}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"] for d in (64, 128, 256, "_fp8")},
     "fa_bwd_dq.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "fa_bwd_kv.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "fa_quant_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "fa_fwd.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"],
 }
 

@@ -71,21 +71,17 @@ __device__ __forceinline__ int64_t lse_at(const QuantFwdArgs& a, int b, int h, i
     return a.cu_q ? (int64_t)h * a.lse_sh + a.cu_q[b] + i : (int64_t)b * a.lse_sb + (int64_t)h * a.lse_sh + i;
 }
 
-// eight 16-bit values of either type as fp32
-__device__ __forceinline__ f32x8 load8(const void* base, int64_t off, bool bf16) {
-    const u32x4 r = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(base) + off);
+// eight 16-bit values as fp32
+template <int DT>
+__device__ __forceinline__ f32x8 widen8(u32x4 r) {
     f32x8 y;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const uint16_t h = (uint16_t)(r[e >> 1] >> (16 * (e & 1)));
-        y[e] = bf16 ? f16_to_32<DT_BF16>(h) : f16_to_32<DT_FP16>(h);
-    }
+    for (int e = 0; e < 8; ++e) y[e] = f16_to_32<DT>((uint16_t)(r[e >> 1] >> (16 * (e & 1))));
     return y;
 }
-__device__ __forceinline__ uint32_t pack2(float x, float y, bool bf16) {
-    const uint32_t b = (uint32_t)f32_to_16<DT_BF16>(x) | (uint32_t)f32_to_16<DT_BF16>(y) << 16;
-    const uint32_t h = (uint32_t)f32_to_16<DT_FP16>(x) | (uint32_t)f32_to_16<DT_FP16>(y) << 16;
-    return bf16 ? b : h;
+template <int DT>
+__device__ __forceinline__ f32x8 load8(const void* base, int64_t off) {
+    return widen8<DT>(*reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(base) + off));
 }
 
 }  // namespace fa

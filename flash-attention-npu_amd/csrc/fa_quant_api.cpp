@@ -16,7 +16,7 @@ namespace fa {
 fa_status_t report_error(fa_status_t st, const char* msg);
 hipError_t launch_page_table(const PageTableArgs& a, hipStream_t stream);
 hipError_t launch_quant_append(QuantAppendArgs a, int dtype, int ct, hipStream_t stream);
-int quant_decode_workers(int grid);
+int quant_decode_workers(int kd, int grid);
 hipError_t launch_quant_decode(const QuantFwdArgs& a, int ct, int kd, int nr, int grid, hipStream_t stream);
 int quant_prefill_rows(int kd);
 int quant_prefill_keys(int kd);
@@ -141,7 +141,7 @@ fa_status_t check_fwd(const fa_quant_fwd_params* p) {
 }
 
 constexpr int kMaxBatch = 2048;  // sequences of one launch (their list lives in LDS)
-constexpr int kDecodeRows = 64;  // packed rows of a kv head that the decode kernel takes
+constexpr int kDecodeRows = 32;  // packed rows of a kv head that the decode kernel takes
 
 struct Plan {
     int kd;          // kernel head dim
@@ -165,13 +165,13 @@ Plan make_plan(const fa_quant_fwd_params* p) {
     pl.prefill = rows > kDecodeRows;
     // of a ragged batch with longer sequences the ones at their next token or two
     pl.dec_rows = !pl.prefill ? (int)rows : p->cu_seqlens_q ? 16 : 0;
-    pl.nr = pl.dec_rows <= 16 ? 1 : pl.dec_rows <= 32 ? 2 : 4;
+    pl.nr = pl.dec_rows <= 16 ? 1 : 2;
     const int cus = fa::compute_units();
     const size_t nb = std::min(p->batch, kMaxBatch);
     pl.grid = cus;
     size_t off = 0;
     if (pl.dec_rows) {
-        const size_t parts = (size_t)fa::quant_decode_workers(pl.grid) * 2 * 16 * pl.nr;
+        const size_t parts = (size_t)fa::quant_decode_workers(pl.kd, pl.grid) * 2 * 16 * pl.nr;
         pl.off_lse = off = align256(sizeof(int) * (nb + 1));
         pl.off_o = off = align256(off + sizeof(float) * parts);
         off = align256(off + sizeof(float) * parts * pl.kd);

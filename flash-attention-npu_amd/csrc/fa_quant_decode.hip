@@ -1,47 +1,74 @@
 // fa_quant_decode.hip -- attention over 8-bit codes for few query rows (a kv
-// head's g query heads x positions, at most 64 packed rows): the cache is
+// head's g query heads x positions, at most 32 packed rows): the cache is
 // streamed once, at the rate that HBM gives.
 //
 // Split: the 64-key tiles (32 at head dim 256) of all sequences and kv heads form
 // one list, built in LDS by each workgroup from cache_seqlens and cut into equal
-// contiguous ranges, one per wave (fa_decode_split.h); waves of a CU take
-// adjacent kv heads of one range, so that a key row is requested by a CU at once. A
-// range that ends inside a sequence leaves a partial, merged by the second launch.
+// contiguous ranges, one per wave; waves of a CU take adjacent kv heads of one
+// range, so that a key row is requested by a CU at once. A range that ends inside a
+// sequence leaves a partial, merged by the second launch.
 //
-// A tile: lane (li, G) of a wave loads a quarter of key row li, which is its operand
-// of S^T = K.Q^T as it stands once widened, and columns li * D/16 .. of value rows
-// 4G .. 4G + 3, which two byte permutations turn into its operand of O^T = V^T.P^T:
-// no shared memory and no barrier on the way, and each wave keeps the next tiles
-// (32 KB) in flight in registers. Page ids and scales come through a small table in
-// LDS, filled 32 tiles at a time.
+// Loads go straight into LDS: each wave has two tiles of keys and two of values there
+// and asks for tile t + 2 of either as soon as it is through with tile t's, so no
+// barrier is needed and 8 waves (4 at head dim 256) keep about 96 KB in flight. Two
+// waves per SIMD, since the chain of one tile (reads, products, maximum over lanes,
+// exponentials, products) takes 2500 clocks, as long as HBM takes for two. Rows are
+// swizzled by the order in which the lanes load. A lane reads the quarter of a key row
+// that is its operand of S^T = K.Q^T once widened, and V^T for O^T = V^T.P^T by byte
+// transpose reads of the key rows that its weights belong to. Page ids and scales
+// come through a small table in LDS, filled 32 blocks of 16 keys at a time, in steps
+// some tiles apart: a wait for the table would be one for every row asked for before.
 //
 // Scales: the K scale of 16 keys multiplies their scores. The V scale t multiplies
 // the weights p, which are then rounded to fp16, so they are kept relative to a
 // running power of two R >= t that moves up like a maximum, w = p * t / R * 2^14: a
 // weight keeps its 11 bits as long as p * t / R > 2^-28.
 #include "fa_quant.h"
-#include "fa_decode_split.h"
+#include "fa_pipe.h"
 
 namespace fa {
 
 namespace {
 
-constexpr int NWAVE = 4;
 constexpr int MAXB = 2048;
-constexpr int TAB = 32;  // tiles of one half of a wave's table
 
 template <int HD>
 struct Cfg {
-    static constexpr int KT = HD == 256 ? 32 : 64;     // keys of a tile
-    static constexpr int NH = KT / 16;
-    static constexpr int KL = HD / 64;                 // 16-byte loads of a lane for its quarter key row
+    static constexpr int NWAVE = HD == 256 ? 4 : 8;    // waves of a workgroup
+    static constexpr int KT = HD == 64 ? 64 : 32;      // keys of a tile
+    static constexpr int NH = KT / 16;                 // blocks of 16
+    static constexpr int TAB = 32 / NH;                // tiles of one half of a wave's table
+    static constexpr int KL = HD / 64;                 // 16-byte reads of a lane for its quarter key row
     static constexpr int KSTEPS = HD / 32;
-    static constexpr int VW = HD / 64;                 // words of a lane for its columns of a value row
-    static constexpr int VB = HD / 16;                 // columns of a lane, PV products of a 16-row tile
-    static constexpr int STAGES = HD == 64 ? 5 : 3;
+    static constexpr int DBLK = HD / 16;
+    static constexpr int LPB = HD / 64;                // 1 KB loads of a block
+    static constexpr int TILE = KT * HD;               // bytes of a tile of keys or of values
+    static constexpr int LOADS = NH * LPB;             // loads of it
+    // swizzle of the 16-byte chunks of row r
+    static __device__ __forceinline__ int f(int r) { return HD == 64 ? (r >> 1) & 3 : HD == 128 ? r & 7 : r & 15; }
 };
 
 __device__ __forceinline__ int heads_per_group(const QuantFwdArgs& a) { return a.Hk % 4 == 0 ? 4 : a.Hk % 2 == 0 ? 2 : 1; }
+
+// The list holds T tiles, sequence by sequence and head group by head group; the
+// first We of W workers share it, T = q We + r: r of them take q + 1 tiles. Workers
+// have kMinTiles at least, since a partial costs its merge about what a tile costs here.
+constexpr int kMinTiles = 2;
+struct Split {
+    int We, q, r;
+    __device__ __forceinline__ int first(int w) const { return w < We ? w * q + min(w, r) : We * q + r; }
+    __device__ __forceinline__ int owner(int t) const {
+        const uint32_t u = (uint32_t)t, big = (uint32_t)r * (uint32_t)(q + 1);
+        return (int)(u < big ? u / (uint32_t)(q + 1) : (uint32_t)r + (u - big) / (uint32_t)q);
+    }
+};
+__device__ __forceinline__ Split split_list(int T, int W) {
+    Split s;
+    s.We = max(min(W, T / kMinTiles), 1);
+    s.q = (int)((uint32_t)T / (uint32_t)s.We);
+    s.r = T - s.q * s.We;
+    return s;
+}
 
 struct Seg {
     int S, n;      // first tile of the list, tiles
@@ -50,8 +77,7 @@ struct Seg {
     QuantSeq q;
 };
 
-__device__ __forceinline__ Seg seg_of(const QuantFwdArgs& a, const int* s_pref, const QuantSeq* s_seq, int t, int hs, int h,
-                                      int KT) {
+__device__ __forceinline__ Seg seg_of(const QuantFwdArgs& a, const int* s_pref, int t, int hs, int h, int KT) {
     int bl = 0, bh = a.B;
     while (bh - bl > 1) {
         const int mid = (bl + bh) >> 1;
@@ -60,35 +86,74 @@ __device__ __forceinline__ Seg seg_of(const QuantFwdArgs& a, const int* s_pref, 
     }
     Seg s;
     s.b = bl;
-    s.n = (s_pref[bl + 1] - s_pref[bl]) / (a.Hk / hs);
-    const int hg = s.n > 0 ? (t - s_pref[bl]) / s.n : 0;
+    s.q = quant_seq(a, bl);
+    s.lo_tile = s.q.lo / KT;
+    s.n = (s.q.hi + KT - 1) / KT - s.lo_tile;
+    const int hg = (int)((uint32_t)(t - s_pref[bl]) / (uint32_t)max(s.n, 1));
     s.hk = hg * hs + h;
     s.S = s_pref[bl] + hg * s.n;
-    s.q = s_seq[bl];
-    s.lo_tile = s.q.lo / KT;
     return s;
 }
 
-// CT: cache type; HD: kernel head dim (HDM: the cache's is smaller, columns past it
-// are zero); NR: 16-row tiles of packed rows.
-template <int CT, int HD, int NR, bool HDM>
-__global__ void __launch_bounds__(256, 1) fa_quant_decode_kernel(QuantFwdArgs a) {
-    using C = Cfg<HD>;
-    constexpr int KT = C::KT, NH = C::NH, KL = C::KL, KSTEPS = C::KSTEPS, VW = C::VW, VB = C::VB, STAGES = C::STAGES;
-    __shared__ int s_pref[MAXB + 1];
-    __shared__ QuantSeq s_seq[MAXB];
-    __shared__ int64_t s_koff[NWAVE][2 * TAB * NH], s_voff[NWAVE][2 * TAB * NH];
-    __shared__ __attribute__((aligned(16))) float s_ks[NWAVE][2 * TAB * NH], s_vs[NWAVE][2 * TAB * NH];
-    __shared__ int s_ok[NWAVE][2 * TAB];
+// One 16-key block of K or V into LDS: LPB loads of 1 KB, as dma16x4 (fa_pipe.h).
+template <int LPB>
+__device__ __forceinline__ void dma_block(unsigned lds, const char* base, const unsigned (&off)[LPB]) {
+    if constexpr (LPB == 4) {
+        dma16x4(lds, base, off);
+    } else {
+        base = uniform(base);
+        lds = __builtin_amdgcn_readfirstlane(lds);
+        if constexpr (LPB == 2)
+            asm volatile(
+                "s_mov_b32 m0, %0\n\ts_nop 3\n\t"
+                "global_load_lds_dwordx4 %2, %1\n\t"
+                "global_load_lds_dwordx4 %3, %1 offset:1024" ::"s"(lds), "s"(base), "v"(off[0]), "v"(off[1])
+                : "memory", "m0");
+        else
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %2, %1" ::"s"(lds), "s"(base), "v"(off[0])
+                         : "memory", "m0");
+    }
+}
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// max over the lanes l, l ^ 16, l ^ 32, l ^ 48. A swap exchanges the odd rows of 16
+// (32) lanes of one register with the even ones of the other. In assembly, since the
+// compiler's builtin gives the first result for both; it wants two wait states after
+// its operands' last write.
+__device__ __forceinline__ float max4(float v) {
+    float w = v;
+    asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(v), "+v"(w));
+    v = w = fmaxf(v, w);
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(v), "+v"(w));
+    return fmaxf(v, w);
+}
+
+// DT: type of q and out; CT: cache type; HD: kernel head dim (the cache's may be smaller: columns past it
+// repeat the row's first and meet zeros of q); NR: 16-row tiles of packed rows.
+template <int DT, int CT, int HD, int NR>
+__global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel(QuantFwdArgs a) {
+    using C = Cfg<HD>;
+    constexpr int NWAVE = C::NWAVE, NT = NWAVE * 64, KT = C::KT, NH = C::NH, TAB = C::TAB, KL = C::KL, KSTEPS = C::KSTEPS,
+                  DBLK = C::DBLK, LPB = C::LPB;
+    __shared__ __attribute__((aligned(1024))) uint8_t s_ring[NWAVE][4 * C::TILE];
+    __shared__ int s_pref[MAXB + 1];
+    __shared__ int64_t s_koff[NWAVE][64], s_voff[NWAVE][64];
+    __shared__ float s_ks[NWAVE][64], s_vs[NWAVE][64];
+    __shared__ int s_ok[NWAVE][64 / NH];
+
+    // The arguments read anew where they are used once in many tiles (the assembly hides
+    // that they stay the same): held all along they would not fit in scalar registers.
+    auto anew = []() -> const QuantFwdArgs& {
+        auto p = __builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(p));
+        return *(const QuantFwdArgs*)p;
+    };
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, G = lane >> 4;
     const int hs = heads_per_group(a), hgs = a.Hk / hs;
 
     // ---- the list of tiles ----------------------------------------------------------
-    for (int b = tid; b < a.B; b += 256) {
+    for (int b = tid; b < a.B; b += NT) {
         const QuantSeq s = quant_seq(a, b);
-        s_seq[b] = s;
         s_pref[b + 1] = s.hi > s.lo && s.sq * a.g <= a.dec_rows ? hgs * ((s.hi + KT - 1) / KT - s.lo / KT) : 0;
     }
     __syncthreads();
@@ -113,156 +178,154 @@ __global__ void __launch_bounds__(256, 1) fa_quant_decode_kernel(QuantFwdArgs a)
     }
     __syncthreads();
     if (blockIdx.x == 0)
-        for (int b = tid; b <= a.B; b += 256) a.sched[b] = s_pref[b];
+        for (int b = tid; b <= a.B; b += NT) a.sched[b] = s_pref[b];
 
-    const long long T = s_pref[a.B];
     const int hsel = wave % hs;
-    const long long W = (long long)gridDim.x * (NWAVE / hs);
-    const long long gw = (long long)(wave / hs) * gridDim.x + blockIdx.x;  // wave-major, as in fa_decode.hip
-    const long long wid = gw * hs + hsel;
-    const long long ovh = dec::seg_ovh(T, W, (long long)a.B * hgs);
-    const long long CT_ = dec::split_total(T, ovh, a.B, hgs);
-    const int t0 = dec::split_tfirst(gw * CT_ / W, s_pref, a.B, hgs, ovh, T, CT_);
-    const int t1 = dec::split_tfirst((gw + 1) * CT_ / W, s_pref, a.B, hgs, ovh, T, CT_);
+    const int gw = (wave / hs) * gridDim.x + blockIdx.x;  // wave-major, as in fa_decode.hip
+    const int64_t wid = (int64_t)gw * hs + hsel;
+    const Split sp = split_list(s_pref[a.B], gridDim.x * (NWAVE / hs));
+    const int t0 = __builtin_amdgcn_readfirstlane(sp.first(gw)), t1 = __builtin_amdgcn_readfirstlane(sp.first(gw + 1));
     if (t0 >= t1) return;  // no barrier follows: the waves go on alone
 
+    // ---- the table: offsets, scales and visibility of the 16-key blocks ------------------
+    // Tiles base .. base + TAB - 1, a block for each of 32 lanes. A block without a visible
+    // key has the offset of a row that is there and scales 0. In
+    // steps: page ids asked for; offsets, scales asked for; scales.
     int64_t* koff = s_koff[wave];
     int64_t* voff = s_voff[wave];
-    float* tks = s_ks[wave];
-    float* tvs = s_vs[wave];
+    float *tks = s_ks[wave], *tvs = s_vs[wave];
     int* tok = s_ok[wave];
-
-    // Offsets, scales and visibility of the 16-key blocks of tiles base .. base + TAB
-    // - 1, into their half of the table. A block without a visible key has offset 0
-    // and scales 0.
-    auto fill = [&](int base) {
-        constexpr int PER = TAB * NH / 64;
-        const int at0 = (((base - t0) / TAB) & 1) * TAB * NH;
-        int id[PER], inp[PER], kvh[PER];
-        bool ok[PER];
-#pragma unroll
-        for (int u = 0; u < PER; ++u) {
-            const int t = base + (u * 64 + lane) / NH;
-            id[u] = -1;
-            inp[u] = 0;
-            kvh[u] = 0;
-            if (t < t1) {
-                const Seg s = seg_of(a, s_pref, s_seq, t, hs, hsel, KT);
-                const int key = (s.lo_tile + (t - s.S)) * KT + (lane % NH) * 16;
-                kvh[u] = s.hk;
-                if (key < s.q.hi && key + 16 > s.q.lo) {
-                    const int pi = a.table ? (int)udiv(a.page, (uint32_t)key) : 0;
-                    inp[u] = key - pi * a.page_size;
-                    id[u] = a.table ? a.table[(int64_t)s.q.crow * a.t_stride + pi] : s.q.crow;
-                }
+    int id, inp, kvh;
+    float ksv, vsv;
+    auto fill_ids = [&](int base) {
+        const QuantFwdArgs& A = anew();
+        const int t = base + lane / NH;
+        id = -1;
+        inp = kvh = 0;
+        if (lane < 32 && t < t1) {
+            const Seg s = seg_of(A, s_pref, t, hs, hsel, KT);
+            const int key = (s.lo_tile + (t - s.S)) * KT + (lane % NH) * 16;
+            kvh = s.hk;
+            if (key < s.q.hi && key + 16 > s.q.lo) {
+                const int pi = A.table ? (int)udiv(A.page, (uint32_t)key) : 0;
+                inp = key - pi * A.page_size;
+                id = A.table ? A.table[(int64_t)s.q.crow * A.t_stride + pi] : s.q.crow;
             }
         }
-        float ks[PER], vs[PER];
-#pragma unroll
-        for (int u = 0; u < PER; ++u) {
-            ok[u] = id[u] >= 0 && id[u] < a.num_pages;
-            const int64_t p = ok[u] ? id[u] : 0, r = ok[u] ? inp[u] : 0, h = kvh[u];
-            const int64_t sb = udiv(a.sblk, (uint32_t)r);
-            ks[u] = a.ks[p * a.ks_sp + sb * a.ks_sb + h * a.ks_sh];
-            vs[u] = a.vs[p * a.vs_sp + sb * a.vs_sb + h * a.vs_sh];
-            const int at = at0 + u * 64 + lane;
-            koff[at] = p * a.k_sp + r * a.k_si + h * a.k_sh;
-            voff[at] = p * a.v_sp + r * a.v_si + h * a.v_sh;
-            const unsigned long long m = __ballot(ok[u]);
+    };
+    auto slot_of = [&](int base) { return (((base - t0) / TAB) & 1) * 32 + (lane & 31); };
+    auto fill_rows = [&](int base) {
+        const QuantFwdArgs& A = anew();
+        const bool ok = id >= 0 && id < A.num_pages;
+        const int64_t p = ok ? id : 0, r = ok ? inp : 0, h = kvh;
+        const int64_t sb = udiv(A.sblk, (uint32_t)r);
+        ksv = A.ks[p * A.ks_sp + sb * A.ks_sb + h * A.ks_sh];
+        vsv = A.vs[p * A.vs_sp + sb * A.vs_sb + h * A.vs_sh];
+        const int at = slot_of(base);
+        const unsigned long long m = __ballot(ok);
+        if (lane < 32) {
+            koff[at] = p * A.k_sp + r * A.k_si + h * A.k_sh;
+            voff[at] = p * A.v_sp + r * A.v_si + h * A.v_sh;
             if (lane % NH == 0) tok[at / NH] = (int)(m >> lane) & ((1 << NH) - 1);
         }
-#pragma unroll
-        for (int u = 0; u < PER; ++u) {
-            const int at = at0 + u * 64 + lane;
-            tks[at] = ok[u] ? ks[u] : 0.f;
-            tvs[at] = ok[u] ? vs[u] : 0.f;
+    };
+    auto fill_scales = [&](int base) {
+        const bool ok = id >= 0 && id < a.num_pages;
+        const int at = slot_of(base);
+        if (lane < 32) {
+            tks[at] = ok ? ksv : 0.f;
+            tvs[at] = ok ? vsv : 0.f;
         }
     };
-    fill(t0);
 
     // ---- loads ------------------------------------------------------------------------
-    u32x4 kr[STAGES][NH][KL];
-    uint32_t vr[STAGES][NH][4][VW];
-    const uint32_t kin = (uint32_t)li * (uint32_t)a.k_si + G * (HD / 4);
-    uint32_t vin[4];
+    const unsigned ring = lds_addr(s_ring[wave]);
+    unsigned kin[LPB], vin[LPB];  // what a lane loads of a block: chunk c ^ f(r) of row r to chunk c
 #pragma unroll
-    for (int i = 0; i < 4; ++i) vin[i] = (uint32_t)(4 * G + i) * (uint32_t)a.v_si + li * VB;
-    auto uniform64 = [](int64_t x) -> int64_t {
-        const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)x);
-        const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)x >> 32));
-        return (int64_t)((uint64_t)hi << 32 | lo);
-    };
-    auto issue = [&](int t, u32x4 (&kk)[NH][KL], uint32_t (&vv)[NH][4][VW]) {
+    for (int u = 0; u < LPB; ++u) {
+        const int at = u * 64 + lane, r = at / DBLK, c = (at % DBLK) ^ C::f(r), col = c * 16 < a.hd ? c * 16 : 0;
+        kin[u] = (unsigned)r * (unsigned)a.k_si + col + (LPB - 1 - u) * 1024;
+        vin[u] = (unsigned)r * (unsigned)a.v_si + col + (LPB - 1 - u) * 1024;
+    }
+    auto issue_k = [&](int t) {
         if (t >= t1) return;
-        const int at = ((t - t0) % (2 * TAB)) * NH;
+        const int at = (t - t0) % (2 * TAB) * NH;
+        const unsigned to = ring + ((t - t0) & 1) * C::TILE;
+        int64_t off[NH];
 #pragma unroll
-        for (int h = 0; h < NH; ++h) {
-            const uint8_t* kb = a.k + uniform64(koff[at + h]);
-            const uint8_t* vb = a.v + uniform64(voff[at + h]);
+        for (int h = 0; h < NH; ++h) off[h] = koff[at + h];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // also: the reads of the tile that is written over are done
 #pragma unroll
-            for (int s = 0; s < KL; ++s)
-                kk[h][s] = !HDM || G * (HD / 4) + 16 * s < a.hd ? *reinterpret_cast<const u32x4*>(kb + kin + 16 * s)
-                                                                : u32x4{0u, 0u, 0u, 0u};
-            const bool in = !HDM || li * VB < a.hd;
+        for (int h = 0; h < NH; ++h)
+            dma_block<LPB>(to + h * (16 * HD), reinterpret_cast<const char*>(a.k + off[h]) - (LPB - 1) * 1024, kin);
+    };
+    auto issue_v = [&](int t) {
+        if (t >= t1) return;
+        const int at = (t - t0) % (2 * TAB) * NH;
+        const unsigned to = ring + (2 + ((t - t0) & 1)) * C::TILE;
+        int64_t off[NH];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (VW == 1) {
-                    vv[h][i][0] = in ? *reinterpret_cast<const uint32_t*>(vb + vin[i]) : 0u;
-                } else if constexpr (VW == 2) {
-                    const u32x2 x = in ? *reinterpret_cast<const u32x2*>(vb + vin[i]) : u32x2{0u, 0u};
-                    vv[h][i][0] = x[0];
-                    vv[h][i][1] = x[1];
-                } else {
-                    const u32x4 x = in ? *reinterpret_cast<const u32x4*>(vb + vin[i]) : u32x4{0u, 0u, 0u, 0u};
+        for (int h = 0; h < NH; ++h) off[h] = voff[at + h];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) vv[h][i][w] = x[w];
-                }
-            }
-        }
+        for (int h = 0; h < NH; ++h)
+            dma_block<LPB>(to + h * (16 * HD), reinterpret_cast<const char*>(a.v + off[h]) - (LPB - 1) * 1024, vin);
     };
 
     // ---- a segment: q, sums ----------------------------------------------------------------
-    Seg cs = seg_of(a, s_pref, s_seq, t0, hs, hsel, KT);
+    Seg cs;
     u32x4 qreg[NR][KSTEPS];
     float qs[NR];              // what the scores of a row are to be multiplied by for its q_shift
     int qi[NR];
-    f32x4 oacc[NR][VB];
+    f32x4 oacc[NR][DBLK];
     float m_run[NR], l_run[NR];
     int rows = 0, eR = 30;     // R = 2^(eR - 127)
     int flo = 0, fhi = 0;      // keys that every row sees
-    auto begin_seg = [&]() {
-        rows = cs.q.sq * a.g;
-        flo = key_lo(cs.q.sk - 1, a.wl, 0);
-        fhi = key_hi(cs.q.sk - cs.q.sq, a.wr, 0);
-        eR = 30;
+    auto load_q = [&](int t) {
+        const QuantFwdArgs& A = anew();
+        cs = seg_of(A, s_pref, t, hs, hsel, KT);
+        rows = cs.q.sq * A.g;
 #pragma unroll
         for (int rt = 0; rt < NR; ++rt) {
             const int r = rt * 16 + li;
             const bool ok = r < rows;
-            qi[rt] = ok ? r / a.g : 0;
-            const int h = cs.hk * a.g + (ok ? r % a.g : 0);
-            const int64_t base = q_row(a, cs.b, qi[rt], a.q_sb, a.q_si) + (int64_t)h * a.q_sh;
-            f32x8 x[KSTEPS];
-            float most = 0.f;
+            qi[rt] = ok ? r / A.g : 0;
+            const int h = cs.hk * A.g + (ok ? r % A.g : 0);
+            const uint16_t* q = static_cast<const uint16_t*>(A.q) + q_row(A, cs.b, qi[rt], A.q_sb, A.q_si) + (int64_t)h * A.q_sh;
 #pragma unroll
             for (int s = 0; s < KSTEPS; ++s) {
                 const int d = G * (HD / 4) + 8 * s;
-                x[s] = ok && (!HDM || d < a.hd) ? load8(a.q, base + d, a.bf16) : f32x8{0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[s][e]));
+                qreg[rt][s] = ok && d < A.hd ? *reinterpret_cast<const u32x4*>(q + d) : u32x4{0u, 0u, 0u, 0u};
             }
-            const int sh = q_shift(wave_max16x4(most));
-            const float up = exp2i(sh);
-            qs[rt] = exp2i(-sh);
+        }
+    };
+    const float scale2 = a.softcap > 0.f ? a.scale / a.softcap : a.scale * kLog2e;
+    auto begin_seg = [&]() {
+        flo = key_lo(cs.q.sk - 1, a.wl, 0);
+        fhi = min(key_hi(cs.q.sk - cs.q.sq, a.wr, 0), cs.q.sk - 1);
+        eR = 30;
 #pragma unroll
-            for (int s = 0; s < KSTEPS; ++s) qreg[rt][s] = pack8<DT_FP16>(x[s] * up);
+        for (int rt = 0; rt < NR; ++rt) {
+            float most = 0.f;
+#pragma unroll
+            for (int s = 0; s < KSTEPS; ++s) {
+                const f32x8 x = widen8<DT>(qreg[rt][s]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[e]));
+            }
+            const int sh = q_shift(max4(most));
+            const float up = exp2i(sh);
+            qs[rt] = exp2i(-sh) * scale2;
+#pragma unroll
+            for (int s = 0; s < KSTEPS; ++s) qreg[rt][s] = pack8<DT_FP16>(widen8<DT>(qreg[rt][s]) * up);
             m_run[rt] = -INFINITY;
             l_run[rt] = 0.f;
 #pragma unroll
-            for (int j = 0; j < VB; ++j) oacc[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int db = 0; db < DBLK; ++db) oacc[rt][db] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
     };
     auto end_seg = [&]() {
+        const QuantFwdArgs& A = anew();
         const bool whole = cs.S >= t0 && cs.S + cs.n <= t1;
         const float back = exp2i(eR - 127 - 14);
 #pragma unroll
@@ -274,38 +337,38 @@ __global__ void __launch_bounds__(256, 1) fa_quant_decode_kernel(QuantFwdArgs a)
             const float lse = some ? (m_run[rt] + fast_log2(l)) * kLn2 : INFINITY;
             if (r >= rows) continue;
             if (whole) {
-                const int h = cs.hk * a.g + r % a.g;
-                uint16_t* o = static_cast<uint16_t*>(a.out) + q_row(a, cs.b, qi[rt], a.o_sb, a.o_si) + (int64_t)h * a.o_sh;
+                const int h = cs.hk * A.g + r % A.g;
+                uint16_t* o = static_cast<uint16_t*>(A.out) + q_row(A, cs.b, qi[rt], A.o_sb, A.o_si) + (int64_t)h * A.o_sh;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int d = (4 * G + i) * VB;
-                    if (HDM && d >= a.hd) continue;
-#pragma unroll
-                    for (int j = 0; j < VB; j += 4)
-                        *reinterpret_cast<u32x2*>(o + d + j) =
-                            u32x2{pack2(oacc[rt][j][i] * inv, oacc[rt][j + 1][i] * inv, a.bf16),
-                                  pack2(oacc[rt][j + 2][i] * inv, oacc[rt][j + 3][i] * inv, a.bf16)};
+                for (int db = 0; db < DBLK; ++db) {
+                    if (16 * db >= A.hd) continue;
+                    const f32x4 y = oacc[rt][db] * inv;
+                    *reinterpret_cast<u32x2*>(o + 16 * db + 4 * G) = u32x2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
                 }
-                if (G == 0) a.lse[lse_at(a, cs.b, h, qi[rt])] = lse;
+                if (G == 0) A.lse[lse_at(A, cs.b, h, qi[rt])] = lse;
             } else {
                 const int slot = cs.S <= t0 ? 0 : 1;  // this worker's first segment, else its last
                 const int64_t row = (wid * 2 + slot) * (16 * NR) + r;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < VB; j += 4)
-                        *reinterpret_cast<f32x4*>(a.part_o + row * HD + (4 * G + i) * VB + j) =
-                            f32x4{oacc[rt][j][i], oacc[rt][j + 1][i], oacc[rt][j + 2][i], oacc[rt][j + 3][i]} * inv;
-                if (G == 0) a.part_lse[row] = some ? lse : -INFINITY;
+                for (int db = 0; db < DBLK; ++db)
+                    *reinterpret_cast<f32x4*>(A.part_o + row * HD + 16 * db + 4 * G) = oacc[rt][db] * inv;
+                if (G == 0) A.part_lse[row] = some ? lse : -INFINITY;
             }
         }
     };
 
     // ---- a tile ----------------------------------------------------------------------------
-    const float scale2 = a.scale * kLog2e;
-    auto compute = [&](int t, const u32x4 (&kk)[NH][KL], uint32_t (&vv)[NH][4][VW]) {
+    const int kx = C::f(li) << 4;
+    // the key row of the transpose reads, in the first of two blocks for lanes 0-7 of
+    // a group of 16 and in the second for the others
+    const int vrow = (li >> 3) * 16 + 4 * G + ((li >> 1) & 3), vx = C::f(vrow) << 4;
+    auto compute = [&](int t) {
         const int key0 = (cs.lo_tile + (t - cs.S)) * KT;
         const int at = (t - t0) % (2 * TAB);
+        const unsigned kt = ring + ((t - t0) & 1) * C::TILE, vt = kt + 2 * C::TILE;
+        // behind tile t's keys: its values, the next tile's keys and values
+        if (t + 1 < t1) wait_loads<3 * C::LOADS>();
+        else wait_loads<C::LOADS>();
         float ks[NH], vs[NH];
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
@@ -313,7 +376,7 @@ __global__ void __launch_bounds__(256, 1) fa_quant_decode_kernel(QuantFwdArgs a)
             vs[h] = tvs[at * NH + h];
         }
         const int ok = __builtin_amdgcn_readfirstlane(tok[at]);
-        const bool full = ok == (1 << NH) - 1 && key0 + KT <= cs.q.sk && key0 >= flo && key0 + KT - 1 <= fhi;
+        const bool full = ok == (1 << NH) - 1 && key0 >= flo && key0 + KT - 1 <= fhi;
         // S^T = K . Q^T on the codes
         f32x4 x[NR][NH];
 #pragma unroll
@@ -321,29 +384,30 @@ __global__ void __launch_bounds__(256, 1) fa_quant_decode_kernel(QuantFwdArgs a)
 #pragma unroll
             for (int rt = 0; rt < NR; ++rt) x[rt][h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int s = 0; s < KL; ++s)
+            for (int s = 0; s < KL; ++s) {
+                const u32x4 k = row_read(kt + (h * 16 + li) * HD + (((G * KL + s) << 4) ^ kx));
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const u32x2 lo = widen4<CT>(kk[h][s][2 * u]), hi = widen4<CT>(kk[h][s][2 * u + 1]);
+                    const u32x2 lo = widen4<CT>(k[2 * u]), hi = widen4<CT>(k[2 * u + 1]);
                     const u32x4 op = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
                     for (int rt = 0; rt < NR; ++rt) x[rt][h] = mfma_f16(op, qreg[rt][2 * s + u], x[rt][h]);
                 }
+            }
         }
+        issue_k(t + 2);
         // scores in log2 units
 #pragma unroll
         for (int rt = 0; rt < NR; ++rt)
 #pragma unroll
-            for (int h = 0; h < NH; ++h) {
-                if (a.softcap > 0.f) {
-                    const float c = qs[rt] * a.scale * ks[h];
+            for (int h = 0; h < NH; ++h) x[rt][h] *= qs[rt] * ks[h];
+        if (a.softcap > 0.f)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        x[rt][h][e] = a.softcap * kLog2e * fast_tanh(x[rt][h][e] * c * (1.f / a.softcap));
-                } else {
-                    x[rt][h] *= qs[rt] * scale2 * ks[h];
-                }
-            }
+            for (int rt = 0; rt < NR; ++rt)
+#pragma unroll
+                for (int h = 0; h < NH; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[rt][h][e] = a.softcap * kLog2e * fast_tanh(x[rt][h][e]);
         if (!full) {
 #pragma unroll
             for (int rt = 0; rt < NR; ++rt) {
@@ -357,16 +421,6 @@ __global__ void __launch_bounds__(256, 1) fa_quant_decode_kernel(QuantFwdArgs a)
                         x[rt][h][e] = (ok >> h & 1) && j >= rlo && j <= rhi ? x[rt][h][e] : -INFINITY;
                     }
             }
-            // values that no row sees must not meet the products, where 0 x NaN is NaN
-#pragma unroll
-            for (int h = 0; h < NH; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int j = key0 + h * 16 + G * 4 + i;
-                    const bool seen = (ok >> h & 1) && j >= cs.q.lo && j < cs.q.hi;
-#pragma unroll
-                    for (int w = 0; w < VW; ++w) vv[h][i][w] = seen ? vv[h][i][w] : 0u;
-                }
         }
         // R, and the weights' factor for each block
         float vmax = 0.f;
@@ -385,7 +439,7 @@ __global__ void __launch_bounds__(256, 1) fa_quant_decode_kernel(QuantFwdArgs a)
             float mx = -INFINITY;
 #pragma unroll
             for (int h = 0; h < NH; ++h) mx = fmaxf(mx, fmaxf(fmaxf(x[rt][h][0], x[rt][h][1]), fmaxf(x[rt][h][2], x[rt][h][3])));
-            mx = fmaxf(m_run[rt], wave_max16x4(mx));
+            mx = fmaxf(m_run[rt], max4(mx));
             const float m = mx == -INFINITY ? 0.f : mx;
             const float alpha = fast_exp2(m_run[rt] - m);
             m_run[rt] = mx;
@@ -405,104 +459,106 @@ __global__ void __launch_bounds__(256, 1) fa_quant_decode_kernel(QuantFwdArgs a)
             l_run[rt] = l_run[rt] * alpha + sum;
             const float c = alpha * shrink;
 #pragma unroll
-            for (int j = 0; j < VB; ++j) oacc[rt][j] *= c;
+            for (int db = 0; db < DBLK; ++db) oacc[rt][db] *= c;
         }
-        // O^T += V^T . P^T: columns 4w .. 4w + 3 of two blocks at a time
+        // behind tile t's values: the next tile's keys and values, the keys after that
+        if (t + 2 < t1) wait_loads<3 * C::LOADS>();
+        else if (t + 1 < t1) wait_loads<2 * C::LOADS>();
+        else wait_loads<0>();
+        if (!full) {
+            // values that no row sees must not meet the products, where 0 x NaN is NaN
+#pragma unroll 1
+            for (int c = lane; c < KT * DBLK; c += 64) {
+                const int r = c / DBLK, j = key0 + r;
+                if (!(ok >> (r >> 4) & 1) || j < cs.q.lo || j >= cs.q.hi) row_write(vt + c * 16, u32x4{0u, 0u, 0u, 0u});
+            }
+        }
+        // O^T += V^T . P^T
 #pragma unroll
         for (int k2 = 0; k2 < NH / 2; ++k2)
 #pragma unroll
-            for (int w = 0; w < VW; ++w) {
-                u32x4 op[4];
+            for (int db = 0; db < DBLK; ++db) {
+                const u32x2 v = tr8_read(vt + (32 * k2 + vrow) * HD + ((db << 4) ^ vx) + (li & 1) * 8);
+                const u32x2 lo = widen4<CT>(v[0]), hi = widen4<CT>(v[1]);
+                const u32x4 op = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {  // block c >> 1, keys 2 (c & 1) and the next
-                    const uint32_t r0 = vv[2 * k2 + (c >> 1)][2 * (c & 1)][w], r1 = vv[2 * k2 + (c >> 1)][2 * (c & 1) + 1][w];
-                    const u32x2 lo = widen4<CT>(byte_perm(r1, r0, 0x05010400u)), hi = widen4<CT>(byte_perm(r1, r0, 0x07030602u));
-                    op[0][c] = lo[0];
-                    op[1][c] = lo[1];
-                    op[2][c] = hi[0];
-                    op[3][c] = hi[1];
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int rt = 0; rt < NR; ++rt) oacc[rt][4 * w + j] = mfma_f16(op[j], pk[rt][k2], oacc[rt][4 * w + j]);
+                for (int rt = 0; rt < NR; ++rt) oacc[rt][db] = mfma_f16(op, pk[rt][k2], oacc[rt][db]);
             }
+        issue_v(t + 2);
     };
 
-    begin_seg();
-#pragma unroll
-    for (int st = 0; st < STAGES - 1; ++st) issue(t0 + st, kr[st], vr[st]);
-    int filled = t0 + TAB;
-    for (int tb = t0; tb < t1; tb += STAGES) {
-        // the loads of this round reach tile tb + 2 STAGES - 2; the half that is
-        // written over lies a half behind
-        static_assert(2 * STAGES <= TAB, "");
-        if (tb + 2 * STAGES > filled && filled < t1) {
-            fill(filled);
-            filled += TAB;
+    // q and the first page ids are asked for together, then key rows and scales.
+    fill_ids(t0);
+    load_q(t0);
+    fill_rows(t0);
+#pragma unroll 1
+    for (int t = t0; t < t0 + 2; ++t) {
+        issue_k(t);
+        issue_v(t);
+    }
+    fill_scales(t0);
+    int qat = t0, send = min(cs.S + cs.n, t1);
+#pragma unroll 1
+    for (int t = t0; t < t1; ++t) {
+        // the other half of the table, whose tiles are done
+        static_assert(TAB >= 8, "");
+        const int step = (t - t0) % TAB, next = t - step + TAB;
+        if (next < t1) {
+            if (step == 0) fill_ids(next);
+            else if (step == 2) fill_rows(next);
+            else if (step == 4) fill_scales(next);
         }
-#pragma unroll
-        for (int st = 0; st < STAGES; ++st) {
-            const int t = tb + st;
-            if (t < t1) {
-                issue(t + STAGES - 1, kr[(st + STAGES - 1) % STAGES], vr[(st + STAGES - 1) % STAGES]);
-                if (t >= cs.S + cs.n) {
-                    end_seg();
-                    cs = seg_of(a, s_pref, s_seq, t, hs, hsel, KT);
-                    begin_seg();
-                }
-                compute(t, kr[st], vr[st]);
+        if (t == qat) {
+            if (t > t0) {
+                load_q(t);
+                send = min(cs.S + cs.n, t1);
             }
+            begin_seg();
+        }
+        compute(t);
+        if (t + 1 == send) {
+            end_seg();
+            qat = send;
         }
     }
-    end_seg();
 }
 
-// Merge of what a segment's workers left (fa_decode_merge_kernel's rules for which
-// they are): 16 rows of a segment per workgroup and blockIdx.y; groups of threads
-// fold a share of the partials each, with a running maximum, and meet in LDS.
-template <int HD>
-__global__ void __launch_bounds__(256) fa_quant_merge_kernel(QuantFwdArgs a, int workers, int nr) {
-    __shared__ __attribute__((aligned(16))) float s_acc[256][8];
-    __shared__ float s_gm[256], s_gs[256];
-    constexpr int CH = HD / 2 / 8;  // 8-column chunks of a row, half of them in each workgroup
-    const int sig = blockIdx.x >> 1, half = blockIdx.x & 1;
-    const int b = sig / a.Hk, hk = sig % a.Hk;
-    const int hs = heads_per_group(a), hgs = a.Hk / hs, hg = hk / hs, hsel = hk % hs;
-    int sq = a.cu_q ? a.cu_q[b + 1] - a.cu_q[b] : a.Sq;
-    sq = min(max(sq, 0), a.Sq);
-    const int row0 = blockIdx.y * 16, rows = min(sq * a.g - row0, 16);
-    if (rows <= 0 || sq * a.g > a.dec_rows) return;
-    const long long T = a.sched[a.B], W = workers / hs;
-    const int per = (a.sched[b + 1] - a.sched[b]) / hgs;
-    const long long S = a.sched[b] + (long long)hg * per;
-    const long long ovh = dec::seg_ovh(T, W, (long long)a.B * hgs);
-    const long long CT_ = dec::split_total(T, ovh, a.B, hgs);
-    auto owner = [&](long long t) { return dec::split_owner(t + ovh * ((long long)b * hgs + hg), W, CT_); };
-    long long wf = 0;
-    int n = 0;
+// Merge of what a segment's workers left: 16 rows and 32 columns of a segment per
+// workgroup; groups of threads fold a share of the partials each, with a running
+// maximum, and meet in LDS.
+constexpr int MT = 512;
+template <int DT, int HD>
+__global__ void __launch_bounds__(MT) fa_quant_merge_kernel(QuantFwdArgs a, int grid, int nr) {
+    __shared__ __attribute__((aligned(16))) float s_acc[MT][8];
+    __shared__ float s_gm[MT], s_gs[MT];
+    constexpr int KT = Cfg<HD>::KT, COLS = HD / 32, CH = 4;  // 8-column chunks of a workgroup
+    const int sig = blockIdx.x / COLS, part = blockIdx.x % COLS;
+    const int b = (int)((uint32_t)sig / (uint32_t)a.Hk), hk = sig - b * a.Hk;
+    const int hs = heads_per_group(a), hg = hk / hs, hsel = hk - hg * hs;
+    const QuantSeq q = quant_seq(a, b);
+    const int T = a.sched[a.B], S0 = a.sched[b];
+    const int row0 = blockIdx.y * 16, rows = min(q.sq * a.g - row0, 16);
+    if (rows <= 0 || q.sq * a.g > a.dec_rows) return;
+    const int per = q.hi > q.lo ? (q.hi + KT - 1) / KT - q.lo / KT : 0, S = S0 + hg * per;
+    const Split sp = split_list(T, grid * (Cfg<HD>::NWAVE / hs));
+    int wf = 0, n = 0;
     if (per > 0) {
-        wf = owner(S);
-        n = T >= W ? (int)(owner(S + per - 1) - wf + 1) : per;
+        wf = sp.owner(S);
+        n = sp.owner(S + per - 1) - wf + 1;
         if (n == 1) return;  // written by its one worker
     }
-    bool slot1 = false;  // the first partial is its worker's last
-    if (per > 0 && S > 0) {
-        const long long jp = ovh > 0 ? dec::split_prev_segment(b, hg, hgs, a.sched) : 0;
-        slot1 = dec::split_owner(S - 1 + ovh * jp, W, CT_) == wf;
-    }
+    const bool slot1 = per > 0 && sp.first(wf) < S;  // the first partial is its worker's last
     const int tid = threadIdx.x;
     int rp = 1;
     while (rp < rows) rp <<= 1;
-    const int GS = CH * rp, NG = 256 / GS;
-    const int grp = tid / GS, rr = tid % GS / CH, d0 = half * (HD / 2) + tid % CH * 8;
+    const int GS = CH * rp, NG = MT / GS;
+    const int grp = tid / GS, rr = tid % GS / CH, d0 = part * 32 + tid % CH * 8;
     float m = -INFINITY, sum = 0.f;
     f32x4 acc0 = {0.f, 0.f, 0.f, 0.f}, acc1 = acc0;
     if (rr < rows) {
 #pragma unroll 4
         for (int j = grp; j < n; j += NG) {
-            const long long w = T >= W ? wf + j : owner(S + j);
-            const int64_t pr = ((w * hs + hsel) * 2 + (j == 0 && slot1 ? 1 : 0)) * (16 * nr) + row0 + rr;
+            const int64_t pr = (((int64_t)(wf + j) * hs + hsel) * 2 + (j == 0 && slot1 ? 1 : 0)) * (16 * nr) + row0 + rr;
             const float v = a.part_lse[pr];
             const f32x4 o0 = *reinterpret_cast<const f32x4*>(a.part_o + pr * HD + d0);
             const f32x4 o1 = *reinterpret_cast<const f32x4*>(a.part_o + pr * HD + d0 + 4);
@@ -516,67 +572,65 @@ __global__ void __launch_bounds__(256) fa_quant_merge_kernel(QuantFwdArgs a, int
             }
         }
     }
-    if (NG > 1) {
-        *reinterpret_cast<f32x4*>(&s_acc[tid][0]) = acc0;
-        *reinterpret_cast<f32x4*>(&s_acc[tid][4]) = acc1;
-        s_gm[tid] = m;
-        s_gs[tid] = sum;
+    *reinterpret_cast<f32x4*>(&s_acc[tid][0]) = acc0;
+    *reinterpret_cast<f32x4*>(&s_acc[tid][4]) = acc1;
+    s_gm[tid] = m;
+    s_gs[tid] = sum;
+    // halve the groups until one is left
+    for (int half = NG / 2; half > 0; half /= 2) {
         __syncthreads();
-        if (grp != 0) return;
-        float M = m;
-        for (int q = 1; q < NG; ++q) M = fmaxf(M, s_gm[tid + q * GS]);
-        if (M != -INFINITY) {
-            const float c = fast_exp2((m - M) * kLog2e);
-            acc0 *= c;
-            acc1 *= c;
-            sum *= c;
-            for (int q = 1; q < NG; ++q) {
-                const int o = tid + q * GS;
-                const float cg = fast_exp2((s_gm[o] - M) * kLog2e);
-                acc0 += *reinterpret_cast<const f32x4*>(&s_acc[o][0]) * cg;
-                acc1 += *reinterpret_cast<const f32x4*>(&s_acc[o][4]) * cg;
-                sum += s_gs[o] * cg;
+        if (grp < half) {
+            const int o = tid + half * GS;
+            const float mo = s_gm[o], M = fmaxf(m, mo);
+            if (M != -INFINITY) {
+                const float c = fast_exp2((m - M) * kLog2e), co = fast_exp2((mo - M) * kLog2e);
+                acc0 = acc0 * c + *reinterpret_cast<const f32x4*>(&s_acc[o][0]) * co;
+                acc1 = acc1 * c + *reinterpret_cast<const f32x4*>(&s_acc[o][4]) * co;
+                sum = sum * c + s_gs[o] * co;
+                m = M;
+                *reinterpret_cast<f32x4*>(&s_acc[tid][0]) = acc0;
+                *reinterpret_cast<f32x4*>(&s_acc[tid][4]) = acc1;
+                s_gm[tid] = m;
+                s_gs[tid] = sum;
             }
         }
-        m = M;
     }
-    if (rr >= rows) return;
+    if (grp != 0 || rr >= rows) return;
     const float inv = m == -INFINITY ? 0.f : 1.f / sum;
     acc0 *= inv;
     acc1 *= inv;
     const int r = row0 + rr, i = r / a.g, h = hk * a.g + r % a.g;
     uint16_t* o = static_cast<uint16_t*>(a.out) + q_row(a, b, i, a.o_sb, a.o_si) + (int64_t)h * a.o_sh;
     if (d0 < a.hd)
-        *reinterpret_cast<u32x4*>(o + d0) = u32x4{pack2(acc0[0], acc0[1], a.bf16), pack2(acc0[2], acc0[3], a.bf16),
-                                                  pack2(acc1[0], acc1[1], a.bf16), pack2(acc1[2], acc1[3], a.bf16)};
+        *reinterpret_cast<u32x4*>(o + d0) = u32x4{pack2<DT>(acc0[0], acc0[1]), pack2<DT>(acc0[2], acc0[3]),
+                                                  pack2<DT>(acc1[0], acc1[1]), pack2<DT>(acc1[2], acc1[3])};
     if (d0 == 0) a.lse[lse_at(a, b, h, i)] = m == -INFINITY ? INFINITY : m + fast_log2(sum) * kLn2;
 }
 
-template <int CT, int HD, int NR>
-void launch_h(const QuantFwdArgs& a, int grid, hipStream_t stream) {
-    if (a.hd < HD) hipLaunchKernelGGL((fa_quant_decode_kernel<CT, HD, NR, true>), dim3(grid), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((fa_quant_decode_kernel<CT, HD, NR, false>), dim3(grid), dim3(256), 0, stream, a);
-}
-
-template <int CT, int HD>
+template <int DT, int CT, int HD>
 void launch_n(const QuantFwdArgs& a, int nr, int grid, hipStream_t stream) {
-    if (nr == 1) launch_h<CT, HD, 1>(a, grid, stream);
-    else if (nr == 2) launch_h<CT, HD, 2>(a, grid, stream);
-    else launch_h<CT, HD, 4>(a, grid, stream);
-    hipLaunchKernelGGL((fa_quant_merge_kernel<HD>), dim3(a.B * a.Hk * 2, nr), dim3(256), 0, stream, a, grid * NWAVE, nr);
+    const dim3 nt(Cfg<HD>::NWAVE * 64);
+    if (nr == 1) hipLaunchKernelGGL((fa_quant_decode_kernel<DT, CT, HD, 1>), dim3(grid), nt, 0, stream, a);
+    else hipLaunchKernelGGL((fa_quant_decode_kernel<DT, CT, HD, 2>), dim3(grid), nt, 0, stream, a);
+    hipLaunchKernelGGL((fa_quant_merge_kernel<DT, HD>), dim3(a.B * a.Hk * (HD / 32), nr), dim3(MT), 0, stream, a, grid, nr);
 }
 
 template <int HD>
 void launch_d(const QuantFwdArgs& a, int ct, int nr, int grid, hipStream_t stream) {
-    if (ct == CT_INT8) launch_n<CT_INT8, HD>(a, nr, grid, stream);
-    else launch_n<CT_E4M3, HD>(a, nr, grid, stream);
+    if (a.bf16) {
+        if (ct == CT_INT8) launch_n<DT_BF16, CT_INT8, HD>(a, nr, grid, stream);
+        else launch_n<DT_BF16, CT_E4M3, HD>(a, nr, grid, stream);
+    } else {
+        if (ct == CT_INT8) launch_n<DT_FP16, CT_INT8, HD>(a, nr, grid, stream);
+        else launch_n<DT_FP16, CT_E4M3, HD>(a, nr, grid, stream);
+    }
 }
 
 }  // namespace
 
-int quant_decode_workers(int grid) { return grid * NWAVE; }
+int quant_decode_workers(int kd, int grid) { return grid * (kd == 256 ? Cfg<256>::NWAVE : Cfg<128>::NWAVE); }
 
-// kd: kernel head dim; nr: 16-row tiles (1, 2 or 4)
+// kd: kernel head dim; nr: 16-row tiles (1 or 2)
 hipError_t launch_quant_decode(const QuantFwdArgs& a, int ct, int kd, int nr, int grid, hipStream_t stream) {
     if (kd == 64) launch_d<64>(a, ct, nr, grid, stream);
     else if (kd == 128) launch_d<128>(a, ct, nr, grid, stream);

@@ -13,6 +13,7 @@
 // running power of two (fa_quant_decode.hip). The running maximum is lazy: it moves
 // only where a new score exceeds it by 2^4, and the weights' unit leaves room for that
 // (2^10 in place of 2^14: a weight keeps its 11 bits as long as p t / R > 2^-24).
+#include "fa_pipe.h"
 #include "fa_quant.h"
 
 #include <type_traits>
@@ -129,7 +130,7 @@ __device__ void build_list(const QuantFwdArgs& a, int* s_pref, long long* s_red,
 }
 
 // CAP: soft cap
-template <int CT, int HD, bool CAP>
+template <int DT, int CT, int HD, bool CAP>
 __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a) {
     using C = Cfg<HD>;
     constexpr int RB = C::RB, BM = C::BM, BN = C::BN, NB = C::NB, DCH = C::DCH, KSTEPS = C::KSTEPS, DBLK = C::DBLK,
@@ -275,7 +276,7 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
 #pragma unroll
             for (int s = 0; s < KSTEPS; ++s) {
                 const int d = (4 * s + G) * 8;
-                x[s] = ok && d < a.hd ? load8(a.q, at + d, a.bf16) : f32x8{0, 0, 0, 0, 0, 0, 0, 0};
+                x[s] = ok && d < a.hd ? load8<DT>(a.q, at + d) : f32x8{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
                 for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[s][e]));
             }
@@ -431,7 +432,7 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
                 for (int db = 0; db < DBLK; ++db) {
                     if (16 * db >= a.hd) continue;
                     const f32x4 y = oacc[rb][db] * inv;
-                    *reinterpret_cast<u32x2*>(o + 16 * db + 4 * G) = u32x2{pack2(y[0], y[1], a.bf16), pack2(y[2], y[3], a.bf16)};
+                    *reinterpret_cast<u32x2*>(o + 16 * db + 4 * G) = u32x2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
                 }
                 if (G == 0) a.lse[lse_at(a, b, h, i)] = lse;
             } else {
@@ -446,7 +447,7 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
 }
 
 // Merge of split items: a thread for each row and 8 columns.
-template <int HD>
+template <int DT, int HD>
 __global__ void __launch_bounds__(256) fa_quant_prefill_merge_kernel(QuantFwdArgs a, int mt_max) {
     constexpr int BM = Cfg<HD>::BM, DCH = HD / 8, RPB = 256 / DCH, BPT = BM / RPB;
     const int blk = blockIdx.x % BPT, item = blockIdx.x / BPT;
@@ -479,25 +480,30 @@ __global__ void __launch_bounds__(256) fa_quant_prefill_merge_kernel(QuantFwdArg
     const int i = r / a.g, h = hk * a.g + r % a.g;
     uint16_t* o = static_cast<uint16_t*>(a.out) + q_row(a, b, i, a.o_sb, a.o_si) + (int64_t)h * a.o_sh;
     if (d0 < a.hd)
-        *reinterpret_cast<u32x4*>(o + d0) = u32x4{pack2(acc0[0], acc0[1], a.bf16), pack2(acc0[2], acc0[3], a.bf16),
-                                                  pack2(acc1[0], acc1[1], a.bf16), pack2(acc1[2], acc1[3], a.bf16)};
+        *reinterpret_cast<u32x4*>(o + d0) = u32x4{pack2<DT>(acc0[0], acc0[1]), pack2<DT>(acc0[2], acc0[3]),
+                                                  pack2<DT>(acc1[0], acc1[1]), pack2<DT>(acc1[2], acc1[3])};
     if (d0 == 0) a.lse[lse_at(a, b, h, i)] = lse;
 }
 
-template <int CT, int HD>
+template <int DT, int CT, int HD>
 void launch_c(const QuantFwdArgs& a, int grid, int mt_max, hipStream_t stream) {
-    if (a.softcap > 0.f) hipLaunchKernelGGL((fa_quant_prefill_kernel<CT, HD, true>), dim3(grid), dim3(NT), 0, stream, a);
-    else hipLaunchKernelGGL((fa_quant_prefill_kernel<CT, HD, false>), dim3(grid), dim3(NT), 0, stream, a);
+    if (a.softcap > 0.f) hipLaunchKernelGGL((fa_quant_prefill_kernel<DT, CT, HD, true>), dim3(grid), dim3(NT), 0, stream, a);
+    else hipLaunchKernelGGL((fa_quant_prefill_kernel<DT, CT, HD, false>), dim3(grid), dim3(NT), 0, stream, a);
     if (!a.allow_split) return;
     constexpr int RPB = 256 / (HD / 8);
-    hipLaunchKernelGGL((fa_quant_prefill_merge_kernel<HD>), dim3((unsigned)(a.B * mt_max * a.Hk * (Cfg<HD>::BM / RPB))), dim3(256), 0,
-                       stream, a, mt_max);
+    hipLaunchKernelGGL((fa_quant_prefill_merge_kernel<DT, HD>), dim3((unsigned)(a.B * mt_max * a.Hk * (Cfg<HD>::BM / RPB))), dim3(256),
+                       0, stream, a, mt_max);
 }
 
 template <int HD>
 void launch_d(const QuantFwdArgs& a, int ct, int grid, int mt_max, hipStream_t stream) {
-    if (ct == CT_INT8) launch_c<CT_INT8, HD>(a, grid, mt_max, stream);
-    else launch_c<CT_E4M3, HD>(a, grid, mt_max, stream);
+    if (a.bf16) {
+        if (ct == CT_INT8) launch_c<DT_BF16, CT_INT8, HD>(a, grid, mt_max, stream);
+        else launch_c<DT_BF16, CT_E4M3, HD>(a, grid, mt_max, stream);
+    } else {
+        if (ct == CT_INT8) launch_c<DT_FP16, CT_INT8, HD>(a, grid, mt_max, stream);
+        else launch_c<DT_FP16, CT_E4M3, HD>(a, grid, mt_max, stream);
+    }
 }
 
 }  // namespace
