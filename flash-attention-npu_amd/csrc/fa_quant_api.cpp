@@ -18,9 +18,9 @@ hipError_t launch_page_table(const PageTableArgs& a, hipStream_t stream);
 hipError_t launch_quant_append(QuantAppendArgs a, int dtype, int ct, hipStream_t stream);
 int quant_decode_workers(int kd, int grid);
 hipError_t launch_quant_decode(const QuantFwdArgs& a, int ct, int kd, int nr, int grid, hipStream_t stream);
-int quant_prefill_rows(int kd);
+int quant_prefill_rows(int kd, bool many);
 int quant_prefill_keys(int kd);
-hipError_t launch_quant_prefill(const QuantFwdArgs& a, int ct, int kd, int grid, int mt_max, hipStream_t stream);
+hipError_t launch_quant_prefill(const QuantFwdArgs& a, int ct, int kd, int rows, int grid, int mt_max, hipStream_t stream);
 int compute_units();
 }  // namespace fa
 
@@ -149,7 +149,7 @@ struct Plan {
     int dec_rows;    // sequences of at most so many packed rows run on the decode kernel
     bool prefill;    // some may have more
     int nr, grid;    // decode: 16-row tiles, workgroups
-    int pf_grid, mt_max;
+    int pf_rows, pf_grid, mt_max;
     bool allow_split;
     int target_items, min_chunk;
     size_t off_lse, off_o, off_psched, off_plse, off_po, total;
@@ -177,12 +177,15 @@ Plan make_plan(const fa_quant_fwd_params* p) {
         off = align256(off + sizeof(float) * parts * pl.kd);
     }
     if (pl.prefill) {
-        const int bm = fa::quant_prefill_rows(pl.kd);
+        // ragged batches go by their mean
+        const int64_t each = p->cu_seqlens_q ? (int64_t)p->total_q * pl.g / p->batch : rows;
+        const int bm = pl.pf_rows = fa::quant_prefill_rows(pl.kd, each > 192);
         pl.mt_max = (int)((rows + bm - 1) / bm);
         int64_t items = (int64_t)nb * pl.mt_max * p->nheads_k;
         // ragged: a part tile more per sequence than the rows fill
         if (p->cu_seqlens_q) items = std::min(items, ((int64_t)p->total_q * pl.g / bm + (int64_t)nb) * p->nheads_k);
-        pl.allow_split = items < cus;
+        // the items of a ragged batch differ in length, whatever their number
+        pl.allow_split = items < cus || (p->cu_seqlens_q && items < 8 * cus);
         pl.target_items = cus;
         pl.min_chunk = 4 * fa::quant_prefill_keys(pl.kd);
         // pieces: each item's keys in chunks of at least the mean work, so at most one part chunk more each
@@ -368,7 +371,7 @@ fa_status_t fa_quant_fwd(const fa_quant_fwd_params* p, void* stream) {
         if (a.batch_idx) c.batch_idx = a.batch_idx + b0;
         hipError_t e = hipSuccess;
         if (pl.dec_rows) e = fa::launch_quant_decode(c, p->cache_dtype, pl.kd, pl.nr, pl.grid, static_cast<hipStream_t>(stream));
-        if (e == hipSuccess && pl.prefill) e = fa::launch_quant_prefill(c, p->cache_dtype, pl.kd, pl.pf_grid, pl.mt_max, static_cast<hipStream_t>(stream));
+        if (e == hipSuccess && pl.prefill) e = fa::launch_quant_prefill(c, p->cache_dtype, pl.kd, pl.pf_rows, pl.pf_grid, pl.mt_max, static_cast<hipStream_t>(stream));
         if (e != hipSuccess) return fail(FA_EHIP, "attention launch failed: %s", hipGetErrorString(e));
     }
     return FA_OK;

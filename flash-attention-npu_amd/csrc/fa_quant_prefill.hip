@@ -14,7 +14,7 @@
 // only where a new score exceeds it by 2^4, and the weights' unit leaves room for that
 // (2^10 in place of 2^14: a weight keeps its 11 bits as long as p t / R > 2^-24).
 #include "fa_pipe.h"
-#include "fa_quant.h"
+#include "fa_quant_items.h"
 
 #include <type_traits>
 
@@ -22,14 +22,13 @@ namespace fa {
 
 namespace {
 
-constexpr int MAXB = 2048;
 constexpr int NW = 8, NT = NW * 64;
 constexpr float kLazy = 4.f;
 constexpr int kUnit = 10;  // w = p t / R 2^kUnit, p <= 2^kLazy
 
-template <int HD>
+template <int HD, int RB_>
 struct Cfg {
-    static constexpr int RB = HD == 64 ? 4 : HD == 128 ? 2 : 1;   // 16-row blocks of a wave
+    static constexpr int RB = RB_;                                 // 16-row blocks of a wave
     static constexpr int BM = NW * RB * 16;                        // rows of a work item
     static constexpr int BN = 8192 / HD;                           // keys of a tile: 16 codes per thread
     static constexpr int NB = BN / 16;
@@ -39,113 +38,26 @@ struct Cfg {
     static constexpr int VPRE = HD == 64 ? 4 : 8;                  // V^T operands read ahead of the softmax
 };
 
-struct Rows {
-    int rows, mt;
-    QuantSeq q;
-};
-
-template <int BM>
-__device__ __forceinline__ Rows rows_of(const QuantFwdArgs& a, int b) {
-    Rows r;
-    r.q = quant_seq(a, b);
-    if (r.q.hi < r.q.lo) r.q.hi = r.q.lo;
-    r.rows = r.q.sq * a.g > a.dec_rows ? r.q.sq * a.g : 0;
-    r.mt = (r.rows + BM - 1) / BM;
-    return r;
-}
-
-__device__ __forceinline__ void split_of(const QuantFwdArgs& a, int range, int chunk_auto, int& ns, int& chunk) {
-    chunk = chunk_auto;
-    ns = a.allow_split && range > 0 ? (range + chunk - 1) / chunk : 1;
-}
-
-// The list of work items: prefix over the sequences in LDS, made by every
-// workgroup alike; workgroup 0 leaves it for the merge. Keys are cut into chunks so
-// that there are about target_items pieces, none under min_chunk keys.
-template <int BM, int BN>
-__device__ void build_list(const QuantFwdArgs& a, int* s_pref, long long* s_red, int& total, int& chunk_auto) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    chunk_auto = 0x3fffffff;
-    if (a.allow_split) {
-        long long work = 0, base = 0;
-        for (int b = tid; b < a.B; b += NT) {
-            const Rows r = rows_of<BM>(a, b);
-            base += (long long)a.Hk * r.mt;
-            work += (long long)a.Hk * r.mt * (r.q.hi - r.q.lo);
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            work += __shfl_xor(work, o);
-            base += __shfl_xor(base, o);
-        }
-        if (lane == 0) {
-            s_red[wave * 2] = work;
-            s_red[wave * 2 + 1] = base;
-        }
-        __syncthreads();
-        work = 0;
-        base = 0;
-        for (int w = 0; w < NW; ++w) {
-            work += s_red[w * 2];
-            base += s_red[w * 2 + 1];
-        }
-        if (base < a.target_items) {
-            long long c = (work + a.target_items - 1) / a.target_items;
-            c = c < a.min_chunk ? a.min_chunk : c;
-            c = (c + BN - 1) / BN * BN;
-            chunk_auto = (int)(c > 0x3fffffff ? 0x3fffffff : c);
-        }
-    }
-    for (int b = tid; b < a.B; b += NT) {
-        const Rows r = rows_of<BM>(a, b);
-        int ns, chunk;
-        split_of(a, r.q.hi - r.q.lo, chunk_auto, ns, chunk);
-        s_pref[b + 1] = a.Hk * r.mt * ns;
-        if (blockIdx.x == 0 && a.allow_split) a.pf_sched[a.B + 1 + b] = ns;
-    }
-    __syncthreads();
-    if (wave == 0) {
-        const int seg = (a.B + 63) / 64, b0 = lane * seg;
-        int local = 0;
-        for (int k = 0; k < seg; ++k)
-            if (b0 + k < a.B) local += s_pref[b0 + k + 1];
-        int incl = local;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(incl, o);
-            if (lane >= o) incl += v;
-        }
-        int run = incl - local;
-        for (int k = 0; k < seg; ++k)
-            if (b0 + k < a.B) {
-                run += s_pref[b0 + k + 1];
-                s_pref[b0 + k + 1] = run;
-            }
-        if (lane == 0) s_pref[0] = 0;
-    }
-    __syncthreads();
-    total = s_pref[a.B];
-    if (blockIdx.x == 0 && a.allow_split)
-        for (int b = tid; b <= a.B; b += NT) a.pf_sched[b] = s_pref[b];
-}
-
 // CAP: soft cap
-template <int DT, int CT, int HD, bool CAP>
+template <int DT, int CT, int HD, int RB_, bool CAP>
 __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a) {
-    using C = Cfg<HD>;
+    using C = Cfg<HD, RB_>;
     constexpr int RB = C::RB, BM = C::BM, BN = C::BN, NB = C::NB, DCH = C::DCH, KSTEPS = C::KSTEPS, DBLK = C::DBLK,
                   VPRE = C::VPRE;
     __shared__ __attribute__((aligned(16))) uint16_t s_k[2][BN * HD];
     __shared__ __attribute__((aligned(16))) uint16_t s_v[2][BN * HD];
-    __shared__ float s_ks[2][NB], s_vs[2][NB];
-    __shared__ int s_ok[2][NB];
-    __shared__ int s_pref[MAXB + 1];
-    __shared__ long long s_red[2 * NW];
+    // of the blocks of 16 keys: K scale; V scale, its log2 and inverse; whether the page
+    // is in the cache; of the tile: whether the softmax scale and all of these are positive
+    __shared__ float s_ks[2][NB], s_vs[2][NB], s_lv[2][NB], s_iv[2][NB];
+    __shared__ int s_ok[2][NB], s_plain[2];
+    __shared__ int64_t s_koff[2][NB], s_voff[2][NB];  // where its rows are; below 0: nowhere
+    __shared__ int s_pref[kQuantMaxB + 1];
+    __shared__ long long s_red[NW];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int li = lane & 15, G = lane >> 4;
     int total, chunk_auto;
-    build_list<BM, BN>(a, s_pref, s_red, total, chunk_auto);
+    build_list<BM, BN, NW>(a, s_pref, s_red, total, chunk_auto);
 
     auto swzk = [](int r, int c) { return HD == 64 ? swz_k64(r, c) : swz_k(r, c); };
     auto swzv = [](int r, int c) { return HD == 64 ? swz_v64(r, c) : swz_v(r, c); };
@@ -159,7 +71,13 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
     // this thread's part of a tile: 16 codes of one row of K and of V
     const int kk = tid / DCH, dch = tid % DCH;
     const bool in = dch * 16 < a.hd;
-    const int sblk = tid % NB, swhich = tid / NB;  // threads below 2 NB carry the scales
+    const uint32_t kin = (uint32_t)(kk & 15) * (uint32_t)a.k_si + (in ? dch * 16 : 0);
+    const uint32_t vin = (uint32_t)(kk & 15) * (uint32_t)a.v_si + (in ? dch * 16 : 0);
+    auto anew = []() -> const QuantFwdArgs& {  // as in fa_quant_decode.hip
+        auto p = __builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(p));
+        return *(const QuantFwdArgs*)p;
+    };
 
     for (int k = 0; k * (int)gridDim.x < total; ++k) {
         // items are numbered heaviest first within a sequence; odd passes run the other way
@@ -196,39 +114,47 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
         const int f_lo = max(k_lo, key_lo(i_hi + diag0, a.wl, 0)), f_hi = min(k_hi - 1, key_hi(i_lo + diag0, a.wr, 0));
 
         // ---- tiles: registers -> widened -> LDS ---------------------------------------------
+        // The blocks of 16 keys of a tile are looked after by the first NB lanes of the
+        // last wave, which causal items leave idle soonest: page id, three tiles ahead
+        // of the products; rows' place and scales, two tiles; all others read the place.
         const int* trow = a.table ? a.table + (int64_t)R.q.crow * a.t_stride : nullptr;
-        auto page_of = [&](int j, int& inp) -> int {  // -1: no key of this item
-            inp = 0;
-            if (j >= k_hi || j + 16 <= k_lo) return -1;
-            const int pi = trow ? (int)udiv(a.page, (uint32_t)j) : 0;
-            inp = j - pi * a.page_size;
-            return trow ? trow[pi] : R.q.crow;
+        const bool keeper = tid >= NT - 64 && tid < NT - 64 + NB;
+        int bid = -1, binp = 0;
+        float bks = 0.f, bvs = 0.f;
+        bool bok = false;
+        auto block_id = [&](int t) {
+            const QuantFwdArgs& A = anew();
+            const int j = base + t * BN + lane * 16;
+            bid = -1;
+            binp = 0;
+            if (j < k_hi && j + 16 > k_lo) {
+                const int pi = trow ? (int)udiv(A.page, (uint32_t)j) : 0;
+                binp = j - pi * A.page_size;
+                bid = trow ? trow[pi] : R.q.crow;
+            }
         };
+        auto block_place = [&](int t) {
+            const QuantFwdArgs& A = anew();
+            bok = bid >= 0 && bid < A.num_pages;
+            const int64_t p = bok ? bid : 0, r = bok ? binp : 0;
+            s_koff[t & 1][lane] = bok ? p * A.k_sp + r * A.k_si : -1;
+            s_voff[t & 1][lane] = p * A.v_sp + r * A.v_si;
+            const int64_t sb = udiv(A.sblk, (uint32_t)r);
+            bks = A.ks[p * A.ks_sp + sb * A.ks_sb + (int64_t)hk * A.ks_sh];
+            bvs = A.vs[p * A.vs_sp + sb * A.vs_sb + (int64_t)hk * A.vs_sh];
+        };
+        const uint8_t* kbase = a.k + (int64_t)hk * a.k_sh;
+        const uint8_t* vbase = a.v + (int64_t)hk * a.v_sh;
         u32x4 kr, vr;
-        float sc = 0.f;
-        int sok = 0;
-        int id, inp, sid = -1, sinp = 0;
-        auto ids = [&](int t0) {
-            id = page_of(t0 + kk, inp);
-            if (t0 + kk < k_lo) id = -1;
-            if (tid < 2 * NB) sid = page_of(t0 + sblk * 16, sinp);
-        };
-        auto load_tile = [&]() {  // the rows that `ids` found
-            const bool ok = id >= 0 && id < a.num_pages && in;
+        auto load_tile = [&](int t) {
+            const int64_t ko = s_koff[t & 1][kk >> 4], vo = s_voff[t & 1][kk >> 4];
+            const int j = base + t * BN + kk;
+            const bool ok = ko >= 0 && j >= k_lo && j < k_hi && in;
             kr = u32x4{0u, 0u, 0u, 0u};
             vr = kr;
             if (ok) {
-                kr = *reinterpret_cast<const u32x4*>(a.k + (int64_t)id * a.k_sp + (int64_t)inp * a.k_si + (int64_t)hk * a.k_sh + dch * 16);
-                vr = *reinterpret_cast<const u32x4*>(a.v + (int64_t)id * a.v_sp + (int64_t)inp * a.v_si + (int64_t)hk * a.v_sh + dch * 16);
-            }
-            if (tid < 2 * NB) {
-                sok = sid >= 0 && sid < a.num_pages;
-                sc = 0.f;
-                if (sok) {
-                    const int64_t sb = udiv(a.sblk, (uint32_t)sinp);
-                    sc = swhich ? a.vs[(int64_t)sid * a.vs_sp + sb * a.vs_sb + (int64_t)hk * a.vs_sh]
-                                : a.ks[(int64_t)sid * a.ks_sp + sb * a.ks_sb + (int64_t)hk * a.ks_sh];
-                }
+                kr = *reinterpret_cast<const u32x4*>(kbase + ko + kin);
+                vr = *reinterpret_cast<const u32x4*>(vbase + vo + vin);
             }
         };
         auto store_tile = [&](int buf) {
@@ -239,25 +165,25 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
                 *reinterpret_cast<u32x4*>(&s_k[buf][kk * HD + (swzk(kk & 15, 2 * dch + u) << 3)]) = u32x4{k0[0], k0[1], k1[0], k1[1]};
                 *reinterpret_cast<u32x4*>(&s_v[buf][kk * HD + (swzv(kk & 15, 2 * dch + u) << 3)]) = u32x4{v0[0], v0[1], v1[0], v1[1]};
             }
-            if (tid < NB) {
-                s_ks[buf][sblk] = sc;
-                s_ok[buf][sblk] = sok;
-            } else if (tid < 2 * NB) {
-                s_vs[buf][sblk] = sc;
+            if (keeper) {
+                s_ks[buf][lane] = bok ? bks : 0.f;
+                s_vs[buf][lane] = bok ? bvs : 0.f;
+                s_lv[buf][lane] = fast_log2(bvs);
+                s_iv[buf][lane] = 1.f / bvs;
+                s_ok[buf][lane] = bok;
+                const unsigned long long odd = __ballot(!bok || !(anew().scale > 0.f && bks > 0.f && bks < INFINITY && bvs > 0x1p-100f && bvs < 0x1p100f));
+                if (lane == 0) s_plain[buf] = odd == 0;
             }
         };
-        // a page outside the cache anywhere in the item: its tiles all test each key
-        int bad = 0;
-        if (trow && ntiles > 0) {
-            const int p0 = (int)udiv(a.page, (uint32_t)k_lo), p1 = (int)udiv(a.page, (uint32_t)(k_hi - 1));
-            for (int p = p0 + tid; p <= p1; p += NT) bad |= trow[p] < 0 || trow[p] >= a.num_pages;
+        // the tiles of the item before are read by all when the first barrier is passed
+        __syncthreads();
+        if (ntiles > 0 && keeper) {
+            block_id(0);
+            block_place(0);
+            block_id(1);
         }
-        if (ntiles > 0) {
-            ids(base);
-            load_tile();
-            ids(base + BN);
-        }
-        bad = __syncthreads_or(bad);  // also: the tiles of the item before are read
+        __syncthreads();
+        if (ntiles > 0) load_tile(0);
 
         // ---- Q --------------------------------------------------------------------------------
         u32x4 qreg[RB][KSTEPS];
@@ -297,9 +223,12 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
             for (int db = 0; db < DBLK; ++db) oacc[rb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
 
-        // 32 keys of the tile in buf, those at 32 hh
-        auto tile = [&](int buf, int hh, int s0, auto mask_tag) {
-            constexpr bool MASK = decltype(mask_tag)::value;
+        // 32 keys of the tile in buf, those at 32 hh. PLAIN: all rows see all of them and
+        // the scales are positive. Scores then stay as the products give them until
+        // the exponential's argument, and the V scale goes there too, as its log2, so
+        // that the weight comes out whole; the sum of p takes it back, once for a block.
+        auto tile = [&](int buf, int hh, int s0, auto plain_tag) {
+            constexpr bool PLAIN = decltype(plain_tag)::value;
             f32x4 x[RB][2];
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) x[rb][0] = x[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -326,22 +255,27 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
             const int up = max((int)(__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, vmax)) >> 23) + 1 - eR, 0);
             bool need = up > 0;
             float xmax[RB];
+            constexpr bool RAW = PLAIN && !CAP;  // x stays raw
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
                 float mx = -INFINITY;
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) {
                     const float c = qs[rb] * ks[kb];
+                    if constexpr (RAW) {
+                        mx = fmaxf(mx, c * fmaxf(fmaxf(x[rb][kb][0], x[rb][kb][1]), fmaxf(x[rb][kb][2], x[rb][kb][3])));
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float y = x[rb][kb][e] * c;
-                        if constexpr (CAP) y = a.softcap * kLog2e * fast_tanh(y);
-                        if constexpr (MASK) {
-                            const int j = s0 + kb * 16 + G * 4 + e;
-                            y = s_ok[buf][2 * hh + kb] && j >= rlo[rb] && j <= rhi[rb] ? y : -INFINITY;
+                        for (int e = 0; e < 4; ++e) {
+                            float y = x[rb][kb][e] * c;
+                            if constexpr (CAP) y = a.softcap * kLog2e * fast_tanh(y);
+                            if constexpr (!PLAIN) {
+                                const int j = s0 + kb * 16 + G * 4 + e;
+                                y = s_ok[buf][2 * hh + kb] && j >= rlo[rb] && j <= rhi[rb] ? y : -INFINITY;
+                            }
+                            x[rb][kb][e] = y;
+                            mx = fmaxf(mx, y);
                         }
-                        x[rb][kb][e] = y;
-                        mx = fmaxf(mx, y);
                     }
                 }
                 xmax[rb] = mx;
@@ -364,22 +298,40 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
                     }
                 }
             }
-            const float toR = exp2i(127 + kUnit - eR);
-            vs[0] *= toR;
-            vs[1] *= toR;
             u32x4 pk[RB];
+            if constexpr (PLAIN) {
+                const float unit = (float)(127 + kUnit - eR), back = exp2i(eR - 127 - kUnit);
+                const float lv[2] = {s_lv[buf][2 * hh] + unit, s_lv[buf][2 * hh + 1] + unit};
+                const float iv[2] = {s_iv[buf][2 * hh] * back, s_iv[buf][2 * hh + 1] * back};
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-                f32x8 wt;
-                float sum = 0.f;
+                for (int rb = 0; rb < RB; ++rb) {
+                    f32x8 wt;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float p = fast_exp2(x[rb][e >> 2][e & 3] - m_run[rb]);
-                    sum += p;
-                    wt[e] = p * vs[e >> 2];
+                    for (int kb = 0; kb < 2; ++kb) {
+                        const float c = RAW ? qs[rb] * ks[kb] : 1.f, d = lv[kb] - m_run[rb];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) wt[4 * kb + e] = fast_exp2(__builtin_fmaf(x[rb][kb][e], c, d));
+                        l_run[rb] += ((wt[4 * kb] + wt[4 * kb + 1]) + (wt[4 * kb + 2] + wt[4 * kb + 3])) * iv[kb];
+                    }
+                    pk[rb] = pack8<DT_FP16>(wt);
                 }
-                l_run[rb] += sum;
-                pk[rb] = pack8<DT_FP16>(wt);
+            } else {
+                const float toR = exp2i(127 + kUnit - eR);
+                vs[0] *= toR;
+                vs[1] *= toR;
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    f32x8 wt;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float p = fast_exp2(x[rb][e >> 2][e & 3] - m_run[rb]);
+                        sum += p;
+                        wt[e] = p * vs[e >> 2];
+                    }
+                    l_run[rb] += sum;
+                    pk[rb] = pack8<DT_FP16>(wt);
+                }
             }
             __builtin_amdgcn_s_setprio(1);  // the SIMD's other wave fills the slots between these products
 #pragma unroll
@@ -392,27 +344,39 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
             __builtin_amdgcn_s_setprio(0);
         };
 
+        // Turn t: tile t's products, tile t + 1 from registers to LDS, tile t + 2 asked
+        // for at the place left in turn t - 1, and tile t + 3's left in this one. The
+        // keeper's scales of tile t + 1 go down before it asks for tile t + 2's.
         if (ntiles > 0) {
             store_tile(0);
-            if (ntiles > 1) load_tile();
-            ids(base + 2 * BN);
+            if (keeper) {
+                block_place(1);
+                block_id(2);
+            }
         }
         __syncthreads();
+        if (ntiles > 1) load_tile(1);
         for (int t = 0; t < ntiles; ++t) {
             const int buf = t & 1, s0 = base + t * BN;
             if (live && s0 <= w_hi && s0 + BN > w_lo) {
+                const bool plain = __builtin_amdgcn_readfirstlane(s_plain[buf]);
 #pragma unroll
                 for (int hh = 0; hh < BN / 32; ++hh) {
                     const int h0 = s0 + 32 * hh;
                     if (h0 > w_hi || h0 + 32 <= w_lo) continue;
-                    if (!bad && h0 >= f_lo && h0 + 31 <= f_hi) tile(buf, hh, h0, std::integral_constant<bool, false>{});
-                    else tile(buf, hh, h0, std::integral_constant<bool, true>{});
+                    if (plain && h0 >= f_lo && h0 + 31 <= f_hi) tile(buf, hh, h0, std::integral_constant<bool, true>{});
+                    else tile(buf, hh, h0, std::integral_constant<bool, false>{});
                 }
             }
-            if (t + 1 < ntiles) store_tile(buf ^ 1);
-            if (t + 2 < ntiles) load_tile();
-            ids(base + (t + 3) * BN);
+            if (t + 1 < ntiles) {
+                store_tile(buf ^ 1);
+                if (keeper) {
+                    block_place(t + 2);
+                    block_id(t + 3);
+                }
+            }
             __syncthreads();
+            if (t + 2 < ntiles) load_tile(t + 2);
         }
 
         // ---- results --------------------------------------------------------------------------
@@ -446,75 +410,36 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
     }
 }
 
-// Merge of split items: a thread for each row and 8 columns.
-template <int DT, int HD>
-__global__ void __launch_bounds__(256) fa_quant_prefill_merge_kernel(QuantFwdArgs a, int mt_max) {
-    constexpr int BM = Cfg<HD>::BM, DCH = HD / 8, RPB = 256 / DCH, BPT = BM / RPB;
-    const int blk = blockIdx.x % BPT, item = blockIdx.x / BPT;
-    const int hk = item % a.Hk, mt = item / a.Hk % mt_max, b = item / a.Hk / mt_max;
-    const int ns = a.pf_sched[a.B + 1 + b];
-    if (ns <= 1) return;
-    int sq = a.cu_q ? a.cu_q[b + 1] - a.cu_q[b] : a.Sq;
-    sq = min(max(sq, 0), a.Sq);
-    const int rows = sq * a.g > a.dec_rows ? sq * a.g : 0, mt_b = (rows + BM - 1) / BM;
-    const int rr = blk * RPB + threadIdx.x / DCH, d0 = threadIdx.x % DCH * 8, r = mt * BM + rr;
-    if (mt >= mt_b || r >= rows) return;
-    const int w0 = a.pf_sched[b] + (mt_b - 1 - mt) * ns * a.Hk + hk;
-    float m = -INFINITY;
-    for (int s = 0; s < ns; ++s) m = fmaxf(m, a.pf_lse[(int64_t)(w0 + s * a.Hk) * BM + rr]);
-    f32x4 acc0 = {0.f, 0.f, 0.f, 0.f}, acc1 = acc0;
-    float lse = INFINITY;
-    if (m != -INFINITY) {
-        float sum = 0.f;
-        for (int s = 0; s < ns; ++s) {
-            const int64_t prow = (int64_t)(w0 + s * a.Hk) * BM + rr;
-            const float wgt = fast_exp2((a.pf_lse[prow] - m) * kLog2e);
-            sum += wgt;
-            acc0 += *reinterpret_cast<const f32x4*>(a.pf_o + prow * HD + d0) * wgt;
-            acc1 += *reinterpret_cast<const f32x4*>(a.pf_o + prow * HD + d0 + 4) * wgt;
-        }
-        acc0 *= 1.f / sum;
-        acc1 *= 1.f / sum;
-        lse = m + fast_log2(sum) * kLn2;
-    }
-    const int i = r / a.g, h = hk * a.g + r % a.g;
-    uint16_t* o = static_cast<uint16_t*>(a.out) + q_row(a, b, i, a.o_sb, a.o_si) + (int64_t)h * a.o_sh;
-    if (d0 < a.hd)
-        *reinterpret_cast<u32x4*>(o + d0) = u32x4{pack2<DT>(acc0[0], acc0[1]), pack2<DT>(acc0[2], acc0[3]),
-                                                  pack2<DT>(acc1[0], acc1[1]), pack2<DT>(acc1[2], acc1[3])};
-    if (d0 == 0) a.lse[lse_at(a, b, h, i)] = lse;
+template <int DT, int CT, int HD, int RB>
+void launch_r(const QuantFwdArgs& a, int grid, int mt_max, hipStream_t stream) {
+    if (a.softcap > 0.f) hipLaunchKernelGGL((fa_quant_prefill_kernel<DT, CT, HD, RB, true>), dim3(grid), dim3(NT), 0, stream, a);
+    else hipLaunchKernelGGL((fa_quant_prefill_kernel<DT, CT, HD, RB, false>), dim3(grid), dim3(NT), 0, stream, a);
+    launch_items_merge<DT, HD, Cfg<HD, RB>::BM>(a, mt_max, stream);
 }
 
-template <int DT, int CT, int HD>
-void launch_c(const QuantFwdArgs& a, int grid, int mt_max, hipStream_t stream) {
-    if (a.softcap > 0.f) hipLaunchKernelGGL((fa_quant_prefill_kernel<DT, CT, HD, true>), dim3(grid), dim3(NT), 0, stream, a);
-    else hipLaunchKernelGGL((fa_quant_prefill_kernel<DT, CT, HD, false>), dim3(grid), dim3(NT), 0, stream, a);
-    if (!a.allow_split) return;
-    constexpr int RPB = 256 / (HD / 8);
-    hipLaunchKernelGGL((fa_quant_prefill_merge_kernel<DT, HD>), dim3((unsigned)(a.B * mt_max * a.Hk * (Cfg<HD>::BM / RPB))), dim3(256),
-                       0, stream, a, mt_max);
-}
-
-template <int HD>
-void launch_d(const QuantFwdArgs& a, int ct, int grid, int mt_max, hipStream_t stream) {
+template <int HD, int RB>
+void launch_c(const QuantFwdArgs& a, int ct, int grid, int mt_max, hipStream_t stream) {
     if (a.bf16) {
-        if (ct == CT_INT8) launch_c<DT_BF16, CT_INT8, HD>(a, grid, mt_max, stream);
-        else launch_c<DT_BF16, CT_E4M3, HD>(a, grid, mt_max, stream);
+        if (ct == CT_INT8) launch_r<DT_BF16, CT_INT8, HD, RB>(a, grid, mt_max, stream);
+        else launch_r<DT_BF16, CT_E4M3, HD, RB>(a, grid, mt_max, stream);
     } else {
-        if (ct == CT_INT8) launch_c<DT_FP16, CT_INT8, HD>(a, grid, mt_max, stream);
-        else launch_c<DT_FP16, CT_E4M3, HD>(a, grid, mt_max, stream);
+        if (ct == CT_INT8) launch_r<DT_FP16, CT_INT8, HD, RB>(a, grid, mt_max, stream);
+        else launch_r<DT_FP16, CT_E4M3, HD, RB>(a, grid, mt_max, stream);
     }
 }
 
 }  // namespace
 
-int quant_prefill_rows(int kd) { return kd == 64 ? Cfg<64>::BM : kd == 128 ? Cfg<128>::BM : Cfg<256>::BM; }
-int quant_prefill_keys(int kd) { return kd == 64 ? Cfg<64>::BN : kd == 128 ? Cfg<128>::BN : Cfg<256>::BN; }
+// Rows of an item: 128, or as many as the registers take where sequences have them.
+int quant_prefill_rows(int kd, bool many) { return many && kd < 256 ? 256 : 128; }
+int quant_prefill_keys(int kd) { return 8192 / kd; }
 
-hipError_t launch_quant_prefill(const QuantFwdArgs& a, int ct, int kd, int grid, int mt_max, hipStream_t stream) {
-    if (kd == 64) launch_d<64>(a, ct, grid, mt_max, stream);
-    else if (kd == 128) launch_d<128>(a, ct, grid, mt_max, stream);
-    else launch_d<256>(a, ct, grid, mt_max, stream);
+hipError_t launch_quant_prefill(const QuantFwdArgs& a, int ct, int kd, int rows, int grid, int mt_max, hipStream_t stream) {
+    if (kd == 64 && rows == 256) launch_c<64, 2>(a, ct, grid, mt_max, stream);
+    else if (kd == 64) launch_c<64, 1>(a, ct, grid, mt_max, stream);
+    else if (kd == 128 && rows == 256) launch_c<128, 2>(a, ct, grid, mt_max, stream);
+    else if (kd == 128) launch_c<128, 1>(a, ct, grid, mt_max, stream);
+    else launch_c<256, 1>(a, ct, grid, mt_max, stream);
     return hipGetLastError();
 }
 
