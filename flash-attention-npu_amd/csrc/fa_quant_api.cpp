@@ -19,8 +19,7 @@ hipError_t launch_quant_append(QuantAppendArgs a, int dtype, int ct, hipStream_t
 int quant_decode_workers(int kd, int grid);
 hipError_t launch_quant_decode(const QuantFwdArgs& a, int ct, int kd, int nr, int grid, hipStream_t stream);
 int quant_prefill_rows(int kd, bool many);
-int quant_prefill_keys(int kd);
-hipError_t launch_quant_prefill(const QuantFwdArgs& a, int ct, int kd, int rows, int grid, int mt_max, hipStream_t stream);
+hipError_t launch_quant_prefill(const QuantFwdArgs& a, int ct, int kd, int rows, int grid, hipStream_t stream);
 int compute_units();
 }  // namespace fa
 
@@ -149,10 +148,9 @@ struct Plan {
     int dec_rows;    // sequences of at most so many packed rows run on the decode kernel
     bool prefill;    // some may have more
     int nr, grid;    // decode: 16-row tiles, workgroups
-    int pf_rows, pf_grid, mt_max;
-    bool allow_split;
-    int target_items, min_chunk;
-    size_t off_lse, off_o, off_psched, off_plse, off_po, total;
+    int pf_rows, pf_grid;
+    bool cut;        // prefill: the items are cut over the workgroups
+    size_t off_lse, off_o, off_pcut, off_plse, off_po, total;
 };
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -180,22 +178,21 @@ Plan make_plan(const fa_quant_fwd_params* p) {
         // ragged batches go by their mean
         const int64_t each = p->cu_seqlens_q ? (int64_t)p->total_q * pl.g / p->batch : rows;
         const int bm = pl.pf_rows = fa::quant_prefill_rows(pl.kd, each > 192);
-        pl.mt_max = (int)((rows + bm - 1) / bm);
-        int64_t items = (int64_t)nb * pl.mt_max * p->nheads_k;
+        int64_t entries = (int64_t)nb * ((rows + bm - 1) / bm);
         // ragged: a part tile more per sequence than the rows fill
-        if (p->cu_seqlens_q) items = std::min(items, ((int64_t)p->total_q * pl.g / bm + (int64_t)nb) * p->nheads_k);
-        // the items of a ragged batch differ in length, whatever their number
-        pl.allow_split = items < cus || (p->cu_seqlens_q && items < 8 * cus);
-        pl.target_items = cus;
-        pl.min_chunk = 4 * fa::quant_prefill_keys(pl.kd);
-        // pieces: each item's keys in chunks of at least the mean work, so at most one part chunk more each
-        const int64_t pieces = pl.allow_split ? items + pl.target_items : items;
-        pl.pf_grid = (int)std::min<int64_t>(pieces, pl.allow_split ? 2 * cus : cus);
-        if (pl.allow_split) {
-            pl.off_psched = off;
-            pl.off_plse = off = align256(off + sizeof(int) * (2 * nb + 1));
-            pl.off_po = off = align256(off + sizeof(float) * pieces * bm);
-            off = align256(off + sizeof(float) * pieces * bm * pl.kd);
+        if (p->cu_seqlens_q) entries = std::min(entries, (int64_t)p->total_q * pl.g / bm + (int64_t)nb);
+        const int64_t items = entries * p->nheads_k;
+        // Cutting costs its pieces' sums a way through memory (chunks of 2048 onto 4096 keys,
+        // four items to a workgroup: 921 -> 971 us). It pays where items differ in
+        // length (ragged) or a last round would leave workgroups without one.
+        const int64_t rounds = (items + cus - 1) / cus;
+        pl.cut = entries <= kMaxBatch && items < 8 * cus && (p->cu_seqlens_q || rounds * cus * 12 > items * 13);
+        pl.pf_grid = pl.cut ? cus : (int)std::min<int64_t>(items, cus);
+        if (pl.cut) {
+            pl.off_pcut = off;
+            pl.off_plse = off = align256(off + sizeof(int) * 4 * pl.pf_grid);
+            pl.off_po = off = align256(off + sizeof(float) * 2 * pl.pf_grid * bm);
+            off = align256(off + sizeof(float) * 2 * pl.pf_grid * bm * pl.kd);
         }
     }
     pl.total = off;
@@ -348,10 +345,8 @@ fa_status_t fa_quant_fwd(const fa_quant_fwd_params* p, void* stream) {
     a.sched = reinterpret_cast<int*>(ws);
     a.part_lse = reinterpret_cast<float*>(ws + pl.off_lse);
     a.part_o = reinterpret_cast<float*>(ws + pl.off_o);
-    a.allow_split = pl.allow_split;
-    a.target_items = pl.target_items;
-    a.min_chunk = pl.min_chunk;
-    a.pf_sched = reinterpret_cast<int*>(ws + pl.off_psched);
+    a.cut = pl.cut;
+    a.pf_cut = reinterpret_cast<int*>(ws + pl.off_pcut);
     a.pf_lse = reinterpret_cast<float*>(ws + pl.off_plse);
     a.pf_o = reinterpret_cast<float*>(ws + pl.off_po);
     // a batch of more sequences than a launch lists runs in parts, one after another
@@ -371,7 +366,7 @@ fa_status_t fa_quant_fwd(const fa_quant_fwd_params* p, void* stream) {
         if (a.batch_idx) c.batch_idx = a.batch_idx + b0;
         hipError_t e = hipSuccess;
         if (pl.dec_rows) e = fa::launch_quant_decode(c, p->cache_dtype, pl.kd, pl.nr, pl.grid, static_cast<hipStream_t>(stream));
-        if (e == hipSuccess && pl.prefill) e = fa::launch_quant_prefill(c, p->cache_dtype, pl.kd, pl.pf_rows, pl.pf_grid, pl.mt_max, static_cast<hipStream_t>(stream));
+        if (e == hipSuccess && pl.prefill) e = fa::launch_quant_prefill(c, p->cache_dtype, pl.kd, pl.pf_rows, pl.pf_grid, static_cast<hipStream_t>(stream));
         if (e != hipSuccess) return fail(FA_EHIP, "attention launch failed: %s", hipGetErrorString(e));
     }
     return FA_OK;

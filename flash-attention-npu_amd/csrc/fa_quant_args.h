@@ -78,12 +78,11 @@ struct QuantFwdArgs {
     int* sched;                    // [0..B]: tile prefix
     float* part_lse;               // [worker][2][16 * row tiles]
     float* part_o;                 // [worker][2][16 * row tiles][kernel head dim]
-    // prefill kernel: items may be cut over the keys into about target_items
-    // pieces of at least min_chunk keys; their scratch
-    int allow_split, target_items, min_chunk;
-    int* pf_sched;                 // [0..B]: item prefix, [B+1..2B]: pieces of each sequence's items
-    float* pf_lse;                 // [item][rows of an item]
-    float* pf_o;                   // [item][rows of an item][kernel head dim]
+    // prefill kernel: whether its items are cut, and the scratch of that
+    int cut;
+    int* pf_cut;                   // [workgroup][4]: the cut item that begins there
+    float* pf_lse;                 // [workgroup][2][rows of an item]
+    float* pf_o;                   // [workgroup][2][rows of an item][kernel head dim]
 };
 
 }  // namespace fa

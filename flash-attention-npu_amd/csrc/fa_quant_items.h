@@ -1,5 +1,5 @@
-// fa_quant_items.h -- the work items of the prefill kernels over 8-bit codes: their
-// list, their split over the keys, and the merge of the pieces.
+// fa_quant_items.h -- the work items of the prefill kernel over 8-bit codes: their
+// list, their cut over the workgroups, and the merge of the pieces.
 #pragma once
 #include "fa_quant.h"
 #include "fa_pipe.h"
@@ -10,7 +10,7 @@ namespace fa {
 
 namespace {
 
-constexpr int kQuantMaxB = 2048;  // sequences of a launch: their list lives in LDS
+constexpr int kQuantMaxB = 2048;  // sequences of a launch, and entries of a list that is cut: they live in LDS
 
 struct Rows {
     int rows, mt;
@@ -27,114 +27,148 @@ __device__ __forceinline__ Rows rows_of(const QuantFwdArgs& a, int b) {
     return r;
 }
 
-__device__ __forceinline__ void split_of(const QuantFwdArgs& a, int range, int chunk_auto, int& ns, int& chunk) {
-    chunk = chunk_auto;
-    ns = a.allow_split && range > 0 ? (range + chunk - 1) / chunk : 1;
+// Keys that rows [row0, row0 + n) see; those of a tile from base on
+struct Keys {
+    int lo, hi;
+};
+__device__ __forceinline__ Keys keys_of(const QuantFwdArgs& a, const QuantSeq& q, int row0, int n) {
+    const int diag0 = q.sk - q.sq;
+    Keys k;
+    k.lo = max(0, key_lo(row0 / a.g + diag0, a.wl, 0));
+    k.hi = max(k.lo, min(q.sk, key_hi((row0 + n - 1) / a.g + diag0, a.wr, 0) + 1));
+    return k;
+}
+template <int BN>
+__device__ __forceinline__ int tiles_of(const Keys& k) {
+    return (k.hi - (k.lo & ~15) + BN - 1) / BN;  // tiles start at a block of 16 keys
 }
 
-// The list of work items: prefix over the sequences in LDS, made by every
-// workgroup alike; workgroup 0 leaves it for the merge. Keys are cut into chunks so
-// that there are about target_items pieces, none under min_chunk keys.
+// Exclusive prefix sums in place over s[1 .. n], by one wave; s[0] = 0
+template <typename T>
+__device__ void prefix_sums(T* s, int n) {
+    const int lane = threadIdx.x & 63, seg = (n + 63) / 64, b0 = lane * seg;
+    T local = 0;
+    for (int k = 0; k < seg; ++k)
+        if (b0 + k < n) local += s[b0 + k + 1];
+    T incl = local;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const T v = __shfl_up(incl, o);
+        if (lane >= o) incl += v;
+    }
+    T run = incl - local;
+    for (int k = 0; k < seg; ++k)
+        if (b0 + k < n) {
+            run += s[b0 + k + 1];
+            s[b0 + k + 1] = run;
+        }
+    if (lane == 0) s[0] = 0;
+}
+
+template <typename T, typename X>
+__device__ __forceinline__ int find_in(const T* s, int n, X x) {  // the last i of [0, n) with s[i] <= x
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// The list: an entry is a tile of BM rows of a sequence, an item an entry of one kv
+// head. Every workgroup makes the list alike, in LDS.
+//
+// Few items, or ragged ones, are cut: laid end to end, head after head, their costs
+// make a line that the workgroups share evenly, so one piece begins and one ends
+// inside an item at most. An item costs kStart and for each tile of keys kTile and one
+// for each wave with rows; a workgroup takes at least kLeast.
+constexpr int kStart = 24, kTile = 4, kLeast = 72;
+
+struct Line {
+    int64_t len;   // of one head
+    int64_t total;
+    int workers;
+    __device__ int64_t cut(int w) const { return w * total / workers; }
+    // the worker that holds place x: the last w with cut(w) <= x
+    __device__ int holder(int64_t x) const { return (int)(((x + 1) * workers - 1) / total); }
+};
+
+template <int BM, int WROWS>
+__device__ __forceinline__ int tile_cost(int rows, int mt) {
+    return kTile + (min(BM, rows - mt * BM) + WROWS - 1) / WROWS;
+}
+
 template <int BM, int BN, int NW>
-__device__ void build_list(const QuantFwdArgs& a, int* s_pref, long long* s_red, int& total, int& chunk_auto) {
+__device__ void build_list(const QuantFwdArgs& a, int* s_pref, int64_t* s_line) {
     constexpr int NT = NW * 64;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    chunk_auto = 0x3fffffff;
-    if (a.allow_split) {
-        long long work = 0;
-        for (int b = tid; b < a.B; b += NT) {
-            const Rows r = rows_of<BM>(a, b);
-            work += (long long)a.Hk * r.mt * (r.q.hi - r.q.lo);
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) work += __shfl_xor(work, o);
-        if (lane == 0) s_red[wave] = work;
-        __syncthreads();
-        work = 0;
-        for (int w = 0; w < NW; ++w) work += s_red[w];
-        long long c = (work + a.target_items - 1) / a.target_items;
-        c = c < a.min_chunk ? a.min_chunk : c;
-        c = (c + BN - 1) / BN * BN;
-        chunk_auto = (int)(c > 0x3fffffff ? 0x3fffffff : c);
-    }
-    for (int b = tid; b < a.B; b += NT) {
+    const int tid = threadIdx.x;
+    for (int b = tid; b < a.B; b += NT) s_pref[b + 1] = rows_of<BM>(a, b).mt;
+    __syncthreads();
+    if (tid < 64) prefix_sums(s_pref, a.B);
+    __syncthreads();
+    if (!a.cut) return;
+    const int n = min(s_pref[a.B], kQuantMaxB);
+    for (int e = tid; e < n; e += NT) {
+        const int b = find_in(s_pref, a.B, e);
         const Rows r = rows_of<BM>(a, b);
-        int ns, chunk;
-        split_of(a, r.q.hi - r.q.lo, chunk_auto, ns, chunk);
-        s_pref[b + 1] = a.Hk * r.mt * ns;
-        if (blockIdx.x == 0 && a.allow_split) a.pf_sched[a.B + 1 + b] = ns;
+        const int mt = e - s_pref[b];
+        const Keys k = keys_of(a, r.q, mt * BM, min(BM, r.rows - mt * BM));
+        s_line[e + 1] = kStart + (int64_t)tiles_of<BN>(k) * tile_cost<BM, BM / NW>(r.rows, mt);
     }
     __syncthreads();
-    if (wave == 0) {
-        const int seg = (a.B + 63) / 64, b0 = lane * seg;
-        int local = 0;
-        for (int k = 0; k < seg; ++k)
-            if (b0 + k < a.B) local += s_pref[b0 + k + 1];
-        int incl = local;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(incl, o);
-            if (lane >= o) incl += v;
-        }
-        int run = incl - local;
-        for (int k = 0; k < seg; ++k)
-            if (b0 + k < a.B) {
-                run += s_pref[b0 + k + 1];
-                s_pref[b0 + k + 1] = run;
-            }
-        if (lane == 0) s_pref[0] = 0;
-    }
+    if (tid < 64) prefix_sums(s_line, n);
     __syncthreads();
-    total = s_pref[a.B];
-    if (blockIdx.x == 0 && a.allow_split)
-        for (int b = tid; b <= a.B; b += NT) a.pf_sched[b] = s_pref[b];
 }
 
-// Merge of split items: a thread for each row and 8 columns.
+// An item that was cut, left by the worker that holds its start for the merge
+struct CutItem {
+    int pieces, b, mt, hk;
+};
+
+// Merge of the pieces of cut items: the first is the second slot of the worker that
+// left the item, the others the first slots of those after it. A thread for each row
+// and 8 columns.
 template <int DT, int HD, int BM>
-__global__ void __launch_bounds__(256) fa_quant_prefill_merge_kernel(QuantFwdArgs a, int mt_max) {
+__global__ void __launch_bounds__(256) fa_quant_prefill_merge_kernel(QuantFwdArgs a) {
     constexpr int DCH = HD / 8, RPB = 256 / DCH, BPT = BM / RPB;
-    const int blk = blockIdx.x % BPT, item = blockIdx.x / BPT;
-    const int hk = item % a.Hk, mt = item / a.Hk % mt_max, b = item / a.Hk / mt_max;
-    const int ns = a.pf_sched[a.B + 1 + b];
-    if (ns <= 1) return;
-    int sq = a.cu_q ? a.cu_q[b + 1] - a.cu_q[b] : a.Sq;
+    const int blk = blockIdx.x % BPT, w = blockIdx.x / BPT;
+    const CutItem c = reinterpret_cast<const CutItem*>(a.pf_cut)[w];
+    if (c.pieces == 0) return;
+    int sq = a.cu_q ? a.cu_q[c.b + 1] - a.cu_q[c.b] : a.Sq;
     sq = min(max(sq, 0), a.Sq);
-    const int rows = sq * a.g > a.dec_rows ? sq * a.g : 0, mt_b = (rows + BM - 1) / BM;
-    const int rr = blk * RPB + threadIdx.x / DCH, d0 = threadIdx.x % DCH * 8, r = mt * BM + rr;
-    if (mt >= mt_b || r >= rows) return;
-    const int w0 = a.pf_sched[b] + (mt_b - 1 - mt) * ns * a.Hk + hk;
+    const int rr = blk * RPB + threadIdx.x / DCH, d0 = threadIdx.x % DCH * 8, r = c.mt * BM + rr;
+    if (r >= sq * a.g) return;
+    auto row = [&](int s) { return (int64_t)(s == 0 ? 2 * w + 1 : 2 * (w + s)) * BM + rr; };
     float m = -INFINITY;
-    for (int s = 0; s < ns; ++s) m = fmaxf(m, a.pf_lse[(int64_t)(w0 + s * a.Hk) * BM + rr]);
+    for (int s = 0; s < c.pieces; ++s) m = fmaxf(m, a.pf_lse[row(s)]);
     f32x4 acc0 = {0.f, 0.f, 0.f, 0.f}, acc1 = acc0;
     float lse = INFINITY;
     if (m != -INFINITY) {
         float sum = 0.f;
-        for (int s = 0; s < ns; ++s) {
-            const int64_t prow = (int64_t)(w0 + s * a.Hk) * BM + rr;
-            const float wgt = fast_exp2((a.pf_lse[prow] - m) * kLog2e);
+        for (int s = 0; s < c.pieces; ++s) {
+            const float wgt = fast_exp2((a.pf_lse[row(s)] - m) * kLog2e);
             sum += wgt;
-            acc0 += *reinterpret_cast<const f32x4*>(a.pf_o + prow * HD + d0) * wgt;
-            acc1 += *reinterpret_cast<const f32x4*>(a.pf_o + prow * HD + d0 + 4) * wgt;
+            acc0 += *reinterpret_cast<const f32x4*>(a.pf_o + row(s) * HD + d0) * wgt;
+            acc1 += *reinterpret_cast<const f32x4*>(a.pf_o + row(s) * HD + d0 + 4) * wgt;
         }
         acc0 *= 1.f / sum;
         acc1 *= 1.f / sum;
         lse = m + fast_log2(sum) * kLn2;
     }
-    const int i = r / a.g, h = hk * a.g + r % a.g;
-    uint16_t* o = static_cast<uint16_t*>(a.out) + q_row(a, b, i, a.o_sb, a.o_si) + (int64_t)h * a.o_sh;
+    const int i = r / a.g, h = c.hk * a.g + r % a.g;
+    uint16_t* o = static_cast<uint16_t*>(a.out) + q_row(a, c.b, i, a.o_sb, a.o_si) + (int64_t)h * a.o_sh;
     if (d0 < a.hd)
         *reinterpret_cast<u32x4*>(o + d0) = u32x4{pack2<DT>(acc0[0], acc0[1]), pack2<DT>(acc0[2], acc0[3]),
                                                   pack2<DT>(acc1[0], acc1[1]), pack2<DT>(acc1[2], acc1[3])};
-    if (d0 == 0) a.lse[lse_at(a, b, h, i)] = lse;
+    if (d0 == 0) a.lse[lse_at(a, c.b, h, i)] = lse;
 }
 
 template <int DT, int HD, int BM>
-void launch_items_merge(const QuantFwdArgs& a, int mt_max, hipStream_t stream) {
-    if (!a.allow_split) return;
+void launch_items_merge(const QuantFwdArgs& a, int grid, hipStream_t stream) {
+    if (!a.cut) return;
     constexpr int RPB = 256 / (HD / 8);
-    hipLaunchKernelGGL((fa_quant_prefill_merge_kernel<DT, HD, BM>), dim3((unsigned)(a.B * mt_max * a.Hk * (BM / RPB))), dim3(256), 0,
-                       stream, a, mt_max);
+    hipLaunchKernelGGL((fa_quant_prefill_merge_kernel<DT, HD, BM>), dim3((unsigned)(grid * (BM / RPB))), dim3(256), 0, stream, a);
 }
 
 }  // namespace

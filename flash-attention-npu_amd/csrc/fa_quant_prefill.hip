@@ -1,8 +1,8 @@
 // fa_quant_prefill.hip -- attention over 8-bit codes for many query rows (prompts
 // and their chunks, speculated tokens of many heads).
 //
-// Rows of a work item are (query position, q head) pairs of one kv head; items with
-// few rows and long keys are cut over the keys and merged by a second launch. Eight
+// Rows of a work item are (query position, q head) pairs of one kv head; few or
+// ragged items are cut over the keys (fa_quant_items.h), the pieces merged by a second launch. Eight
 // waves (two per SIMD) of 16-row blocks share tiles of keys in LDS, double buffered,
 // one barrier a tile. The codes are widened to fp16 once, on their way into LDS, so the
 // products meet what 16-bit rows would give them: S^T = K.Q^T, whose accumulator
@@ -52,12 +52,11 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
     __shared__ int s_ok[2][NB], s_plain[2];
     __shared__ int64_t s_koff[2][NB], s_voff[2][NB];  // where its rows are; below 0: nowhere
     __shared__ int s_pref[kQuantMaxB + 1];
-    __shared__ long long s_red[NW];
+    __shared__ int64_t s_line[kQuantMaxB + 1];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int li = lane & 15, G = lane >> 4;
-    int total, chunk_auto;
-    build_list<BM, BN, NW>(a, s_pref, s_red, total, chunk_auto);
+    build_list<BM, BN, NW>(a, s_pref, s_line);
 
     auto swzk = [](int r, int c) { return HD == 64 ? swz_k64(r, c) : swz_k(r, c); };
     auto swzv = [](int r, int c) { return HD == 64 ? swz_v64(r, c) : swz_v(r, c); };
@@ -79,32 +78,65 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
         return *(const QuantFwdArgs*)p;
     };
 
-    for (int k = 0; k * (int)gridDim.x < total; ++k) {
-        // items are numbered heaviest first within a sequence; odd passes run the other way
-        const int w = k * (int)gridDim.x + ((k & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
-        if (w >= total) continue;
-        int bl = 0, bh = a.B;
-        while (bh - bl > 1) {
-            const int mid = (bl + bh) >> 1;
-            if (s_pref[mid] <= w) bl = mid;
-            else bh = mid;
+    const int entries = s_pref[a.B], grid = (int)gridDim.x;
+    Line line{};
+    int worker = blockIdx.x;
+    int64_t at = 0, end;  // places on the line, or numbers of whole items
+    if (a.cut) {
+        line.len = s_line[min(entries, kQuantMaxB)];
+        line.total = line.len * a.Hk;
+        line.workers = (int)min((int64_t)grid, max((int64_t)1, line.total / kLeast));
+        // all at work: neighbours on the line, who read the same keys, share an XCD's L2
+        if (line.workers == grid && grid % 8 == 0) worker = worker % 8 * (grid / 8) + worker / 8;
+        if (tid == 0) reinterpret_cast<CutItem*>(a.pf_cut)[worker] = CutItem{0, 0, 0, 0};
+        end = 0;
+        if (line.total > 0 && worker < line.workers) {
+            at = line.cut(worker);
+            end = line.cut(worker + 1);
         }
-        const int b = bl, g = a.g;
+    } else {
+        end = (entries * (int64_t)a.Hk + grid - 1) / grid;
+    }
+
+    while (at < end) {
+        int e, hk, t_lo = 0, t_hi = 0x7fffffff, slot = -1;  // tiles and slot of a piece
+        const int g = a.g;
+        if (a.cut) {
+            hk = (int)(at / line.len);
+            const int64_t p0 = hk * line.len;
+            e = find_in(s_line, min(entries, kQuantMaxB), at - p0);
+        } else {
+            // items are numbered heaviest first within a sequence; odd passes run the other way
+            const int64_t w = at * grid + ((at & 1) ? grid - 1 - (int)blockIdx.x : (int)blockIdx.x);
+            ++at;
+            if (w >= entries * (int64_t)a.Hk) continue;
+            hk = (int)(w % a.Hk);
+            e = (int)(w / a.Hk);
+        }
+        const int b = find_in(s_pref, a.B, e);
         const Rows R = rows_of<BM>(a, b);
-        int ns, chunk;
-        split_of(a, R.q.hi - R.q.lo, chunk_auto, ns, chunk);
-        const int local = w - s_pref[b];
-        const int hk = local % a.Hk, split = local / a.Hk % ns, mt = R.mt - 1 - local / a.Hk / ns;
+        const int mt = a.cut ? e - s_pref[b] : s_pref[b + 1] - 1 - e;
         const int diag0 = R.q.sk - R.q.sq;
-        const int row0 = mt * BM, item_rows = min(BM, R.rows - row0);
-        int k_lo = max(0, key_lo(row0 / g + diag0, a.wl, 0));
-        int k_hi = min(R.q.sk, key_hi((row0 + item_rows - 1) / g + diag0, a.wr, 0) + 1);
-        if (ns > 1) {
-            k_lo = max(k_lo, R.q.lo + split * chunk);
-            k_hi = min(k_hi, R.q.lo + (split + 1) * chunk);
+        const int row0 = mt * BM;
+        const Keys K = keys_of(a, R.q, row0, min(BM, R.rows - row0));
+        int k_lo = K.lo, k_hi = K.hi;
+        if (a.cut) {
+            const int64_t p0 = hk * line.len + s_line[e], p1 = hk * line.len + s_line[e + 1], upto = min(end, p1);
+            const int cost = tile_cost<BM, BM / NW>(R.rows, mt);
+            if (at > p0) t_lo = max(0, (int)((at - p0 - kStart) / cost));
+            if (upto < p1) t_hi = max(0, (int)((upto - p0 - kStart) / cost));
+            if (at > p0 || upto < p1) {
+                slot = at > p0 ? 2 * worker : 2 * worker + 1;
+                if (at == p0 && tid == 0)
+                    reinterpret_cast<CutItem*>(a.pf_cut)[worker] = CutItem{line.holder(p1 - 1) - worker + 1, b, mt, hk};
+                const int base = k_lo & ~15;
+                if (t_hi < tiles_of<BN>(K)) k_hi = min(k_hi, base + t_hi * BN);
+                k_lo = max(k_lo, base + t_lo * BN);
+                k_hi = max(k_hi, k_lo);
+            }
+            at = upto;
         }
-        k_hi = max(k_hi, k_lo);
-        const int base = k_lo & ~15;  // tiles start at a block of 16 keys
+        const int base = k_lo & ~15;
         const int ntiles = (k_hi - base + BN - 1) / BN;
 
         const int wrow0 = row0 + wave * RB * 16, wrows = min(RB * 16, R.rows - wrow0);
@@ -389,7 +421,7 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
             const float inv = some ? back / l : 0.f;
             const float lse = some ? (m_run[rb] + fast_log2(l)) * kLn2 : INFINITY;
             if (r >= R.rows) continue;
-            if (ns == 1) {
+            if (slot < 0) {
                 const int i = r / g, h = hk * g + r % g;
                 uint16_t* o = static_cast<uint16_t*>(a.out) + q_row(a, b, i, a.o_sb, a.o_si) + (int64_t)h * a.o_sh;
 #pragma unroll
@@ -400,7 +432,7 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
                 }
                 if (G == 0) a.lse[lse_at(a, b, h, i)] = lse;
             } else {
-                const int64_t prow = (int64_t)w * BM + (r - row0);
+                const int64_t prow = (int64_t)slot * BM + (r - row0);
 #pragma unroll
                 for (int db = 0; db < DBLK; ++db)
                     *reinterpret_cast<f32x4*>(a.pf_o + prow * HD + 16 * db + 4 * G) = oacc[rb][db] * inv;
@@ -411,20 +443,20 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
 }
 
 template <int DT, int CT, int HD, int RB>
-void launch_r(const QuantFwdArgs& a, int grid, int mt_max, hipStream_t stream) {
+void launch_r(const QuantFwdArgs& a, int grid, hipStream_t stream) {
     if (a.softcap > 0.f) hipLaunchKernelGGL((fa_quant_prefill_kernel<DT, CT, HD, RB, true>), dim3(grid), dim3(NT), 0, stream, a);
     else hipLaunchKernelGGL((fa_quant_prefill_kernel<DT, CT, HD, RB, false>), dim3(grid), dim3(NT), 0, stream, a);
-    launch_items_merge<DT, HD, Cfg<HD, RB>::BM>(a, mt_max, stream);
+    launch_items_merge<DT, HD, Cfg<HD, RB>::BM>(a, grid, stream);
 }
 
 template <int HD, int RB>
-void launch_c(const QuantFwdArgs& a, int ct, int grid, int mt_max, hipStream_t stream) {
+void launch_c(const QuantFwdArgs& a, int ct, int grid, hipStream_t stream) {
     if (a.bf16) {
-        if (ct == CT_INT8) launch_r<DT_BF16, CT_INT8, HD, RB>(a, grid, mt_max, stream);
-        else launch_r<DT_BF16, CT_E4M3, HD, RB>(a, grid, mt_max, stream);
+        if (ct == CT_INT8) launch_r<DT_BF16, CT_INT8, HD, RB>(a, grid, stream);
+        else launch_r<DT_BF16, CT_E4M3, HD, RB>(a, grid, stream);
     } else {
-        if (ct == CT_INT8) launch_r<DT_FP16, CT_INT8, HD, RB>(a, grid, mt_max, stream);
-        else launch_r<DT_FP16, CT_E4M3, HD, RB>(a, grid, mt_max, stream);
+        if (ct == CT_INT8) launch_r<DT_FP16, CT_INT8, HD, RB>(a, grid, stream);
+        else launch_r<DT_FP16, CT_E4M3, HD, RB>(a, grid, stream);
     }
 }
 
@@ -432,14 +464,13 @@ void launch_c(const QuantFwdArgs& a, int ct, int grid, int mt_max, hipStream_t s
 
 // Rows of an item: 128, or as many as the registers take where sequences have them.
 int quant_prefill_rows(int kd, bool many) { return many && kd < 256 ? 256 : 128; }
-int quant_prefill_keys(int kd) { return 8192 / kd; }
 
-hipError_t launch_quant_prefill(const QuantFwdArgs& a, int ct, int kd, int rows, int grid, int mt_max, hipStream_t stream) {
-    if (kd == 64 && rows == 256) launch_c<64, 2>(a, ct, grid, mt_max, stream);
-    else if (kd == 64) launch_c<64, 1>(a, ct, grid, mt_max, stream);
-    else if (kd == 128 && rows == 256) launch_c<128, 2>(a, ct, grid, mt_max, stream);
-    else if (kd == 128) launch_c<128, 1>(a, ct, grid, mt_max, stream);
-    else launch_c<256, 1>(a, ct, grid, mt_max, stream);
+hipError_t launch_quant_prefill(const QuantFwdArgs& a, int ct, int kd, int rows, int grid, hipStream_t stream) {
+    if (kd == 64 && rows == 256) launch_c<64, 2>(a, ct, grid, stream);
+    else if (kd == 64) launch_c<64, 1>(a, ct, grid, stream);
+    else if (kd == 128 && rows == 256) launch_c<128, 2>(a, ct, grid, stream);
+    else if (kd == 128) launch_c<128, 1>(a, ct, grid, stream);
+    else launch_c<256, 1>(a, ct, grid, stream);
     return hipGetLastError();
 }
 
