@@ -62,6 +62,7 @@ SRC_FLAGS = {
     "fa_bwd_dq.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "fa_bwd_kv.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "fa_quant_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "fa_quant_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "fa_fwd.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"],
 }
 

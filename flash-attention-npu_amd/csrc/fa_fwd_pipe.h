@@ -34,13 +34,6 @@ namespace pipe {
 constexpr int NT = 256, NBUF = 4;
 constexpr float kLazy = 8.f;  // log2 headroom before the running maximum moves
 
-// Slot of chunk c in row r: fa_pipe.h's; 128-byte rows (two to a line of LDS
-// banks) take theirs from the row pair, conflict free for the same reads.
-template <int ROW>
-__device__ __forceinline__ int slot_of(int r, int c) {
-    return ROW == 128 ? c ^ ((((r >> 1) & 1) << 2) | ((r >> 2) & 3)) : swz(r, c);
-}
-
 // EB: bytes per element of q, K and V
 template <int HD, int RBLK, int EB>
 struct PipeCfg {

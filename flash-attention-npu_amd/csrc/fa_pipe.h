@@ -34,6 +34,13 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
 // one chunk of 32 rows and for the transpose reads of 4 rows x 4 chunks.
 __device__ __forceinline__ int swz(int r, int c) { return c ^ (((r & 3) << 2) | ((r >> 2) & 3)); }
 
+// The same for rows of ROW bytes: 128-byte rows (two to a line of LDS
+// banks) take theirs from the row pair, conflict free for the same reads.
+template <int ROW>
+__device__ __forceinline__ int slot_of(int r, int c) {
+    return ROW == 128 ? c ^ ((((r >> 1) & 1) << 2) | ((r >> 2) & 3)) : swz(r, c);
+}
+
 __device__ __forceinline__ u32x4 tr_read(unsigned lo, unsigned hi) {
     const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(size_t)lo));
     const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(size_t)hi));

@@ -79,11 +79,11 @@ __device__ __forceinline__ int find_in(const T* s, int n, X x) {  // the last i 
 // The list: an entry is a tile of BM rows of a sequence, an item an entry of one kv
 // head. Every workgroup makes the list alike, in LDS.
 //
-// Few items, or ragged ones, are cut: laid end to end, head after head, their costs
+// Ragged items, or few, are cut: laid end to end, head after head, their costs
 // make a line that the workgroups share evenly, so one piece begins and one ends
-// inside an item at most. An item costs kStart and for each tile of keys kTile and one
-// for each wave with rows; a workgroup takes at least kLeast.
-constexpr int kStart = 24, kTile = 4, kLeast = 72;
+// inside an item at most. Costs are in units of 32 keys: an item takes kStart more than
+// its tiles of keys, and a workgroup takes at least kLeast.
+constexpr int kStart = 16, kLeast = 48;
 
 struct Line {
     int64_t len;   // of one head
@@ -93,11 +93,6 @@ struct Line {
     // the worker that holds place x: the last w with cut(w) <= x
     __device__ int holder(int64_t x) const { return (int)(((x + 1) * workers - 1) / total); }
 };
-
-template <int BM, int WROWS>
-__device__ __forceinline__ int tile_cost(int rows, int mt) {
-    return kTile + (min(BM, rows - mt * BM) + WROWS - 1) / WROWS;
-}
 
 template <int BM, int BN, int NW>
 __device__ void build_list(const QuantFwdArgs& a, int* s_pref, int64_t* s_line) {
@@ -114,7 +109,7 @@ __device__ void build_list(const QuantFwdArgs& a, int* s_pref, int64_t* s_line) 
         const Rows r = rows_of<BM>(a, b);
         const int mt = e - s_pref[b];
         const Keys k = keys_of(a, r.q, mt * BM, min(BM, r.rows - mt * BM));
-        s_line[e + 1] = kStart + (int64_t)tiles_of<BN>(k) * tile_cost<BM, BM / NW>(r.rows, mt);
+        s_line[e + 1] = kStart + (int64_t)tiles_of<BN>(k) * (BN / 32);
     }
     __syncthreads();
     if (tid < 64) prefix_sums(s_line, n);

@@ -2,17 +2,25 @@
 // and their chunks, speculated tokens of many heads).
 //
 // Rows of a work item are (query position, q head) pairs of one kv head; few or
-// ragged items are cut over the keys (fa_quant_items.h), the pieces merged by a second launch. Eight
-// waves (two per SIMD) of 16-row blocks share tiles of keys in LDS, double buffered,
-// one barrier a tile. The codes are widened to fp16 once, on their way into LDS, so the
-// products meet what 16-bit rows would give them: S^T = K.Q^T, whose accumulator
-// holds the P^T operand of O^T = V^T.P^T, V^T by transpose reads. Page ids are read a
-// tile ahead of the rows that they lead to.
-//
-// K's scale multiplies the scores of its 16 keys; V's the weights, kept relative to a
-// running power of two (fa_quant_decode.hip). The running maximum is lazy: it moves
-// only where a new score exceeds it by 2^4, and the weights' unit leaves room for that
-// (2^10 in place of 2^14: a weight keeps its 11 bits as long as p t / R > 2^-24).
+// ragged items are cut over the keys (fa_quant_items.h), the pieces merged by a
+// second launch. Four waves, one per SIMD, of RB x 32 rows.
+//   * A tile's codes go from memory straight into LDS, two tiles before they are
+//     widened to fp16 there, once for all rows, so the products meet what 16-bit rows
+//     would give them.
+//   * Per 32 keys a wave forms S^T = K.Q^T and O^T += V^T.P^T with 32x32x16 MFMA: a
+//     lane holds one row and 16 keys, which is the packed P^T operand; V^T by transpose
+//     reads. While the softmax of 32 keys runs, the scores of the next 32 are formed,
+//     and their maximum is taken under the P.V products, in slots of one MFMA and a
+//     share of the vector work (unit()).
+//   * K's scale multiplies the scores of its 16 keys. V's multiplies the weights, kept
+//     relative to a running power of two R (fa_quant_decode.hip): as its log2 in the
+//     exponential's argument, so that the weight comes out whole; the row's sum takes it
+//     back once for a block. The running maximum is lazy: it moves only where a
+//     new score exceeds it by 2^4, and the weights' unit leaves room for that
+//     (2^10 in place of 2^14: a weight keeps its 11 bits as long as p t / R > 2^-24).
+//   * Tiles with masked keys, pages outside the cache or scales that are not plain
+//     positive numbers go through a second copy of the unit, which scales the scores
+//     as they are formed and multiplies the weights by V's scale.
 #include "fa_pipe.h"
 #include "fa_quant_items.h"
 
@@ -22,56 +30,77 @@ namespace fa {
 
 namespace {
 
-constexpr int NW = 8, NT = NW * 64;
+constexpr int NW = 4, NT = NW * 64, NBUF = 3;
 constexpr float kLazy = 4.f;
 constexpr int kUnit = 10;  // w = p t / R 2^kUnit, p <= 2^kLazy
 
 template <int HD, int RB_>
 struct Cfg {
-    static constexpr int RB = RB_;                                 // 16-row blocks of a wave
-    static constexpr int BM = NW * RB * 16;                        // rows of a work item
-    static constexpr int BN = 8192 / HD;                           // keys of a tile: 16 codes per thread
-    static constexpr int NB = BN / 16;
-    static constexpr int DCH = HD / 16;                            // 16-code chunks of a row
-    static constexpr int KSTEPS = HD / 32;
-    static constexpr int DBLK = HD / 16;
-    static constexpr int VPRE = HD == 64 ? 4 : 8;                  // V^T operands read ahead of the softmax
+    static constexpr int RB = RB_;             // 32-row blocks of a wave
+    static constexpr int BM = NW * RB * 32;    // rows of a work item
+    static constexpr int ROW = 2 * HD;         // bytes of a widened row
+    static constexpr int NH = 512 / ROW;       // 32-key units of a tile
+    static constexpr int BN = 32 * NH;         // keys of a tile: 32 codes of K and of V per thread
+    static constexpr int NB = BN / 16;         // blocks of 16 keys of a tile
+    static constexpr int TPG = 64 / NB;        // tiles of a group: its blocks are a wave's lanes
+    static constexpr int KS = HD / 16;         // K operands of a unit
+    static constexpr int DB = HD / 32;         // 32-dim blocks of O
+    static constexpr int DCH = HD / 16;        // 16-code chunks of a row
+    static constexpr int KT = BN * ROW;        // bytes of a tile of K (or V) in LDS
+    static constexpr int TILE = 2 * KT;
 };
+
+// 16 bytes per lane from each of four bases (k, k, v, v) + off to LDS address lds + 1024 u
+// + 16 lane; the wait states are fa_pipe.h's. b<u> is 1024 u less than the base.
+__device__ __forceinline__ void dma16_kkvv(unsigned lds, uint64_t b0, uint64_t b1, uint64_t b2, uint64_t b3, unsigned koff,
+                                           unsigned voff) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 3\n\t"
+        "global_load_lds_dwordx4 %5, %1\n\t"
+        "global_load_lds_dwordx4 %5, %2 offset:1024\n\t"
+        "global_load_lds_dwordx4 %6, %3 offset:2048\n\t"
+        "global_load_lds_dwordx4 %6, %4 offset:3072" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "s"(b0), "s"(b1), "s"(b2), "s"(b3),
+        "v"(koff), "v"(voff)
+        : "memory", "m0");
+}
+
+// x y, and 0 where x is 0, whatever y
+__device__ __forceinline__ float mul_or_0(float x, float y) {
+    float r;
+    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "s"(y), "v"(x));
+    return r;
+}
 
 // CAP: soft cap
 template <int DT, int CT, int HD, int RB_, bool CAP>
 __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a) {
     using C = Cfg<HD, RB_>;
-    constexpr int RB = C::RB, BM = C::BM, BN = C::BN, NB = C::NB, DCH = C::DCH, KSTEPS = C::KSTEPS, DBLK = C::DBLK,
-                  VPRE = C::VPRE;
-    __shared__ __attribute__((aligned(16))) uint16_t s_k[2][BN * HD];
-    __shared__ __attribute__((aligned(16))) uint16_t s_v[2][BN * HD];
-    // of the blocks of 16 keys: K scale; V scale, its log2 and inverse; whether the page
-    // is in the cache; of the tile: whether the softmax scale and all of these are positive
-    __shared__ float s_ks[2][NB], s_vs[2][NB], s_lv[2][NB], s_iv[2][NB];
-    __shared__ int s_ok[2][NB], s_plain[2];
-    __shared__ int64_t s_koff[2][NB], s_voff[2][NB];  // where its rows are; below 0: nowhere
+    constexpr int RB = C::RB, BM = C::BM, BN = C::BN, NB = C::NB, TPG = C::TPG, NH = C::NH, KS = C::KS, DB = C::DB, DCH = C::DCH, ROW = C::ROW,
+                  KT = C::KT, TILE = C::TILE, NE = 16 * RB;
+    // slots: S products, then the P.V products of the first and the last 16 keys
+    constexpr int SS = KS * RB, SP = DB * RB;
+    __shared__ __attribute__((aligned(256))) char s_t[NBUF * TILE];
+    __shared__ __attribute__((aligned(256))) char s_raw[2 * NT * 64];  // codes of two tiles, each thread's own
     __shared__ int s_pref[kQuantMaxB + 1];
     __shared__ int64_t s_line[kQuantMaxB + 1];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int li = lane & 15, G = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, hi = lane >> 5;
     build_list<BM, BN, NW>(a, s_pref, s_line);
 
-    auto swzk = [](int r, int c) { return HD == 64 ? swz_k64(r, c) : swz_k(r, c); };
-    auto swzv = [](int r, int c) { return HD == 64 ? swz_v64(r, c) : swz_v(r, c); };
-    int offk[KSTEPS], offv[DBLK];
-#pragma unroll
-    for (int s = 0; s < KSTEPS; ++s) offk[s] = li * HD + (swzk(li, 4 * s + G) << 3);
-    const int r4 = li >> 2, c4 = li & 3;
-#pragma unroll
-    for (int db = 0; db < DBLK; ++db)
-        offv[db] = (4 * G + r4) * HD + (swzv(4 * G + r4, 2 * db + (c4 >> 1)) << 3) + (c4 & 1) * 4;
-    // this thread's part of a tile: 16 codes of one row of K and of V
+    const unsigned lds0 = lds_addr(s_t);
+    const unsigned rowa = lds0 + col * ROW + (slot_of<ROW>(col, hi) << 4);  // chunk 2s + hi: ^ (s << 5)
+    const int tr_r = 4 * hi + ((lane & 15) >> 2), tr_c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    const unsigned tra = lds0 + KT + (lane & 1) * 8 + tr_r * ROW + (slot_of<ROW>(tr_r, tr_c) << 4);  // dim block db: ^ (db << 6)
+    // This thread's part of a tile: of K and of V the 16 codes of chunk dch of rows kk
+    // and kk + NT / DCH. A wave's rows of either lie in one block of 16 keys.
     const int kk = tid / DCH, dch = tid % DCH;
-    const bool in = dch * 16 < a.hd;
+    const bool in = dch * 16 < a.hd, full = a.hd == HD;
     const uint32_t kin = (uint32_t)(kk & 15) * (uint32_t)a.k_si + (in ? dch * 16 : 0);
     const uint32_t vin = (uint32_t)(kk & 15) * (uint32_t)a.v_si + (in ? dch * 16 : 0);
+    const unsigned put0 = lds0 + kk * ROW + (slot_of<ROW>(kk, 2 * dch) << 4), put1 = lds0 + kk * ROW + (slot_of<ROW>(kk, 2 * dch + 1) << 4);
+    const unsigned raw = __builtin_amdgcn_readfirstlane(lds_addr(s_raw)) + wave * 4096;
+    auto block_of = [&](int u) { return (u * (NT / DCH) + wave * (64 / DCH)) >> 4; };
     auto anew = []() -> const QuantFwdArgs& {  // as in fa_quant_decode.hip
         auto p = __builtin_amdgcn_kernarg_segment_ptr();
         asm volatile("" : "+s"(p));
@@ -103,8 +132,7 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
         const int g = a.g;
         if (a.cut) {
             hk = (int)(at / line.len);
-            const int64_t p0 = hk * line.len;
-            e = find_in(s_line, min(entries, kQuantMaxB), at - p0);
+            e = find_in(s_line, min(entries, kQuantMaxB), at - hk * line.len);
         } else {
             // items are numbered heaviest first within a sequence; odd passes run the other way
             const int64_t w = at * grid + ((at & 1) ? grid - 1 - (int)blockIdx.x : (int)blockIdx.x);
@@ -113,18 +141,19 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
             hk = (int)(w % a.Hk);
             e = (int)(w / a.Hk);
         }
-        const int b = find_in(s_pref, a.B, e);
+        hk = __builtin_amdgcn_readfirstlane(hk);
+        e = __builtin_amdgcn_readfirstlane(e);
+        const int b = __builtin_amdgcn_readfirstlane(find_in(s_pref, a.B, e));
         const Rows R = rows_of<BM>(a, b);
-        const int mt = a.cut ? e - s_pref[b] : s_pref[b + 1] - 1 - e;
+        const int mt = __builtin_amdgcn_readfirstlane(a.cut ? e - s_pref[b] : s_pref[b + 1] - 1 - e);
         const int diag0 = R.q.sk - R.q.sq;
-        const int row0 = mt * BM;
-        const Keys K = keys_of(a, R.q, row0, min(BM, R.rows - row0));
+        const int row0 = mt * BM, item_rows = min(BM, R.rows - row0);
+        const Keys K = keys_of(a, R.q, row0, item_rows);
         int k_lo = K.lo, k_hi = K.hi;
         if (a.cut) {
             const int64_t p0 = hk * line.len + s_line[e], p1 = hk * line.len + s_line[e + 1], upto = min(end, p1);
-            const int cost = tile_cost<BM, BM / NW>(R.rows, mt);
-            if (at > p0) t_lo = max(0, (int)((at - p0 - kStart) / cost));
-            if (upto < p1) t_hi = max(0, (int)((upto - p0 - kStart) / cost));
+            if (at > p0) t_lo = max(0, (int)((at - p0 - kStart) / NH));
+            if (upto < p1) t_hi = max(0, (int)((upto - p0 - kStart) / NH));
             if (at > p0 || upto < p1) {
                 slot = at > p0 ? 2 * worker : 2 * worker + 1;
                 if (at == p0 && tid == 0)
@@ -136,307 +165,516 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
             }
             at = upto;
         }
-        const int base = k_lo & ~15;
+        k_lo = __builtin_amdgcn_readfirstlane(k_lo);
+        k_hi = __builtin_amdgcn_readfirstlane(k_hi);
+        slot = __builtin_amdgcn_readfirstlane(slot);
+        const int base = k_lo & ~15;  // tiles start at a block of 16 keys
         const int ntiles = (k_hi - base + BN - 1) / BN;
-
-        const int wrow0 = row0 + wave * RB * 16, wrows = min(RB * 16, R.rows - wrow0);
-        const bool live = wrows > 0;
-        const int i_lo = live ? wrow0 / g : 0, i_hi = live ? (wrow0 + wrows - 1) / g : 0;
-        const int w_lo = max(k_lo, key_lo(i_lo + diag0, a.wl, 0)), w_hi = min(k_hi - 1, key_hi(i_hi + diag0, a.wr, 0));
-        const int f_lo = max(k_lo, key_lo(i_hi + diag0, a.wl, 0)), f_hi = min(k_hi - 1, key_hi(i_lo + diag0, a.wr, 0));
+        // tiles all of whose keys are visible to all rows: [t1, t2)
+        const int i_lo = row0 / g, i_hi = (row0 + item_rows - 1) / g;
+        const int f_lo = max(k_lo, key_lo(i_hi + diag0, a.wl, 0)), f_hi = min(k_hi, key_hi(i_lo + diag0, a.wr, 0) + 1);
+        const int t1 = min(ntiles, (f_lo - base + BN - 1) / BN), t2 = max(t1, (f_hi - base) / BN);
 
         // ---- tiles: registers -> widened -> LDS ---------------------------------------------
-        // The blocks of 16 keys of a tile are looked after by the first NB lanes of the
-        // last wave, which causal items leave idle soonest: page id, three tiles ahead
-        // of the products; rows' place and scales, two tiles; all others read the place.
+        // The lanes of every wave look after a group of 64 blocks of 16 keys: where their
+        // rows are and their scales. Page ids are read a group ahead.
         const int* trow = a.table ? a.table + (int64_t)R.q.crow * a.t_stride : nullptr;
-        const bool keeper = tid >= NT - 64 && tid < NT - 64 + NB;
-        int bid = -1, binp = 0;
-        float bks = 0.f, bvs = 0.f;
-        bool bok = false;
-        auto block_id = [&](int t) {
+        constexpr int kNoKeys = -0x7fffffff - 1;  // page of a block past the item's keys
+        const float low = 0x1p-97f;               // no R is below it
+        struct Scales {
+            float k, v;
+            uint64_t ok, odd;  // blocks whose page is in the cache; those whose scales are not plain
+        };
+        Scales sc, sc_new;      // of the group at hand, and of the next once asked for
+        sc_new = Scales{1.f, low, 0, 0};
+        float lv = 0.f, iv_ = 0.f, wv_ = 0.f;  // of sc.v against R: log2, inverse, ratio
+        int64_t ko = 0, vo = 0;  // where the blocks of the group asked for are
+        uint64_t have = 0;       // its sc.ok
+        int id_page, id_row;
+        auto group_ids = [&](int gr) {
             const QuantFwdArgs& A = anew();
-            const int j = base + t * BN + lane * 16;
-            bid = -1;
-            binp = 0;
-            if (j < k_hi && j + 16 > k_lo) {
+            const int64_t j = base + ((int64_t)gr * 64 + lane) * 16;
+            id_page = kNoKeys;
+            id_row = 0;
+            if (j < k_hi) {
                 const int pi = trow ? (int)udiv(A.page, (uint32_t)j) : 0;
-                binp = j - pi * A.page_size;
-                bid = trow ? trow[pi] : R.q.crow;
+                id_row = (int)j - pi * A.page_size;
+                id_page = trow ? trow[pi] : R.q.crow;
             }
         };
-        auto block_place = [&](int t) {
+        auto group_places = [&](Scales& s) {
             const QuantFwdArgs& A = anew();
-            bok = bid >= 0 && bid < A.num_pages;
-            const int64_t p = bok ? bid : 0, r = bok ? binp : 0;
-            s_koff[t & 1][lane] = bok ? p * A.k_sp + r * A.k_si : -1;
-            s_voff[t & 1][lane] = p * A.v_sp + r * A.v_si;
-            const int64_t sb = udiv(A.sblk, (uint32_t)r);
-            bks = A.ks[p * A.ks_sp + sb * A.ks_sb + (int64_t)hk * A.ks_sh];
-            bvs = A.vs[p * A.vs_sp + sb * A.vs_sb + (int64_t)hk * A.vs_sh];
-        };
-        const uint8_t* kbase = a.k + (int64_t)hk * a.k_sh;
-        const uint8_t* vbase = a.v + (int64_t)hk * a.v_sh;
-        u32x4 kr, vr;
-        auto load_tile = [&](int t) {
-            const int64_t ko = s_koff[t & 1][kk >> 4], vo = s_voff[t & 1][kk >> 4];
-            const int j = base + t * BN + kk;
-            const bool ok = ko >= 0 && j >= k_lo && j < k_hi && in;
-            kr = u32x4{0u, 0u, 0u, 0u};
-            vr = kr;
+            const bool ok = id_page >= 0 && id_page < A.num_pages;
+            const int64_t p = ok ? id_page : 0, r = ok ? id_row : 0;
+            // less what load u (K) and 2 + u (V) of the block add
+            const int u = lane % NB / (NB / 2);
+            ko = (int64_t)(A.k + ((int64_t)hk * A.k_sh + p * A.k_sp + r * A.k_si)) - 1024 * u;
+            vo = (int64_t)(A.v + ((int64_t)hk * A.v_sh + p * A.v_sp + r * A.v_si)) - 1024 * (2 + u);
+            s.k = id_page == kNoKeys ? 1.f : 0.f;  // (0: not plain)
+            s.v = low;
             if (ok) {
-                kr = *reinterpret_cast<const u32x4*>(kbase + ko + kin);
-                vr = *reinterpret_cast<const u32x4*>(vbase + vo + vin);
+                const int64_t sb = udiv(A.sblk, (uint32_t)r);
+                s.k = A.ks[p * A.ks_sp + sb * A.ks_sb + (int64_t)hk * A.ks_sh];
+                s.v = A.vs[p * A.vs_sp + sb * A.vs_sb + (int64_t)hk * A.vs_sh];
             }
+            have = s.ok = __ballot(ok);
         };
-        auto store_tile = [&](int buf) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const u32x2 k0 = widen4<CT>(kr[2 * u]), k1 = widen4<CT>(kr[2 * u + 1]);
-                const u32x2 v0 = widen4<CT>(vr[2 * u]), v1 = widen4<CT>(vr[2 * u + 1]);
-                *reinterpret_cast<u32x4*>(&s_k[buf][kk * HD + (swzk(kk & 15, 2 * dch + u) << 3)]) = u32x4{k0[0], k0[1], k1[0], k1[1]};
-                *reinterpret_cast<u32x4*>(&s_v[buf][kk * HD + (swzv(kk & 15, 2 * dch + u) << 3)]) = u32x4{v0[0], v0[1], v1[0], v1[1]};
-            }
-            if (keeper) {
-                s_ks[buf][lane] = bok ? bks : 0.f;
-                s_vs[buf][lane] = bok ? bvs : 0.f;
-                s_lv[buf][lane] = fast_log2(bvs);
-                s_iv[buf][lane] = 1.f / bvs;
-                s_ok[buf][lane] = bok;
-                const unsigned long long odd = __ballot(!bok || !(anew().scale > 0.f && bks > 0.f && bks < INFINITY && bvs > 0x1p-100f && bvs < 0x1p100f));
-                if (lane == 0) s_plain[buf] = odd == 0;
-            }
+        auto find_odd = [&](Scales& s) {
+            s.odd = __ballot(!(anew().scale > 0.f && s.k > 0.f && s.k < INFINITY && s.v > 0x1p-100f && s.v < 0x1p100f));
         };
-        // the tiles of the item before are read by all when the first barrier is passed
-        __syncthreads();
-        if (ntiles > 0 && keeper) {
-            block_id(0);
-            block_place(0);
-            block_id(1);
-        }
-        __syncthreads();
-        if (ntiles > 0) load_tile(0);
-
-        // ---- Q --------------------------------------------------------------------------------
-        u32x4 qreg[RB][KSTEPS];
-        float qs[RB];
-        int rlo[RB], rhi[RB];
+        // Rows outside the item, blocks of pages outside the cache and columns past the
+        // head dim are read where there is memory, and put down as 0.
+        constexpr uint64_t kTileBlocks = ((uint64_t)1 << NB) - 1;
+        bool part_a = false, part_b = false;  // the two tiles asked for: whether they have such
+        uint64_t have_a = 0, have_b = 0;
+        auto ask = [&](int t, int tg) {  // tg: the tile's number in its group
+            auto from = [&](int64_t o, int u) {
+                const int bl = tg * NB + block_of(u);
+                return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(o >> 32), bl) << 32 |
+                       (uint32_t)__builtin_amdgcn_readlane((int)o, bl);
+            };
+            part_a = part_b;
+            have_a = have_b;
+            have_b = have >> (tg * NB);
+            part_b = base + t * BN < k_lo || base + (t + 1) * BN > k_hi || !full || (have_b & kTileBlocks) != kTileBlocks;
+            dma16_kkvv(raw + (t & 1) * (NT * 64), from(ko, 0), from(ko, 1), from(vo, 0), from(vo, 1), kin, vin);
+        };
+        u32x4 got[2];
+        auto get_part = [&](int t, int part) {  // part 0 .. 3: K of u = 0, 1, then V
+            got[part & 1] = row_read(raw + (t & 1) * (NT * 64) + part * 1024 + lane * 16);
+        };
+        auto put_part = [&](int t, int part, unsigned tile) {
+            u32x4 x = got[part & 1];
+            const int u = part & 1;
+            if (part_a) {
+                const int j = base + t * BN + u * (NT / DCH) + kk;
+                if (!(in && j >= k_lo && j < k_hi && (have_a >> block_of(u) & 1))) x = u32x4{0u, 0u, 0u, 0u};
+            }
+            const unsigned to = tile + u * (NT / DCH) * ROW + (part >> 1) * KT;
+            const u32x2 c0 = widen4<CT>(x[0]), c1 = widen4<CT>(x[1]), c2 = widen4<CT>(x[2]), c3 = widen4<CT>(x[3]);
+            row_write(put0 + to, u32x4{c0[0], c0[1], c1[0], c1[1]});
+            row_write(put1 + to, u32x4{c2[0], c2[1], c3[0], c3[1]});
+        };
+        // the loads of an item's start in the order in which they are waited for
+        group_ids(0);
+        // ---- q as B operands: lane holds row col, chunks 2s + hi -------------------------------
+        const int wrow0 = row0 + wave * RB * 32;
+        u32x4 qreg[RB][KS];
+        int rlo[RB];       // the row's visible keys: the first, as offset from the item's first tile, and
+        unsigned rsee[RB]; // their number
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
-            const int r = wrow0 + rb * 16 + li;
+            const int r = wrow0 + rb * 32 + col;
             const bool ok = r < R.rows;
             const int i = ok ? r / g : 0, h = hk * g + (ok ? r % g : 0);
-            rlo[rb] = max(k_lo, key_lo(i + diag0, a.wl, 0));
-            rhi[rb] = min(k_hi - 1, key_hi(i + diag0, a.wr, 0));
-            const int64_t at = q_row(a, b, i, a.q_sb, a.q_si) + (int64_t)h * a.q_sh;
-            f32x8 x[KSTEPS];
+            const int first = max(k_lo, key_lo(i + diag0, a.wl, 0));
+            rlo[rb] = first - base - 4 * hi;
+            rsee[rb] = (unsigned)max(min(k_hi - 1, key_hi(i + diag0, a.wr, 0)) + 1 - first, 0);
+            const int64_t qat = q_row(a, b, i, a.q_sb, a.q_si) + (int64_t)h * a.q_sh;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int d = (2 * s + hi) * 8;
+                qreg[rb][s] = ok && d < a.hd ? *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + qat + d)
+                                             : u32x4{0u, 0u, 0u, 0u};
+            }
+        }
+        if (ntiles > 0) {
+            group_places(sc);
+            group_ids(1);
+            ask(0, 0);
+            ask(1, 1);
+        }
+        float qs[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
             float most = 0.f;
 #pragma unroll
-            for (int s = 0; s < KSTEPS; ++s) {
-                const int d = (4 * s + G) * 8;
-                x[s] = ok && d < a.hd ? load8<DT>(a.q, at + d) : f32x8{0, 0, 0, 0, 0, 0, 0, 0};
+            for (int s = 0; s < KS; ++s) {
+                const f32x8 x = widen8<DT>(qreg[rb][s]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[s][e]));
+                for (int e2 = 0; e2 < 8; ++e2) most = fmaxf(most, fabsf(x[e2]));
             }
-            const int sh = q_shift(wave_max16x4(most));
+            const int sh = q_shift(fmaxf(most, __shfl_xor(most, 32)));
             const float up = exp2i(sh);
             qs[rb] = exp2i(-sh) * a.scale * (CAP ? 1.f / a.softcap : kLog2e);
 #pragma unroll
-            for (int s = 0; s < KSTEPS; ++s) qreg[rb][s] = pack8<DT_FP16>(x[s] * up);
+            for (int s = 0; s < KS; ++s) {
+                qreg[rb][s] = pack8<DT_FP16>(widen8<DT>(qreg[rb][s]) * up);
+                asm volatile("" : "+a"(qreg[rb][s]));  // one tuple per operand, in accumulation registers
+            }
         }
-        f32x4 oacc[RB][DBLK];
-        float m_run[RB], l_run[RB];
+
+        if (ntiles > 0) {
+            wait_loads<0>();
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    get_part(t, x);
+                    put_part(t, x, t * TILE);
+                }
+                ask(t + 2, t + 2);
+            }
+        }
+
+        f32x16 o[RB][DB];
+        float m[RB], l[RB];
         int eR = 30;
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
-            m_run[rb] = -1e30f;  // finite: exp2(x - m) never forms inf - inf
-            l_run[rb] = 0.f;
+            m[rb] = -1e30f;  // finite floor: exp2(x - m) never forms inf - inf
+            l[rb] = 0.f;
 #pragma unroll
-            for (int db = 0; db < DBLK; ++db) oacc[rb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[rb][db][i] = 0.f;
         }
 
-        // 32 keys of the tile in buf, those at 32 hh. PLAIN: all rows see all of them and
-        // the scales are positive. Scores then stay as the products give them until
-        // the exponential's argument, and the V scale goes there too, as its log2, so
-        // that the weight comes out whole; the sum of p takes it back, once for a block.
-        auto tile = [&](int buf, int hh, int s0, auto plain_tag) {
-            constexpr bool PLAIN = decltype(plain_tag)::value;
-            f32x4 x[RB][2];
+        // LDS addresses of this lane's operands in the tile read next, moved on
+        // with the tile; opaque, so that the rest goes into the instructions' offsets
+        unsigned ra[KS], ta[DB], tb[DB];
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb) x[rb][0] = x[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < KS; ++s) ra[s] = rowa ^ (s << 5);
 #pragma unroll
-            for (int s = 0; s < KSTEPS; ++s)
+        for (int db = 0; db < DB; ++db) {
+            ta[db] = tra ^ (db << 6);
+            tb[db] = (tra ^ (db << 6) ^ 32) + 8 * ROW;
+        }
+        auto move_on = [&](unsigned& x, unsigned by) {
+            x += by;
+            asm volatile("" : "+v"(x));
+        };
+        u32x4 kop[KS], vop[2 * DB];
+        auto read_rows = [&](int h, int s) {  // operands s and s + 1
+            kop[s] = row_read(ra[s] + h * 32 * ROW);
+            kop[s + 1] = row_read(ra[s + 1] + h * 32 * ROW);
+        };
+        auto read_tr = [&](int h, int x) {  // x, x + 1: step of 16 keys, then dim block
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-                    const u32x4 av = *reinterpret_cast<const u32x4*>(&s_k[buf][offk[s] + (hh * 32 + kb * 16) * HD]);
-#pragma unroll
-                    for (int rb = 0; rb < RB; ++rb) x[rb][kb] = mfma_f16(av, qreg[rb][s], x[rb][kb]);
-                }
-            auto read_vt = [&](int db) {
-                const s16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)&s_v[buf][offv[db] + 32 * hh * HD]);
-                const s16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)&s_v[buf][offv[db] + (32 * hh + 16) * HD]);
-                const u32x2 l2 = __builtin_bit_cast(u32x2, lo4), h2 = __builtin_bit_cast(u32x2, hi4);
-                return u32x4{l2[0], l2[1], h2[0], h2[1]};
-            };
-            u32x4 vt[VPRE];
-#pragma unroll
-            for (int db = 0; db < VPRE; ++db) vt[db] = read_vt(db);
-            const float ks[2] = {s_ks[buf][2 * hh], s_ks[buf][2 * hh + 1]};
-            float vs[2] = {s_vs[buf][2 * hh], s_vs[buf][2 * hh + 1]};
-            const float vmax = fmaxf(fabsf(vs[0]), fabsf(vs[1]));
-            const int up = max((int)(__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, vmax)) >> 23) + 1 - eR, 0);
-            bool need = up > 0;
-            float xmax[RB];
-            constexpr bool RAW = PLAIN && !CAP;  // x stays raw
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-                float mx = -INFINITY;
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-                    const float c = qs[rb] * ks[kb];
-                    if constexpr (RAW) {
-                        mx = fmaxf(mx, c * fmaxf(fmaxf(x[rb][kb][0], x[rb][kb][1]), fmaxf(x[rb][kb][2], x[rb][kb][3])));
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float y = x[rb][kb][e] * c;
-                            if constexpr (CAP) y = a.softcap * kLog2e * fast_tanh(y);
-                            if constexpr (!PLAIN) {
-                                const int j = s0 + kb * 16 + G * 4 + e;
-                                y = s_ok[buf][2 * hh + kb] && j >= rlo[rb] && j <= rhi[rb] ? y : -INFINITY;
-                            }
-                            x[rb][kb][e] = y;
-                            mx = fmaxf(mx, y);
-                        }
-                    }
-                }
-                xmax[rb] = mx;
-                need |= mx > m_run[rb] + kLazy;
+            for (int i = x; i < x + 2; ++i) {
+                const int o_ = (h * 32 + i / DB * 16) * ROW;
+                vop[i] = tr_read(ta[i % DB] + o_, tb[i % DB] + o_);
             }
-            if (__ballot(need)) {
-                eR += up;
-                const float shrink = up > 126 ? 0.f : exp2i(-up);
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    const float mn = fmaxf(m_run[rb], wave_max16x4(xmax[rb]));
-                    const float alpha = fast_exp2(m_run[rb] - mn);
-                    m_run[rb] = mn;
-                    l_run[rb] *= alpha;
-#pragma unroll
-                    for (int db = 0; db < DBLK; ++db) {
-                        f32x4 o = oacc[rb][db];
-                        asm volatile("" : "+v"(o));  // pins the multiply inside this branch
-                        oacc[rb][db] = o * (alpha * shrink);
-                    }
-                }
-            }
-            u32x4 pk[RB];
-            if constexpr (PLAIN) {
-                const float unit = (float)(127 + kUnit - eR), back = exp2i(eR - 127 - kUnit);
-                const float lv[2] = {s_lv[buf][2 * hh] + unit, s_lv[buf][2 * hh + 1] + unit};
-                const float iv[2] = {s_iv[buf][2 * hh] * back, s_iv[buf][2 * hh + 1] * back};
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    f32x8 wt;
-#pragma unroll
-                    for (int kb = 0; kb < 2; ++kb) {
-                        const float c = RAW ? qs[rb] * ks[kb] : 1.f, d = lv[kb] - m_run[rb];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) wt[4 * kb + e] = fast_exp2(__builtin_fmaf(x[rb][kb][e], c, d));
-                        l_run[rb] += ((wt[4 * kb] + wt[4 * kb + 1]) + (wt[4 * kb + 2] + wt[4 * kb + 3])) * iv[kb];
-                    }
-                    pk[rb] = pack8<DT_FP16>(wt);
-                }
-            } else {
-                const float toR = exp2i(127 + kUnit - eR);
-                vs[0] *= toR;
-                vs[1] *= toR;
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    f32x8 wt;
-                    float sum = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float p = fast_exp2(x[rb][e >> 2][e & 3] - m_run[rb]);
-                        sum += p;
-                        wt[e] = p * vs[e >> 2];
-                    }
-                    l_run[rb] += sum;
-                    pk[rb] = pack8<DT_FP16>(wt);
-                }
-            }
-            __builtin_amdgcn_s_setprio(1);  // the SIMD's other wave fills the slots between these products
-#pragma unroll
-            for (int db = 0; db < DBLK; ++db) {
-                const u32x4 cur = vt[db % VPRE];
-                if (db + VPRE < DBLK) vt[db % VPRE] = read_vt(db + VPRE);
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) oacc[rb][db] = mfma_f16(cur, pk[rb], oacc[rb][db]);
-            }
-            __builtin_amdgcn_s_setprio(0);
+        };
+        auto lane_of = [](float x, int i) {
+            return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), i));
         };
 
-        // Turn t: tile t's products, tile t + 1 from registers to LDS, tile t + 2 asked
-        // for at the place left in turn t - 1, and tile t + 3's left in this one. The
-        // keeper's scales of tile t + 1 go down before it asks for tile t + 2's.
-        if (ntiles > 0) {
-            store_tile(0);
-            if (keeper) {
-                block_place(1);
-                block_id(2);
-            }
-        }
-        __syncthreads();
-        if (ntiles > 1) load_tile(1);
-        for (int t = 0; t < ntiles; ++t) {
-            const int buf = t & 1, s0 = base + t * BN;
-            if (live && s0 <= w_hi && s0 + BN > w_lo) {
-                const bool plain = __builtin_amdgcn_readfirstlane(s_plain[buf]);
+        // Scores of the unit at hand are raw products times cc, or scores themselves (cc =
+        // 1); peak: their largest, in log2 units.
+        float cc[RB][2], peak[RB];
+        auto scored = [&](f32x16 (&n)[RB], int el, int s0, float c, unsigned ok) {  // s0: key offset of the unit
+            const int rb = el / 16, i = el % 16;
+            float y = n[rb][i] * c;
+            if constexpr (CAP) y = anew().softcap * kLog2e * fast_tanh(y);
+            const unsigned seen = ok >> (i / 8) & 1 ? rsee[rb] : 0;
+            n[rb][i] = (unsigned)(s0 - rlo[rb] + 8 * (i / 4) + i % 4) < seen ? y : -INFINITY;
+        };
+        // moves the running maximum to that of the scores where they exceed it by 2^4; the
+        // sums are multiplied by shrink too
+        auto raise = [&](bool live, float shrink) {
+            bool need = shrink != 1.f;
 #pragma unroll
-                for (int hh = 0; hh < BN / 32; ++hh) {
-                    const int h0 = s0 + 32 * hh;
-                    if (h0 > w_hi || h0 + 32 <= w_lo) continue;
-                    if (plain && h0 >= f_lo && h0 + 31 <= f_hi) tile(buf, hh, h0, std::integral_constant<bool, true>{});
-                    else tile(buf, hh, h0, std::integral_constant<bool, false>{});
+            for (int rb = 0; rb < RB; ++rb) need |= peak[rb] > m[rb] + kLazy;
+            if (live && __ballot(need)) {
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    const float mn = fmaxf(m[rb], fmaxf(peak[rb], __shfl_xor(peak[rb], 32)));
+                    const float alpha = fast_exp2(m[rb] - mn);
+                    m[rb] = mn;
+                    l[rb] *= alpha;
+                    const float by = alpha * shrink;
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[rb][db][i] *= by;
+                    }
                 }
             }
-            if (t + 1 < ntiles) {
-                store_tile(buf ^ 1);
-                if (keeper) {
-                    block_place(t + 2);
-                    block_id(t + 3);
-                }
-            }
-            __syncthreads();
-            if (t + 2 < ntiles) load_tile(t + 2);
-        }
+        };
+        // A group's scales come into force: R moves above its V scales, and the sums are to
+        // shrink by what is returned
+        auto begin_group = [&]() {
+            // scales that are no numbers are left out: rows may not see them
+            int top = __builtin_bit_cast(int, sc.v) >> 23 & 255;
+            top = top == 255 ? 0 : top;
+#pragma unroll
+            for (int x = 1; x < 64; x <<= 1) top = max(top, __shfl_xor(top, x));
+            const int up = max(__builtin_amdgcn_readfirstlane(top) + 1 - eR, 0);
+            eR += up;
+            lv = fast_log2(sc.v) + (float)(127 + kUnit - eR);
+            iv_ = exp2i(eR - 127 - kUnit) / sc.v;
+            wv_ = sc.v * exp2i(127 + kUnit - eR);
+            return up > 126 ? 0.f : exp2i(-up);
+        };
+        const f32x16 zero = {};
 
-        // ---- results --------------------------------------------------------------------------
+        // One unit: its softmax and P.V while the scores of the next are formed (n_), one
+        // MFMA to a slot. Each score takes three slots: scaled, its exponential,
+        // summed and packed; they are spread evenly up to the last keys' P.V products.
+        // H: the unit at hand in its tile; its successor's K is read from place A of a tile.
+        u32x4 pk[RB][2];
+        float px[NE];
+        auto unit = [&](f32x16 (&c_)[RB], f32x16 (&n_)[RB], auto hh, int tg, int s0n, auto gen, auto more, auto ahead) {
+            constexpr int H = decltype(hh)::value, A = (H + 1) % NH;
+            constexpr bool GEN = decltype(gen)::value, RAW = !GEN && !CAP;
+            float dd[RB][2], nn[RB][2], iv[2], wv[2];
+            const int bl = tg * NB + 2 * H;  // the unit's blocks; the next unit's follow
+            [[maybe_unused]] const unsigned ok = (unsigned)(sc.ok >> ((bl + 2) & 63));
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const float ks = lane_of(sc.k, (bl + 2 + kb) & 63);
+                const float lk = GEN ? 0.f : lane_of(lv, bl + kb);
+                iv[kb] = GEN ? 1.f : lane_of(iv_, bl + kb);
+                wv[kb] = GEN ? lane_of(wv_, bl + kb) : 1.f;
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    dd[rb][kb] = lk - m[rb];
+                    nn[rb][kb] = qs[rb] * ks;
+                }
+            }
+            float part[RB], top[RB][2];
+            int slot = 0;
+            auto next = [&]() {
+#pragma unroll
+                for (int q = 0; q < NE; ++q) {
+                    // q-th score: the first 16 keys of every row block, then the others
+                    const int ks = q / (8 * RB), rb = q / 8 % RB, i = 8 * ks + q % 8;
+                    const int when = q * (SS + SP - 2) / NE;
+                    if (slot == when) px[q] = __builtin_fmaf(c_[rb][i], cc[rb][ks], dd[rb][ks]);
+                    if (slot == when + 1) px[q] = fast_exp2(px[q]);
+                    if (slot == when + 2) {
+                        part[rb] = q % 8 == 0 ? px[q] : part[rb] + px[q];
+                        if (q % 8 == 7) l[rb] = GEN ? l[rb] + part[rb] : __builtin_fmaf(part[rb], iv[ks], l[rb]);
+                        // (0 times any scale is 0: a hidden key's weight)
+                        if constexpr (GEN) px[q] = mul_or_0(px[q], wv[ks]);
+                        if (q & 1) pk[rb][ks][q / 2 % 4] = pack2<DT_FP16>(px[q - 1], px[q]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < NE; ++e) {
+                    if (slot != SS + 2 + e * (2 * SP - 4) / NE) continue;
+                    const int rb = e / 16, kb = e / 8 % 2;
+                    if constexpr (GEN) {
+                        scored(n_, e, s0n, nn[rb][kb], ok);
+                    } else if constexpr (CAP) {
+                        n_[rb][e % 16] = anew().softcap * kLog2e * fast_tanh(n_[rb][e % 16] * nn[rb][kb]);
+                    }
+                    top[rb][kb] = e % 8 == 0 ? n_[rb][e % 16] : fmaxf(top[rb][kb], n_[rb][e % 16]);
+                }
+                ++slot;
+                fence();
+            };
+            // operands are read two steps ahead, the last one read is used first
+#pragma unroll
+            for (int s = 0; s < KS; s += 2) {
+#pragma unroll
+                for (int d = 1; d >= 0; --d) {
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) {
+                        n_[rb] = mfma32<DT_FP16>(kop[s + d], qreg[rb][s + d], s == 0 && d == 1 ? zero : n_[rb]);
+                        if (d == 1 && rb == 0) {
+                            if (s + 2 < KS) read_rows(A, s + 2);
+                            else read_tr(H, 0);
+                        }
+                        next();
+                    }
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 2 * DB; x += 2) {
+#pragma unroll
+                for (int d = 1; d >= 0; --d) {
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) {
+                        o[rb][(x + d) % DB] = mfma32<DT_FP16>(vop[x + d], pk[rb][(x + d) / DB], o[rb][(x + d) % DB]);
+                        if (d == 1 && rb == 0) {
+                            if (x + 2 < 2 * DB) read_tr(H, x + 2);
+                            else ahead();
+                        }
+                        more(x * RB + (1 - d) * RB + rb);
+                        next();
+                    }
+                }
+            }
+            more(2 * SP);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                peak[rb] = RAW ? fmaxf(top[rb][0] * nn[rb][0], top[rb][1] * nn[rb][1]) : fmaxf(top[rb][0], top[rb][1]);
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) cc[rb][kb] = RAW ? nn[rb][kb] : 1.f;
+            }
+        };
+
+        if (ntiles > 0) {
+            begin_group();  // (the sums are 0)
+            find_odd(sc);
+            __syncthreads();
+            f32x16 s0[RB], s1[RB];
+#pragma unroll
+            for (int s = 0; s < KS; s += 2) read_rows(0, s);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                s0[rb] = zero;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) s0[rb] = mfma32<DT_FP16>(kop[s], qreg[rb][s], s0[rb]);
+            }
+#pragma unroll
+            for (int e2 = 0; e2 < NE; ++e2) {
+                const int rb = e2 / 16;
+                scored(s0, e2, 0, qs[rb] * lane_of(sc.k, e2 / 8 % 2), (unsigned)sc.ok);
+                peak[rb] = e2 % 16 == 0 ? s0[rb][0] : fmaxf(peak[rb], s0[rb][e2 % 16]);
+                cc[rb][0] = cc[rb][1] = 1.f;
+            }
+            raise(true, 1.f);
+            if constexpr (NH == 1) {
+#pragma unroll
+                for (int s = 0; s < KS; ++s) move_on(ra[s], TILE);
+            }
+            read_rows(NH > 1 ? 1 : 0, 0);
+            int t = 0, tg = 0, nb = 1, fb = 2;  // buffers of tiles t + 1 and t + 2
+            auto next_buf = [](int x) { return x == NBUF - 1 ? 0 : x + 1; };
+            auto step_to = [](int x) { return x == 0 ? 0u - (NBUF - 1) * (unsigned)TILE : (unsigned)TILE; };
+            constexpr int LAST = (2 * DB - 2) * RB;  // first product of the last operand pair: `ahead` runs there
+            // Tile t + 2 goes down, in four parts, in tile t's last unit, past its barrier
+            // (a tile of one unit: before it); then tile t + 4 is asked for in its place.
+            auto stage = [&](int x) {
+#pragma unroll
+                for (int part = 0; part < 4; ++part) {
+                    if (x == part * 2 * SP / 4) {
+                        if (part == 0) wait_loads<4>();  // all but tile t + 3's
+                        get_part(t, part);
+                    }
+                    if (x == part * 2 * SP / 4 + 1) put_part(t + 2, part, fb * TILE);
+                }
+                if (x == 2 * SP) {
+                    const int ag = (tg + 4) % TPG;
+                    if (ag == 0) {
+                        group_places(sc_new);
+                        group_ids((t + 4) / TPG + 1);
+                    }
+                    ask(t + 4, ag);
+                }
+            };
+            auto tile = [&](auto gen) {
+                const unsigned by = step_to(nb);  // from tile t's buffer to the next
+                const int s0k = t * BN;
+                if constexpr (NH > 1) {
+                    auto half = [&](auto hh) {
+                        constexpr int H = decltype(hh)::value;
+                        unit(H % 2 ? s1 : s0, H % 2 ? s0 : s1, hh, tg, s0k + 32 * (H + 1), gen,
+                             [&](int x) {
+                                 if (H == NH - 2 && x == SP / 2) {
+#pragma unroll
+                                     for (int s = 0; s < KS; ++s) move_on(ra[s], by);
+                                 }
+                                 if (H == NH - 2 && x == LAST - 1) __syncthreads();
+                                 if (H == NH - 1) stage(x);
+                                 if (H == NH - 1 && x == LAST) {
+#pragma unroll
+                                     for (int db = 0; db < DB; ++db) {
+                                         move_on(ta[db], by);
+                                         move_on(tb[db], by);
+                                     }
+                                 }
+                             },
+                             [&]() { read_rows((H + 2) % NH, 0); });
+                        if constexpr (H < NH - 1) raise(true, 1.f);
+                    };
+                    half(std::integral_constant<int, 0>{});
+                    half(std::integral_constant<int, 1>{});
+                    if constexpr (NH == 4) {
+                        half(std::integral_constant<int, 2>{});
+                        half(std::integral_constant<int, 3>{});
+                    }
+                } else {
+                    const unsigned by2 = step_to(next_buf(nb));  // from tile t + 1's buffer to the next
+                    unit(s0, s1, std::integral_constant<int, 0>{}, tg, s0k + 32, gen,
+                         [&](int x) {
+                             if (x == SP / 2) {
+#pragma unroll
+                                 for (int s = 0; s < KS; ++s) move_on(ra[s], by2);
+                             }
+                             stage(x);
+                             if (x == LAST - 1) __syncthreads();
+                             if (x == LAST) {
+#pragma unroll
+                                 for (int db = 0; db < DB; ++db) {
+                                     move_on(ta[db], by);
+                                     move_on(tb[db], by);
+                                 }
+                             }
+                         },
+                         [&]() { read_rows(0, 0); });
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) s0[rb] = s1[rb];
+                }
+                nb = next_buf(nb);
+                fb = next_buf(fb);
+                ++t;
+                float shrink = 1.f;
+                if (++tg == TPG) {
+                    tg = 0;
+                    sc = sc_new;
+                    shrink = begin_group();
+                } else if (tg + 1 == TPG) {
+                    // the next tile's scores take scales of the next group: K's go where those of
+                    // this group's first tile were
+                    find_odd(sc_new);
+                    sc.k = lane < NB ? sc_new.k : sc.k;
+                    sc.ok = (sc.ok & ~kTileBlocks) | (sc_new.ok & kTileBlocks);
+                    sc.odd = (sc.odd & ~kTileBlocks) | (sc_new.odd & kTileBlocks);
+                }
+                raise(t < ntiles, shrink);
+            };
+            // a tile's copy of the unit covers the weights of it and the scores formed in
+            // it: those of its later units and of the next tile's first
+            auto general = [&]() {
+                const uint64_t odd = sc.odd >> (tg * NB) | sc.odd >> ((tg + 1) % TPG * NB);
+                return t < t1 || t + 1 >= t2 || (odd & kTileBlocks);
+            };
+            while (t < ntiles) {
+                while (t < ntiles && general()) tile(std::true_type{});
+                while (t < ntiles && !general()) tile(std::false_type{});
+            }
+        }
+        wait_loads<0>();  // asked for past the end
+        __syncthreads();  // the next item's tiles go where other waves may still read
+
+        // ---- results: lane holds O^T [dims 32db + 8q + 4hi + i][row col] --------------------------
         const float back = exp2i(eR - 127 - kUnit);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
-            const int r = wrow0 + rb * 16 + li;
-            const float l = wave_sum16x4(l_run[rb]);
-            const bool some = l != 0.f;
-            const float inv = some ? back / l : 0.f;
-            const float lse = some ? (m_run[rb] + fast_log2(l)) * kLn2 : INFINITY;
+            const int r = wrow0 + rb * 32 + col;
+            const float lrow = l[rb] + __shfl_xor(l[rb], 32);
+            const bool some = lrow != 0.f;
+            const float inv = some ? back / lrow : 0.f;
+            const float lse = some ? (m[rb] + fast_log2(lrow)) * kLn2 : INFINITY;
             if (r >= R.rows) continue;
             if (slot < 0) {
                 const int i = r / g, h = hk * g + r % g;
-                uint16_t* o = static_cast<uint16_t*>(a.out) + q_row(a, b, i, a.o_sb, a.o_si) + (int64_t)h * a.o_sh;
+                uint16_t* orow = static_cast<uint16_t*>(a.out) + q_row(a, b, i, a.o_sb, a.o_si) + (int64_t)h * a.o_sh;
 #pragma unroll
-                for (int db = 0; db < DBLK; ++db) {
-                    if (16 * db >= a.hd) continue;
-                    const f32x4 y = oacc[rb][db] * inv;
-                    *reinterpret_cast<u32x2*>(o + 16 * db + 4 * G) = u32x2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
-                }
-                if (G == 0) a.lse[lse_at(a, b, h, i)] = lse;
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int d = 32 * db + 8 * q + 4 * hi;
+                        if (d >= a.hd) continue;
+                        *reinterpret_cast<u32x2*>(orow + d) =
+                            u32x2{pack2<DT>(o[rb][db][4 * q] * inv, o[rb][db][4 * q + 1] * inv),
+                                  pack2<DT>(o[rb][db][4 * q + 2] * inv, o[rb][db][4 * q + 3] * inv)};
+                    }
+                if (hi == 0) a.lse[lse_at(a, b, h, i)] = lse;
             } else {
                 const int64_t prow = (int64_t)slot * BM + (r - row0);
 #pragma unroll
-                for (int db = 0; db < DBLK; ++db)
-                    *reinterpret_cast<f32x4*>(a.pf_o + prow * HD + 16 * db + 4 * G) = oacc[rb][db] * inv;
-                if (G == 0) a.pf_lse[prow] = some ? lse : -INFINITY;
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<f32x4*>(a.pf_o + prow * HD + 32 * db + 8 * q + 4 * hi) =
+                            f32x4{o[rb][db][4 * q] * inv, o[rb][db][4 * q + 1] * inv, o[rb][db][4 * q + 2] * inv,
+                                  o[rb][db][4 * q + 3] * inv};
+                if (hi == 0) a.pf_lse[prow] = some ? lse : -INFINITY;
             }
         }
     }
