@@ -71,6 +71,13 @@ __device__ __forceinline__ int64_t lse_at(const QuantFwdArgs& a, int b, int h, i
     return a.cu_q ? (int64_t)h * a.lse_sh + a.cu_q[b] + i : (int64_t)b * a.lse_sb + (int64_t)h * a.lse_sh + i;
 }
 
+// x y, and 0 where x is 0, whatever y: a hidden key's weight
+__device__ __forceinline__ float mul_or_0(float x, float y) {
+    float r;
+    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(y));
+    return r;
+}
+
 // eight 16-bit values as fp32
 template <int DT>
 __device__ __forceinline__ f32x8 widen8(u32x4 r) {

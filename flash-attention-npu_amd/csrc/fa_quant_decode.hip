@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
         // R, and the weights' factor for each block
         float vmax = 0.f;
 #pragma unroll
-        for (int h = 0; h < NH; ++h) vmax = fmaxf(vmax, fabsf(vs[h]));
+        for (int h = 0; h < NH; ++h) vmax = fmaxf(vmax, fabsf(vs[h]) < INFINITY ? fabsf(vs[h]) : 0.f);  // rows may not see what is no number
         const int e = (int)(__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, vmax)) >> 23) + 1;
         const int up = max(e - eR, 0);
         eR += up;
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
                     const int h = 2 * k2 + (e2 >> 2);
                     const float p = fast_exp2(x[rt][h][e2 & 3] - m);
                     sum += p;
-                    w[e2] = p * vs[h];
+                    w[e2] = mul_or_0(p, vs[h]);
                 }
                 pk[rt][k2] = pack8<DT_FP16>(w);
             }

@@ -64,13 +64,6 @@ __device__ __forceinline__ void dma16_kkvv(unsigned lds, uint64_t b0, uint64_t b
         : "memory", "m0");
 }
 
-// x y, and 0 where x is 0, whatever y
-__device__ __forceinline__ float mul_or_0(float x, float y) {
-    float r;
-    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "s"(y), "v"(x));
-    return r;
-}
-
 // CAP: soft cap
 template <int DT, int CT, int HD, int RB_, bool CAP>
 __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a) {

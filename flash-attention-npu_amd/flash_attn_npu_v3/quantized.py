@@ -88,7 +88,10 @@ def flash_attn_with_quantized_kvcache(q, k_cache, v_cache, k_scale, v_scale, cac
     last key). page_table (rows, max_pages) int32 as from update_page_table, or
     None for a contiguous cache. cache_batch_idx (batch_size,) int32: the row
     of the page table (of the contiguous cache) of each sequence. Keys on a page
-    whose id is not in the cache are not visible. The scales may have any value.
+    whose id is not in the cache are not visible. The scales may have any value, and
+    reach only the rows that see their keys. A NaN code of v_cache (e4m3) at a key that
+    some row of the sequence sees may reach rows that do not see it, as a NaN of v does in
+    flash_attn_with_kvcache.
 
     The scores are softmax_scale (default headdim ** -0.5) * k_scale * (q . c)
     of each key's codes, the weights of the values carry v_scale, and both
