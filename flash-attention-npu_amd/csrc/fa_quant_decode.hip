@@ -2,7 +2,7 @@
 // head's g query heads x positions, at most 32 packed rows): the cache is
 // streamed once, at the rate that HBM gives.
 //
-// Split: the 64-key tiles (32 at head dim 256) of all sequences and kv heads form
+// Split: the 32-key tiles (64 at head dim 64) of all sequences and kv heads form
 // one list, built in LDS by each workgroup from cache_seqlens and cut into equal
 // contiguous ranges, one per wave; waves of a CU take adjacent kv heads of one
 // range, so that a key row is requested by a CU at once. A range that ends inside a
@@ -23,6 +23,12 @@
 // the weights p, which are then rounded to fp16, so they are kept relative to a
 // running power of two R >= t that moves up like a maximum, w = p * t / R * 2^14: a
 // weight keeps its 11 bits as long as p * t / R > 2^-28.
+//
+// Measured (D128, g 4 and 8): 64 paged e4m3 sequences, 966 MB: 187-194 us, 5.0-5.2 TB/s; 32
+// contiguous int8 ones, 194 MB: 52 us; 4 tokens over a window of 4096, 8 sequences:
+// 31.6 us; one sequence of 777 keys: 15 us, of which the start before the first
+// tile (list, ids, rows, scales: each waits for the one before) takes 5 and the merge 6.
+// Tiles in registers instead of LDS, with one wave per SIMD: 190, 55, 36 and 15 us.
 #include "fa_quant.h"
 #include "fa_pipe.h"
 
