@@ -120,6 +120,8 @@ fa_status_t check_fwd(const fa_quant_fwd_params* p) {
     } else {
         FA_CHECK(p->cache_batch_idx || p->num_pages >= p->batch, "the cache must have a row per sequence");
     }
+    // masks count keys from -2^30 to 2^30
+    FA_CHECK((int64_t)(p->page_table ? p->max_pages : 1) * p->page_size <= 1 << 30, "a sequence holds at most 2^30 tokens");
     const int64_t rows = p->cu_seqlens_q ? (int64_t)p->total_q : (int64_t)p->batch * p->seqlen_q;
     if (rows == 0 || p->seqlen_q == 0) return FA_OK;
     FA_CHECK(rows * (p->nheads / p->nheads_k) <= INT_MAX, "too many query rows");

@@ -109,6 +109,7 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
         return *(const QuantFwdArgs*)p;
     };
 
+    [[maybe_unused]] const float cap = a.softcap * kLog2e;
     const int entries = s_pref[a.B], grid = (int)gridDim.x;
     Line line{};
     int worker = blockIdx.x;
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
         auto scored = [&](f32x16 (&n)[RB], int el, int s0, float c, unsigned ok) {  // s0: key offset of the unit
             const int rb = el / 16, i = el % 16;
             float y = n[rb][i] * c;
-            if constexpr (CAP) y = anew().softcap * kLog2e * fast_tanh(y);
+            if constexpr (CAP) y = cap * fast_tanh(y);
             const unsigned seen = ok >> (i / 8) & 1 ? rsee[rb] : 0;
             n[rb][i] = (unsigned)(s0 - rlo[rb] + 8 * (i / 4) + i % 4) < seen ? y : -INFINITY;
         };
@@ -460,7 +461,7 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
                     if constexpr (GEN) {
                         scored(n_, e, s0n, nn[rb][kb], ok);
                     } else if constexpr (CAP) {
-                        n_[rb][e % 16] = anew().softcap * kLog2e * fast_tanh(n_[rb][e % 16] * nn[rb][kb]);
+                        n_[rb][e % 16] = cap * fast_tanh(n_[rb][e % 16] * nn[rb][kb]);
                     }
                     top[rb][kb] = e % 8 == 0 ? n_[rb][e % 16] : fmaxf(top[rb][kb], n_[rb][e % 16]);
                 }
