@@ -68,7 +68,7 @@ __device__ __forceinline__ void dma16_kkvv(unsigned lds, uint64_t b0, uint64_t b
         "global_load_lds_dwordx4 %5, %1\n\t"
         "global_load_lds_dwordx4 %5, %2 offset:1024\n\t"
         "global_load_lds_dwordx4 %6, %3 offset:2048\n\t"
-        "global_load_lds_dwordx4 %6, %4 offset:3072" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "s"(b0), "s"(b1), "s"(b2), "s"(b3),
+        "global_load_lds_dwordx4 %6, %4 offset:0xc00" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "s"(b0), "s"(b1), "s"(b2), "s"(b3),
         "v"(koff), "v"(voff)
         : "memory", "m0");
 }
