@@ -531,7 +531,8 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
 
 // Merge of what a segment's workers left: 16 rows and 32 columns of a segment per
 // workgroup; groups of threads fold a share of the partials each, with a running
-// maximum, and meet in LDS.
+// maximum, and meet in LDS. A row is empty where its weights sum to 0, which says so
+// for NaN as well: such partials have no part in the maximum (fmaxf).
 constexpr int MT = 512;
 template <int DT, int HD>
 __global__ void __launch_bounds__(MT) fa_quant_merge_kernel(QuantFwdArgs a, int grid, int nr) {
@@ -588,7 +589,7 @@ __global__ void __launch_bounds__(MT) fa_quant_merge_kernel(QuantFwdArgs a, int 
         if (grp < half) {
             const int o = tid + half * GS;
             const float mo = s_gm[o], M = fmaxf(m, mo);
-            if (M != -INFINITY) {
+            if (s_gs[o] != 0.f || sum != 0.f) {
                 const float c = fast_exp2((m - M) * kLog2e), co = fast_exp2((mo - M) * kLog2e);
                 acc0 = acc0 * c + *reinterpret_cast<const f32x4*>(&s_acc[o][0]) * co;
                 acc1 = acc1 * c + *reinterpret_cast<const f32x4*>(&s_acc[o][4]) * co;
@@ -602,7 +603,7 @@ __global__ void __launch_bounds__(MT) fa_quant_merge_kernel(QuantFwdArgs a, int 
         }
     }
     if (grp != 0 || rr >= rows) return;
-    const float inv = m == -INFINITY ? 0.f : 1.f / sum;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     acc0 *= inv;
     acc1 *= inv;
     const int r = row0 + rr, i = r / a.g, h = hk * a.g + r % a.g;
@@ -610,7 +611,7 @@ __global__ void __launch_bounds__(MT) fa_quant_merge_kernel(QuantFwdArgs a, int 
     if (d0 < a.hd)
         *reinterpret_cast<u32x4*>(o + d0) = u32x4{pack2<DT>(acc0[0], acc0[1]), pack2<DT>(acc0[2], acc0[3]),
                                                   pack2<DT>(acc1[0], acc1[1]), pack2<DT>(acc1[2], acc1[3])};
-    if (d0 == 0) a.lse[lse_at(a, b, h, i)] = m == -INFINITY ? INFINITY : m + fast_log2(sum) * kLn2;
+    if (d0 == 0) a.lse[lse_at(a, b, h, i)] = sum == 0.f ? INFINITY : m + fast_log2(sum) * kLn2;
 }
 
 template <int DT, int CT, int HD>

@@ -138,10 +138,15 @@ __global__ void __launch_bounds__(256) fa_quant_prefill_merge_kernel(QuantFwdArg
     if (r >= sq * a.g) return;
     auto row = [&](int s) { return (int64_t)(s == 0 ? 2 * w + 1 : 2 * (w + s)) * BM + rr; };
     float m = -INFINITY;
-    for (int s = 0; s < c.pieces; ++s) m = fmaxf(m, a.pf_lse[row(s)]);
+    bool some = false;  // a piece with a key for the row; one that is NaN has no part in the maximum
+    for (int s = 0; s < c.pieces; ++s) {
+        const float v = a.pf_lse[row(s)];
+        m = fmaxf(m, v);
+        some |= v != -INFINITY;
+    }
     f32x4 acc0 = {0.f, 0.f, 0.f, 0.f}, acc1 = acc0;
     float lse = INFINITY;
-    if (m != -INFINITY) {
+    if (some) {
         float sum = 0.f;
         for (int s = 0; s < c.pieces; ++s) {
             const float wgt = fast_exp2((a.pf_lse[row(s)] - m) * kLog2e);
