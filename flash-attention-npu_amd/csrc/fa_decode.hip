@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(256, 1) fa_decode_kernel(FwdArgs a) {
 
     auto end_seg = [&](const DecSeg& s) {
         const float lrow = wave_sum16x4(l_run);
-        const bool nonempty = lrow > 0.f;
+        const bool nonempty = lrow != 0.f;  // a NaN sum has keys
         const float inv = nonempty ? (F8 ? sc_v / lrow : 1.f / lrow) : 0.f;
         const bool whole = s.S >= t0 && s.S + s.n <= t1;
         if (li >= rows) return;
@@ -722,7 +722,8 @@ __global__ void __launch_bounds__(256) fa_decode_merge_kernel(FwdArgs a, int wor
     };
     // ---- one pass: each of NG thread groups folds its share of the partials
     // with a running maximum (lse and O of a partial are loaded together), then
-    // the groups are combined through LDS ----------------------------------------------
+    // the groups are combined through LDS. A row is empty where its weights sum to 0:
+    // NaN partials have no part in the maximum (fmaxf) --------------------------------------
     int rp = 1;
     while (rp < rows) rp <<= 1;
     const int GS = CH * rp;  // threads per group: one per (row, 8-dim chunk)
@@ -755,9 +756,12 @@ __global__ void __launch_bounds__(256) fa_decode_merge_kernel(FwdArgs a, int wor
         s_gs[tid] = sum;
         __syncthreads();
         if (grp != 0) return;
-        float M = m;
-        for (int gq = 1; gq < NG; ++gq) M = fmaxf(M, s_gm[tid + gq * GS]);
-        if (M != -INFINITY) {
+        float M = m, some = sum;
+        for (int gq = 1; gq < NG; ++gq) {
+            M = fmaxf(M, s_gm[tid + gq * GS]);
+            some += s_gs[tid + gq * GS];
+        }
+        if (some != 0.f) {
             const float c = fast_exp2((m - M) * kLog2e);
             acc0 *= c;
             acc1 *= c;
@@ -773,10 +777,10 @@ __global__ void __launch_bounds__(256) fa_decode_merge_kernel(FwdArgs a, int wor
         m = M;
     }
     // lse of the row; -inf marks a row with no visible key (out = 0, lse = +inf)
-    const float inv = m == -INFINITY ? 0.f : 1.f / sum;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     acc0 *= inv;
     acc1 *= inv;
-    const float L = m == -INFINITY ? -INFINITY : m + fast_log2(sum) * kLn2;
+    const float L = sum == 0.f ? -INFINITY : m + fast_log2(sum) * kLn2;
     if (rr >= rows) return;
     const int i = rr / a.g, h = hk * a.g + rr % a.g;
     uint16_t* op = static_cast<uint16_t*>(a.out);

@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(PfCfg<HD>::NT, 1) fa_prefill_kernel(FwdArgs a)
         for (int rb = 0; rb < RB; ++rb) {
             const int r = wrow0 + rb * 16 + li;
             const float lrow = wave_sum16x4(l_run[rb]);
-            const bool nonempty = lrow > 0.f;
+            const bool nonempty = lrow != 0.f;  // a NaN sum has keys
             const float inv = nonempty ? (F8 ? sc_v / lrow : 1.f / lrow) : 0.f;
             const float lse = nonempty ? (m_run[rb] + fast_log2(lrow)) * kLn2 : (final_out ? INFINITY : -INFINITY);
             if (r < bi.rows) {
@@ -543,10 +543,15 @@ __global__ void __launch_bounds__(256) fa_merge_kernel(FwdArgs a) {
     const int sst = a.Hk;  // split s of this tile is item w0 + s * Hk
     const int w0 = a.sched[b] + mt_r * ns * a.Hk + hk;
     float m = -INFINITY;
-    for (int s = 0; s < ns; ++s) m = fmaxf(m, a.part_lse[(int64_t)(w0 + s * sst) * BM + rr]);
+    bool some = false;  // a split with a key for the row; one that is NaN has no part in the maximum
+    for (int s = 0; s < ns; ++s) {
+        const float v = a.part_lse[(int64_t)(w0 + s * sst) * BM + rr];
+        m = fmaxf(m, v);
+        some |= v != -INFINITY;
+    }
     f32x4 acc0 = {0.f, 0.f, 0.f, 0.f}, acc1 = {0.f, 0.f, 0.f, 0.f};
     float lse = INFINITY;
-    if (m != -INFINITY) {
+    if (some) {
         float sum = 0.f;
         for (int s = 0; s < ns; ++s) {
             const int64_t prow = (int64_t)(w0 + s * sst) * BM + rr;

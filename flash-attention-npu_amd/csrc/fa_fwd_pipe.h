@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(NT, 1) fa_prefill_pipe_kernel(FwdArgs a) {
         for (int rb = 0; rb < RB; ++rb) {
             const int r = wrow0 + rb * 32 + col;
             const float lrow = l[rb] + __shfl_xor(l[rb], 32);
-            const bool nonempty = lrow > 0.f;
+            const bool nonempty = lrow != 0.f;  // a NaN sum has keys
             const float inv = nonempty ? (F8 ? sc_v / lrow : 1.f / lrow) : 0.f;
             const float lse = nonempty ? (m[rb] + fast_log2(lrow)) * kLn2 : (final_out ? INFINITY : -INFINITY);
             if (r >= bi.rows) continue;
