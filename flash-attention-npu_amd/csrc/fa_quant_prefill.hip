@@ -619,7 +619,8 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
                 if (++tg == TPG) {
                     tg = 0;
                     sc = sc_new;
-                    shrink = begin_group();
+                    // past the last tile there is no group, and nothing left to shrink
+                    if (t < ntiles) shrink = begin_group();
                 } else if (tg + 1 == TPG) {
                     // the next tile's scores take scales of the next group: K's go where those of
                     // this group's first tile were
