@@ -78,6 +78,28 @@ __device__ __forceinline__ float mul_or_0(float x, float y) {
     return r;
 }
 
+// Weights. A code c of V with scale t enters its row's sum as p t c, x the score in log2
+// units. A row keeps a running maximum u of x + log2 t, and with w = 2^(x + log2 t - u)
+//   O = sum of w c,   l = sum of w / t,   out = O / l,   log2 of the sum of 2^x = u + log2 l,
+// so that a weight is as precise as it is large in its row's sum, and keys that the row
+// does not see have no part in that. w / t keeps its bits while a row's scales are
+// within 2^100 of each other, so this is for plain ones. For others l has a running maximum
+// of its own, m of x: l = sum of 2^(x - m), out = O / l 2^(u - m).
+__device__ __forceinline__ bool plain_scale(float t) { return t > 0x1p-40f && t < 0x1p40f; }
+
+// log2 |t|; -inf for 0 and for what is no number, whose weights are formed apart
+__device__ __forceinline__ float scale_log2(float t) {
+    const float a = fabsf(t);
+    const bool small = a < 0x1p-100f;  // the logarithm takes no subnormal
+    const float y = fast_log2(small ? a * 0x1p64f : a) - (small ? 64.f : 0.f);
+    return a < INFINITY ? y : -INFINITY;
+}
+
+// u + log2 l, the exponent of l added first: l is far from 1 where t is
+__device__ __forceinline__ float add_log2(float u, float l) {
+    return u + (float)__builtin_amdgcn_frexp_expf(l) + fast_log2(__builtin_amdgcn_frexp_mantf(l));
+}
+
 // eight 16-bit values as fp32
 template <int DT>
 __device__ __forceinline__ f32x8 widen8(u32x4 r) {

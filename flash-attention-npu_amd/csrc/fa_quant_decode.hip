@@ -19,10 +19,9 @@
 // come through a small table in LDS, filled 32 blocks of 16 keys at a time, in steps
 // some tiles apart: a wait for the table would be one for every row asked for before.
 //
-// Scales: the K scale of 16 keys multiplies their scores. The V scale t multiplies
-// the weights p, which are then rounded to fp16, so they are kept relative to a
-// running power of two R >= t that moves up like a maximum, w = p * t / R * 2^14: a
-// weight keeps its 11 bits as long as p * t / R > 2^-28.
+// Scales: the K scale of 16 keys multiplies their scores, the V scale t goes into the
+// weights' exponent (fa_quant.h), 2^14 w rounded to fp16: a weight keeps its 11 bits as
+// long as it is more than 2^-28 of its row's largest.
 //
 // Measured (D128, g 4 and 8): 64 paged e4m3 sequences, 966 MB: 187-194 us, 5.0-5.2 TB/s; 32
 // contiguous int8 ones, 194 MB: 52 us; 4 tokens over a window of 4096, 8 sequences:
@@ -143,7 +142,7 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
     __shared__ __attribute__((aligned(1024))) uint8_t s_ring[NWAVE][4 * C::TILE];
     __shared__ int s_pref[MAXB + 1];
     __shared__ int64_t s_koff[NWAVE][64], s_voff[NWAVE][64];
-    __shared__ float s_ks[NWAVE][64], s_vs[NWAVE][64];
+    __shared__ float s_ks[NWAVE][64], s_vs[NWAVE][64], s_lv[NWAVE][64], s_iv[NWAVE][64];
     __shared__ int s_ok[NWAVE][64 / NH];
 
     // The arguments read anew where they are used once in many tiles (the assembly hides
@@ -195,11 +194,12 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
 
     // ---- the table: offsets, scales and visibility of the 16-key blocks ------------------
     // Tiles base .. base + TAB - 1, a block for each of 32 lanes. A block without a visible
-    // key has the offset of a row that is there and scales 0. In
-    // steps: page ids asked for; offsets, scales asked for; scales.
+    // key has the offset of a row that is there and plain scales. In
+    // steps: page ids asked for; offsets, scales asked for; scales. tlv, tiv: log2 and
+    // inverse (times 2^-14) of V's scale; tok: the tile's visible blocks, and bit 8 where V's scales are plain.
     int64_t* koff = s_koff[wave];
     int64_t* voff = s_voff[wave];
-    float *tks = s_ks[wave], *tvs = s_vs[wave];
+    float *tks = s_ks[wave], *tvs = s_vs[wave], *tlv = s_lv[wave], *tiv = s_iv[wave];
     int* tok = s_ok[wave];
     int id, inp, kvh;
     float ksv, vsv;
@@ -228,19 +228,23 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
         ksv = A.ks[p * A.ks_sp + sb * A.ks_sb + h * A.ks_sh];
         vsv = A.vs[p * A.vs_sp + sb * A.vs_sb + h * A.vs_sh];
         const int at = slot_of(base);
-        const unsigned long long m = __ballot(ok);
         if (lane < 32) {
             koff[at] = p * A.k_sp + r * A.k_si + h * A.k_sh;
             voff[at] = p * A.v_sp + r * A.v_si + h * A.v_sh;
-            if (lane % NH == 0) tok[at / NH] = (int)(m >> lane) & ((1 << NH) - 1);
         }
     };
     auto fill_scales = [&](int base) {
         const bool ok = id >= 0 && id < a.num_pages;
         const int at = slot_of(base);
+        const float v = ok ? vsv : 1.f, lv = scale_log2(v);
+        const unsigned long long mo = __ballot(ok), mp = __ballot(plain_scale(v));
         if (lane < 32) {
-            tks[at] = ok ? ksv : 0.f;
-            tvs[at] = ok ? vsv : 0.f;
+            constexpr int kAll = (1 << NH) - 1;
+            tks[at] = ok ? ksv : 1.f;
+            tvs[at] = v;
+            tlv[at] = lv;
+            tiv[at] = fast_exp2(-14.f - lv);
+            if (lane % NH == 0) tok[at / NH] = ((int)(mo >> lane) & kAll) | ((((int)(mp >> lane) & kAll) == kAll) << 8);
         }
     };
 
@@ -284,8 +288,9 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
     float qs[NR];              // what the scores of a row are to be multiplied by for its q_shift
     int qi[NR];
     f32x4 oacc[NR][DBLK];
-    float m_run[NR], l_run[NR];
-    int rows = 0, eR = 30;     // R = 2^(eR - 127)
+    float u_run[NR], l_run[NR], m_run[NR];
+    bool apart = false;        // l is relative to m, else to u
+    int rows = 0;
     int flo = 0, fhi = 0;      // keys that every row sees
     auto load_q = [&](int t) {
         const QuantFwdArgs& A = anew();
@@ -309,7 +314,7 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
     auto begin_seg = [&]() {
         flo = key_lo(cs.q.sk - 1, a.wl, 0);
         fhi = min(key_hi(cs.q.sk - cs.q.sq, a.wr, 0), cs.q.sk - 1);
-        eR = 30;
+        apart = false;
 #pragma unroll
         for (int rt = 0; rt < NR; ++rt) {
             float most = 0.f;
@@ -324,7 +329,7 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
             qs[rt] = exp2i(-sh) * scale2;
 #pragma unroll
             for (int s = 0; s < KSTEPS; ++s) qreg[rt][s] = pack8<DT_FP16>(widen8<DT>(qreg[rt][s]) * up);
-            m_run[rt] = -INFINITY;
+            u_run[rt] = m_run[rt] = -INFINITY;
             l_run[rt] = 0.f;
 #pragma unroll
             for (int db = 0; db < DBLK; ++db) oacc[rt][db] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -333,14 +338,19 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
     auto end_seg = [&]() {
         const QuantFwdArgs& A = anew();
         const bool whole = cs.S >= t0 && cs.S + cs.n <= t1;
-        const float back = exp2i(eR - 127 - 14);
 #pragma unroll
         for (int rt = 0; rt < NR; ++rt) {
             const int r = rt * 16 + li;
             const float l = wave_sum16x4(l_run[rt]);
             const bool some = l != 0.f;  // NaN: some
-            const float inv = some ? back / l : 0.f;
-            const float lse = some ? (m_run[rt] + fast_log2(l)) * kLn2 : INFINITY;
+            // 2^(u - m) may be out of range where the quotient is not: half of it on either side
+            const float up = apart && some ? fast_exp2(0.5f * (u_run[rt] - m_run[rt])) : 1.f;
+            if (apart) {
+#pragma unroll
+                for (int db = 0; db < DBLK; ++db) oacc[rt][db] *= up;
+            }
+            const float inv = some ? up * 0x1p-14f / l : 0.f;
+            const float lse = some ? add_log2(apart ? m_run[rt] : u_run[rt], l) * kLn2 : INFINITY;
             if (r >= rows) continue;
             if (whole) {
                 const int h = cs.hk * A.g + r % A.g;
@@ -375,13 +385,15 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
         // behind tile t's keys: its values, the next tile's keys and values
         if (t + 1 < t1) wait_loads<3 * C::LOADS>();
         else wait_loads<C::LOADS>();
-        float ks[NH], vs[NH];
+        float ks[NH], lv[NH], iv[NH];
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
             ks[h] = tks[at * NH + h];
-            vs[h] = tvs[at * NH + h];
+            lv[h] = tlv[at * NH + h];
+            iv[h] = tiv[at * NH + h];
         }
-        const int ok = __builtin_amdgcn_readfirstlane(tok[at]);
+        const int bits = __builtin_amdgcn_readfirstlane(tok[at]), ok = bits & ((1 << NH) - 1);
+        const bool plain = bits >> 8 & 1;
         const bool full = ok == (1 << NH) - 1 && key0 >= flo && key0 + KT - 1 <= fhi;
         // S^T = K . Q^T on the codes
         f32x4 x[NR][NH];
@@ -402,18 +414,46 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
             }
         }
         issue_k(t + 2);
-        // scores in log2 units
+        // one reference again where the two are close
+        if (plain && apart) {
+            float d[NR];
+            bool far = false;
 #pragma unroll
-        for (int rt = 0; rt < NR; ++rt)
+            for (int rt = 0; rt < NR; ++rt) {
+                d[rt] = m_run[rt] == u_run[rt] ? 0.f : m_run[rt] - u_run[rt];
+                far |= !(fabsf(d[rt]) <= 60.f);
+            }
+            if (!__ballot(far)) {
+                apart = false;
 #pragma unroll
-            for (int h = 0; h < NH; ++h) x[rt][h] *= qs[rt] * ks[h];
-        if (a.softcap > 0.f)
+                for (int rt = 0; rt < NR; ++rt) l_run[rt] *= fast_exp2(d[rt]);
+            }
+        }
+        if (!plain && !apart) {
+            apart = true;
+#pragma unroll
+            for (int rt = 0; rt < NR; ++rt) m_run[rt] = u_run[rt];
+        }
+        // scores in log2 units, the log2 of V's scale added where there is one reference
+        float add[NH];
+#pragma unroll
+        for (int h = 0; h < NH; ++h) add[h] = apart ? 0.f : lv[h];
+        if (a.softcap > 0.f) {
 #pragma unroll
             for (int rt = 0; rt < NR; ++rt)
 #pragma unroll
                 for (int h = 0; h < NH; ++h)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[rt][h][e] = a.softcap * kLog2e * fast_tanh(x[rt][h][e]);
+                    for (int e = 0; e < 4; ++e)
+                        x[rt][h][e] = __builtin_fmaf(a.softcap * kLog2e, fast_tanh(x[rt][h][e] * (qs[rt] * ks[h])), add[h]);
+        } else {
+#pragma unroll
+            for (int rt = 0; rt < NR; ++rt)
+#pragma unroll
+                for (int h = 0; h < NH; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[rt][h][e] = __builtin_fmaf(x[rt][h][e], qs[rt] * ks[h], add[h]);
+        }
         if (!full) {
 #pragma unroll
             for (int rt = 0; rt < NR; ++rt) {
@@ -428,44 +468,63 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
                     }
             }
         }
-        // R, and the weights' factor for each block
-        float vmax = 0.f;
-#pragma unroll
-        for (int h = 0; h < NH; ++h) vmax = fmaxf(vmax, fabsf(vs[h]) < INFINITY ? fabsf(vs[h]) : 0.f);  // rows may not see what is no number
-        const int e = (int)(__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, vmax)) >> 23) + 1;
-        const int up = max(e - eR, 0);
-        eR += up;
-        const float shrink = up > 126 ? 0.f : exp2i(-up), toR = exp2i(127 + 14 - eR);
-#pragma unroll
-        for (int h = 0; h < NH; ++h) vs[h] *= toR;
-
         u32x4 pk[NR][NH / 2];
+        auto top = [&](const f32x4& y) { return fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])); };
+        if (!apart) {
 #pragma unroll
-        for (int rt = 0; rt < NR; ++rt) {
-            float mx = -INFINITY;
+            for (int rt = 0; rt < NR; ++rt) {
+                float mx = -INFINITY;
 #pragma unroll
-            for (int h = 0; h < NH; ++h) mx = fmaxf(mx, fmaxf(fmaxf(x[rt][h][0], x[rt][h][1]), fmaxf(x[rt][h][2], x[rt][h][3])));
-            mx = fmaxf(m_run[rt], max4(mx));
-            const float m = mx == -INFINITY ? 0.f : mx;
-            const float alpha = fast_exp2(m_run[rt] - m);
-            m_run[rt] = mx;
-            float sum = 0.f;
+                for (int h = 0; h < NH; ++h) mx = fmaxf(mx, top(x[rt][h]));
+                mx = fmaxf(u_run[rt], max4(mx));
+                const float u = mx == -INFINITY ? 0.f : mx;
+                const float alpha = fast_exp2(u_run[rt] - u);
+                u_run[rt] = mx;
+                l_run[rt] *= alpha;
 #pragma unroll
-            for (int k2 = 0; k2 < NH / 2; ++k2) {
-                f32x8 w;
+                for (int k2 = 0; k2 < NH / 2; ++k2) {
+                    f32x8 w;
 #pragma unroll
-                for (int e2 = 0; e2 < 8; ++e2) {
-                    const int h = 2 * k2 + (e2 >> 2);
-                    const float p = fast_exp2(x[rt][h][e2 & 3] - m);
-                    sum += p;
-                    w[e2] = mul_or_0(p, vs[h]);
+                    for (int e2 = 0; e2 < 8; ++e2) w[e2] = fast_exp2(x[rt][2 * k2 + (e2 >> 2)][e2 & 3] - (u - 14.f));
+                    l_run[rt] = __builtin_fmaf((w[0] + w[1]) + (w[2] + w[3]), iv[2 * k2], l_run[rt]);
+                    l_run[rt] = __builtin_fmaf((w[4] + w[5]) + (w[6] + w[7]), iv[2 * k2 + 1], l_run[rt]);
+                    pk[rt][k2] = pack8<DT_FP16>(w);
                 }
-                pk[rt][k2] = pack8<DT_FP16>(w);
-            }
-            l_run[rt] = l_run[rt] * alpha + sum;
-            const float c = alpha * shrink;
 #pragma unroll
-            for (int db = 0; db < DBLK; ++db) oacc[rt][db] *= c;
+                for (int db = 0; db < DBLK; ++db) oacc[rt][db] *= alpha;
+            }
+        } else {
+#pragma unroll
+            for (int rt = 0; rt < NR; ++rt) {
+                float mx = -INFINITY, ux = -INFINITY;
+#pragma unroll
+                for (int h = 0; h < NH; ++h) {
+                    mx = fmaxf(mx, top(x[rt][h]));
+                    ux = fmaxf(ux, top(x[rt][h]) + lv[h]);
+                }
+                mx = fmaxf(m_run[rt], max4(mx));
+                ux = fmaxf(u_run[rt], max4(ux));
+                const float m = mx == -INFINITY ? 0.f : mx, u = ux == -INFINITY ? 0.f : ux;
+                const float alpha = fast_exp2(u_run[rt] - u);
+                l_run[rt] *= fast_exp2(m_run[rt] - m);
+                m_run[rt] = mx;
+                u_run[rt] = ux;
+#pragma unroll
+                for (int k2 = 0; k2 < NH / 2; ++k2) {
+                    f32x8 w;
+#pragma unroll
+                    for (int e2 = 0; e2 < 8; ++e2) {
+                        const int h = 2 * k2 + (e2 >> 2);
+                        const float t = tvs[at * NH + h], y = x[rt][h][e2 & 3], p = fast_exp2(y - m);
+                        l_run[rt] += p;
+                        // a scale that is no number multiplies what is visible
+                        w[e2] = copysignf(fast_exp2(y + lv[h] - (u - 14.f)), t) + mul_or_0(p, fabsf(t) < INFINITY ? 0.f : t);
+                    }
+                    pk[rt][k2] = pack8<DT_FP16>(w);
+                }
+#pragma unroll
+                for (int db = 0; db < DBLK; ++db) oacc[rt][db] *= alpha;
+            }
         }
         // behind tile t's values: the next tile's keys and values, the keys after that
         if (t + 2 < t1) wait_loads<3 * C::LOADS>();

@@ -12,15 +12,14 @@
 //     reads. While the softmax of 32 keys runs, the scores of the next 32 are formed,
 //     and their maximum is taken under the P.V products, in slots of one MFMA and a
 //     share of the vector work (unit()).
-//   * K's scale multiplies the scores of its 16 keys. V's multiplies the weights, kept
-//     relative to a running power of two R (fa_quant_decode.hip): as its log2 in the
-//     exponential's argument, so that the weight comes out whole; the row's sum takes it
+//   * K's scale multiplies the scores of its 16 keys. V's goes into the weights'
+//     exponent (fa_quant.h), so that the weight comes out whole; the row's sum takes it
 //     back once for a block. The running maximum is lazy: it moves only where a
-//     new score exceeds it by 2^4, and the weights' unit leaves room for that
-//     (2^10 in place of 2^14: a weight keeps its 11 bits as long as p t / R > 2^-24).
-//   * Tiles with masked keys, pages outside the cache or scales that are not plain
-//     positive numbers go through a second copy of the unit, which scales the scores
-//     as they are formed and multiplies the weights by V's scale.
+//     new one exceeds it by 2^4, and the weights' unit leaves room for that (the largest
+//     is 2^10 to 2^14: a weight keeps its 11 bits as long as it is more than 2^-24 of that).
+//   * Tiles with masked keys, pages outside the cache or K scales that are not plain
+//     go through a second copy of the unit, which scales the scores as they are formed,
+//     and tiles with V scales that are not plain through a third, with two references a row.
 //
 // What bounds it: the instructions of one wave. 32 keys of 64 rows take 1024 clocks of
 // products; beside them go 32 exponentials (16 clocks each), about 200 other vector
@@ -41,7 +40,8 @@ namespace {
 
 constexpr int NW = 4, NT = NW * 64, NBUF = 3;
 constexpr float kLazy = 4.f;
-constexpr int kUnit = 10;  // w = p t / R 2^kUnit, p <= 2^kLazy
+constexpr float kUnit = 10.f;  // references of weights are this much below their maximum: weights are at most 2^(kUnit + kLazy)
+enum : int { FAST, MASKED, WILD };  // copies of a unit
 
 template <int HD, int RB_>
 struct Cfg {
@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
     __shared__ __attribute__((aligned(256))) char s_raw[2 * NT * 64];  // codes of two tiles, each thread's own
     __shared__ int s_pref[kQuantMaxB + 1];
     __shared__ int64_t s_line[kQuantMaxB + 1];
+    __shared__ float s_m[RB][NT];  // each thread's m of its rows (fa_quant.h), used where V's scales are not plain
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, hi = lane >> 5;
@@ -183,14 +184,14 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
         // rows are and their scales. Page ids are read a group ahead.
         const int* trow = a.table ? a.table + (int64_t)R.q.crow * a.t_stride : nullptr;
         constexpr int kNoKeys = -0x7fffffff - 1;  // page of a block past the item's keys
-        const float low = 0x1p-97f;               // no R is below it
         struct Scales {
             float k, v;
-            uint64_t ok, odd;  // blocks whose page is in the cache; those whose scales are not plain
+            uint64_t ok;        // blocks whose page is in the cache
         };
         Scales sc, sc_new;      // of the group at hand, and of the next once asked for
-        sc_new = Scales{1.f, low, 0, 0};
-        float lv = 0.f, iv_ = 0.f, wv_ = 0.f;  // of sc.v against R: log2, inverse, ratio
+        sc_new = Scales{1.f, 1.f, 0};
+        float lv = 0.f, iv_ = 1.f;     // log2 and inverse of sc.v, which for 0 is 0 and for no number itself
+        uint64_t hard = 0, wild = 0;   // blocks that are not in the cache or whose scales are not plain; whose V scales are not
         int64_t ko = 0, vo = 0;  // where the blocks of the group asked for are
         uint64_t have = 0;       // its sc.ok
         int id_page, id_row;
@@ -213,8 +214,7 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
             const int u = lane % NB / (NB / 2);
             ko = (int64_t)(A.k + ((int64_t)hk * A.k_sh + p * A.k_sp + r * A.k_si)) - 1024 * u;
             vo = (int64_t)(A.v + ((int64_t)hk * A.v_sh + p * A.v_sp + r * A.v_si)) - 1024 * (2 + u);
-            s.k = id_page == kNoKeys ? 1.f : 0.f;  // (0: not plain)
-            s.v = low;
+            s.k = s.v = 1.f;
             if (ok) {
                 const int64_t sb = udiv(A.sblk, (uint32_t)r);
                 s.k = A.ks[p * A.ks_sp + sb * A.ks_sb + (int64_t)hk * A.ks_sh];
@@ -222,8 +222,16 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
             }
             have = s.ok = __ballot(ok);
         };
-        auto find_odd = [&](Scales& s) {
-            s.odd = __ballot(!(anew().scale > 0.f && s.k > 0.f && s.k < INFINITY && s.v > 0x1p-100f && s.v < 0x1p100f));
+        auto wild_of = [&](const Scales& s) { return __ballot(!plain_scale(s.v)); };
+        auto hard_of = [&](const Scales& s) {
+            return ~s.ok | __ballot(!(anew().scale > 0.f && s.k > 0.f && s.k < INFINITY && plain_scale(s.v)));
+        };
+        auto begin_group = [&]() {
+            lv = scale_log2(sc.v);
+            iv_ = copysignf(fminf(fast_exp2(-lv), 0x1p127f), sc.v);
+            iv_ = lv == -INFINITY ? sc.v : iv_;
+            hard = hard_of(sc);
+            wild = wild_of(sc);
         };
         // Rows outside the item, blocks of pages outside the cache and columns past the
         // head dim are read where there is memory, and put down as 0.
@@ -321,11 +329,11 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
         }
 
         f32x16 o[RB][DB];
-        float m[RB], l[RB];
-        int eR = 30;
+        float u[RB], l[RB];  // references (fa_quant.h; less kUnit) and sums of the rows
+        bool apart = false;  // l is relative to m, else to u
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
-            m[rb] = -1e30f;  // finite floor: exp2(x - m) never forms inf - inf
+            u[rb] = -1e30f;  // finite floor: exp2(x - u) never forms inf - inf
             l[rb] = 0.f;
 #pragma unroll
             for (int db = 0; db < DB; ++db)
@@ -364,8 +372,8 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
         };
 
         // Scores of the unit at hand are raw products times cc, or scores themselves (cc =
-        // 1); peak: their largest, in log2 units.
-        float cc[RB][2], peak[RB];
+        // 1); peak: the largest of them with log2 of V's scale added, peakx: of the scores alone.
+        float cc[RB][2], peak[RB], peakx[RB];
         auto scored = [&](f32x16 (&n)[RB], int el, int s0, float c, unsigned ok) {  // s0: key offset of the unit
             const int rb = el / 16, i = el % 16;
             float y = n[rb][i] * c;
@@ -373,42 +381,35 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
             const unsigned seen = ok >> (i / 8) & 1 ? rsee[rb] : 0;
             n[rb][i] = (unsigned)(s0 - rlo[rb] + 8 * (i / 4) + i % 4) < seen ? y : -INFINITY;
         };
-        // moves the running maximum to that of the scores where they exceed it by 2^4; the
-        // sums are multiplied by shrink too
-        auto raise = [&](bool live, float shrink) {
-            bool need = shrink != 1.f;
+        // moves the running maxima to those of the scores where they exceed them by 2^4
+        auto raise = [&](bool live, auto kind) {
+            constexpr bool TWO = decltype(kind)::value == WILD;
+            bool need = false;
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb) need |= peak[rb] > m[rb] + kLazy;
+            for (int rb = 0; rb < RB; ++rb) {
+                need |= peak[rb] > u[rb] + (kUnit + kLazy);
+                if constexpr (TWO) need |= peakx[rb] > s_m[rb][tid] + kLazy;
+            }
             if (live && __ballot(need)) {
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
-                    const float mn = fmaxf(m[rb], fmaxf(peak[rb], __shfl_xor(peak[rb], 32)));
-                    const float alpha = fast_exp2(m[rb] - mn);
-                    m[rb] = mn;
-                    l[rb] *= alpha;
-                    const float by = alpha * shrink;
+                    const float un = fmaxf(u[rb], fmaxf(peak[rb], __shfl_xor(peak[rb], 32)) - kUnit);
+                    const float alpha = fast_exp2(u[rb] - un);
+                    u[rb] = un;
+                    if constexpr (TWO) {
+                        const float m = s_m[rb][tid], mn = fmaxf(m, fmaxf(peakx[rb], __shfl_xor(peakx[rb], 32)));
+                        l[rb] *= fast_exp2(m - mn);
+                        s_m[rb][tid] = mn;
+                    } else {
+                        l[rb] *= alpha;
+                    }
 #pragma unroll
                     for (int db = 0; db < DB; ++db) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[rb][db][i] *= by;
+                        for (int i = 0; i < 16; ++i) o[rb][db][i] *= alpha;
                     }
                 }
             }
-        };
-        // A group's scales come into force: R moves above its V scales, and the sums are to
-        // shrink by what is returned
-        auto begin_group = [&]() {
-            // scales that are no numbers are left out: rows may not see them
-            int top = __builtin_bit_cast(int, sc.v) >> 23 & 255;
-            top = top == 255 ? 0 : top;
-#pragma unroll
-            for (int x = 1; x < 64; x <<= 1) top = max(top, __shfl_xor(top, x));
-            const int up = max(__builtin_amdgcn_readfirstlane(top) + 1 - eR, 0);
-            eR += up;
-            lv = fast_log2(sc.v) + (float)(127 + kUnit - eR);
-            iv_ = exp2i(eR - 127 - kUnit) / sc.v;
-            wv_ = sc.v * exp2i(127 + kUnit - eR);
-            return up > 126 ? 0.f : exp2i(-up);
         };
         const f32x16 zero = {};
 
@@ -417,24 +418,33 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
         // summed and packed; they are spread evenly up to the last keys' P.V products.
         // H: the unit at hand in its tile; its successor's K is read from place A of a tile.
         u32x4 pk[RB][2];
-        float px[NE];
-        auto unit = [&](f32x16 (&c_)[RB], f32x16 (&n_)[RB], auto hh, int tg, int s0n, auto gen, auto more, auto ahead) {
-            constexpr int H = decltype(hh)::value, A = (H + 1) % NH;
-            constexpr bool GEN = decltype(gen)::value, RAW = !GEN && !CAP;
-            float dd[RB][2], nn[RB][2], iv[2], wv[2];
+        float px[NE], lk[2];  // lk: log2 of V's scales of the unit at hand
+        auto unit = [&](f32x16 (&c_)[RB], f32x16 (&n_)[RB], auto hh, int tg, int s0n, auto kind, auto more, auto ahead) {
+            constexpr int H = decltype(hh)::value, A = (H + 1) % NH, KIND = decltype(kind)::value;
+            constexpr bool RAW = KIND == FAST && !CAP, TWO = KIND == WILD;
+            float dd[RB][2], nn[RB][2], iv[2], ln[2];
+            [[maybe_unused]] float sg[2], no[2], m[RB], pw[NE];  // TWO: V's sign, its scale where that is no number, m, weights
             const int bl = tg * NB + 2 * H;  // the unit's blocks; the next unit's follow
             [[maybe_unused]] const unsigned ok = (unsigned)(sc.ok >> ((bl + 2) & 63));
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
                 const float ks = lane_of(sc.k, (bl + 2 + kb) & 63);
-                const float lk = GEN ? 0.f : lane_of(lv, bl + kb);
-                iv[kb] = GEN ? 1.f : lane_of(iv_, bl + kb);
-                wv[kb] = GEN ? lane_of(wv_, bl + kb) : 1.f;
+                ln[kb] = lane_of(lv, (bl + 2 + kb) & 63);
+                iv[kb] = TWO ? 1.f : lane_of(iv_, bl + kb);
+                if constexpr (TWO) {
+                    const float t = lane_of(iv_, bl + kb);
+                    sg[kb] = copysignf(1.f, t);
+                    no[kb] = fabsf(t) < INFINITY ? 0.f : t;
+                }
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
-                    dd[rb][kb] = lk - m[rb];
+                    dd[rb][kb] = lk[kb] - u[rb];
                     nn[rb][kb] = qs[rb] * ks;
                 }
+            }
+            if constexpr (TWO) {
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) m[rb] = s_m[rb][tid];
             }
             float part[RB], top[RB][2];
             int slot = 0;
@@ -444,13 +454,22 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
                     // q-th score: the first 16 keys of every row block, then the others
                     const int ks = q / (8 * RB), rb = q / 8 % RB, i = 8 * ks + q % 8;
                     const int when = q * (SS + SP - 2) / NE;
-                    if (slot == when) px[q] = __builtin_fmaf(c_[rb][i], cc[rb][ks], dd[rb][ks]);
-                    if (slot == when + 1) px[q] = fast_exp2(px[q]);
+                    if (slot == when) {
+                        if constexpr (TWO) {
+                            pw[q] = __builtin_fmaf(c_[rb][i], cc[rb][ks], dd[rb][ks]);
+                            px[q] = __builtin_fmaf(c_[rb][i], cc[rb][ks], -m[rb]);
+                        } else {
+                            px[q] = __builtin_fmaf(c_[rb][i], cc[rb][ks], dd[rb][ks]);
+                        }
+                    }
+                    if (slot == when + 1) {
+                        px[q] = fast_exp2(px[q]);
+                        if constexpr (TWO) pw[q] = fast_exp2(pw[q]);
+                    }
                     if (slot == when + 2) {
                         part[rb] = q % 8 == 0 ? px[q] : part[rb] + px[q];
-                        if (q % 8 == 7) l[rb] = GEN ? l[rb] + part[rb] : __builtin_fmaf(part[rb], iv[ks], l[rb]);
-                        // (0 times any scale is 0: a hidden key's weight)
-                        if constexpr (GEN) px[q] = mul_or_0(px[q], wv[ks]);
+                        if (q % 8 == 7) l[rb] = TWO ? l[rb] + part[rb] : __builtin_fmaf(part[rb], iv[ks], l[rb]);
+                        if constexpr (TWO) px[q] = __builtin_fmaf(pw[q], sg[ks], mul_or_0(px[q], no[ks]));
                         if (q & 1) pk[rb][ks][q / 2 % 4] = pack2<DT_FP16>(px[q - 1], px[q]);
                     }
                 }
@@ -458,7 +477,7 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
                 for (int e = 0; e < NE; ++e) {
                     if (slot != SS + 2 + e * (2 * SP - 4) / NE) continue;
                     const int rb = e / 16, kb = e / 8 % 2;
-                    if constexpr (GEN) {
+                    if constexpr (KIND != FAST) {
                         scored(n_, e, s0n, nn[rb][kb], ok);
                     } else if constexpr (CAP) {
                         n_[rb][e % 16] = cap * fast_tanh(n_[rb][e % 16] * nn[rb][kb]);
@@ -503,15 +522,18 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
             more(2 * SP);
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
-                peak[rb] = RAW ? fmaxf(top[rb][0] * nn[rb][0], top[rb][1] * nn[rb][1]) : fmaxf(top[rb][0], top[rb][1]);
+                if constexpr (RAW) peak[rb] = fmaxf(__builtin_fmaf(top[rb][0], nn[rb][0], ln[0]), __builtin_fmaf(top[rb][1], nn[rb][1], ln[1]));
+                else peak[rb] = fmaxf(top[rb][0] + ln[0], top[rb][1] + ln[1]);
+                if constexpr (TWO) peakx[rb] = fmaxf(top[rb][0], top[rb][1]);
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) cc[rb][kb] = RAW ? nn[rb][kb] : 1.f;
             }
+            lk[0] = ln[0];
+            lk[1] = ln[1];
         };
 
         if (ntiles > 0) {
-            begin_group();  // (the sums are 0)
-            find_odd(sc);
+            begin_group();
             __syncthreads();
             f32x16 s0[RB], s1[RB];
 #pragma unroll
@@ -522,14 +544,21 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
 #pragma unroll
                 for (int s = 0; s < KS; ++s) s0[rb] = mfma32<DT_FP16>(kop[s], qreg[rb][s], s0[rb]);
             }
+            lk[0] = lane_of(lv, 0);
+            lk[1] = lane_of(lv, 1);
 #pragma unroll
-            for (int e2 = 0; e2 < NE; ++e2) {
-                const int rb = e2 / 16;
-                scored(s0, e2, 0, qs[rb] * lane_of(sc.k, e2 / 8 % 2), (unsigned)sc.ok);
-                peak[rb] = e2 % 16 == 0 ? s0[rb][0] : fmaxf(peak[rb], s0[rb][e2 % 16]);
+            for (int rb = 0; rb < RB; ++rb) {  // (the sums are 0)
+                float top[2];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    scored(s0, rb * 16 + i, 0, qs[rb] * lane_of(sc.k, i / 8), (unsigned)sc.ok);
+                    top[i / 8] = i % 8 == 0 ? s0[rb][i] : fmaxf(top[i / 8], s0[rb][i]);
+                }
+                const float mx = fmaxf(top[0], top[1]), ux = fmaxf(top[0] + lk[0], top[1] + lk[1]);
+                u[rb] = fmaxf(u[rb], fmaxf(ux, __shfl_xor(ux, 32)) - kUnit);
+                s_m[rb][tid] = fmaxf(-1e30f, fmaxf(mx, __shfl_xor(mx, 32)));
                 cc[rb][0] = cc[rb][1] = 1.f;
             }
-            raise(true, 1.f);
             if constexpr (NH == 1) {
 #pragma unroll
                 for (int s = 0; s < KS; ++s) move_on(ra[s], TILE);
@@ -559,13 +588,13 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
                     ask(t + 4, ag);
                 }
             };
-            auto tile = [&](auto gen) {
+            auto tile = [&](auto kind) {
                 const unsigned by = step_to(nb);  // from tile t's buffer to the next
                 const int s0k = t * BN;
                 if constexpr (NH > 1) {
                     auto half = [&](auto hh) {
                         constexpr int H = decltype(hh)::value;
-                        unit(H % 2 ? s1 : s0, H % 2 ? s0 : s1, hh, tg, s0k + 32 * (H + 1), gen,
+                        unit(H % 2 ? s1 : s0, H % 2 ? s0 : s1, hh, tg, s0k + 32 * (H + 1), kind,
                              [&](int x) {
                                  if (H == NH - 2 && x == SP / 2) {
 #pragma unroll
@@ -582,7 +611,7 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
                                  }
                              },
                              [&]() { read_rows((H + 2) % NH, 0); });
-                        if constexpr (H < NH - 1) raise(true, 1.f);
+                        if constexpr (H < NH - 1) raise(true, kind);
                     };
                     half(std::integral_constant<int, 0>{});
                     half(std::integral_constant<int, 1>{});
@@ -592,7 +621,7 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
                     }
                 } else {
                     const unsigned by2 = step_to(next_buf(nb));  // from tile t + 1's buffer to the next
-                    unit(s0, s1, std::integral_constant<int, 0>{}, tg, s0k + 32, gen,
+                    unit(s0, s1, std::integral_constant<int, 0>{}, tg, s0k + 32, kind,
                          [&](int x) {
                              if (x == SP / 2) {
 #pragma unroll
@@ -615,45 +644,71 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
                 nb = next_buf(nb);
                 fb = next_buf(fb);
                 ++t;
-                float shrink = 1.f;
                 if (++tg == TPG) {
                     tg = 0;
                     sc = sc_new;
-                    // past the last tile there is no group, and nothing left to shrink
-                    if (t < ntiles) shrink = begin_group();
+                    begin_group();
                 } else if (tg + 1 == TPG) {
-                    // the next tile's scores take scales of the next group: K's go where those of
+                    // the next tile's scores take scales of the next group: they go where those of
                     // this group's first tile were
-                    find_odd(sc_new);
                     sc.k = lane < NB ? sc_new.k : sc.k;
+                    lv = lane < NB ? scale_log2(sc_new.v) : lv;
                     sc.ok = (sc.ok & ~kTileBlocks) | (sc_new.ok & kTileBlocks);
-                    sc.odd = (sc.odd & ~kTileBlocks) | (sc_new.odd & kTileBlocks);
+                    hard = (hard & ~kTileBlocks) | (hard_of(sc_new) & kTileBlocks);
+                    wild = (wild & ~kTileBlocks) | (wild_of(sc_new) & kTileBlocks);
                 }
-                raise(t < ntiles, shrink);
+                raise(t < ntiles, kind);
             };
             // a tile's copy of the unit covers the weights of it and the scores formed in
             // it: those of its later units and of the next tile's first
-            auto general = [&]() {
-                const uint64_t odd = sc.odd >> (tg * NB) | sc.odd >> ((tg + 1) % TPG * NB);
-                return t < t1 || t + 1 >= t2 || (odd & kTileBlocks);
-            };
+            auto among = [&](uint64_t x) { return ((x >> (tg * NB) | x >> ((tg + 1) % TPG * NB)) & kTileBlocks) != 0; };
+            auto odd = [&]() { return t < t1 || t + 1 >= t2 || among(hard); };
+            apart = among(wild);
             while (t < ntiles) {
-                while (t < ntiles && general()) tile(std::true_type{});
-                while (t < ntiles && !general()) tile(std::false_type{});
+                while (t < ntiles && (apart || among(wild))) {
+                    if (!apart) {
+                        apart = true;
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) s_m[rb][tid] = u[rb];
+                    }
+                    tile(std::integral_constant<int, WILD>{});
+                    if (among(wild)) continue;
+                    // one reference again where the two are close
+                    bool far = false;
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) far |= !(fabsf(s_m[rb][tid] - u[rb]) <= 60.f);
+                    if (__ballot(far) == 0) {
+                        apart = false;
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) l[rb] *= fast_exp2(s_m[rb][tid] - u[rb]);
+                    }
+                }
+                while (t < ntiles && odd() && !among(wild)) tile(std::integral_constant<int, MASKED>{});
+                while (t < ntiles && !odd()) tile(std::integral_constant<int, FAST>{});
             }
         }
         wait_loads<0>();  // asked for past the end
         __syncthreads();  // the next item's tiles go where other waves may still read
 
         // ---- results: lane holds O^T [dims 32db + 8q + 4hi + i][row col] --------------------------
-        const float back = exp2i(eR - 127 - kUnit);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             const int r = wrow0 + rb * 32 + col;
             const float lrow = l[rb] + __shfl_xor(l[rb], 32);
             const bool some = lrow != 0.f;
-            const float inv = some ? back / lrow : 0.f;
-            const float lse = some ? (m[rb] + fast_log2(lrow)) * kLn2 : INFINITY;
+            // 2^(u - m) may be out of range where the quotient is not: half of it on either side
+            float m = u[rb], up = 1.f;
+            if (apart) {
+                m = s_m[rb][tid];
+                up = fast_exp2(0.5f * (u[rb] - m));
+#pragma unroll
+                for (int db = 0; db < DB; ++db) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[rb][db][i] *= up;
+                }
+            }
+            const float inv = some ? up / lrow : 0.f;
+            const float lse = some ? add_log2(m, lrow) * kLn2 : INFINITY;
             if (r >= R.rows) continue;
             if (slot < 0) {
                 const int i = r / g, h = hk * g + r % g;
