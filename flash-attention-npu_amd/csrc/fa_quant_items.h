@@ -132,8 +132,7 @@ __global__ void __launch_bounds__(256) fa_quant_prefill_merge_kernel(QuantFwdArg
     const int blk = blockIdx.x % BPT, w = blockIdx.x / BPT;
     const CutItem c = reinterpret_cast<const CutItem*>(a.pf_cut)[w];
     if (c.pieces == 0) return;
-    int sq = a.cu_q ? a.cu_q[c.b + 1] - a.cu_q[c.b] : a.Sq;
-    sq = min(max(sq, 0), a.Sq);
+    const int sq = quant_seq(a, c.b).sq;
     const int rr = blk * RPB + threadIdx.x / DCH, d0 = threadIdx.x % DCH * 8, r = c.mt * BM + rr;
     if (r >= sq * a.g) return;
     auto row = [&](int s) { return (int64_t)(s == 0 ? 2 * w + 1 : 2 * (w + s)) * BM + rr; };

@@ -82,7 +82,9 @@ def flash_attn_with_quantized_kvcache(q, k_cache, v_cache, k_scale, v_scale, cac
     """Attention against a quantised cache (append_quantized_kvcache fills it).
 
     q: (batch_size, seqlen, nheads, headdim) fp16 or bf16 or, with cu_seqlens_q
-    (batch_size + 1,) int32 and max_seqlen_q, (total_q, nheads, headdim).
+    (batch_size + 1,) int32 and max_seqlen_q, at least the rows of each sequence,
+    (total_q, nheads, headdim). Where cu_seqlens_q goes past total_q (update_page_table
+    with too small a total_new), the tokens past it are not there, rows and keys.
     cache_seqlens (batch_size,) int32: the keys of each sequence, the tokens
     that this step appended among them (the last query row is aligned with the
     last key). page_table (rows, max_pages) int32 as from update_page_table, or

@@ -390,7 +390,8 @@ typedef struct fa_quant_fwd_params {
     float* softmax_lse;              /* (B, H, Sq), with cu_seqlens_q (H, total_q) */
     const int32_t* cache_seqlens;    /* (B,) keys of each sequence, the step's own among them */
     const int32_t* cu_seqlens_q;     /* (B + 1,) or NULL */
-    int32_t total_q;                 /* with cu_seqlens_q */
+    int32_t total_q;                 /* with cu_seqlens_q: the rows of q, out and softmax_lse. Rows past it, as of new
+                                        tokens that slot_mapping had no room for, are not there, nor are their keys */
     const int32_t* page_table;       /* (table_rows, max_pages) or NULL: contiguous */
     int64_t page_table_row_stride;
     int32_t table_rows, max_pages;
