@@ -120,11 +120,11 @@ fa_status_t check_fwd(const fa_quant_fwd_params* p) {
     } else {
         FA_CHECK(p->cache_batch_idx || p->num_pages >= p->batch, "the cache must have a row per sequence");
     }
-    // masks count keys from -2^30 to 2^30
+    // positions of rows and keys count from -2^30 to 2^30
     FA_CHECK((int64_t)(p->page_table ? p->max_pages : 1) * p->page_size <= 1 << 30, "a sequence holds at most 2^30 tokens");
     const int64_t rows = p->cu_seqlens_q ? (int64_t)p->total_q : (int64_t)p->batch * p->seqlen_q;
     if (rows == 0 || p->seqlen_q == 0) return FA_OK;
-    FA_CHECK(rows * (p->nheads / p->nheads_k) <= INT_MAX, "too many query rows");
+    FA_CHECK(rows * (p->nheads / p->nheads_k) <= 1 << 30, "too many query rows");
     FA_CHECK(p->q && p->out && p->softmax_lse && p->k && p->v && p->k_scale && p->v_scale,
              "q, out, softmax_lse, the caches and the scales are required");
     FA_CHECK(aligned16(p->q) && aligned16(p->out) && aligned16(p->k) && aligned16(p->v),
@@ -201,7 +201,9 @@ Plan make_plan(const fa_quant_fwd_params* p) {
     return pl;
 }
 
-int window_bound(int32_t w) { return w < 0 ? -1 : std::min(w, 1 << 30); }
+// A window of 2^30 - 1 reaches every key, and the masks' bounds then stay in 32 bits: key_hi
+// + 1 is at most (2^30 - 1) + (2^30 - 1) + 1, key_lo at least -2^30 - (2^30 - 1).
+int window_bound(int32_t w) { return w < 0 ? -1 : std::min(w, (1 << 30) - 1); }
 
 }  // namespace
 
