@@ -14,6 +14,7 @@
 #include "fa_common.h"
 #include "fa_quant_args.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace fa {
@@ -83,10 +84,10 @@ __global__ void __launch_bounds__(256, KEEP > 4 ? 3 : 4) fa_quant_append_kernel(
     constexpr int UNITS = 4 / WPU, LANES = 64 * WPU;
     constexpr uint32_t kInf = DT == DT_FP16 ? 0x7c00u : 0x7f80u;
     const int lane = threadIdx.x & 63, ul = threadIdx.x % LANES;
-    // launch_t: fewer than 2^32. What a wave has in common is told to be in scalar registers.
+    // launch_t: fewer than 2^26. What a wave has in common is told to be in scalar registers.
     const uint32_t unit = blockIdx.x * UNITS + __builtin_amdgcn_readfirstlane(threadIdx.x / LANES);
     const uint32_t chunk = unit / (uint32_t)(2 * a.Hk);
-    const int64_t c0 = (int64_t)chunk * a.rows_per_unit;
+    const int64_t c0 = a.row0 + (int64_t)chunk * a.rows_per_unit;
     if (c0 >= a.total_new) return;  // WPU 4: the whole workgroup
     const int uh = (int)(unit - chunk * (uint32_t)(2 * a.Hk)), kv = uh >= a.Hk ? 1 : 0, h = uh - kv * a.Hk;
     const int ch = a.hd / 8, rp = LANES / ch;            // lanes of a row, rows of a pass
@@ -249,11 +250,19 @@ void launch_t(QuantAppendArgs& a, hipStream_t stream) {
     a.block = udiv_make((uint32_t)a.scale_block);
     a.page = udiv_make((uint32_t)a.page_size);
     a.chunks = udiv_make((uint32_t)a.hd / 8);
-    const int64_t units = (a.total_new + a.rows_per_unit - 1) / a.rows_per_unit * 2 * a.Hk;
-    const dim3 one((unsigned)units), four((unsigned)((units + 3) / 4)), nt(256);
-    if (few) hipLaunchKernelGGL((fa_quant_append_kernel<DT, CT, 1, 4>), four, nt, 0, stream, a);
-    else if (wide) hipLaunchKernelGGL((fa_quant_append_kernel<DT, CT, 4, 16>), one, nt, 0, stream, a);
-    else hipLaunchKernelGGL((fa_quant_append_kernel<DT, CT, 1, 16>), four, nt, 0, stream, a);
+    const int64_t chunks = (a.total_new + a.rows_per_unit - 1) / a.rows_per_unit;
+    // A launch has fewer than 2^32 threads; chunks past that many go into others, one after
+    // another (an even number, so that they fill their workgroups of four units). A run belongs to
+    // the chunk in which it begins.
+    const int64_t most = ((1ll << 32) / 256 - 1) * (wide && !few ? 1 : 4) / (2 * a.Hk) & ~1ll;
+    for (int64_t c = 0; c < chunks; c += most) {
+        a.row0 = c * a.rows_per_unit;
+        const int64_t units = std::min(chunks - c, most) * 2 * a.Hk;
+        const dim3 one((unsigned)units), four((unsigned)((units + 3) / 4)), nt(256);
+        if (few) hipLaunchKernelGGL((fa_quant_append_kernel<DT, CT, 1, 4>), four, nt, 0, stream, a);
+        else if (wide) hipLaunchKernelGGL((fa_quant_append_kernel<DT, CT, 4, 16>), one, nt, 0, stream, a);
+        else hipLaunchKernelGGL((fa_quant_append_kernel<DT, CT, 1, 16>), four, nt, 0, stream, a);
+    }
 }
 
 }  // namespace

@@ -39,6 +39,7 @@ struct QuantAppendArgs {
     int64_t total_new, num_slots;  // num_slots: num_pages * page_size
     int Hk, hd, page_size, scale_block;
     int rows_per_unit;             // rows among which a unit looks for the beginning of a run
+    int64_t row0;                  // first row of the launch
     UDiv block, page, chunks;      // division by scale_block, page_size and hd / 8
 };
 
