@@ -16,6 +16,7 @@ namespace fa {
 fa_status_t report_error(fa_status_t st, const char* msg);
 hipError_t launch_page_table(const PageTableArgs& a, hipStream_t stream);
 hipError_t launch_quant_append(QuantAppendArgs a, int dtype, int ct, hipStream_t stream);
+int64_t quant_decode_batch(int kd, int Hk, int64_t capacity);
 int quant_decode_workers(int kd, int grid);
 hipError_t launch_quant_decode(const QuantFwdArgs& a, int ct, int kd, int nr, int grid, hipStream_t stream);
 int quant_prefill_rows(int kd, bool many);
@@ -101,6 +102,15 @@ fa_status_t check_append(const fa_quant_append_params* p) {
     return FA_OK;
 }
 
+constexpr int kMaxBatch = 2048;  // sequences of one launch (their list lives in LDS)
+
+int kernel_headdim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+int64_t batch_of_launch(const fa_quant_fwd_params* p) {
+    const int64_t capacity = (int64_t)(p->page_table ? p->max_pages : 1) * p->page_size;
+    return std::min<int64_t>(kMaxBatch, fa::quant_decode_batch(kernel_headdim(p->headdim), p->nheads_k, capacity));
+}
+
 fa_status_t check_fwd(const fa_quant_fwd_params* p) {
     FA_CHECK(p != nullptr, "params must not be null");
     FA_CHECK(p->abi_version == FA_MI355X_ABI_VERSION, "abi_version %d does not match library ABI %d", p->abi_version,
@@ -124,6 +134,7 @@ fa_status_t check_fwd(const fa_quant_fwd_params* p) {
     FA_CHECK((int64_t)(p->page_table ? p->max_pages : 1) * p->page_size <= 1 << 30, "a sequence holds at most 2^30 tokens");
     const int64_t rows = p->cu_seqlens_q ? (int64_t)p->total_q : (int64_t)p->batch * p->seqlen_q;
     if (rows == 0 || p->seqlen_q == 0) return FA_OK;
+    FA_CHECK(batch_of_launch(p) >= 1, "a sequence has too many key/value heads and tokens");
     FA_CHECK(rows * (p->nheads / p->nheads_k) <= 1 << 30, "too many query rows");
     FA_CHECK(p->q && p->out && p->softmax_lse && p->k && p->v && p->k_scale && p->v_scale,
              "q, out, softmax_lse, the caches and the scales are required");
@@ -141,11 +152,11 @@ fa_status_t check_fwd(const fa_quant_fwd_params* p) {
     return FA_OK;
 }
 
-constexpr int kMaxBatch = 2048;  // sequences of one launch (their list lives in LDS)
 constexpr int kDecodeRows = 32;  // packed rows of a kv head that the decode kernel takes
 
 struct Plan {
     int kd;          // kernel head dim
+    int nb;          // sequences of a launch
     int g;
     int dec_rows;    // sequences of at most so many packed rows run on the decode kernel
     bool prefill;    // some may have more
@@ -159,7 +170,8 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 Plan make_plan(const fa_quant_fwd_params* p) {
     Plan pl{};
-    pl.kd = p->headdim <= 64 ? 64 : p->headdim <= 128 ? 128 : 256;
+    pl.kd = kernel_headdim(p->headdim);
+    pl.nb = (int)std::min<int64_t>(p->batch, batch_of_launch(p));
     pl.g = p->nheads / p->nheads_k;
     const int64_t rows = (int64_t)p->seqlen_q * pl.g;
     pl.prefill = rows > kDecodeRows;
@@ -167,7 +179,7 @@ Plan make_plan(const fa_quant_fwd_params* p) {
     pl.dec_rows = !pl.prefill ? (int)rows : p->cu_seqlens_q ? 16 : 0;
     pl.nr = pl.dec_rows <= 16 ? 1 : 2;
     const int cus = fa::compute_units();
-    const size_t nb = std::min(p->batch, kMaxBatch);
+    const size_t nb = pl.nb;
     pl.grid = cus;
     size_t off = 0;
     if (pl.dec_rows) {
@@ -355,17 +367,17 @@ fa_status_t fa_quant_fwd(const fa_quant_fwd_params* p, void* stream) {
     a.pf_o = reinterpret_cast<float*>(ws + pl.off_po);
     // a batch of more sequences than a launch lists runs in parts, one after another
     // on the stream and on the same scratch
-    for (int b0 = 0; b0 < p->batch; b0 += kMaxBatch) {
+    for (int64_t b0 = 0; b0 < p->batch; b0 += pl.nb) {
         fa::QuantFwdArgs c = a;
-        c.B = std::min(p->batch - b0, kMaxBatch);
-        c.row0 = b0;
+        c.B = (int)std::min<int64_t>(p->batch - b0, pl.nb);
+        c.row0 = (int)b0;
         c.seqlens = a.seqlens + b0;
         if (a.cu_q) {
             c.cu_q = a.cu_q + b0;
         } else {
-            c.q = static_cast<const uint16_t*>(a.q) + (int64_t)b0 * a.q_sb;
-            c.out = static_cast<uint16_t*>(a.out) + (int64_t)b0 * a.o_sb;
-            c.lse = a.lse + (int64_t)b0 * a.lse_sb;
+            c.q = static_cast<const uint16_t*>(a.q) + b0 * a.q_sb;
+            c.out = static_cast<uint16_t*>(a.out) + b0 * a.o_sb;
+            c.lse = a.lse + b0 * a.lse_sb;
         }
         if (a.batch_idx) c.batch_idx = a.batch_idx + b0;
         hipError_t e = hipSuccess;

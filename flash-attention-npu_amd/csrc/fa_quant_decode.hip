@@ -31,6 +31,8 @@
 #include "fa_quant.h"
 #include "fa_pipe.h"
 
+#include <algorithm>
+
 namespace fa {
 
 namespace {
@@ -693,6 +695,13 @@ void launch_d(const QuantFwdArgs& a, int ct, int nr, int grid, hipStream_t strea
 }
 
 }  // namespace
+
+// Sequences of `capacity` keys that one launch takes: its list of tiles counts in 32 bits, and the
+// merge has fewer than 2^32 threads (kd: kernel head dim)
+int64_t quant_decode_batch(int kd, int Hk, int64_t capacity) {
+    const int64_t hgs = Hk % 4 == 0 ? Hk / 4 : Hk % 2 == 0 ? Hk / 2 : Hk, kt = kd == 64 ? Cfg<64>::KT : Cfg<128>::KT;
+    return std::min(0x7fffffffll / (hgs * (capacity / kt + 2)), 0xffffffffll / MT / ((int64_t)Hk * (kd / 32)));
+}
 
 int quant_decode_workers(int kd, int grid) { return grid * (kd == 256 ? Cfg<256>::NWAVE : Cfg<128>::NWAVE); }
 
