@@ -54,16 +54,20 @@ struct QuantSeq {
 __device__ __forceinline__ QuantSeq quant_seq(const QuantFwdArgs& a, int b) {
     QuantSeq s;
     s.sk = min(max(a.seqlens[b], 0), a.capacity);
+    s.crow = a.row0 + b;
+    if (a.batch_idx) {  // a row that is not there has no keys
+        s.crow = a.batch_idx[b];
+        if ((unsigned)s.crow >= (unsigned)a.rows) s.crow = s.sk = 0;
+    }
     s.sq = a.Sq;
     if (a.cu_q) {
         // rows past total_q are not there, nor are their keys, the sequence's last
-        const int first = a.cu_q[b], end = max(a.cu_q[b + 1], first), in = min(end, a.total_q);
-        s.sk = max(s.sk - (end - max(in, first)), 0);
-        s.sq = first < 0 ? 0 : min(max(in - first, 0), a.Sq);
+        const int first = a.cu_q[b], end = max(a.cu_q[b + 1], first), upto = min(end, a.total_q);
+        s.sk = max(s.sk - (end - max(upto, first)), 0);
+        s.sq = first < 0 ? 0 : min(max(upto - first, 0), a.Sq);
     }
     s.lo = max(0, key_lo(s.sk - s.sq, a.wl, 0));
     s.hi = min(s.sk, key_hi(s.sk - 1, a.wr, 0) + 1);
-    s.crow = a.batch_idx ? min(max(a.batch_idx[b], 0), a.rows - 1) : a.row0 + b;
     if (s.sq == 0) s.hi = s.lo;
     return s;
 }

@@ -64,7 +64,7 @@ struct QuantFwdArgs {
     const int* table;              // null: contiguous, the sequence's row is its page
     int64_t t_stride;
     const int* batch_idx;
-    int rows;                      // rows of the page table, or pages when contiguous (clamp bound of batch_idx)
+    int rows;                      // rows of the page table, or pages when contiguous (bound of batch_idx)
     int num_pages, max_pages, page_size;
     UDiv page, sblk;               // division by page_size and scale_block
     int capacity;                  // keys addressable per sequence

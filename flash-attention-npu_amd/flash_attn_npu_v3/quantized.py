@@ -89,8 +89,8 @@ def flash_attn_with_quantized_kvcache(q, k_cache, v_cache, k_scale, v_scale, cac
     that this step appended among them (the last query row is aligned with the
     last key). page_table (rows, max_pages) int32 as from update_page_table, or
     None for a contiguous cache. cache_batch_idx (batch_size,) int32: the row
-    of the page table (of the contiguous cache) of each sequence. Keys on a page
-    whose id is not in the cache are not visible. A sequence holds at most 2 ** 30
+    of the page table (of the contiguous cache) of each sequence; one whose row is not there has
+    no keys. Keys on a page whose id is not in the cache are not visible. A sequence holds at most 2 ** 30
     tokens. The scales may have any value, and
     reach only the rows that see their keys. A NaN code of v_cache (e4m3) at a key that
     some row of the sequence sees may reach rows that do not see it, as a NaN of v does in

@@ -395,7 +395,8 @@ typedef struct fa_quant_fwd_params {
     const int32_t* page_table;       /* (table_rows, max_pages) or NULL: contiguous */
     int64_t page_table_row_stride;
     int32_t table_rows, max_pages;
-    const int32_t* cache_batch_idx;  /* (B,) row of the page table (of the cache when contiguous), or NULL: row b */
+    const int32_t* cache_batch_idx;  /* (B,) row of the page table (of the cache when contiguous), or NULL: row b.
+                                        A sequence whose row is not there has no keys */
     float softmax_scale;
     float softcap;                   /* 0 = off */
     int32_t is_causal;
