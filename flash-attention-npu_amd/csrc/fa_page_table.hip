@@ -27,14 +27,27 @@ namespace {
 
 constexpr int NT = 1024;
 
+// Sums of counts, none negative. Pages of all requests fit in 32 bits (the host checks),
+// new tokens need not, the lengths being the caller's: their sums (SAT) end at 2^31 - 1.
+template <bool SAT>
+__device__ __forceinline__ int add(int x, int y) {
+    return SAT ? __builtin_elementwise_add_sat(x, y) : x + y;
+}
+
 // exclusive prefix over the workgroup of v, total in `sum`
+template <bool SAT = false>
 __device__ __forceinline__ int block_scan(int v, int* s_w, int& sum) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int incl = v;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const int u = __shfl_up(incl, o);
-        if (lane >= o) incl += u;
+        if (lane >= o) incl = add<SAT>(incl, u);
+    }
+    int excl = incl - v;
+    if constexpr (SAT) {
+        const int u = __shfl_up(incl, 1);
+        excl = lane > 0 ? u : 0;
     }
     __syncthreads();
     if (lane == 63) s_w[wave] = incl;
@@ -42,10 +55,10 @@ __device__ __forceinline__ int block_scan(int v, int* s_w, int& sum) {
     int pre = 0;
     sum = 0;
     for (int w = 0; w < NT / 64; ++w) {
-        pre += w < wave ? s_w[w] : 0;
-        sum += s_w[w];
+        pre = add<SAT>(pre, w < wave ? s_w[w] : 0);
+        sum = add<SAT>(sum, s_w[w]);
     }
-    return pre + incl - v;
+    return add<SAT>(pre, excl);
 }
 
 struct Req {
@@ -71,16 +84,16 @@ __device__ __forceinline__ Req request(const PageTableArgs& a, int b) {
 
 constexpr int MAXB = 4096;  // requests whose sums fit in LDS
 
-// Inclusive prefix of s[1..n] over the workgroup, in place (s[0] = 0); `carry` is
-// scratch.
+// Inclusive prefix of s[1..n] over the workgroup, in place (s[0] = 0); s_w is scratch.
+template <bool SAT = false>
 __device__ __forceinline__ void scan_lds(int* s, int n, int* s_w) {
     int carry = 0;
     for (int b0 = 0; b0 < n; b0 += NT) {
         const int b = b0 + threadIdx.x, v = b < n ? s[b + 1] : 0;
         int sum;
-        const int pre = carry + block_scan(v, s_w, sum);
-        carry += sum;
-        if (b < n) s[b + 1] = pre + v;
+        const int pre = add<SAT>(carry, block_scan<SAT>(v, s_w, sum));
+        carry = add<SAT>(carry, sum);
+        if (b < n) s[b + 1] = add<SAT>(pre, v);
     }
     if (threadIdx.x == 0) s[0] = 0;
     __syncthreads();
@@ -103,7 +116,7 @@ __global__ void __launch_bounds__(NT) fa_page_table_kernel(PageTableArgs a) {
     }
     scan_lds(s_rel, B, s_w);
     scan_lds(s_take, B, s_w);
-    scan_lds(s_fresh, B, s_w);
+    scan_lds<true>(s_fresh, B, s_w);
     const int raw = s_rel[B], taken = s_take[B], fresh = s_fresh[B];
     // released entry f of the requests in turn: its request, place among the request's, id
     auto entry = [&](int f, int& b, int& j) -> int {
@@ -211,8 +224,8 @@ __global__ void __launch_bounds__(NT) fa_page_table_large_kernel(PageTableArgs a
             const int at = top - 1 - (t0 + j - r.have);
             row[j] = at >= 0 ? a.free_pages[at] : -1;
         }
-        const int f0 = fresh + block_scan(r.fresh, s_w, sum);
-        fresh += sum;
+        const int f0 = add<true>(fresh, block_scan<true>(r.fresh, s_w, sum));
+        fresh = add<true>(fresh, sum);
         if (b < a.B) a.cu_new[b] = f0;
     }
     if (threadIdx.x == 0) {

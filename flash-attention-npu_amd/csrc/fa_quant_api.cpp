@@ -52,6 +52,8 @@ fa_status_t check_table(const fa_page_table_params* p) {
     FA_CHECK(p->table_rows >= 0 && p->max_pages >= 0, "page_table sizes must not be negative");
     FA_CHECK(p->cache_batch_idx || p->table_rows >= p->batch, "page_table must have a row per request");
     FA_CHECK((int64_t)p->max_pages * p->page_size <= INT_MAX, "page_table rows hold at most 2^31 - 1 tokens");
+    // the kernel's counters of pages go a few thousand past the last
+    FA_CHECK((int64_t)p->batch * p->max_pages <= 1 << 30, "the requests of a step have at most 2^30 pages");
     FA_CHECK(p->page_table || (int64_t)p->table_rows * p->max_pages == 0, "page_table is required");
     FA_CHECK(p->page_table_row_stride >= p->max_pages || p->table_rows <= 1, "page_table rows must not overlap");
     FA_CHECK(p->free_capacity >= 0 && (p->free_pages || p->free_capacity == 0), "free_pages is required");

@@ -45,7 +45,7 @@ def update_page_table(page_table, cache_seqlens, new_seqlens, free_pages, num_fr
       slot_mapping (total_new,) int64: the slots, page * page_size + row, of the
         new tokens of all requests in turn; -1 for a token without a page
         (stack empty, past max_pages * page_size) and behind the last one;
-      cu_seqlens_new (batch_size + 1,) int32: their starts;
+      cu_seqlens_new (batch_size + 1,) int32: their starts, at most 2 ** 31 - 1;
       num_free_out (1,) int32: the stack's new count, to be given to the next
         step, or less than 0 by as many pages as were missing.
 

@@ -323,7 +323,7 @@ typedef struct fa_page_table_params {
     int32_t free_capacity;
     const int32_t* num_free;         /* (1,) ids on the stack; taken as within [0, free_capacity] */
     int32_t* num_free_out;           /* (1,) ids on it after the step, negative by the pages that were missing */
-    int32_t* cu_seqlens_new;         /* (batch + 1,) prefix of the new tokens of the requests */
+    int32_t* cu_seqlens_new;         /* (batch + 1,) prefix of the new tokens of the requests, 2^31 - 1 where it is more */
     int64_t* slot_mapping;           /* (total_new,) slot of each new token, -1 where there is none */
     int64_t total_new;
 } fa_page_table_params;
