@@ -16,6 +16,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 
@@ -701,6 +702,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> varlen_bwd(const Tensor& dout, const 
 }
 
 // ---- the quantised cache: page table, append, attention ----------------------------------------
+// Sizes that the C entries take in 32 bits.
+int32_t i32(int64_t n, const char* name) {
+    TORCH_CHECK(n <= INT32_MAX, name, " must be less than 2^31, got ", n);
+    return (int32_t)n;
+}
+
 const int32_t* i32_vec(const Tensor& t, const Tensor& on, int64_t n, const char* name) {
     check_dev(t, on, name);
     TORCH_CHECK(t.scalar_type() == at::kInt, name, " must have dtype int32");
@@ -724,17 +731,17 @@ std::tuple<Tensor, Tensor, Tensor> update_page_table(Tensor& page_table, const T
     TORCH_CHECK(B >= 1, "batch size must be positive");
     fa_page_table_params p{};
     p.abi_version = FA_MI355X_ABI_VERSION;
-    p.batch = (int32_t)B;
+    p.batch = i32(B, "batch size");
     p.page_size = (int32_t)page_size;
-    p.table_rows = (int32_t)page_table.size(0);
-    p.max_pages = (int32_t)page_table.size(1);
+    p.table_rows = i32(page_table.size(0), "rows of page_table");
+    p.max_pages = i32(page_table.size(1), "columns of page_table");
     p.page_table = page_table.data_ptr<int32_t>();
     p.page_table_row_stride = page_table.stride(0);
     if (cache_batch_idx.has_value()) p.cache_batch_idx = i32_vec(*cache_batch_idx, page_table, B, "cache_batch_idx");
     p.cache_seqlens = i32_vec(cache_seqlens, page_table, B, "cache_seqlens");
     p.new_seqlens = i32_vec(new_seqlens, page_table, B, "new_seqlens");
     p.free_pages = const_cast<int32_t*>(i32_vec(free_pages, page_table, free_pages.numel(), "free_pages"));
-    p.free_capacity = (int32_t)free_pages.size(0);
+    p.free_capacity = i32(free_pages.size(0), "size of free_pages");
     p.num_free = i32_vec(num_free, page_table, 1, "num_free");
     Tensor slots = at::empty({total_new}, page_table.options().dtype(at::kLong));
     Tensor cu = at::empty({B + 1}, page_table.options());
@@ -779,10 +786,10 @@ void set_quant_cache(P& p, const Tensor& kcache, const Tensor& vcache, const Ten
     p.abi_version = FA_MI355X_ABI_VERSION;
     p.dtype = dtype_code(q);
     p.cache_dtype = cache_code(kcache, "k_cache");
-    p.nheads_k = (int32_t)kcache.size(2);
-    p.headdim = (int32_t)headdim;
-    p.num_pages = (int32_t)kcache.size(0);
-    p.page_size = (int32_t)page;
+    p.nheads_k = i32(kcache.size(2), "number of key/value heads");
+    p.headdim = i32(headdim, "head size");
+    p.num_pages = i32(kcache.size(0), "number of pages");
+    p.page_size = i32(page, "page size");
     p.scale_block = (int32_t)(page / kscale.size(1));
     p.k_page_stride = kcache.stride(0);
     p.k_row_stride = kcache.stride(1);
@@ -856,8 +863,8 @@ std::tuple<Tensor, Tensor> quant_fwd(const Tensor& q, const Tensor& kcache, cons
                           : q.contiguous();
     const int64_t B = ragged ? cu_seqlens_q->numel() - 1 : q.size(0);
     TORCH_CHECK(B >= 1, "batch size must be positive");
-    p.batch = (int32_t)B;
-    p.nheads = (int32_t)q.size(-2);
+    p.batch = i32(B, "batch size");
+    p.nheads = i32(q.size(-2), "number of heads");
     Tensor out = at::empty(q.sizes(), q.options());
     Tensor lse = ragged ? at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat))
                         : at::empty({B, q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
@@ -867,13 +874,13 @@ std::tuple<Tensor, Tensor> quant_fwd(const Tensor& q, const Tensor& kcache, cons
     if (ragged) {
         p.cu_seqlens_q = i32_vec(*cu_seqlens_q, q, B + 1, "cu_seqlens_q");
         p.seqlen_q = (int32_t)max_seqlen_q;
-        p.total_q = (int32_t)q.size(0);
+        p.total_q = i32(q.size(0), "rows of q");
         p.q_row_stride = qc.stride(0);
         p.q_head_stride = qc.stride(1);
         p.out_row_stride = out.stride(0);
         p.out_head_stride = out.stride(1);
     } else {
-        p.seqlen_q = (int32_t)q.size(1);
+        p.seqlen_q = i32(q.size(1), "seqlen_q");
         p.q_batch_stride = qc.stride(0);
         p.q_row_stride = qc.stride(1);
         p.q_head_stride = qc.stride(2);
@@ -888,16 +895,16 @@ std::tuple<Tensor, Tensor> quant_fwd(const Tensor& q, const Tensor& kcache, cons
                     "page_table must be an int32 matrix with contiguous rows");
         p.page_table = page_table->data_ptr<int32_t>();
         p.page_table_row_stride = page_table->stride(0);
-        p.table_rows = (int32_t)page_table->size(0);
-        p.max_pages = (int32_t)page_table->size(1);
+        p.table_rows = i32(page_table->size(0), "rows of page_table");
+        p.max_pages = i32(page_table->size(1), "columns of page_table");
         TORCH_CHECK(p.table_rows >= 1 && p.max_pages >= 1, "page_table must have rows and columns");
     }
     if (cache_batch_idx.has_value()) p.cache_batch_idx = i32_vec(*cache_batch_idx, q, B, "cache_batch_idx");
     p.softmax_scale = (float)softmax_scale;
     p.softcap = (float)softcap;
     p.is_causal = is_causal ? 1 : 0;
-    p.window_size_left = (int32_t)std::min<int64_t>(window_size_left, INT32_MAX);
-    p.window_size_right = (int32_t)std::min<int64_t>(window_size_right, INT32_MAX);
+    p.window_size_left = (int32_t)std::clamp<int64_t>(window_size_left, -1, INT32_MAX);
+    p.window_size_right = (int32_t)std::clamp<int64_t>(window_size_right, -1, INT32_MAX);
     size_t bytes = 0;
     check_status(fa_quant_fwd_workspace_size(&p, &bytes));
     Tensor ws;
