@@ -200,7 +200,9 @@ Plan make_plan(const fa_quant_fwd_params* p) {
         const int64_t items = entries * p->nheads_k;
         // Cutting costs its pieces' sums a way through memory (chunks of 2048 onto 4096 keys,
         // four items to a workgroup: 921 -> 971 us). It pays where items differ in
-        // length (ragged) or a last round would leave workgroups without one.
+        // length or a last round would leave workgroups without one. The host sees the latter,
+        // and of the former only ragged queries: key lengths that differ under queries of
+        // one length leave whole items to be shared out by their number.
         const int64_t rounds = (items + cus - 1) / cus;
         pl.cut = entries <= kMaxBatch && items < 8 * cus && (p->cu_seqlens_q || rounds * cus * 12 > items * 13);
         pl.pf_grid = pl.cut ? cus : (int)std::min<int64_t>(items, cus);

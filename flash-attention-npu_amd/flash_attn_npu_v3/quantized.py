@@ -40,7 +40,8 @@ def update_page_table(page_table, cache_seqlens, new_seqlens, free_pages, num_fr
 
     Pages that are no longer needed go onto the stack first, then needed ones
     come off it, both in the order of the requests. Where the stack runs empty
-    the table gets -1. Returns (slot_mapping, cu_seqlens_new, num_free_out):
+    the table gets -1, and keeps it until the request shrinks below that page or ends: later steps
+    count the page as held, and its tokens have no slots. Returns (slot_mapping, cu_seqlens_new, num_free_out):
 
       slot_mapping (total_new,) int64: the slots, page * page_size + row, of the
         new tokens of all requests in turn; -1 for a token without a page
@@ -69,7 +70,9 @@ def append_quantized_kvcache(k, v, k_cache, v_cache, k_scale, v_scale, slot_mapp
     its row 0) keeps its scale if that is the larger; otherwise the codes before that row
     are rounded to the new scale. Codes are x / s rounded to the nearest, ties
     to even. +-inf counts as the type's largest finite value; NaN becomes 0 in
-    int8 and NaN in e4m3."""
+    int8 and NaN in e4m3. The new rows of one block and head are one workgroup's work, and so are the
+    codes before them that move: blocks of thousands of tokens (a contiguous cache with one scale a
+    sequence) are slow."""
     _append(k, v, k_cache, v_cache, k_scale, v_scale, maybe_contiguous(slot_mapping))
 
 
@@ -100,7 +103,8 @@ def flash_attn_with_quantized_kvcache(q, k_cache, v_cache, k_scale, v_scale, cac
     of each key's codes, the weights of the values carry v_scale, and both
     products run on the codes without rounding them (fp32 sums). causal,
     window_size and softcap as in flash_attn_with_kvcache. A row that sees no
-    key gets 0 and a softmax_lse of +inf. Returns out, or (out, softmax_lse)
+    key gets 0 and a softmax_lse of +inf. Rows behind the last sequence of cu_seqlens_q are not
+    written: what out and softmax_lse hold there means nothing. Returns out, or (out, softmax_lse)
     with softmax_lse (batch_size, nheads, seqlen) or (nheads, total_q) fp32."""
     if softmax_scale is None:
         softmax_scale = q.shape[-1] ** (-0.5)

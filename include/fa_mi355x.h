@@ -331,7 +331,7 @@ typedef struct fa_page_table_params {
 /* Takes the step in this order. Pages that requests no longer need go onto the
  * stack, request by request (ids below 0 and ids that the stack has no room for
  * are dropped). Pages that requests need come off its top, request by request; an
- * empty stack gives -1. Tokens past max_pages * page_size have no page. Entries
+ * empty stack gives -1, which stays until the request shrinks below that page or ends. Tokens past max_pages * page_size have no page. Entries
  * of num_free_out, cu_seqlens_new and slot_mapping may not overlap the inputs. */
 fa_status_t fa_update_page_table(const fa_page_table_params* p, void* stream);
 
