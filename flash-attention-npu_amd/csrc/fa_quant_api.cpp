@@ -137,7 +137,7 @@ fa_status_t check_fwd(const fa_quant_fwd_params* p) {
     const int64_t rows = p->cu_seqlens_q ? (int64_t)p->total_q : (int64_t)p->batch * p->seqlen_q;
     if (rows == 0 || p->seqlen_q == 0) return FA_OK;
     FA_CHECK(batch_of_launch(p) >= 1, "a sequence has too many key/value heads and tokens");
-    FA_CHECK(rows * (p->nheads / p->nheads_k) <= 1 << 30, "too many query rows");
+    FA_CHECK(rows <= 1 << 30 && rows * (p->nheads / p->nheads_k) <= 1 << 30, "too many query rows");
     FA_CHECK(p->q && p->out && p->softmax_lse && p->k && p->v && p->k_scale && p->v_scale,
              "q, out, softmax_lse, the caches and the scales are required");
     FA_CHECK(aligned16(p->q) && aligned16(p->out) && aligned16(p->k) && aligned16(p->v),
@@ -175,7 +175,8 @@ Plan make_plan(const fa_quant_fwd_params* p) {
     pl.kd = kernel_headdim(p->headdim);
     pl.nb = (int)std::min<int64_t>(p->batch, batch_of_launch(p));
     pl.g = p->nheads / p->nheads_k;
-    const int64_t rows = (int64_t)p->seqlen_q * pl.g;
+    // of a ragged batch seqlen_q is a bound, and may be beyond the 2^30 rows of a call
+    const int64_t rows = std::min<int64_t>((int64_t)p->seqlen_q * pl.g, 1 << 30);
     pl.prefill = rows > kDecodeRows;
     // of a ragged batch with longer sequences the ones at their next token or two
     pl.dec_rows = !pl.prefill ? (int)rows : p->cu_seqlens_q ? 16 : 0;
