@@ -30,6 +30,7 @@
 // Tiles in registers instead of LDS, with one wave per SIMD: 190, 55, 36 and 15 us.
 #include "fa_quant.h"
 #include "fa_pipe.h"
+#include "fa_quant_split.h"
 
 #include <algorithm>
 
@@ -56,26 +57,6 @@ struct Cfg {
 };
 
 __device__ __forceinline__ int heads_per_group(const QuantFwdArgs& a) { return a.Hk % 4 == 0 ? 4 : a.Hk % 2 == 0 ? 2 : 1; }
-
-// The list holds T tiles, sequence by sequence and head group by head group; the
-// first We of W workers share it, T = q We + r: r of them take q + 1 tiles. Workers
-// have kMinTiles at least, since a partial costs its merge about what a tile costs here.
-constexpr int kMinTiles = 2;
-struct Split {
-    int We, q, r;
-    __device__ __forceinline__ int first(int w) const { return w < We ? w * q + min(w, r) : We * q + r; }
-    __device__ __forceinline__ int owner(int t) const {
-        const uint32_t u = (uint32_t)t, big = (uint32_t)r * (uint32_t)(q + 1);
-        return (int)(u < big ? u / (uint32_t)(q + 1) : (uint32_t)r + (u - big) / (uint32_t)q);
-    }
-};
-__device__ __forceinline__ Split split_list(int T, int W) {
-    Split s;
-    s.We = max(min(W, T / kMinTiles), 1);
-    s.q = (int)((uint32_t)T / (uint32_t)s.We);
-    s.r = T - s.q * s.We;
-    return s;
-}
 
 struct Seg {
     int S, n;      // first tile of the list, tiles

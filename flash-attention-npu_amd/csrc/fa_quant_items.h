@@ -3,6 +3,7 @@
 #pragma once
 #include "fa_quant.h"
 #include "fa_pipe.h"
+#include "fa_quant_split.h"
 
 #include <type_traits>
 
@@ -78,24 +79,7 @@ __device__ __forceinline__ int find_in(const T* s, int n, X x) {  // the last i 
 
 // The list: an entry is a tile of BM rows of a sequence, an item an entry of one kv
 // head. Every workgroup makes the list alike, in LDS.
-//
-// Ragged items, or few, are cut: laid end to end, head after head, their costs
-// make a line that the workgroups share evenly, so one piece begins and one ends
-// inside an item at most. Costs are in units of 32 keys: an item takes kStart more than
-// its tiles of keys, and a workgroup takes at least kLeast. Ragged batch of 40 sequences
-// of 64 to 8192 keys: 281 us with whole items in turn, 194 cut; kStart of 8, 16, 24: 207,
-// 185, 183 us.
-constexpr int kStart = 16, kLeast = 48;
-
-struct Line {
-    int64_t len;   // of one head
-    int64_t total;
-    int workers;
-    __device__ int64_t cut(int w) const { return w * total / workers; }
-    // the worker that holds place x: the last w with cut(w) <= x
-    __device__ int holder(int64_t x) const { return (int)(((x + 1) * workers - 1) / total); }
-};
-
+// Ragged items, or few, are cut (fa_quant_split.h).
 template <int BM, int BN, int NW>
 __device__ void build_list(const QuantFwdArgs& a, int* s_pref, int64_t* s_line) {
     constexpr int NT = NW * 64;

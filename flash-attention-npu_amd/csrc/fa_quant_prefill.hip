@@ -116,9 +116,7 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
     int worker = blockIdx.x;
     int64_t at = 0, end;  // places on the line, or numbers of whole items
     if (a.cut) {
-        line.len = s_line[min(entries, kQuantMaxB)];
-        line.total = line.len * a.Hk;
-        line.workers = (int)min((int64_t)grid, max((int64_t)1, line.total / kLeast));
+        line = make_line(s_line[min(entries, kQuantMaxB)], a.Hk, grid);
         // all at work: neighbours on the line, who read the same keys, share an XCD's L2
         if (line.workers == grid && grid % 8 == 0) worker = worker % 8 * (grid / 8) + worker / 8;
         if (tid == 0) reinterpret_cast<CutItem*>(a.pf_cut)[worker] = CutItem{0, 0, 0, 0};
@@ -156,8 +154,8 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
         int k_lo = K.lo, k_hi = K.hi;
         if (a.cut) {
             const int64_t p0 = hk * line.len + s_line[e], p1 = hk * line.len + s_line[e + 1], upto = min(end, p1);
-            if (at > p0) t_lo = max(0, (int)((at - p0 - kStart) / NH));
-            if (upto < p1) t_hi = max(0, (int)((upto - p0 - kStart) / NH));
+            if (at > p0) t_lo = tile_at(at - p0, NH);
+            if (upto < p1) t_hi = tile_at(upto - p0, NH);
             if (at > p0 || upto < p1) {
                 slot = at > p0 ? 2 * worker : 2 * worker + 1;
                 if (at == p0 && tid == 0)

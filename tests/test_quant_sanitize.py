@@ -27,3 +27,9 @@ def build_and_run(tmp_path, *args):
 def test_checks_and_plans(tmp_path):
     build_and_run(tmp_path, "-D__HIP_PLATFORM_AMD__=1", "-I", "/opt/rocm/include", "-I", os.path.join(REPO, "include"),
                   os.path.join(CSRC, "fa_quant_api.cpp"), os.path.join(HOST, "fa_quant_host_harness.cpp"))
+
+
+def test_split_against_brute_force(tmp_path):
+    """The decode list's and the prefill line's split (csrc/fa_quant_split.h, host and device code alike): ranges, owners,
+    pieces of items and the counts that the merges go by."""
+    build_and_run(tmp_path, os.path.join(HOST, "fa_quant_split_check.cpp"))
