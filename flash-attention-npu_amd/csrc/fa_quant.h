@@ -80,6 +80,28 @@ __device__ __forceinline__ int64_t lse_at(const QuantFwdArgs& a, int b, int h, i
     return a.cu_q ? (int64_t)h * a.lse_sh + a.cu_q[b] + i : (int64_t)b * a.lse_sb + (int64_t)h * a.lse_sh + i;
 }
 
+// Inclusive prefix sums in place over s[1 .. n], by one wave; s[0] = 0
+template <typename T>
+__device__ __forceinline__ void prefix_sums(T* s, int n) {
+    const int lane = threadIdx.x & 63, seg = (n + 63) / 64, b0 = lane * seg;
+    T local = 0;
+    for (int k = 0; k < seg; ++k)
+        if (b0 + k < n) local += s[b0 + k + 1];
+    T incl = local;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const T v = __shfl_up(incl, o);
+        if (lane >= o) incl += v;
+    }
+    T run = incl - local;
+    for (int k = 0; k < seg; ++k)
+        if (b0 + k < n) {
+            run += s[b0 + k + 1];
+            s[b0 + k + 1] = run;
+        }
+    if (lane == 0) s[0] = 0;
+}
+
 // x y, and 0 where x is 0, whatever y: a hidden key's weight
 __device__ __forceinline__ float mul_or_0(float x, float y) {
     float r;

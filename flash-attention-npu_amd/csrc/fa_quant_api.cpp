@@ -104,13 +104,11 @@ fa_status_t check_append(const fa_quant_append_params* p) {
     return FA_OK;
 }
 
-constexpr int kMaxBatch = 2048;  // sequences of one launch (their list lives in LDS)
-
 int kernel_headdim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 int64_t batch_of_launch(const fa_quant_fwd_params* p) {
     const int64_t capacity = (int64_t)(p->page_table ? p->max_pages : 1) * p->page_size;
-    return std::min<int64_t>(kMaxBatch, fa::quant_decode_batch(kernel_headdim(p->headdim), p->nheads_k, capacity));
+    return std::min<int64_t>(fa::kQuantMaxB, fa::quant_decode_batch(kernel_headdim(p->headdim), p->nheads_k, capacity));
 }
 
 fa_status_t check_fwd(const fa_quant_fwd_params* p) {
@@ -205,7 +203,7 @@ Plan make_plan(const fa_quant_fwd_params* p) {
         // and of the former only ragged queries: key lengths that differ under queries of
         // one length leave whole items to be shared out by their number.
         const int64_t rounds = (items + cus - 1) / cus;
-        pl.cut = entries <= kMaxBatch && items < 8 * cus && (p->cu_seqlens_q || rounds * cus * 12 > items * 13);
+        pl.cut = entries <= fa::kQuantMaxB && items < 8 * cus && (p->cu_seqlens_q || rounds * cus * 12 > items * 13);
         pl.pf_grid = pl.cut ? cus : (int)std::min<int64_t>(items, cus);
         if (pl.cut) {
             pl.off_pcut = off;

@@ -10,6 +10,8 @@ namespace fa {
 // Cache types, as FA_DTYPE_FP8_E4M3 and FA_DTYPE_INT8.
 enum : int { CT_E4M3 = 3, CT_INT8 = 4 };
 
+constexpr int kQuantMaxB = 2048;  // sequences of an attention launch, and entries of a list that is cut: they live in LDS
+
 struct PageTableArgs {
     int* table;
     int64_t t_stride;

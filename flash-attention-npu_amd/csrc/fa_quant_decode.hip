@@ -38,8 +38,6 @@ namespace fa {
 
 namespace {
 
-constexpr int MAXB = 2048;
-
 template <int HD>
 struct Cfg {
     static constexpr int NWAVE = HD == 256 ? 4 : 8;    // waves of a workgroup
@@ -123,7 +121,7 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
     constexpr int NWAVE = C::NWAVE, NT = NWAVE * 64, KT = C::KT, NH = C::NH, TAB = C::TAB, KL = C::KL, KSTEPS = C::KSTEPS,
                   DBLK = C::DBLK, LPB = C::LPB;
     __shared__ __attribute__((aligned(1024))) uint8_t s_ring[NWAVE][4 * C::TILE];
-    __shared__ int s_pref[MAXB + 1];
+    __shared__ int s_pref[kQuantMaxB + 1];
     __shared__ int64_t s_koff[NWAVE][64], s_voff[NWAVE][64];
     __shared__ float s_ks[NWAVE][64], s_vs[NWAVE][64], s_lv[NWAVE][64], s_iv[NWAVE][64];
     __shared__ int s_ok[NWAVE][64 / NH];
@@ -145,25 +143,7 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
         s_pref[b + 1] = s.hi > s.lo && s.sq * a.g <= a.dec_rows ? hgs * ((s.hi + KT - 1) / KT - s.lo / KT) : 0;
     }
     __syncthreads();
-    if (wave == 0) {
-        const int seg = (a.B + 63) / 64, b0 = lane * seg;
-        int local = 0;
-        for (int k = 0; k < seg; ++k)
-            if (b0 + k < a.B) local += s_pref[b0 + k + 1];
-        int incl = local;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(incl, o);
-            if (lane >= o) incl += v;
-        }
-        int run = incl - local;
-        for (int k = 0; k < seg; ++k)
-            if (b0 + k < a.B) {
-                run += s_pref[b0 + k + 1];
-                s_pref[b0 + k + 1] = run;
-            }
-        if (lane == 0) s_pref[0] = 0;
-    }
+    if (wave == 0) prefix_sums(s_pref, a.B);
     __syncthreads();
     if (blockIdx.x == 0)
         for (int b = tid; b <= a.B; b += NT) a.sched[b] = s_pref[b];

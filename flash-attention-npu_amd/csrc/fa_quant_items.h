@@ -11,8 +11,6 @@ namespace fa {
 
 namespace {
 
-constexpr int kQuantMaxB = 2048;  // sequences of a launch, and entries of a list that is cut: they live in LDS
-
 struct Rows {
     int rows, mt;
     QuantSeq q;
@@ -42,28 +40,6 @@ __device__ __forceinline__ Keys keys_of(const QuantFwdArgs& a, const QuantSeq& q
 template <int BN>
 __device__ __forceinline__ int tiles_of(const Keys& k) {
     return (k.hi - (k.lo & ~15) + BN - 1) / BN;  // tiles start at a block of 16 keys
-}
-
-// Exclusive prefix sums in place over s[1 .. n], by one wave; s[0] = 0
-template <typename T>
-__device__ void prefix_sums(T* s, int n) {
-    const int lane = threadIdx.x & 63, seg = (n + 63) / 64, b0 = lane * seg;
-    T local = 0;
-    for (int k = 0; k < seg; ++k)
-        if (b0 + k < n) local += s[b0 + k + 1];
-    T incl = local;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const T v = __shfl_up(incl, o);
-        if (lane >= o) incl += v;
-    }
-    T run = incl - local;
-    for (int k = 0; k < seg; ++k)
-        if (b0 + k < n) {
-            run += s[b0 + k + 1];
-            s[b0 + k + 1] = run;
-        }
-    if (lane == 0) s[0] = 0;
 }
 
 template <typename T, typename X>
