@@ -14,7 +14,7 @@
 // read from L2) and then writes its share of stack, table and slots; an id that
 // this step both releases and takes is found in the table, where its owner's row
 // is not written, so no workgroup waits for another. Measured: 64 requests 6 us
-// (10 with the call, as the host is slower than the kernel), 1024 of which an eighth
+// (10 with the call: the host dispatches and allocates three results), 1024 of which an eighth
 // end 18, 96 prompts of 512 to 8192 tokens 10; as two launches the last two took 77 and 75.
 #include "fa_common.h"
 #include "fa_quant_args.h"

@@ -23,10 +23,10 @@
 // weights' exponent (fa_quant.h), 2^14 w rounded to fp16: a weight keeps its 11 bits as
 // long as it is more than 2^-28 of its row's largest.
 //
-// Measured (D128, g 4 and 8): 64 paged e4m3 sequences, 966 MB: 187-194 us, 5.0-5.2 TB/s; 32
-// contiguous int8 ones, 194 MB: 52 us; 4 tokens over a window of 4096, 8 sequences:
-// 31.6 us; one sequence of 777 keys: 15 us, of which the start before the first
-// tile (list, ids, rows, scales: each waits for the one before) takes 5 and the merge 6.
+// Measured (D128, g 4 and 8): 64 paged e4m3 sequences, 966 MB: 188-194 us, 5.0-5.2 TB/s; 32
+// contiguous int8 ones, 194 MB: 53 us; 4 tokens over a window of 4096, 8 sequences:
+// 32 us; one sequence of 777 keys: 15.3 us, 12 here, of which the start before the first
+// tile (list, ids, rows, scales: each waits for the one before) is most, and 4 in the merge.
 // Tiles in registers instead of LDS, with one wave per SIMD: 190, 55, 36 and 15 us.
 #include "fa_quant.h"
 #include "fa_pipe.h"

@@ -21,14 +21,14 @@
 //     go through a second copy of the unit, which scales the scores as they are formed,
 //     and tiles with V scales that are not plain through a third, with two references a row.
 //
-// What bounds it: the instructions of one wave. 32 keys of 64 rows take 1024 clocks of
-// products; beside them go 32 exponentials (16 clocks each), about 200 other vector
+// What bounds it: the instructions of one wave. 32 keys of 64 rows take about 2640 clocks,
+// 1024 of them products; beside them go 32 exponentials (16 clocks each), about 200 other vector
 // instructions and the reads. Measured: chunk of 2048 onto 4096 keys, B4 H32/8 D128 e4m3:
-// 725 us, 948 TFLOP/s (two waves per SIMD of 32 rows each, which do products and softmax
+// 742-757 us, 910-930 TFLOP/s (two waves per SIMD of 32 rows each, which do products and softmax
 // mostly one after the other: 921; page ids and scales of each tile looked up
 // in that tile instead of for 64 blocks at once: 927); 40 ragged sequences, H24/8 D64
-// int8: 185 us, of which the 800 starts of items (ids, rows, q one after another)
-// are a third.
+// int8: 185 us, 150 of them here, where waves wait 27 % of the time, for the 800 starts of items (ids,
+// rows, q one after another) above all.
 #include "fa_pipe.h"
 #include "fa_quant_items.h"
 
