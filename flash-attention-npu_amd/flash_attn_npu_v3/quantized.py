@@ -94,7 +94,7 @@ def flash_attn_with_quantized_kvcache(q, k_cache, v_cache, k_scale, v_scale, cac
     None for a contiguous cache. cache_batch_idx (batch_size,) int32: the row
     of the page table (of the contiguous cache) of each sequence; one whose row is not there has
     no keys. Keys on a page whose id is not in the cache are not visible. A sequence holds at most 2 ** 30
-    tokens. The scales may have any value, and
+    tokens. The scales may have any value (scale * code in the range of fp32), and
     reach only the rows that see their keys. A NaN code of v_cache (e4m3) at a key that
     some row of the sequence sees may reach rows that do not see it, as a NaN of v does in
     flash_attn_with_kvcache.

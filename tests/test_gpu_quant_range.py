@@ -25,7 +25,7 @@ def attend(c, q, **kw):
 def v_scales(c, b):
     """Of each key (n, Hk)."""
     j = torch.arange(c.lens[b])
-    pages = torch.tensor(c.pages[b])[j // c.page]
+    pages = torch.tensor(c.pages[b], dtype=torch.long)[j // c.page]
     return c.scales[1][pages, j % c.page // c.block].double()
 
 
