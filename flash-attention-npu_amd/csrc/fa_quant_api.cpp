@@ -176,7 +176,9 @@ Plan make_plan(const fa_quant_fwd_params* p) {
     // of a ragged batch seqlen_q is a bound, and may be beyond the 2^30 rows of a call
     const int64_t rows = std::min<int64_t>((int64_t)p->seqlen_q * pl.g, 1 << 30);
     pl.prefill = rows > kDecodeRows;
-    // of a ragged batch with longer sequences the ones at their next token or two
+    // Of a ragged batch with longer sequences the ones at their next token or two: with 32 rows in place of
+    // 16 the two row tiles of the decode kernel cost a mixed batch 2 us of 185, where its shorter ones
+    // are single tokens; 64 sequences of 2 to 7 tokens of 8 heads take 353 us in place of 403.
     pl.dec_rows = !pl.prefill ? (int)rows : p->cu_seqlens_q ? 16 : 0;
     pl.nr = pl.dec_rows <= 16 ? 1 : 2;
     const int cus = fa::compute_units();
