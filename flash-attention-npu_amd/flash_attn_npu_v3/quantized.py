@@ -51,7 +51,8 @@ def update_page_table(page_table, cache_seqlens, new_seqlens, free_pages, num_fr
         step, or less than 0 by as many pages as were missing.
 
     No new token is dropped if total_new is at least the sum of
-    max(new_seqlens - cache_seqlens, 0). Nothing is read back to the host."""
+    max(new_seqlens - cache_seqlens, 0). batch_size * max_pages is at most 2 ** 30. Nothing is read
+    back to the host."""
     return _update_page_table(page_table, maybe_contiguous(cache_seqlens), maybe_contiguous(new_seqlens), free_pages,
                               num_free, int(page_size), int(total_new), maybe_contiguous(cache_batch_idx))
 
@@ -94,7 +95,7 @@ def flash_attn_with_quantized_kvcache(q, k_cache, v_cache, k_scale, v_scale, cac
     None for a contiguous cache. cache_batch_idx (batch_size,) int32: the row
     of the page table (of the contiguous cache) of each sequence; one whose row is not there has
     no keys. Keys on a page whose id is not in the cache are not visible. A sequence holds at most 2 ** 30
-    tokens. The scales may have any value (scale * code in the range of fp32), and
+    tokens, a call 2 ** 30 query rows x query heads of a kv head. The scales may have any value (scale * code in the range of fp32), and
     reach only the rows that see their keys. A NaN code of v_cache (e4m3) at a key that
     some row of the sequence sees may reach rows that do not see it, as a NaN of v does in
     flash_attn_with_kvcache.
