@@ -7,8 +7,8 @@
 
 namespace fa {
 
-// Cache types, as FA_DTYPE_FP8_E4M3 and FA_DTYPE_INT8.
-enum : int { CT_E4M3 = 3, CT_INT8 = 4 };
+// Cache types, as FA_DTYPE_FP8_E4M3, FA_DTYPE_INT8 and FA_DTYPE_FP4_E2M1.
+enum : int { CT_E4M3 = 3, CT_INT8 = 4, CT_FP4 = 5 };
 
 constexpr int kQuantMaxB = 2048;  // sequences of an attention launch, and entries of a list that is cut: they live in LDS
 

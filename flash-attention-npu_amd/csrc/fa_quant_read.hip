@@ -1,0 +1,124 @@
+// fa_quant_read.hip -- rows of a quantised cache as values of 16 or 32 bits: fa_quant_read.
+//
+// One pass: codes and scales in, values out, which are most of what moves (2 bytes
+// for 0.53 of a 4-bit cache).
+#include "fa_fp4.h"
+#include "fa_quant_read_args.h"
+
+#include <algorithm>
+
+namespace fa {
+
+namespace {
+
+constexpr int kMostRows = 32;  // rows of a workgroup
+enum : int { DT_F32 = 2 };
+
+// A thread makes 8 channels of a row and head, of k and of v.
+template <int OT, int CT>
+__global__ void __launch_bounds__(256) fa_quant_read_kernel(QuantReadArgs a, int rows_per_group) {
+    __shared__ int64_t s_at[4][kMostRows];  // k, v, their scales; -1: the row has no place
+    const int64_t r0 = a.row0 + (int64_t)blockIdx.x * rows_per_group;
+    const int n = (int)min((int64_t)rows_per_group, a.total - r0);
+    if ((int)threadIdx.x < n) {
+        const int64_t row = r0 + threadIdx.x;
+        int64_t page = -1, j = 0;
+        if (a.slots) {
+            const int64_t s = a.slots[row];
+            if (s >= 0 && s < a.num_slots) {
+                page = a.num_slots <= 0xffffffffll ? (int64_t)udiv(a.page, (uint32_t)s) : s / a.page_size;
+                j = s - page * a.page_size;
+            }
+        } else if (row >= a.cu[0] && row < a.cu[a.B]) {
+            const int b = seq_of(a.cu, a.B, (int)row);
+            const int64_t key = row - a.cu[b];  // below 0 where cu is no prefix sum
+            int64_t at = b;
+            if (a.batch_idx) at = a.batch_idx[b];
+            if (at >= 0 && at < a.rows && key >= 0 && key < a.capacity) {
+                const int64_t pi = udiv(a.page, (uint32_t)key);
+                j = key - pi * a.page_size;
+                page = a.table ? (int64_t)a.table[at * a.t_stride + pi] : at;
+                if (page >= a.num_pages) page = -1;
+            }
+        }
+        const bool ok = page >= 0;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+            s_at[kv][threadIdx.x] = ok ? page * a.c_sp[kv] + j * a.c_si[kv] : -1;
+            s_at[2 + kv][threadIdx.x] = ok ? page * a.s_sp[kv] + (CT == CT_FP4 ? j : (int64_t)udiv(a.sblk, (uint32_t)j)) * a.s_sb[kv] : 0;
+        }
+    }
+    __syncthreads();
+    for (uint32_t id = threadIdx.x; id < (uint32_t)n * a.per_row.d; id += 256) {
+        const int r = (int)udiv(a.per_row, id);
+        const uint32_t in = id - (uint32_t)r * a.per_row.d, h = udiv(a.chunks, in), c = in - h * a.chunks.d;
+        const bool ok = s_at[0][r] != -1;
+        const int64_t to = ((r0 + r) * (int64_t)a.per_row.d + in) * 8;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+            f32x8 y = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            u32x4 o = {0u, 0u, 0u, 0u};
+            if (ok) {
+                const uint8_t* codes = a.c[kv] + s_at[kv][r] + (int64_t)h * a.c_sh[kv];
+                const int64_t sat = s_at[2 + kv][r] + (int64_t)h * a.s_sh[kv];
+                if constexpr (CT == CT_FP4) {
+                    const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + c * 4);
+                    const float s = fp4_scale(static_cast<const uint8_t*>(a.s[kv])[sat + c / 4]);
+                    if constexpr (OT == DT_F32) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            typedef float f32x2 __attribute__((ext_vector_type(2)));
+                            f32x2 p;
+                            if (e == 0) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0);
+                            else if (e == 1) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
+                            else if (e == 2) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2);
+                            else p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
+                            y[2 * e] = p[0];
+                            y[2 * e + 1] = p[1];
+                        }
+                    } else {
+                        o = fp4_widen8<OT>(w, s);
+                    }
+                } else {
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(codes + c * 8);
+                    const float s = static_cast<const float*>(a.s[kv])[sat];
+                    const u32x2 lo = widen4<CT>(w[0]), hi = widen4<CT>(w[1]);  // exact in fp16
+                    y = widen8<DT_FP16>(u32x4{lo[0], lo[1], hi[0], hi[1]}) * s;
+                    if constexpr (OT != DT_F32) o = pack8<OT>(y);
+                }
+            }
+            if constexpr (OT == DT_F32) {
+                float* t = static_cast<float*>(a.o[kv]) + to;
+                *reinterpret_cast<f32x4*>(t) = f32x4{y[0], y[1], y[2], y[3]};
+                *reinterpret_cast<f32x4*>(t + 4) = f32x4{y[4], y[5], y[6], y[7]};
+            } else {
+                *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.o[kv]) + to) = o;
+            }
+        }
+    }
+}
+
+template <int OT>
+void launch_read_t(const QuantReadArgs& a, int ct, int rows, dim3 grid, hipStream_t stream) {
+    const dim3 nt(256);
+    if (ct == CT_FP4) hipLaunchKernelGGL((fa_quant_read_kernel<OT, CT_FP4>), grid, nt, 0, stream, a, rows);
+    else if (ct == CT_INT8) hipLaunchKernelGGL((fa_quant_read_kernel<OT, CT_INT8>), grid, nt, 0, stream, a, rows);
+    else hipLaunchKernelGGL((fa_quant_read_kernel<OT, CT_E4M3>), grid, nt, 0, stream, a, rows);
+}
+
+}  // namespace
+
+hipError_t launch_quant_read(QuantReadArgs a, int dtype, int ct, hipStream_t stream) {
+    const int rows = (int)std::min<int64_t>(std::max<int64_t>(a.total / 2048, 1), kMostRows);
+    const int64_t groups = (a.total + rows - 1) / rows, most = (1 << 24) - 1;  // less than 2^32 threads of a launch
+    for (int64_t g = 0; g < groups; g += most) {
+        a.row0 = g * rows;
+        const dim3 grid((unsigned)std::min(groups - g, most));
+        if (dtype == DT_F32) launch_read_t<DT_F32>(a, ct, rows, grid, stream);
+        else if (dtype == DT_BF16) launch_read_t<DT_BF16>(a, ct, rows, grid, stream);
+        else launch_read_t<DT_FP16>(a, ct, rows, grid, stream);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace fa

@@ -1,7 +1,8 @@
 // fa_torch_ops.cpp -- PyTorch-ROCm operators over the C ABI (libfa_mi355x.so).
 //
 // Registers torch.ops.fa_mi355x.{fwd_kvcache, fwd_kvcache_v3, fwd, varlen_fwd, fwd_combine,
-// fwd_combine_out, bwd, varlen_bwd, update_page_table, quant_append, quant_fwd}.
+// fwd_combine_out, bwd, varlen_bwd, update_page_table, quant_append, quant_fwd,
+// quant_read, rotary_table, rotary, rotary_}.
 // Argument order and meaning follow the reference pybind entry points
 // (csrc/arch22/flash_attn_npu_v2/flash_api.cpp: mha_fwd_kvcache :356-377,
 // mha_fwd :628-640, mha_varlen_fwd :828-850, bound at :1301-1309). Unlike the
@@ -757,8 +758,11 @@ std::tuple<Tensor, Tensor, Tensor> update_page_table(Tensor& page_table, const T
 int32_t cache_code(const Tensor& t, const char* name) {
     if (t.scalar_type() == at::kChar) return FA_DTYPE_INT8;
     if (t.scalar_type() == at::kFloat8_e4m3fn) return FA_DTYPE_FP8_E4M3;
-    TORCH_CHECK(false, name, " must hold int8 or float8_e4m3fn");
+    if (t.scalar_type() == at::kByte || t.scalar_type() == at::kFloat4_e2m1fn_x2) return FA_DTYPE_FP4_E2M1;
+    TORCH_CHECK(false, name, " must hold int8, float8_e4m3fn or float4_e2m1fn_x2 (or its bytes, uint8)");
 }
+
+constexpr int64_t kGroup = 32;  // channels of a 4-bit cache that share a scale
 
 // The caches and their scales, in the fields that the append and the attention share.
 template <typename P>
@@ -768,29 +772,36 @@ void set_quant_cache(P& p, const Tensor& kcache, const Tensor& vcache, const Ten
     check_dev(vcache, q, "v_cache");
     check_dev(kscale, q, "k_scale");
     check_dev(vscale, q, "v_scale");
-    TORCH_CHECK(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16,
-                "FlashAttention only support fp16 and bf16 data type");
     TORCH_CHECK(kcache.dim() == 4 && vcache.sizes() == kcache.sizes(),
                 "k_cache and v_cache must have shape (num_pages, page_size, num_heads_k, head_size)");
     TORCH_CHECK(kcache.scalar_type() == vcache.scalar_type(), "k_cache and v_cache must have the same dtype");
     TORCH_CHECK(kcache.stride(3) == 1 && vcache.stride(3) == 1, "the caches must have contiguous last dimension");
-    TORCH_CHECK(kcache.size(3) == headdim, "head size of the caches must match");
-    TORCH_CHECK(kscale.scalar_type() == at::kFloat && vscale.scalar_type() == at::kFloat,
-                "k_scale and v_scale must have dtype fp32");
-    const int64_t page = kcache.size(1);
-    TORCH_CHECK(kscale.dim() == 3 && vscale.sizes() == kscale.sizes() && kscale.size(0) == kcache.size(0) &&
-                    kscale.size(2) == kcache.size(2),
-                "k_scale and v_scale must have shape (num_pages, blocks of a page, num_heads_k)");
-    TORCH_CHECK(kscale.size(1) >= 1 && page % kscale.size(1) == 0, "page_size ", page,
-                " must be a multiple of the blocks of a page, ", kscale.size(1));
     p.abi_version = FA_MI355X_ABI_VERSION;
-    p.dtype = dtype_code(q);
     p.cache_dtype = cache_code(kcache, "k_cache");
+    const bool four = p.cache_dtype == FA_DTYPE_FP4_E2M1;
+    TORCH_CHECK(kcache.size(3) * (four ? 2 : 1) == headdim, "head size of the caches must match");
+    const int64_t page = kcache.size(1);
+    if (four) {
+        auto bytes = [](const Tensor& t) { return t.scalar_type() == at::kByte || t.scalar_type() == at::kFloat8_e8m0fnu; };
+        TORCH_CHECK(bytes(kscale) && bytes(vscale), "k_scale and v_scale of a 4-bit cache must have dtype float8_e8m0fnu (or uint8)");
+        TORCH_CHECK(kscale.dim() == 4 && vscale.sizes() == kscale.sizes() && kscale.size(0) == kcache.size(0) &&
+                        kscale.size(1) == page && kscale.size(2) == kcache.size(2) && kscale.size(3) * kGroup == headdim,
+                    "k_scale and v_scale of a 4-bit cache must have shape (num_pages, page_size, num_heads_k, head_size / 32)");
+        TORCH_CHECK(kscale.stride(3) == 1 && vscale.stride(3) == 1, "k_scale and v_scale must have contiguous last dimension");
+    } else {
+        TORCH_CHECK(kscale.scalar_type() == at::kFloat && vscale.scalar_type() == at::kFloat,
+                    "k_scale and v_scale must have dtype fp32");
+        TORCH_CHECK(kscale.dim() == 3 && vscale.sizes() == kscale.sizes() && kscale.size(0) == kcache.size(0) &&
+                        kscale.size(2) == kcache.size(2),
+                    "k_scale and v_scale must have shape (num_pages, blocks of a page, num_heads_k)");
+        TORCH_CHECK(kscale.size(1) >= 1 && page % kscale.size(1) == 0, "page_size ", page,
+                    " must be a multiple of the blocks of a page, ", kscale.size(1));
+    }
     p.nheads_k = i32(kcache.size(2), "number of key/value heads");
     p.headdim = i32(headdim, "head size");
     p.num_pages = i32(kcache.size(0), "number of pages");
     p.page_size = i32(page, "page size");
-    p.scale_block = (int32_t)(page / kscale.size(1));
+    p.scale_block = four ? 1 : (int32_t)(page / kscale.size(1));
     p.k_page_stride = kcache.stride(0);
     p.k_row_stride = kcache.stride(1);
     p.k_head_stride = kcache.stride(2);
@@ -799,14 +810,19 @@ void set_quant_cache(P& p, const Tensor& kcache, const Tensor& vcache, const Ten
     p.v_head_stride = vcache.stride(2);
     p.k = kcache.data_ptr();
     p.v = vcache.data_ptr();
-    p.k_scale = kscale.data_ptr<float>();
+    p.k_scale = kscale.data_ptr();
     p.k_scale_page_stride = kscale.stride(0);
     p.k_scale_block_stride = kscale.stride(1);
     p.k_scale_head_stride = kscale.stride(2);
-    p.v_scale = vscale.data_ptr<float>();
+    p.v_scale = vscale.data_ptr();
     p.v_scale_page_stride = vscale.stride(0);
     p.v_scale_block_stride = vscale.stride(1);
     p.v_scale_head_stride = vscale.stride(2);
+}
+
+void check_16bit(const Tensor& t) {
+    TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16,
+                "FlashAttention only support fp16 and bf16 data type");
 }
 
 void quant_append(const Tensor& k, const Tensor& v, Tensor& kcache, Tensor& vcache, Tensor& kscale, Tensor& vscale,
@@ -816,7 +832,9 @@ void quant_append(const Tensor& k, const Tensor& v, Tensor& kcache, Tensor& vcac
     TORCH_CHECK(k.dim() == 3 && v.sizes() == k.sizes(), "k and v must have shape (total_new, num_heads_k, head_size)");
     check_dev(v, k, "v");
     TORCH_CHECK(v.scalar_type() == k.scalar_type(), "k and v must have the same dtype");
+    check_16bit(k);
     fa_quant_append_params p{};
+    p.dtype = dtype_code(k);
     set_quant_cache(p, kcache, vcache, kscale, vscale, k, k.size(2));
     TORCH_CHECK(k.size(1) == p.nheads_k, "k must have the key/value heads of the cache");
     check_dev(slot_mapping, k, "slot_mapping");
@@ -838,7 +856,7 @@ void quant_append(const Tensor& k, const Tensor& v, Tensor& kcache, Tensor& vcac
     p.vnew_row_stride = vn.stride(0);
     p.vnew_head_stride = vn.stride(1);
     p.slot_mapping = slot_mapping.data_ptr<int64_t>();
-    check_status(fa_quant_append(&p, cur_stream()));
+    check_status(p.cache_dtype == FA_DTYPE_FP4_E2M1 ? fa_fp4_append(&p, cur_stream()) : fa_quant_append(&p, cur_stream()));
 }
 
 std::tuple<Tensor, Tensor> quant_fwd(const Tensor& q, const Tensor& kcache, const Tensor& vcache, const Tensor& kscale,
@@ -855,7 +873,9 @@ std::tuple<Tensor, Tensor> quant_fwd(const Tensor& q, const Tensor& kcache, cons
         TORCH_CHECK(q.dim() == 4, "q must have shape (batch_size, seqlen_q, num_heads, head_size)");
     }
     TORCH_CHECK(max_seqlen_q >= 0 && max_seqlen_q <= INT32_MAX, "max_seqlen_q must be >= 0");
+    check_16bit(q);
     fa_quant_fwd_params p{};
+    p.dtype = dtype_code(q);
     set_quant_cache(p, kcache, vcache, kscale, vscale, q, q.size(-1));
     const Tensor qc = q.stride(-1) == 1 && q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 && q.stride(-2) % 8 == 0 &&
                               ((uintptr_t)q.data_ptr() & 15) == 0
@@ -906,15 +926,211 @@ std::tuple<Tensor, Tensor> quant_fwd(const Tensor& q, const Tensor& kcache, cons
     p.window_size_left = (int32_t)std::clamp<int64_t>(window_size_left, -1, INT32_MAX);
     p.window_size_right = (int32_t)std::clamp<int64_t>(window_size_right, -1, INT32_MAX);
     size_t bytes = 0;
-    check_status(fa_quant_fwd_workspace_size(&p, &bytes));
+    const bool four = p.cache_dtype == FA_DTYPE_FP4_E2M1;
+    check_status(four ? fa_fp4_fwd_workspace_size(&p, &bytes) : fa_quant_fwd_workspace_size(&p, &bytes));
     Tensor ws;
     if (bytes) {
         ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
         p.workspace = ws.data_ptr();
         p.workspace_bytes = bytes;
     }
-    check_status(fa_quant_fwd(&p, cur_stream()));
+    check_status(four ? fa_fp4_fwd(&p, cur_stream()) : fa_quant_fwd(&p, cur_stream()));
     return {out, lse};
+}
+
+std::tuple<Tensor, Tensor> quant_read(const Tensor& kcache, const Tensor& vcache, const Tensor& kscale, const Tensor& vscale,
+                                      const OptT& slot_mapping, const OptT& cu_seqlens_k, int64_t total_k, const OptT& page_table,
+                                      const OptT& cache_batch_idx, at::ScalarType dtype) {
+    c10::DeviceGuard guard(kcache.device());
+    TORCH_CHECK(kcache.is_cuda(), "k_cache must be on a GPU device");
+    TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16 || dtype == at::kFloat, "dtype must be fp16, bf16 or fp32");
+    TORCH_CHECK(kcache.dim() == 4, "k_cache and v_cache must have shape (num_pages, page_size, num_heads_k, head_size)");
+    TORCH_CHECK(slot_mapping.has_value() != cu_seqlens_k.has_value(), "either slot_mapping or cu_seqlens_k is required");
+    fa_quant_read_params p{};
+    p.dtype = dtype == at::kHalf ? FA_DTYPE_FP16 : dtype == at::kBFloat16 ? FA_DTYPE_BF16 : FA_DTYPE_FP32;
+    const int64_t headdim = kcache.size(3) * (cache_code(kcache, "k_cache") == FA_DTYPE_FP4_E2M1 ? 2 : 1);
+    set_quant_cache(p, kcache, vcache, kscale, vscale, kcache, headdim);
+    if (slot_mapping.has_value()) {
+        TORCH_CHECK(!page_table.has_value() && !cache_batch_idx.has_value(), "slot_mapping comes without page_table and cache_batch_idx");
+        check_dev(*slot_mapping, kcache, "slot_mapping");
+        TORCH_CHECK(slot_mapping->scalar_type() == at::kLong && slot_mapping->dim() == 1 && slot_mapping->is_contiguous(),
+                    "slot_mapping must be a contiguous int64 vector");
+        p.total = slot_mapping->size(0);
+        p.slot_mapping = slot_mapping->data_ptr<int64_t>();
+    } else {
+        TORCH_CHECK(total_k >= 0, "total_k must be >= 0");
+        TORCH_CHECK(cu_seqlens_k->numel() >= 2, "cu_seqlens_k must have batch_size + 1 entries");
+        p.batch = i32(cu_seqlens_k->numel() - 1, "batch size");
+        p.cu_seqlens_k = i32_vec(*cu_seqlens_k, kcache, cu_seqlens_k->numel(), "cu_seqlens_k");
+        p.total = total_k;
+        if (page_table.has_value()) {
+            check_dev(*page_table, kcache, "page_table");
+            TORCH_CHECK(page_table->scalar_type() == at::kInt && page_table->dim() == 2 && page_table->stride(1) == 1,
+                        "page_table must be an int32 matrix with contiguous rows");
+            TORCH_CHECK(page_table->numel() > 0, "page_table must have rows and columns");
+            p.page_table = page_table->data_ptr<int32_t>();
+            p.page_table_row_stride = page_table->stride(0);
+            p.table_rows = i32(page_table->size(0), "rows of page_table");
+            p.max_pages = i32(page_table->size(1), "columns of page_table");
+        }
+        if (cache_batch_idx.has_value()) p.cache_batch_idx = i32_vec(*cache_batch_idx, kcache, p.batch, "cache_batch_idx");
+    }
+    const auto opts = kcache.options().dtype(dtype);
+    Tensor k = at::empty({p.total, p.nheads_k, p.headdim}, opts), v = at::empty({p.total, p.nheads_k, p.headdim}, opts);
+    p.k_out = k.data_ptr();
+    p.v_out = v.data_ptr();
+    check_status(fa_quant_read(&p, cur_stream()));
+    return {k, v};
+}
+
+// ---- rotary positions --------------------------------------------------------------------------
+std::tuple<Tensor, Tensor> rotary_table(const Tensor& positions, int64_t rotary_dim, double base, int64_t scaling, double factor,
+                                        double original_length, double low, double high, double attention_factor,
+                                        at::ScalarType dtype) {
+    c10::DeviceGuard guard(positions.device());
+    TORCH_CHECK(positions.is_cuda(), "positions must be on a GPU device");
+    TORCH_CHECK(positions.dim() == 1 && positions.is_contiguous() &&
+                    (positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong),
+                "positions must be a contiguous int32 or int64 vector");
+    TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16 || dtype == at::kFloat, "dtype must be fp16, bf16 or fp32");
+    TORCH_CHECK(rotary_dim >= 16 && rotary_dim <= 256 && rotary_dim % 16 == 0, "rotary_dim must be a multiple of 16, at most 256");
+    fa_rotary_table_params p{};
+    p.abi_version = FA_MI355X_ABI_VERSION;
+    p.dtype = dtype == at::kHalf ? FA_DTYPE_FP16 : dtype == at::kBFloat16 ? FA_DTYPE_BF16 : FA_DTYPE_FP32;
+    p.rotary_dim = (int32_t)rotary_dim;
+    p.scaling = (int32_t)std::clamp<int64_t>(scaling, -1, 100);
+    p.base = base;
+    p.factor = factor;
+    p.original_length = original_length;
+    p.low = low;
+    p.high = high;
+    p.attention_factor = attention_factor;
+    p.num_positions = positions.size(0);
+    p.positions = positions.data_ptr();
+    p.positions_int64 = positions.scalar_type() == at::kLong;
+    const auto opts = positions.options().dtype(dtype);
+    Tensor c = at::empty({p.num_positions, rotary_dim / 2}, opts), s = at::empty({p.num_positions, rotary_dim / 2}, opts);
+    p.cos = c.data_ptr();
+    p.sin = s.data_ptr();
+    check_status(fa_rotary_table(&p, cur_stream()));
+    return {c, s};
+}
+
+bool rows_of_16(const Tensor& t) {
+    bool ok = (t.stride(-1) == 1 || t.size(-1) <= 1) && ((uintptr_t)t.data_ptr() & 15) == 0;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
+    return ok;
+}
+
+// q (and k) turned into qo (and ko), which may be q and k
+void rotary_into(const Tensor& q, const OptT& k, Tensor& qo, const OptT& ko, const Tensor& cos, const Tensor& sin,
+                 const OptT& positions, const OptT& seqlen_offsets, int64_t seqlen_offset, const OptT& cu_seqlens, bool interleaved,
+                 bool conjugate) {
+    const int64_t B = q.dim() == 4 ? q.size(0) : cu_seqlens.has_value() ? cu_seqlens->numel() - 1 : 1;
+    const int64_t S = q.dim() == 4 ? q.size(1) : q.size(0);
+    fa_rotary_params p{};
+    p.abi_version = FA_MI355X_ABI_VERSION;
+    p.dtype = dtype_code(q);
+    p.table_dtype = cos.scalar_type() == at::kFloat ? (int32_t)FA_DTYPE_FP32 : dtype_code(cos);
+    p.nheads = i32(q.size(-2), "number of heads");
+    p.headdim = i32(q.size(-1), "head size");
+    p.rotary_dim = i32(2 * cos.size(1), "rotary_dim");
+    p.batch = i32(B, "batch size");
+    if (cu_seqlens.has_value()) {
+        TORCH_CHECK(q.dim() == 3, "q must have shape (total, num_heads, head_size) with cu_seqlens");
+        TORCH_CHECK(B >= 1, "cu_seqlens must have batch_size + 1 entries");
+        p.total = i32(S, "rows of q");
+        p.cu_seqlens = i32_vec(*cu_seqlens, q, B + 1, "cu_seqlens");
+    } else {
+        p.seqlen = i32(S, "seqlen");
+    }
+    auto step = [](const Tensor& t, int64_t i) { return t.size(i) > 1 ? t.stride(i) : 0; };  // one entry: any stride
+    auto strides = [&](const Tensor& t, int64_t& sb, int64_t& si, int64_t& sh) {
+        sb = t.dim() == 4 ? step(t, 0) : 0;
+        si = step(t, -3);
+        sh = step(t, -2);
+    };
+    p.q = q.data_ptr();
+    strides(q, p.q_batch_stride, p.q_row_stride, p.q_head_stride);
+    p.q_out = qo.data_ptr();
+    strides(qo, p.q_out_batch_stride, p.q_out_row_stride, p.q_out_head_stride);
+    if (k.has_value()) {
+        p.nheads_k = i32(k->size(-2), "number of key/value heads");
+        p.k = k->data_ptr();
+        strides(*k, p.k_batch_stride, p.k_row_stride, p.k_head_stride);
+        p.k_out = ko->data_ptr();
+        strides(*ko, p.k_out_batch_stride, p.k_out_row_stride, p.k_out_head_stride);
+    }
+    auto table = [](const Tensor& t) { return rows_of_16(t) ? t : t.contiguous(); };
+    const Tensor c = table(cos), s = table(sin);
+    p.cos = c.data_ptr();
+    p.cos_row_stride = step(c, 0);
+    p.sin = s.data_ptr();
+    p.sin_row_stride = step(s, 0);
+    p.seqlen_ro = i32(cos.size(0), "rows of cos");
+    if (positions.has_value()) {
+        check_dev(*positions, q, "positions");
+        TORCH_CHECK(!seqlen_offsets.has_value() && seqlen_offset == 0, "positions come without seqlen_offsets");
+        TORCH_CHECK(positions->scalar_type() == at::kInt || positions->scalar_type() == at::kLong, "positions must have dtype int32 or int64");
+        TORCH_CHECK(positions->sizes() == q.sizes().slice(0, q.dim() - 2), "positions must have an entry for each row of q");
+        p.positions = positions->data_ptr();
+        p.positions_int64 = positions->scalar_type() == at::kLong;
+        p.positions_batch_stride = q.dim() == 4 ? positions->stride(0) : 0;
+        p.positions_row_stride = positions->stride(-1);
+    }
+    if (seqlen_offsets.has_value()) p.seqlen_offsets = i32_vec(*seqlen_offsets, q, B, "seqlen_offsets");
+    p.seqlen_offset = seqlen_offset;
+    p.interleaved = interleaved;
+    p.conjugate = conjugate;
+    check_status(fa_rotary(&p, cur_stream()));
+}
+
+void check_rotary(const Tensor& q, const OptT& k, const Tensor& cos, const Tensor& sin) {
+    TORCH_CHECK(q.is_cuda(), "q must be on a GPU device");
+    check_16bit(q);
+    TORCH_CHECK(q.dim() == 3 || q.dim() == 4, "q must have shape (batch_size, seqlen, num_heads, head_size) or (total, num_heads, head_size)");
+    if (k.has_value()) {
+        check_dev(*k, q, "k");
+        TORCH_CHECK(k->scalar_type() == q.scalar_type(), "q and k must have the same dtype");
+        TORCH_CHECK(k->dim() == q.dim() && k->size(-1) == q.size(-1) && k->size(0) == q.size(0) && k->size(1 - (q.dim() == 3)) == q.size(1 - (q.dim() == 3)),
+                    "k must have the rows and the head size of q");
+    }
+    check_dev(cos, q, "rotary_cos");
+    check_dev(sin, q, "rotary_sin");
+    TORCH_CHECK(cos.dim() == 2 && sin.sizes() == cos.sizes(), "rotary_cos and rotary_sin must have shape (seqlen_ro, rotary_dim / 2)");
+    TORCH_CHECK(cos.scalar_type() == sin.scalar_type() && (cos.scalar_type() == at::kFloat || cos.scalar_type() == q.scalar_type()),
+                "rotary_cos and rotary_sin must have the dtype of q, or fp32");
+}
+
+std::tuple<Tensor, Tensor> rotary(const Tensor& q, const OptT& k, const Tensor& cos, const Tensor& sin, const OptT& positions,
+                                  const OptT& seqlen_offsets, int64_t seqlen_offset, const OptT& cu_seqlens, bool interleaved,
+                                  bool conjugate) {
+    c10::DeviceGuard guard(q.device());
+    check_rotary(q, k, cos, sin);
+    const Tensor qc = rows_of_16(q) ? q : q.contiguous();
+    OptT kc, ko;
+    Tensor qo = at::empty(q.sizes(), q.options()), none = at::empty({0}, q.options());
+    if (k.has_value()) {
+        kc = rows_of_16(*k) ? *k : k->contiguous();
+        ko = at::empty(k->sizes(), k->options());
+    }
+    rotary_into(qc, kc, qo, ko, cos, sin, positions, seqlen_offsets, seqlen_offset, cu_seqlens, interleaved, conjugate);
+    return {qo, ko.has_value() ? *ko : none};
+}
+
+void rotary_(Tensor& q, const OptT& k, const Tensor& cos, const Tensor& sin, const OptT& positions, const OptT& seqlen_offsets,
+             int64_t seqlen_offset, const OptT& cu_seqlens, bool interleaved, bool conjugate) {
+    c10::DeviceGuard guard(q.device());
+    check_rotary(q, k, cos, sin);
+    auto check = [](const Tensor& t, const char* name) {
+        TORCH_CHECK(rows_of_16(t), name, " turned in place must have contiguous last dimension, strides of 8 elements and 16-byte alignment");
+        // rows that share memory would be turned more than once
+        for (int64_t i = 0; i + 1 < t.dim(); ++i)
+            TORCH_CHECK(t.size(i) <= 1 || t.stride(i) != 0, name, " turned in place must not repeat rows");
+    };
+    check(q, "q");
+    if (k.has_value()) check(*k, "k");
+    rotary_into(q, k, q, k, cos, sin, positions, seqlen_offsets, seqlen_offset, cu_seqlens, interleaved, conjugate);
 }
 
 }  // namespace
@@ -930,6 +1146,18 @@ TORCH_LIBRARY(fa_mi355x, m) {
         "quant_fwd(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor cache_seqlens, "
         "Tensor? page_table, Tensor? cache_batch_idx, Tensor? cu_seqlens_q, int max_seqlen_q, float softmax_scale, "
         "bool is_causal, int window_size_left, int window_size_right, float softcap) -> (Tensor, Tensor)");
+    m.def(
+        "quant_read(Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor? slot_mapping, Tensor? cu_seqlens_k, "
+        "int total_k, Tensor? page_table, Tensor? cache_batch_idx, ScalarType dtype) -> (Tensor, Tensor)");
+    m.def(
+        "rotary_table(Tensor positions, int rotary_dim, float base, int scaling, float factor, float original_length, float low, "
+        "float high, float attention_factor, ScalarType dtype) -> (Tensor, Tensor)");
+    m.def(
+        "rotary(Tensor q, Tensor? k, Tensor rotary_cos, Tensor rotary_sin, Tensor? positions, Tensor? seqlen_offsets, "
+        "int seqlen_offset, Tensor? cu_seqlens, bool interleaved, bool conjugate) -> (Tensor, Tensor)");
+    m.def(
+        "rotary_(Tensor(a!) q, Tensor(b!)? k, Tensor rotary_cos, Tensor rotary_sin, Tensor? positions, Tensor? seqlen_offsets, "
+        "int seqlen_offset, Tensor? cu_seqlens, bool interleaved, bool conjugate) -> ()");
     m.def(
         "fwd_kvcache(Tensor q, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor? k, Tensor? v, Tensor? seqlens_k, "
         "Tensor? rotary_cos, Tensor? rotary_sin, Tensor? cache_batch_idx, Tensor? leftpad_k, Tensor? block_table, "
@@ -980,4 +1208,8 @@ TORCH_LIBRARY_IMPL(fa_mi355x, CUDA, m) {
     m.impl("update_page_table", &update_page_table);
     m.impl("quant_append", &quant_append);
     m.impl("quant_fwd", &quant_fwd);
+    m.impl("quant_read", &quant_read);
+    m.impl("rotary_table", &rotary_table);
+    m.impl("rotary", &rotary);
+    m.impl("rotary_", &rotary_);
 }

@@ -95,3 +95,29 @@ def _quant_fwd_fake(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, page_t
                     max_seqlen_q, softmax_scale, is_causal, window_size_left, window_size_right, softcap):
     lse = (q.shape[1], q.shape[0]) if cu_seqlens_q is not None else (q.shape[0], q.shape[2], q.shape[1])
     return q.new_empty(q.shape), q.new_empty(lse, dtype=torch.float32)
+
+
+@torch.library.register_fake("fa_mi355x::quant_read")
+def _quant_read_fake(k_cache, v_cache, k_scale, v_scale, slot_mapping, cu_seqlens_k, total_k, page_table, cache_batch_idx,
+                     dtype):
+    four = k_cache.dtype in (torch.uint8, torch.float4_e2m1fn_x2)
+    shape = (slot_mapping.shape[0] if slot_mapping is not None else total_k, k_cache.shape[2],
+             k_cache.shape[3] * (2 if four else 1))
+    return k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype)
+
+
+@torch.library.register_fake("fa_mi355x::rotary_table")
+def _rotary_table_fake(positions, rotary_dim, base, scaling, factor, original_length, low, high, attention_factor, dtype):
+    shape = (positions.shape[0], rotary_dim // 2)
+    return positions.new_empty(shape, dtype=dtype), positions.new_empty(shape, dtype=dtype)
+
+
+@torch.library.register_fake("fa_mi355x::rotary")
+def _rotary_fake(q, k, rotary_cos, rotary_sin, positions, seqlen_offsets, seqlen_offset, cu_seqlens, interleaved, conjugate):
+    return q.new_empty(q.shape), q.new_empty(k.shape if k is not None else (0,))
+
+
+@torch.library.register_fake("fa_mi355x::rotary_")
+def _rotary_inplace_fake(q, k, rotary_cos, rotary_sin, positions, seqlen_offsets, seqlen_offset, cu_seqlens, interleaved,
+                         conjugate):
+    return None

@@ -13,13 +13,15 @@ CORE_LIB = os.path.join(_HERE, "lib", "libfa_mi355x.so")
 
 ABI_VERSION = 4
 FA_OK, FA_EINVAL, FA_EUNSUPPORTED, FA_EHIP, FA_EWORKSPACE = 0, 1, 2, 3, 4
-FA_DTYPE_FP16, FA_DTYPE_BF16, FA_DTYPE_FP32, FA_DTYPE_FP8_E4M3, FA_DTYPE_INT8 = 0, 1, 2, 3, 4
+FA_DTYPE_FP16, FA_DTYPE_BF16, FA_DTYPE_FP32, FA_DTYPE_FP8_E4M3, FA_DTYPE_INT8, FA_DTYPE_FP4_E2M1 = 0, 1, 2, 3, 4, 5
+FA_ROTARY_PLAIN, FA_ROTARY_LINEAR, FA_ROTARY_NTK, FA_ROTARY_BY_PARTS = 0, 1, 2, 3
 FA_KIND_KVCACHE, FA_KIND_DENSE, FA_KIND_VARLEN = 0, 1, 2
 
 EXPORTED = ["fa_abi_version", "fa_validate", "fa_fwd_workspace_size", "fa_mha_fwd_kvcache", "fa_mha_fwd",
             "fa_mha_varlen_fwd", "fa_mha_fwd_kvcache_noalloc", "fa_combine", "fa_last_error", "fa_validate_bwd",
             "fa_bwd_workspace_size", "fa_mha_bwd", "fa_mha_varlen_bwd", "fa_update_page_table", "fa_quant_append",
-            "fa_quant_fwd_workspace_size", "fa_quant_fwd"]
+            "fa_quant_fwd_workspace_size", "fa_quant_fwd", "fa_fp4_append", "fa_fp4_fwd_workspace_size", "fa_fp4_fwd",
+            "fa_quant_read", "fa_rotary_table", "fa_rotary"]
 NOALLOC_SCRATCH_BYTES = 32 << 20  # FA_NOALLOC_SCRATCH_BYTES
 
 _i32 = ctypes.c_int32
@@ -94,7 +96,7 @@ class PageTableParams(ctypes.Structure):
 
 
 def _cache_fields():
-    """The caches and scales of QuantAppendParams and QuantFwdParams."""
+    """The caches and scales of QuantAppendParams, QuantFwdParams and QuantReadParams."""
     f = []
     for n in ("k", "v"):
         f += [(n, _vp), (n + "_page_stride", _i64), (n + "_row_stride", _i64), (n + "_head_stride", _i64)]
@@ -127,6 +129,44 @@ class QuantFwdParams(ctypes.Structure):
     ]
 
 
+class QuantReadParams(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32), ("dtype", _i32), ("cache_dtype", _i32), ("nheads_k", _i32), ("headdim", _i32),
+        ("num_pages", _i32), ("page_size", _i32), ("scale_block", _i32),
+    ] + _cache_fields() + [
+        ("k_out", _vp), ("v_out", _vp), ("total", _i64), ("slot_mapping", _vp), ("cu_seqlens_k", _vp), ("batch", _i32),
+        ("page_table", _vp), ("page_table_row_stride", _i64), ("table_rows", _i32), ("max_pages", _i32),
+        ("cache_batch_idx", _vp),
+    ]
+
+
+class RotaryTableParams(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32), ("dtype", _i32), ("rotary_dim", _i32), ("scaling", _i32),
+        ("base", ctypes.c_double), ("factor", ctypes.c_double), ("original_length", ctypes.c_double), ("low", ctypes.c_double),
+        ("high", ctypes.c_double), ("attention_factor", ctypes.c_double),
+        ("num_positions", _i64), ("positions", _vp), ("positions_int64", _i32), ("cos", _vp), ("sin", _vp),
+    ]
+
+
+def _row_fields(*names):
+    f = []
+    for n in names:
+        f += [(n, _vp), (n + "_batch_stride", _i64), (n + "_row_stride", _i64), (n + "_head_stride", _i64)]
+    return f
+
+
+class RotaryParams(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", _i32), ("dtype", _i32), ("table_dtype", _i32), ("batch", _i32), ("seqlen", _i32), ("total", _i32),
+        ("nheads", _i32), ("nheads_k", _i32), ("headdim", _i32), ("rotary_dim", _i32),
+    ] + _row_fields("q", "k", "q_out", "k_out") + [
+        ("cos", _vp), ("cos_row_stride", _i64), ("sin", _vp), ("sin_row_stride", _i64), ("seqlen_ro", _i32),
+        ("positions", _vp), ("positions_int64", _i32), ("positions_batch_stride", _i64), ("positions_row_stride", _i64),
+        ("seqlen_offsets", _vp), ("seqlen_offset", _i64), ("cu_seqlens", _vp), ("interleaved", _i32), ("conjugate", _i32),
+    ]
+
+
 _lib = None
 
 
@@ -156,11 +196,14 @@ def lib():
             getattr(L, fn).argtypes = [PB, _vp]
             getattr(L, fn).restype = ctypes.c_int
         for fn, params in (("fa_update_page_table", PageTableParams), ("fa_quant_append", QuantAppendParams),
-                           ("fa_quant_fwd", QuantFwdParams)):
+                           ("fa_quant_fwd", QuantFwdParams), ("fa_fp4_append", QuantAppendParams),
+                           ("fa_fp4_fwd", QuantFwdParams), ("fa_quant_read", QuantReadParams),
+                           ("fa_rotary_table", RotaryTableParams), ("fa_rotary", RotaryParams)):
             getattr(L, fn).argtypes = [ctypes.POINTER(params), _vp]
             getattr(L, fn).restype = ctypes.c_int
-        L.fa_quant_fwd_workspace_size.argtypes = [ctypes.POINTER(QuantFwdParams), ctypes.POINTER(ctypes.c_size_t)]
-        L.fa_quant_fwd_workspace_size.restype = ctypes.c_int
+        for fn in ("fa_quant_fwd_workspace_size", "fa_fp4_fwd_workspace_size"):
+            getattr(L, fn).argtypes = [ctypes.POINTER(QuantFwdParams), ctypes.POINTER(ctypes.c_size_t)]
+            getattr(L, fn).restype = ctypes.c_int
         _lib = L
     return _lib
 
@@ -242,3 +285,33 @@ def quant_fwd_workspace_size(p):
 
 def quant_fwd(p, stream=0):
     return lib().fa_quant_fwd(ctypes.byref(p), stream)
+
+
+def fp4_append(stream=0, **kw):
+    """fa_fp4_append with the given fields (zero elsewhere)."""
+    return lib().fa_fp4_append(ctypes.byref(QuantAppendParams(abi_version=ABI_VERSION, **kw)), stream)
+
+
+def fp4_fwd_workspace_size(p):
+    n = ctypes.c_size_t(0)
+    st = lib().fa_fp4_fwd_workspace_size(ctypes.byref(p), ctypes.byref(n))
+    return st, n.value
+
+
+def fp4_fwd(p, stream=0):
+    return lib().fa_fp4_fwd(ctypes.byref(p), stream)
+
+
+def quant_read(stream=0, **kw):
+    """fa_quant_read with the given fields (zero elsewhere)."""
+    return lib().fa_quant_read(ctypes.byref(QuantReadParams(abi_version=ABI_VERSION, **kw)), stream)
+
+
+def rotary_table(stream=0, **kw):
+    """fa_rotary_table with the given fields (zero elsewhere)."""
+    return lib().fa_rotary_table(ctypes.byref(RotaryTableParams(abi_version=ABI_VERSION, **kw)), stream)
+
+
+def rotary(stream=0, **kw):
+    """fa_rotary with the given fields (zero elsewhere)."""
+    return lib().fa_rotary(ctypes.byref(RotaryParams(abi_version=ABI_VERSION, **kw)), stream)

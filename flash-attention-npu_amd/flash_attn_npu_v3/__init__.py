@@ -16,5 +16,10 @@ from .interface import (  # noqa: F401
 from .quantized import (  # noqa: F401
     append_quantized_kvcache,
     flash_attn_with_quantized_kvcache,
+    read_quantized_kvcache,
     update_page_table,
+)
+from .rotary import (  # noqa: F401
+    apply_rotary_emb,
+    rotary_cos_sin,
 )

@@ -1,4 +1,4 @@
-"""Serving over a paged cache of 8-bit keys and values.
+"""Serving over a paged cache of 8-bit or 4-bit keys and values.
 
 A serving step calls these three in turn: update_page_table gives the pages of
 requests that ended to requests that grow and every new token its slot,
@@ -13,6 +13,15 @@ one head: a stored code c stands for c * scale. block is a multiple of 16,
 headdim one of 16 up to 256. A contiguous cache is (batch_size, seqlen_cache,
 nheads_k, headdim) with scales (batch_size, seqlen_cache // block, nheads_k), and
 no page table: slot b * seqlen_cache + j is row j of sequence b.
+
+A 4-bit cache holds half the bytes (OCP Microscaling, MXFP4): k_cache and v_cache are (num_pages, page_size,
+nheads_k, headdim // 2) of torch.float4_e2m1fn_x2 or of its bytes, torch.uint8 (the even channel in the
+lower half); k_scale and v_scale are (num_pages, page_size, nheads_k, headdim // 32)
+of torch.float8_e8m0fnu or its bytes, uint8: 32 channels of a token and head share one. A code (0, 0.5, 1, 1.5, 2, 3, 4
+or 6, and their negatives) under the scale s stands for code * s. headdim is a multiple of 32 up to 256, page_size
+one of 16. All the calls below take it in place of an 8-bit one.
+
+read_quantized_kvcache gives rows of either cache back in 16 or 32 bits.
 """
 from typing import Optional
 
@@ -22,7 +31,8 @@ from fa_mi355x import ops
 
 from .interface import maybe_contiguous
 
-_update_page_table, _append, _fwd = (op.default for op in (ops.update_page_table, ops.quant_append, ops.quant_fwd))
+_update_page_table, _append, _fwd, _read = (op.default for op in (ops.update_page_table, ops.quant_append, ops.quant_fwd,
+                                                                  ops.quant_read))
 
 
 def update_page_table(page_table, cache_seqlens, new_seqlens, free_pages, num_free, page_size, total_new,
@@ -73,7 +83,12 @@ def append_quantized_kvcache(k, v, k_cache, v_cache, k_scale, v_scale, slot_mapp
     to even. +-inf counts as the type's largest finite value; NaN becomes 0 in
     int8 and NaN in e4m3. The new rows of one block and head are one workgroup's work, and so are the
     codes before them that move: blocks of thousands of tokens (a contiguous cache with one scale a
-    sequence) are slow."""
+    sequence) are slow.
+
+    4-bit cache: each 32 channels of a row get the smallest power of two s with max |x| <= 6 s (at least 2 ** -100, at most
+    2 ** 13 for fp16 and 2 ** 125 for bf16, past which codes end at 6), and codes x / s rounded to the nearest, ties to
+    the even code. +-inf counts as the type's largest finite value; a NaN makes its 32 channels NaN. Slots may
+    come in any order, since no row touches another."""
     _append(k, v, k_cache, v_cache, k_scale, v_scale, maybe_contiguous(slot_mapping))
 
 
@@ -104,7 +119,9 @@ def flash_attn_with_quantized_kvcache(q, k_cache, v_cache, k_scale, v_scale, cac
     of each key's codes, the weights of the values carry v_scale, and both
     products run on the codes without rounding them (fp32 sums). causal,
     window_size and softcap as in flash_attn_with_kvcache. A row that sees no
-    key gets 0 and a softmax_lse of +inf. Rows behind the last sequence of cu_seqlens_q are not
+    key gets 0 and a softmax_lse of +inf. Of a 4-bit cache, the products run on the values that it holds, rounded to the type of q:
+    bf16 holds them as they are, fp16 those from 2 ** -14 to 65504 (larger ones become inf, smaller ones lose bits). A value of
+    v_cache that is NaN or inf so, at a key that some row of the sequence sees, may reach rows that do not see it. Rows behind the last sequence of cu_seqlens_q are not
     written: what out and softmax_lse hold there means nothing. Returns out, or (out, softmax_lse)
     with softmax_lse (batch_size, nheads, seqlen) or (nheads, total_q) fp32."""
     if softmax_scale is None:
@@ -116,3 +133,21 @@ def flash_attn_with_quantized_kvcache(q, k_cache, v_cache, k_scale, v_scale, cac
                             maybe_contiguous(cu_seqlens_q), int(max_seqlen_q or 0), float(softmax_scale), bool(causal),
                             int(window_size[0]), int(window_size[1]), float(softcap))
     return (out, softmax_lse) if return_softmax_lse else out
+
+
+def read_quantized_kvcache(k_cache, v_cache, k_scale, v_scale, slot_mapping: Optional[torch.Tensor] = None,
+                           cu_seqlens_k: Optional[torch.Tensor] = None, total_k: Optional[int] = None,
+                           page_table: Optional[torch.Tensor] = None, cache_batch_idx: Optional[torch.Tensor] = None,
+                           dtype=torch.bfloat16):
+    """Rows of a quantised cache as values: (k, v), each (total, nheads_k, headdim) of dtype (bf16, fp16 or fp32).
+
+    Which rows: those of slot_mapping (total,) int64, or the keys of sequences one behind the other, as
+    flash_attn_varlen_func takes them: row cu_seqlens_k[b] + j, cu_seqlens_k (batch_size + 1,) int32, is key j
+    of sequence b, which page_table and cache_batch_idx lead to as in flash_attn_with_quantized_kvcache; total_k is the number of
+    rows of k and v, of which those behind the last sequence are 0. So is a row whose slot or page is not in the cache.
+
+    A value is code * scale, rounded to fp32 and to dtype; of a 4-bit cache it is rounded to dtype alone."""
+    if cu_seqlens_k is not None and total_k is None:
+        raise RuntimeError("total_k is required with cu_seqlens_k")
+    return _read(k_cache, v_cache, k_scale, v_scale, maybe_contiguous(slot_mapping), maybe_contiguous(cu_seqlens_k),
+                 int(total_k or 0), maybe_contiguous(page_table), maybe_contiguous(cache_batch_idx), dtype)

@@ -61,7 +61,8 @@ typedef enum {
     FA_DTYPE_FP32 = 2,     /* fa_combine output only */
     FA_DTYPE_FP8_E4M3 = 3, /* forward only: q, k, v, k_new, v_new in OCP float8 e4m3fn (torch.float8_e4m3fn),
                               out in bf16; see q_descale below. Also a cache type of the quantised cache */
-    FA_DTYPE_INT8 = 4      /* cache type of the quantised cache only */
+    FA_DTYPE_INT8 = 4,     /* cache type of the quantised cache only */
+    FA_DTYPE_FP4_E2M1 = 5  /* cache type of the 4-bit cache only */
 } fa_dtype_t;
 
 typedef enum {
@@ -350,9 +351,9 @@ typedef struct fa_quant_append_params {
     int64_t k_page_stride, k_row_stride, k_head_stride;
     void* v;
     int64_t v_page_stride, v_row_stride, v_head_stride;
-    float* k_scale;
+    void* k_scale;                   /* fp32 (FP4_E2M1: bytes) */
     int64_t k_scale_page_stride, k_scale_block_stride, k_scale_head_stride;
-    float* v_scale;
+    void* v_scale;
     int64_t v_scale_page_stride, v_scale_block_stride, v_scale_head_stride;
     const int64_t* slot_mapping;     /* (total_new,) slot of each row; rows with a slot outside the cache are skipped */
 } fa_quant_append_params;
@@ -381,9 +382,9 @@ typedef struct fa_quant_fwd_params {
     int64_t k_page_stride, k_row_stride, k_head_stride;
     const void* v;
     int64_t v_page_stride, v_row_stride, v_head_stride;
-    const float* k_scale;
+    const void* k_scale;             /* fp32 (FP4_E2M1: bytes) */
     int64_t k_scale_page_stride, k_scale_block_stride, k_scale_head_stride;
-    const float* v_scale;
+    const void* v_scale;
     int64_t v_scale_page_stride, v_scale_block_stride, v_scale_head_stride;
     void* out;                       /* like q */
     int64_t out_batch_stride, out_row_stride, out_head_stride;
@@ -414,6 +415,122 @@ typedef struct fa_quant_fwd_params {
  * are left as they are. */
 fa_status_t fa_quant_fwd_workspace_size(const fa_quant_fwd_params* p, size_t* bytes);
 fa_status_t fa_quant_fwd(const fa_quant_fwd_params* p, void* stream);
+
+/* ---- a cache in 4 bits --------------------------------------------------------
+ * The same parameters with cache_dtype FP4_E2M1. k and v hold two codes to a byte,
+ * (num_pages, page_size, Hk, D / 2) bytes, the even channel in the lower half; the
+ * scales are bytes (num_pages, page_size, Hk, D / 32): 32 channels of a token and
+ * head share one. A code e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) under a scale
+ * byte b stands for code * 2^(b - 127), b = 255 for NaN (OCP Microscaling, MXFP4). D is a
+ * multiple of 32, at most 256, page_size one of 16, scale_block 1: the block strides
+ * are a token's. Strides of caches and scales count bytes, and the scales of a row and head
+ * stand together. */
+
+/* As fa_quant_append. Each group of 32 values has a scale of its own: the smallest
+ * power of two s in [2^-100, most] with max |x| <= 6 s, most = 2^13 for FP16 and
+ * 2^125 for BF16 (so that every value reads back as a finite one of dtype), and its codes are
+ * x / s rounded to the nearest, ties to the even code, at most 6. +-inf counts as the largest
+ * finite value of dtype; a group with a NaN gets the scale NaN. Nothing of the cache
+ * but the new rows is read or written, so their order is free. */
+fa_status_t fa_fp4_append(const fa_quant_append_params* p, void* stream);
+
+/* As fa_quant_fwd, over the values that the cache holds, rounded to the type of q
+ * (bf16 holds each of them up to 6 * 2^125; fp16 those of 2^-14 to 65504 exactly, larger ones as inf). */
+fa_status_t fa_fp4_fwd_workspace_size(const fa_quant_fwd_params* p, size_t* bytes);
+fa_status_t fa_fp4_fwd(const fa_quant_fwd_params* p, void* stream);
+
+typedef struct fa_quant_read_params {
+    int32_t abi_version;
+    int32_t dtype;                   /* of k_out, v_out: FP16, BF16 or FP32 */
+    int32_t cache_dtype;             /* INT8, FP8_E4M3 or FP4_E2M1 */
+    int32_t nheads_k, headdim;
+    int32_t num_pages, page_size, scale_block;
+    const void* k;
+    int64_t k_page_stride, k_row_stride, k_head_stride;
+    const void* v;
+    int64_t v_page_stride, v_row_stride, v_head_stride;
+    const void* k_scale;             /* fp32 (FP4_E2M1: bytes) */
+    int64_t k_scale_page_stride, k_scale_block_stride, k_scale_head_stride;
+    const void* v_scale;
+    int64_t v_scale_page_stride, v_scale_block_stride, v_scale_head_stride;
+    void* k_out;                     /* (total, Hk, D) contiguous */
+    void* v_out;
+    int64_t total;
+    const int64_t* slot_mapping;     /* (total,) slot of each row, or NULL: the rows are those of cu_seqlens_k */
+    const int32_t* cu_seqlens_k;     /* (batch + 1,) row cu_seqlens_k[b] + j is key j of sequence b */
+    int32_t batch;
+    const int32_t* page_table;       /* (table_rows, max_pages) or NULL: contiguous */
+    int64_t page_table_row_stride;
+    int32_t table_rows, max_pages;
+    const int32_t* cache_batch_idx;  /* as in fa_quant_fwd_params */
+} fa_quant_read_params;
+
+/* Rows of any quantised cache as values: code * scale rounded once to fp32 and once to
+ * dtype (FP4_E2M1: exact but for the type's range). A row whose slot or page is not in the cache, or
+ * that belongs to no sequence, is 0. */
+fa_status_t fa_quant_read(const fa_quant_read_params* p, void* stream);
+
+/* ---- rotary positions -------------------------------------------------------------
+ * The reference takes tables of cosines and sines (rotary_cos, rotary_sin of
+ * flash_attn_with_kvcache) and has nothing that makes them, nor a rotation of its own. */
+typedef enum {
+    FA_ROTARY_PLAIN = 0,
+    FA_ROTARY_LINEAR = 1,   /* f / factor */
+    FA_ROTARY_NTK = 2,      /* base * factor^(rd / (rd - 2)) in place of base */
+    FA_ROTARY_BY_PARTS = 3  /* f (g + (1 - g) / factor), g = clamp((original_length f / 2 pi - low) / (high - low), 0, 1) */
+} fa_rotary_scaling_t;
+
+typedef struct fa_rotary_table_params {
+    int32_t abi_version;
+    int32_t dtype;                   /* of cos and sin: FP32, FP16 or BF16 */
+    int32_t rotary_dim;              /* rd: a multiple of 16, at most 256 */
+    int32_t scaling;                 /* fa_rotary_scaling_t */
+    double base, factor, original_length, low, high, attention_factor;
+    int64_t num_positions;
+    const void* positions;           /* (num_positions,) int32 or int64 */
+    int32_t positions_int64;
+    void* cos;                       /* (num_positions, rd / 2) contiguous */
+    void* sin;
+} fa_rotary_table_params;
+
+/* cos[n, i] = attention_factor * cos(positions[n] * f_i), f_i = base^(-2 i / rd) scaled; sin alike.
+ * Angles are formed in 64 bits. */
+fa_status_t fa_rotary_table(const fa_rotary_table_params* p, void* stream);
+
+typedef struct fa_rotary_params {
+    int32_t abi_version;
+    int32_t dtype;                   /* of q, k and their results: FP16 or BF16 */
+    int32_t table_dtype;             /* of cos and sin: dtype or FP32 */
+    int32_t batch, seqlen;           /* with cu_seqlens: sequences, unused */
+    int32_t total;                   /* with cu_seqlens: rows */
+    int32_t nheads, nheads_k;        /* nheads_k 0: no k */
+    int32_t headdim, rotary_dim;     /* multiples of 8 and 16, rotary_dim at most 256 */
+    const void* q;                   /* (B, S, H, D), with cu_seqlens (total, H, D) */
+    int64_t q_batch_stride, q_row_stride, q_head_stride;
+    const void* k;                   /* like q with Hk heads, or NULL */
+    int64_t k_batch_stride, k_row_stride, k_head_stride;
+    void* q_out;                     /* like q; q itself turns it in place (k_out then is k) */
+    int64_t q_out_batch_stride, q_out_row_stride, q_out_head_stride;
+    void* k_out;
+    int64_t k_out_batch_stride, k_out_row_stride, k_out_head_stride;
+    const void* cos;                 /* (seqlen_ro, rotary_dim / 2) */
+    int64_t cos_row_stride;
+    const void* sin;
+    int64_t sin_row_stride;
+    int32_t seqlen_ro;
+    const void* positions;           /* (B, S), with cu_seqlens (total,), int32 or int64, or NULL */
+    int32_t positions_int64;
+    int64_t positions_batch_stride, positions_row_stride;
+    const int32_t* seqlen_offsets;   /* (B,) position of each sequence's first row, or NULL: seqlen_offset */
+    int64_t seqlen_offset;
+    const int32_t* cu_seqlens;       /* (B + 1,) or NULL */
+    int32_t interleaved;             /* pairs (2i, 2i + 1), else (i, i + rd / 2) */
+    int32_t conjugate;               /* turned back: the gradient of the rotation */
+} fa_rotary_params;
+
+/* x1' = x1 cos - x2 sin, x2' = x2 cos + x1 sin of each pair; channels past rotary_dim
+ * and rows that belong to no sequence stay. Positions outside [0, seqlen_ro) take the nearest row. */
+fa_status_t fa_rotary(const fa_rotary_params* p, void* stream);
 
 /* Thread-local message describing the last non-FA_OK status on this thread. */
 const char* fa_last_error(void);
