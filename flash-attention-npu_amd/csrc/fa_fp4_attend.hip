@@ -99,7 +99,6 @@ static hipError_t launch_fp4_attend(const QuantFwdArgs& a, bool few, hipStream_t
     return hipGetLastError();
 }
 
-hipError_t launch_fp4_decode(const QuantFwdArgs& a, int, int, int, int, hipStream_t stream) { return launch_fp4_attend(a, true, stream); }
 hipError_t launch_fp4_prefill(const QuantFwdArgs& a, int, int, int, int, hipStream_t stream) { return launch_fp4_attend(a, false, stream); }
 
 }  // namespace fa

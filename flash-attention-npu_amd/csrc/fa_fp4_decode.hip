@@ -1,0 +1,425 @@
+// fa_fp4_decode.hip -- attention over the 4-bit cache for few query rows (a kv head's g
+// query heads x positions, at most 32 packed rows): the cache is streamed once.
+//
+// Split: as in fa_quant_decode.hip, 64-key tiles of all sequences and kv heads in one
+// list, cut into equal ranges, one per wave; what a range leaves of a sequence is merged by a
+// second launch.
+//
+// A lane loads, of each of 16 keys' rows that four lanes share, its quarter: 32 channels at head dim
+// 128, which have one scale, so a value is one conversion with its scale (fa_fp4.h). Tiles stay in
+// registers, two in flight beside the one at hand. Keys go from there straight into S^T = K.Q^T.
+// Values go through LDS once they are 16 bits wide, 32 keys at a time, since O^T = V^T.P^T wants
+// the keys of a channel side by side: written by rows, read by transpose reads. Nothing waits
+// for another wave.
+//
+// Weights are kept in units that make a row's largest 2^14 in fp16, so that a weight has all
+// its bits down to 2^-28 of that, and 2^-20 in bf16, whose values reach to 2^128: the sum of 2^20 of
+// them stays in fp32. In bf16, whose 8 bits would be most of the result's error, a weight is the
+// sum of two bf16 numbers and meets V twice; the products have the time, since what bounds
+// a step is memory.
+#include "fa_fp4.h"
+#include "fa_quant_list.h"
+
+namespace fa {
+
+namespace {
+
+template <int HD>
+struct Cfg4 {
+    static constexpr int NWAVE = HD == 256 ? 4 : 8;  // waves of a workgroup
+    static constexpr int KT = 64, NB = KT / 16;      // keys of a tile, blocks of 16
+    static constexpr int W = HD / 32;                // words of 8 codes that a lane has of a row
+    static constexpr int NL = HD == 256 ? 2 : 1;     // loads of them, each under one scale
+    static constexpr int DBLK = HD / 16;
+    static constexpr int ROW = 2 * HD;               // bytes of a widened row
+    static constexpr int TILES = 64 / NB;            // tiles whose places a wave's lanes hold
+    // first channel of word w of lane group G
+    static __device__ __forceinline__ int channel(int G, int w) {
+        return HD == 64 ? 16 * G + 8 * w : HD == 128 ? 32 * G + 8 * w : 128 * (w >> 2) + 32 * G + 8 * (w & 3);
+    }
+    // slot of 16-byte chunk c of row r: conflict free for the writes of one chunk of 16 rows and for the
+    // transpose reads of two chunks of 8 rows
+    static __device__ __forceinline__ int slot(int r, int c) {
+        return HD == 64 ? swz_b64(r, c) : c ^ (((r & 7) << 1) | ((r >> 3) & 1));
+    }
+};
+
+// A tile's codes and scales, as a lane loads them
+template <int HD>
+struct Tile {
+    uint32_t k[4][Cfg4<HD>::W], v[4][Cfg4<HD>::W];
+    uint32_t ks[4][Cfg4<HD>::NL], vs[4][Cfg4<HD>::NL];
+};
+
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t* to, const uint8_t* p) {
+    if constexpr (N == 4) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+        to[0] = x[0], to[1] = x[1], to[2] = x[2], to[3] = x[3];
+    } else {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+        to[0] = x[0], to[1] = x[1];
+    }
+}
+
+// DT: type of q and out; HD: kernel head dim (the cache's may be smaller: lanes past it
+// hold the row's first codes and meet zeros of q); NR: 16-row tiles of packed rows.
+template <int DT, int HD, int NR>
+__global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, 1) fa_fp4_decode_kernel(QuantFwdArgs a) {
+    using C = Cfg4<HD>;
+    constexpr int NWAVE = C::NWAVE, NT = NWAVE * 64, KT = C::KT, NB = C::NB, W = C::W, NL = C::NL, DBLK = C::DBLK, ROW = C::ROW, TILES = C::TILES;
+    constexpr bool SPLIT = DT == DT_BF16;
+    constexpr float kTop = DT == DT_BF16 ? -20.f : 14.f;  // log2 of the largest weight
+    __shared__ __attribute__((aligned(1024))) char s_v[NWAVE][32 * ROW];
+    __shared__ int s_pref[kQuantMaxB + 1];
+
+    auto anew = []() -> const QuantFwdArgs& {  // as in fa_quant_decode.hip
+        auto p = __builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(p));
+        return *(const QuantFwdArgs*)p;
+    };
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int li = lane & 15, G = lane >> 4;
+    const int hs = heads_per_group(a), hgs = a.Hk / hs;
+
+    // ---- the list of tiles ----------------------------------------------------------
+    for (int b = tid; b < a.B; b += NT) {
+        const QuantSeq s = quant_seq(a, b);
+        s_pref[b + 1] = s.hi > s.lo && s.sq * a.g <= a.dec_rows ? hgs * ((s.hi + KT - 1) / KT - s.lo / KT) : 0;
+    }
+    __syncthreads();
+    if (wave == 0) prefix_sums(s_pref, a.B);
+    __syncthreads();
+    if (blockIdx.x == 0)
+        for (int b = tid; b <= a.B; b += NT) a.sched[b] = s_pref[b];
+
+    const int hsel = wave % hs;
+    const int gw = (wave / hs) * gridDim.x + blockIdx.x;  // wave-major, as in fa_decode.hip
+    const int64_t wid = (int64_t)gw * hs + hsel;
+    const Split sp = split_list(s_pref[a.B], gridDim.x * (NWAVE / hs));
+    const int t0 = __builtin_amdgcn_readfirstlane(sp.first(gw)), t1 = __builtin_amdgcn_readfirstlane(sp.first(gw + 1));
+    if (t0 >= t1) return;  // no barrier follows: the waves go on alone
+
+    // ---- places: lane l looks after block l % 4 of tile l / 4 of 16 tiles ------------------
+    // A block without a visible key has the place of a row that is there.
+    int id, inp, kvh;
+    int64_t koff, voff, ksoff, vsoff;
+    uint64_t have = 0;  // the blocks of the 16 tiles whose page is in the cache
+    auto ask_ids = [&](int base) {
+        const QuantFwdArgs& A = anew();
+        const int t = base + lane / NB;
+        id = -1;
+        inp = kvh = 0;
+        if (t < t1) {
+            const Seg s = seg_of(A, s_pref, t, hs, hsel, KT);
+            const int key = (s.lo_tile + (t - s.S)) * KT + (lane % NB) * 16;
+            kvh = s.hk;
+            if (key < s.q.hi && key + 16 > s.q.lo) {
+                const int pi = A.table ? (int)udiv(A.page, (uint32_t)key) : 0;
+                inp = key - pi * A.page_size;
+                id = A.table ? A.table[(int64_t)s.q.crow * A.t_stride + pi] : s.q.crow;
+            }
+        }
+    };
+    auto places = [&]() {
+        const QuantFwdArgs& A = anew();
+        const bool ok = id >= 0 && id < A.num_pages;
+        const int64_t p = ok ? id : 0, r = ok ? inp : 0, h = kvh;
+        koff = p * A.k_sp + r * A.k_si + h * A.k_sh;
+        voff = p * A.v_sp + r * A.v_si + h * A.v_sh;
+        ksoff = p * A.ks_sp + r * A.ks_sb + h * A.ks_sh;
+        vsoff = p * A.vs_sp + r * A.vs_sb + h * A.vs_sh;
+        have = __ballot(ok);
+    };
+
+    // ---- loads ------------------------------------------------------------------------
+    const int groups = a.hd / kGroup;
+    uint32_t kin[NL], vin[NL], ksin[NL], vsin[NL];  // where a lane's codes and scales are in a block
+    uint32_t mine[NL];  // the bits of codes that are the lane's own
+#pragma unroll
+    for (int u = 0; u < NL; ++u) {
+        const int grp = HD == 64 ? G >> 1 : 4 * u + G, at = HD == 64 ? 8 * G : 64 * u + 16 * G;
+        const bool in = grp < groups;
+        mine[u] = in ? ~0u : 0u;
+        kin[u] = (uint32_t)li * (uint32_t)a.k_si + (in ? at : 0);
+        vin[u] = (uint32_t)li * (uint32_t)a.v_si + (in ? at : 0);
+        ksin[u] = (uint32_t)li * (uint32_t)a.ks_sb + (in ? grp : 0);
+        vsin[u] = (uint32_t)li * (uint32_t)a.vs_sb + (in ? grp : 0);
+    }
+    const uint8_t* ksb = reinterpret_cast<const uint8_t*>(a.ks);
+    const uint8_t* vsb = reinterpret_cast<const uint8_t*>(a.vs);
+    auto of_lane = [](int64_t x, int l) {
+        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane((int)x, l));
+    };
+    // Past the range the last tile is asked for again, so that every wait counts the same loads. The
+    // places are those of asked tile's 16 until `places` moves on.
+    int asked = t0;
+    unsigned bits0 = 0, bits1 = 0;  // visible blocks of the tile at hand and of the next
+    auto ask_k = [&](Tile<HD>& T) {
+        const int i = asked - t0;
+        if (asked < t1 && i % TILES == 0) {
+            places();
+            ask_ids(asked + TILES);
+        }
+        const int at = (min(asked, t1 - 1) - t0) % TILES * NB;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const uint8_t *p = a.k + of_lane(koff, at + b), *s = ksb + of_lane(ksoff, at + b);
+#pragma unroll
+            for (int u = 0; u < NL; ++u) {
+                load_words<W / NL>(T.k[b] + u * (W / NL), p + kin[u]);
+                T.ks[b][u] = s[ksin[u]];
+            }
+        }
+    };
+    auto ask_v = [&](Tile<HD>& T) {
+        const int at = (min(asked, t1 - 1) - t0) % TILES * NB;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const uint8_t *p = a.v + of_lane(voff, at + b), *s = vsb + of_lane(vsoff, at + b);
+#pragma unroll
+            for (int u = 0; u < NL; ++u) {
+                load_words<W / NL>(T.v[b] + u * (W / NL), p + vin[u]);
+                T.vs[b][u] = s[vsin[u]];
+            }
+        }
+        ++asked;
+    };
+    auto bits_of = [&]() { return (unsigned)(have >> ((min(asked, t1 - 1) - t0) % TILES * NB)) & 15u; };
+
+    // ---- a segment: q, sums ----------------------------------------------------------------
+    Seg cs;
+    u32x4 qreg[NR][W];
+    int qi[NR];
+    f32x4 oacc[NR][DBLK];
+    float m_run[NR], l_run[NR];
+    int rows = 0;
+    int flo = 0, fhi = 0;      // keys that every row sees
+    const float scale2 = a.softcap > 0.f ? a.scale / a.softcap : a.scale * kLog2e;
+    auto begin_seg = [&](int t) {
+        const QuantFwdArgs& A = anew();
+        cs = seg_of(A, s_pref, t, hs, hsel, KT);
+        rows = cs.q.sq * A.g;
+        flo = key_lo(cs.q.sk - 1, A.wl, 0);
+        fhi = min(key_hi(cs.q.sk - cs.q.sq, A.wr, 0), cs.q.sk - 1);
+#pragma unroll
+        for (int rt = 0; rt < NR; ++rt) {
+            const int r = rt * 16 + li;
+            const bool ok = r < rows;
+            qi[rt] = ok ? r / A.g : 0;
+            const int h = cs.hk * A.g + (ok ? r % A.g : 0);
+            const uint16_t* q = static_cast<const uint16_t*>(A.q) + q_row(A, cs.b, qi[rt], A.q_sb, A.q_si) + (int64_t)h * A.q_sh;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const int d = C::channel(G, w);
+                qreg[rt][w] = ok && d < A.hd ? *reinterpret_cast<const u32x4*>(q + d) : u32x4{0u, 0u, 0u, 0u};
+            }
+            m_run[rt] = -INFINITY;
+            l_run[rt] = 0.f;
+#pragma unroll
+            for (int db = 0; db < DBLK; ++db) oacc[rt][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    };
+    auto end_seg = [&]() {
+        const QuantFwdArgs& A = anew();
+        const bool whole = cs.S >= t0 && cs.S + cs.n <= t1;
+#pragma unroll
+        for (int rt = 0; rt < NR; ++rt) {
+            const int r = rt * 16 + li;
+            const float l = wave_sum16x4(l_run[rt]);
+            const bool some = l != 0.f;  // NaN: some
+            const float inv = some ? 1.f / l : 0.f;
+            const float lse = some ? (m_run[rt] - kTop + fast_log2(l)) * kLn2 : INFINITY;
+            if (r >= rows) continue;
+            if (whole) {
+                const int h = cs.hk * A.g + r % A.g;
+                uint16_t* o = static_cast<uint16_t*>(A.out) + q_row(A, cs.b, qi[rt], A.o_sb, A.o_si) + (int64_t)h * A.o_sh;
+#pragma unroll
+                for (int db = 0; db < DBLK; ++db) {
+                    if (16 * db >= A.hd) continue;
+                    const f32x4 y = oacc[rt][db] * inv;
+                    *reinterpret_cast<u32x2*>(o + 16 * db + 4 * G) = u32x2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
+                }
+                if (G == 0) A.lse[lse_at(A, cs.b, h, qi[rt])] = lse;
+            } else {
+                const int slot = cs.S <= t0 ? 0 : 1;  // this worker's first segment, else its last
+                const int64_t row = (wid * 2 + slot) * (16 * NR) + r;
+#pragma unroll
+                for (int db = 0; db < DBLK; ++db)
+                    *reinterpret_cast<f32x4*>(A.part_o + row * HD + 16 * db + 4 * G) = oacc[rt][db] * inv;
+                if (G == 0) A.part_lse[row] = some ? lse : -INFINITY;
+            }
+        }
+    };
+
+    // ---- a tile ----------------------------------------------------------------------------
+    const unsigned vt = lds_addr(s_v[wave]);
+    const int tr_row = 4 * G + (li >> 2);
+    auto compute = [&](int t, Tile<HD>& T) {
+        const int key0 = (cs.lo_tile + (t - cs.S)) * KT;
+        const unsigned ok = bits0;
+        const bool full = ok == 15u && key0 >= flo && key0 + KT - 1 <= fhi;
+        // codes past the head dim are 0, since inf x 0 is NaN
+        if (groups * kGroup != HD) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int w = 0; w < W; ++w) T.k[b][w] &= mine[w * NL / W];
+        }
+        // S^T = K . Q^T
+        f32x4 x[NR][NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int rt = 0; rt < NR; ++rt) x[rt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const u32x4 op = fp4_widen8<DT>(T.k[b][w], fp4_scale(T.ks[b][w * NL / W]));
+#pragma unroll
+                for (int rt = 0; rt < NR; ++rt) x[rt][b] = mfma16x16x32<DT>(op, qreg[rt][w], x[rt][b]);
+            }
+        }
+        ask_k(T);
+        const unsigned bits2 = bits_of();
+        if (a.softcap > 0.f) {
+#pragma unroll
+            for (int rt = 0; rt < NR; ++rt)
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[rt][b][e] = a.softcap * kLog2e * fast_tanh(x[rt][b][e] * scale2);
+        } else {
+#pragma unroll
+            for (int rt = 0; rt < NR; ++rt)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) x[rt][b] *= scale2;
+        }
+        if (!full) {
+#pragma unroll
+            for (int rt = 0; rt < NR; ++rt) {
+                const int d = qi[rt] + cs.q.sk - cs.q.sq;
+                const int rlo = key_lo(d, a.wl, 0), rhi = min(key_hi(d, a.wr, 0), cs.q.sk - 1);
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = key0 + b * 16 + G * 4 + e;
+                        x[rt][b][e] = (ok >> b & 1) && j >= rlo && j <= rhi ? x[rt][b][e] : -INFINITY;
+                    }
+            }
+        }
+        // weights, the running maximum's 2^kTop
+        u32x4 pk[NR][NB / 2], pl[NR][NB / 2];
+        float up[NR];
+        bool moved = false;
+#pragma unroll
+        for (int rt = 0; rt < NR; ++rt) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) mx = fmaxf(mx, fmaxf(fmaxf(x[rt][b][0], x[rt][b][1]), fmaxf(x[rt][b][2], x[rt][b][3])));
+            mx = fmaxf(m_run[rt], max4(mx));
+            moved |= mx > m_run[rt];
+            const float u = mx == -INFINITY ? 0.f : mx;
+            up[rt] = fast_exp2(m_run[rt] - u);
+            m_run[rt] = mx;
+            l_run[rt] *= up[rt];
+#pragma unroll
+            for (int k2 = 0; k2 < NB / 2; ++k2) {
+                f32x8 w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = fast_exp2(x[rt][2 * k2 + (e >> 2)][e & 3] - (u - kTop));
+                l_run[rt] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+                pk[rt][k2] = pack8<DT>(w);
+                if constexpr (SPLIT) pl[rt][k2] = pack8<DT>(w - widen8<DT>(pk[rt][k2]));
+            }
+        }
+        if (__ballot(moved)) {
+#pragma unroll
+            for (int rt = 0; rt < NR; ++rt)
+#pragma unroll
+                for (int db = 0; db < DBLK; ++db) oacc[rt][db] *= up[rt];
+        }
+        // O^T += V^T . P^T, 32 keys at a time
+#pragma unroll
+        for (int k2 = 0; k2 < NB / 2; ++k2) {
+#pragma unroll
+            for (int bb = 0; bb < 2; ++bb) {
+                const int b = 2 * k2 + bb, r = 16 * bb + li, j = key0 + 16 * b + li;
+                // values that no row sees must not meet the products, where 0 x NaN is NaN
+                const bool seen = full || ((ok >> b & 1) && j >= cs.q.lo && j < cs.q.hi);
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    u32x4 y = fp4_widen8<DT>(T.v[b][w], fp4_scale(T.vs[b][w * NL / W]));
+                    if (!full && !seen) y = u32x4{0u, 0u, 0u, 0u};
+                    row_write(vt + r * ROW + (C::slot(li, C::channel(G, w) / 8) << 4), y);
+                }
+            }
+            if (k2 == NB / 2 - 1) ask_v(T);
+#pragma unroll
+            for (int db = 0; db < DBLK; ++db) {
+                const unsigned p = vt + tr_row * ROW + (C::slot(tr_row, 2 * db + ((li & 3) >> 1)) << 4) + (li & 1) * 8;
+                const u32x4 op = tr_read(p, p + 16 * ROW);
+#pragma unroll
+                for (int rt = 0; rt < NR; ++rt) {
+                    oacc[rt][db] = mfma16x16x32<DT>(op, pk[rt][k2], oacc[rt][db]);
+                    if constexpr (SPLIT) oacc[rt][db] = mfma16x16x32<DT>(op, pl[rt][k2], oacc[rt][db]);
+                }
+            }
+        }
+        bits0 = bits1;
+        bits1 = bits2;
+    };
+
+    Tile<HD> A, B;
+    ask_ids(t0);
+    ask_k(A);
+    bits0 = bits_of();
+    ask_v(A);
+    ask_k(B);
+    bits1 = bits_of();
+    ask_v(B);
+    int qat = t0, send = t0;
+    auto step = [&](int t, Tile<HD>& T) {
+        if (t == qat) {
+            begin_seg(t);
+            send = min(cs.S + cs.n, t1);
+        }
+        compute(t, T);
+        if (t + 1 == send) {
+            end_seg();
+            qat = send;
+        }
+    };
+#pragma unroll 1
+    for (int t = t0; t < t1; t += 2) {
+        step(t, A);
+        if (t + 1 < t1) step(t + 1, B);
+    }
+}
+
+template <int DT, int HD>
+void launch_n(const QuantFwdArgs& a, int nr, int grid, hipStream_t stream) {
+    const dim3 nt(Cfg4<HD>::NWAVE * 64);
+    if (nr == 1) hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 1>), dim3(grid), nt, 0, stream, a);
+    else hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 2>), dim3(grid), nt, 0, stream, a);
+    launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE>(a, nr, grid, stream);
+}
+
+template <int HD>
+void launch_d(const QuantFwdArgs& a, int nr, int grid, hipStream_t stream) {
+    if (a.bf16) launch_n<DT_BF16, HD>(a, nr, grid, stream);
+    else launch_n<DT_FP16, HD>(a, nr, grid, stream);
+}
+
+}  // namespace
+
+// kd: kernel head dim; nr: 16-row tiles (1 or 2)
+hipError_t launch_fp4_decode(const QuantFwdArgs& a, int, int kd, int nr, int grid, hipStream_t stream) {
+    if (kd == 64) launch_d<64>(a, nr, grid, stream);
+    else if (kd == 128) launch_d<128>(a, nr, grid, stream);
+    else launch_d<256>(a, nr, grid, stream);
+    return hipGetLastError();
+}
+
+}  // namespace fa

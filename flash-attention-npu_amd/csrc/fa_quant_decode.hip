@@ -28,9 +28,7 @@
 // 32 us; one sequence of 777 keys: 15.3 us, 12 here, of which the start before the first
 // tile (list, ids, rows, scales: each waits for the one before) is most, and 4 in the merge.
 // Tiles in registers instead of LDS, with one wave per SIMD: 190, 55, 36 and 15 us.
-#include "fa_quant.h"
-#include "fa_pipe.h"
-#include "fa_quant_split.h"
+#include "fa_quant_list.h"
 
 #include <algorithm>
 
@@ -54,33 +52,6 @@ struct Cfg {
     static __device__ __forceinline__ int f(int r) { return HD == 64 ? (r >> 1) & 3 : HD == 128 ? r & 7 : r & 15; }
 };
 
-__device__ __forceinline__ int heads_per_group(const QuantFwdArgs& a) { return a.Hk % 4 == 0 ? 4 : a.Hk % 2 == 0 ? 2 : 1; }
-
-struct Seg {
-    int S, n;      // first tile of the list, tiles
-    int b, hk;
-    int lo_tile;
-    QuantSeq q;
-};
-
-__device__ __forceinline__ Seg seg_of(const QuantFwdArgs& a, const int* s_pref, int t, int hs, int h, int KT) {
-    int bl = 0, bh = a.B;
-    while (bh - bl > 1) {
-        const int mid = (bl + bh) >> 1;
-        if (s_pref[mid] <= t) bl = mid;
-        else bh = mid;
-    }
-    Seg s;
-    s.b = bl;
-    s.q = quant_seq(a, bl);
-    s.lo_tile = s.q.lo / KT;
-    s.n = (s.q.hi + KT - 1) / KT - s.lo_tile;
-    const int hg = (int)((uint32_t)(t - s_pref[bl]) / (uint32_t)max(s.n, 1));
-    s.hk = hg * hs + h;
-    s.S = s_pref[bl] + hg * s.n;
-    return s;
-}
-
 // One 16-key block of K or V into LDS: LPB loads of 1 KB, as dma16x4 (fa_pipe.h).
 template <int LPB>
 __device__ __forceinline__ void dma_block(unsigned lds, const char* base, const unsigned (&off)[LPB]) {
@@ -99,18 +70,6 @@ __device__ __forceinline__ void dma_block(unsigned lds, const char* base, const 
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %2, %1" ::"s"(lds), "s"(base), "v"(off[0])
                          : "memory", "m0");
     }
-}
-
-// max over the lanes l, l ^ 16, l ^ 32, l ^ 48. A swap exchanges the odd rows of 16
-// (32) lanes of one register with the even ones of the other. In assembly, since the
-// compiler's builtin gives the first result for both; it wants two wait states after
-// its operands' last write.
-__device__ __forceinline__ float max4(float v) {
-    float w = v;
-    asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(v), "+v"(w));
-    v = w = fmaxf(v, w);
-    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(v), "+v"(w));
-    return fmaxf(v, w);
 }
 
 // DT: type of q and out; CT: cache type; HD: kernel head dim (the cache's may be smaller: columns past it
@@ -551,97 +510,12 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
     }
 }
 
-// Merge of what a segment's workers left: 16 rows and 32 columns of a segment per
-// workgroup; groups of threads fold a share of the partials each, with a running
-// maximum, and meet in LDS. A row is empty where its weights sum to 0, which says so
-// for NaN as well: such partials have no part in the maximum (fmaxf).
-constexpr int MT = 512;
-template <int DT, int HD>
-__global__ void __launch_bounds__(MT) fa_quant_merge_kernel(QuantFwdArgs a, int grid, int nr) {
-    __shared__ __attribute__((aligned(16))) float s_acc[MT][8];
-    __shared__ float s_gm[MT], s_gs[MT];
-    constexpr int KT = Cfg<HD>::KT, COLS = HD / 32, CH = 4;  // 8-column chunks of a workgroup
-    const int sig = blockIdx.x / COLS, part = blockIdx.x % COLS;
-    const int b = (int)((uint32_t)sig / (uint32_t)a.Hk), hk = sig - b * a.Hk;
-    const int hs = heads_per_group(a), hg = hk / hs, hsel = hk - hg * hs;
-    const QuantSeq q = quant_seq(a, b);
-    const int T = a.sched[a.B], S0 = a.sched[b];
-    const int row0 = blockIdx.y * 16, rows = min(q.sq * a.g - row0, 16);
-    if (rows <= 0 || q.sq * a.g > a.dec_rows) return;
-    const int per = q.hi > q.lo ? (q.hi + KT - 1) / KT - q.lo / KT : 0, S = S0 + hg * per;
-    const Split sp = split_list(T, grid * (Cfg<HD>::NWAVE / hs));
-    int wf = 0, n = 0;
-    if (per > 0) {
-        wf = sp.owner(S);
-        n = sp.owner(S + per - 1) - wf + 1;
-        if (n == 1) return;  // written by its one worker
-    }
-    const bool slot1 = per > 0 && sp.first(wf) < S;  // the first partial is its worker's last
-    const int tid = threadIdx.x;
-    int rp = 1;
-    while (rp < rows) rp <<= 1;
-    const int GS = CH * rp, NG = MT / GS;
-    const int grp = tid / GS, rr = tid % GS / CH, d0 = part * 32 + tid % CH * 8;
-    float m = -INFINITY, sum = 0.f;
-    f32x4 acc0 = {0.f, 0.f, 0.f, 0.f}, acc1 = acc0;
-    if (rr < rows) {
-#pragma unroll 4
-        for (int j = grp; j < n; j += NG) {
-            const int64_t pr = (((int64_t)(wf + j) * hs + hsel) * 2 + (j == 0 && slot1 ? 1 : 0)) * (16 * nr) + row0 + rr;
-            const float v = a.part_lse[pr];
-            const f32x4 o0 = *reinterpret_cast<const f32x4*>(a.part_o + pr * HD + d0);
-            const f32x4 o1 = *reinterpret_cast<const f32x4*>(a.part_o + pr * HD + d0 + 4);
-            if (v != -INFINITY) {
-                const float mn = fmaxf(m, v);
-                const float c = fast_exp2((m - mn) * kLog2e), wgt = fast_exp2((v - mn) * kLog2e);
-                acc0 = acc0 * c + o0 * wgt;
-                acc1 = acc1 * c + o1 * wgt;
-                sum = sum * c + wgt;
-                m = mn;
-            }
-        }
-    }
-    *reinterpret_cast<f32x4*>(&s_acc[tid][0]) = acc0;
-    *reinterpret_cast<f32x4*>(&s_acc[tid][4]) = acc1;
-    s_gm[tid] = m;
-    s_gs[tid] = sum;
-    // halve the groups until one is left
-    for (int half = NG / 2; half > 0; half /= 2) {
-        __syncthreads();
-        if (grp < half) {
-            const int o = tid + half * GS;
-            const float mo = s_gm[o], M = fmaxf(m, mo);
-            if (s_gs[o] != 0.f || sum != 0.f) {
-                const float c = fast_exp2((m - M) * kLog2e), co = fast_exp2((mo - M) * kLog2e);
-                acc0 = acc0 * c + *reinterpret_cast<const f32x4*>(&s_acc[o][0]) * co;
-                acc1 = acc1 * c + *reinterpret_cast<const f32x4*>(&s_acc[o][4]) * co;
-                sum = sum * c + s_gs[o] * co;
-                m = M;
-                *reinterpret_cast<f32x4*>(&s_acc[tid][0]) = acc0;
-                *reinterpret_cast<f32x4*>(&s_acc[tid][4]) = acc1;
-                s_gm[tid] = m;
-                s_gs[tid] = sum;
-            }
-        }
-    }
-    if (grp != 0 || rr >= rows) return;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    acc0 *= inv;
-    acc1 *= inv;
-    const int r = row0 + rr, i = r / a.g, h = hk * a.g + r % a.g;
-    uint16_t* o = static_cast<uint16_t*>(a.out) + q_row(a, b, i, a.o_sb, a.o_si) + (int64_t)h * a.o_sh;
-    if (d0 < a.hd)
-        *reinterpret_cast<u32x4*>(o + d0) = u32x4{pack2<DT>(acc0[0], acc0[1]), pack2<DT>(acc0[2], acc0[3]),
-                                                  pack2<DT>(acc1[0], acc1[1]), pack2<DT>(acc1[2], acc1[3])};
-    if (d0 == 0) a.lse[lse_at(a, b, h, i)] = sum == 0.f ? INFINITY : m + fast_log2(sum) * kLn2;
-}
-
 template <int DT, int CT, int HD>
 void launch_n(const QuantFwdArgs& a, int nr, int grid, hipStream_t stream) {
     const dim3 nt(Cfg<HD>::NWAVE * 64);
     if (nr == 1) hipLaunchKernelGGL((fa_quant_decode_kernel<DT, CT, HD, 1>), dim3(grid), nt, 0, stream, a);
     else hipLaunchKernelGGL((fa_quant_decode_kernel<DT, CT, HD, 2>), dim3(grid), nt, 0, stream, a);
-    hipLaunchKernelGGL((fa_quant_merge_kernel<DT, HD>), dim3(a.B * a.Hk * (HD / 32), nr), dim3(MT), 0, stream, a, grid, nr);
+    launch_list_merge<DT, HD, Cfg<HD>::KT, Cfg<HD>::NWAVE>(a, nr, grid, stream);
 }
 
 template <int HD>

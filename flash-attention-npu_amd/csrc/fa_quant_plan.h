@@ -115,6 +115,9 @@ inline fa_status_t check_fwd(const fa_quant_fwd_params* p, Codes codes) {
     // the rows of 16 keys are addressed in 32 bits
     FA_CHECK(p->k_row_stride >= 0 && p->k_row_stride < (1 << 27) && p->v_row_stride >= 0 && p->v_row_stride < (1 << 27),
              "row strides of the caches must be in [0, 2^27)");
+    FA_CHECK(codes == Codes::Eight || (p->k_scale_block_stride >= 0 && p->k_scale_block_stride < (1 << 27) &&
+                                       p->v_scale_block_stride >= 0 && p->v_scale_block_stride < (1 << 27)),
+             "token strides of the scales of a 4-bit cache must be in [0, 2^27)");
     return FA_OK;
 }
 
