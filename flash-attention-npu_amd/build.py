@@ -31,7 +31,7 @@ HIP_SOURCES = ["fa_fwd.hip", "fa_fwd_pipe64.hip", "fa_fwd_pipe128.hip", "fa_fwd_
                "fa_fwd_pipe_fp8.hip", "fa_decode.hip", "fa_kv_prep.hip", "fa_bwd.hip", "fa_bwd_kv.hip",
                "fa_bwd_dq.hip", "fa_api.cpp", "fa_noalloc.hip", "fa_page_table.hip", "fa_quant_append.hip",
                "fa_quant_decode.hip", "fa_quant_prefill.hip", "fa_quant_api.cpp", "fa_quant_read.hip",
-               "fa_fp4_append.hip", "fa_fp4_attend.hip", "fa_fp4_decode.hip", "fa_fp4_api.cpp", "fa_rotary.hip", "fa_rotary_api.cpp"]
+               "fa_fp4_append.hip", "fa_fp4_decode.hip", "fa_fp4_prefill.hip", "fa_fp4_api.cpp", "fa_rotary.hip", "fa_rotary_api.cpp"]
 HIPFLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
     # no packed fp32 ops (v_pk_*_f32) in any generated code
@@ -65,6 +65,7 @@ SRC_FLAGS = {
     "fa_quant_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "fa_quant_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "fa_fp4_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "fa_fp4_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "fa_fwd.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"],
 }
 
