@@ -11,6 +11,7 @@
 
 namespace fa {
 hipError_t launch_fp4_append(QuantAppendArgs a, int dtype, hipStream_t stream);
+int fp4_decode_workers(int kd, int nr, int cus);
 hipError_t launch_fp4_decode(const QuantFwdArgs& a, int ct, int kd, int nr, int grid, hipStream_t stream);
 hipError_t launch_fp4_prefill(const QuantFwdArgs& a, int ct, int kd, int rows, int grid, hipStream_t stream);
 hipError_t launch_quant_read(QuantReadArgs a, int dtype, int ct, hipStream_t stream);
@@ -109,14 +110,14 @@ fa_status_t fa_fp4_fwd_workspace_size(const fa_quant_fwd_params* p, size_t* byte
     if (!bytes) return fail(FA_EINVAL, "bytes must not be null");
     const fa_status_t st = check_fwd(p, Codes::Four);
     if (st != FA_OK) return st;
-    *bytes = p->seqlen_q > 0 ? make_plan(p).total : 0;
+    *bytes = p->seqlen_q > 0 ? make_plan(p, fa::fp4_decode_workers).total : 0;
     return FA_OK;
 }
 
 fa_status_t fa_fp4_fwd(const fa_quant_fwd_params* p, void* stream) {
     const fa_status_t st = check_fwd(p, Codes::Four);
     if (st != FA_OK) return st;
-    return attend(p, stream, fa::launch_fp4_decode, fa::launch_fp4_prefill);
+    return attend(p, stream, fa::fp4_decode_workers, fa::launch_fp4_decode, fa::launch_fp4_prefill);
 }
 
 }  // extern "C"

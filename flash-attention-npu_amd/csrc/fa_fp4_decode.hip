@@ -5,12 +5,12 @@
 // list, cut into equal ranges, one per wave; what a range leaves of a sequence is merged by a
 // second launch.
 //
-// A lane loads, of each of 16 keys' rows that four lanes share, its quarter: 32 channels at head dim
-// 128, which have one scale, so a value is one conversion with its scale (fa_fp4.h). Tiles stay in
-// registers, two in flight beside the one at hand. Keys go from there straight into S^T = K.Q^T.
-// Values go through LDS once they are 16 bits wide, 32 keys at a time, since O^T = V^T.P^T wants
-// the keys of a channel side by side: written by rows, read by transpose reads. Nothing waits
-// for another wave.
+// Four neighbouring lanes load a key's row, 32 channels each at head dim 128, which have one scale, so a
+// value is one conversion with its scale (fa_fp4.h). A tile's registers are asked for again as
+// soon as they are used, so that one tile is always in flight. Keys change lanes through LDS as codes, since the
+// products want a row's quarters 16 lanes apart, and values once they are 16 bits wide, 32 keys at a
+// time, since O^T = V^T.P^T wants the keys of a channel side by side: written by rows, read by transpose
+// reads. Nothing waits for another wave.
 //
 // Weights are kept in units that make a row's largest 2^14 in fp16, so that a weight has all
 // its bits down to 2^-28 of that, and 2^-20 in bf16, whose values reach to 2^128: the sum of 2^20 of
@@ -26,14 +26,15 @@ namespace {
 
 template <int HD>
 struct Cfg4 {
-    static constexpr int NWAVE = HD == 256 ? 4 : 8;  // waves of a workgroup
+    static constexpr int NWAVE = 4;                  // waves of a workgroup
+    static constexpr int HS = 4;                     // heads of a group at most
     static constexpr int KT = 64, NB = KT / 16;      // keys of a tile, blocks of 16
     static constexpr int W = HD / 32;                // words of 8 codes that a lane has of a row
     static constexpr int NL = HD == 256 ? 2 : 1;     // loads of them, each under one scale
     static constexpr int DBLK = HD / 16;
     static constexpr int ROW = 2 * HD;               // bytes of a widened row
     static constexpr int TILES = 64 / NB;            // tiles whose places a wave's lanes hold
-    // first channel of word w of lane group G
+    // first channel of word w of quarter G
     static __device__ __forceinline__ int channel(int G, int w) {
         return HD == 64 ? 16 * G + 8 * w : HD == 128 ? 32 * G + 8 * w : 128 * (w >> 2) + 32 * G + 8 * (w & 3);
     }
@@ -43,6 +44,9 @@ struct Cfg4 {
         return HD == 64 ? swz_b64(r, c) : c ^ (((r & 7) << 1) | ((r >> 3) & 1));
     }
 };
+
+// Workgroups of a compute unit, a wave of each on a SIMD: as many as the registers hold.
+__host__ __device__ constexpr int groups_of_cu(int hd, int nr) { return hd == 256 ? 1 : 2; }
 
 // A tile's codes and scales, as a lane loads them
 template <int HD>
@@ -62,10 +66,26 @@ __device__ __forceinline__ void load_words(uint32_t* to, const uint8_t* p) {
     }
 }
 
+template <int N>
+__device__ __forceinline__ void words_write(unsigned a, const uint32_t* x) {
+    if constexpr (N == 4) row_write(a, u32x4{x[0], x[1], x[2], x[3]});
+    else *(__attribute__((address_space(3))) u32x2*)(size_t)a = u32x2{x[0], x[1]};
+}
+template <int N>
+__device__ __forceinline__ void words_read(uint32_t* to, unsigned a) {
+    if constexpr (N == 4) {
+        const u32x4 x = row_read(a);
+        to[0] = x[0], to[1] = x[1], to[2] = x[2], to[3] = x[3];
+    } else {
+        const u32x2 x = lds_load_u32x2(a);
+        to[0] = x[0], to[1] = x[1];
+    }
+}
+
 // DT: type of q and out; HD: kernel head dim (the cache's may be smaller: lanes past it
 // hold the row's first codes and meet zeros of q); NR: 16-row tiles of packed rows.
 template <int DT, int HD, int NR>
-__global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, 1) fa_fp4_decode_kernel(QuantFwdArgs a) {
+__global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, groups_of_cu(HD, NR)) fa_fp4_decode_kernel(QuantFwdArgs a) {
     using C = Cfg4<HD>;
     constexpr int NWAVE = C::NWAVE, NT = NWAVE * 64, KT = C::KT, NB = C::NB, W = C::W, NL = C::NL, DBLK = C::DBLK, ROW = C::ROW, TILES = C::TILES;
     constexpr bool SPLIT = DT == DT_BF16;
@@ -79,8 +99,9 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, 1) fa_fp4_decode_kernel(
         return *(const QuantFwdArgs*)p;
     };
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int li = lane & 15, G = lane >> 4;
-    const int hs = heads_per_group(a), hgs = a.Hk / hs;
+    const int li = lane & 15, G = lane >> 4;   // row (column) and quarter of a product's operand
+    const int lr = lane >> 2, lq = lane & 3;   // row and quarter that a lane loads of 16 keys: four lanes a row
+    const int hs = heads_per_group<Cfg4<HD>::HS>(a), hgs = a.Hk / hs;
 
     // ---- the list of tiles ----------------------------------------------------------
     for (int b = tid; b < a.B; b += NT) {
@@ -138,13 +159,13 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, 1) fa_fp4_decode_kernel(
     uint32_t mine[NL];  // the bits of codes that are the lane's own
 #pragma unroll
     for (int u = 0; u < NL; ++u) {
-        const int grp = HD == 64 ? G >> 1 : 4 * u + G, at = HD == 64 ? 8 * G : 64 * u + 16 * G;
+        const int grp = HD == 64 ? lq >> 1 : 4 * u + lq, at = HD == 64 ? 8 * lq : 64 * u + 16 * lq;
         const bool in = grp < groups;
         mine[u] = in ? ~0u : 0u;
-        kin[u] = (uint32_t)li * (uint32_t)a.k_si + (in ? at : 0);
-        vin[u] = (uint32_t)li * (uint32_t)a.v_si + (in ? at : 0);
-        ksin[u] = (uint32_t)li * (uint32_t)a.ks_sb + (in ? grp : 0);
-        vsin[u] = (uint32_t)li * (uint32_t)a.vs_sb + (in ? grp : 0);
+        kin[u] = (uint32_t)lr * (uint32_t)a.k_si + (in ? at : 0);
+        vin[u] = (uint32_t)lr * (uint32_t)a.v_si + (in ? at : 0);
+        ksin[u] = (uint32_t)lr * (uint32_t)a.ks_sb + (in ? grp : 0);
+        vsin[u] = (uint32_t)lr * (uint32_t)a.vs_sb + (in ? grp : 0);
     }
     const uint8_t* ksb = reinterpret_cast<const uint8_t*>(a.ks);
     const uint8_t* vsb = reinterpret_cast<const uint8_t*>(a.vs);
@@ -155,7 +176,7 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, 1) fa_fp4_decode_kernel(
     // Past the range the last tile is asked for again, so that every wait counts the same loads. The
     // places are those of asked tile's 16 until `places` moves on.
     int asked = t0;
-    unsigned bits0 = 0, bits1 = 0;  // visible blocks of the tile at hand and of the next
+    unsigned bits = 0;  // visible blocks of the tile at hand
     auto ask_k = [&](Tile<HD>& T) {
         const int i = asked - t0;
         if (asked < t1 && i % TILES == 0) {
@@ -256,9 +277,14 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, 1) fa_fp4_decode_kernel(
     // ---- a tile ----------------------------------------------------------------------------
     const unsigned vt = lds_addr(s_v[wave]);
     const int tr_row = 4 * G + (li >> 2);
+    // Keys' codes use the values' place: 16 rows of KB / 16 bytes, a lane's piece in a slot that sets the rows of
+    // eight lanes' reads on different banks
+    constexpr int KB = 16 * 4 * (W / NL) * 4, PIECE = 4 * (W / NL);
+    const auto piece = [](int r, int q) { return (r * 4 + (q ^ ((HD == 64 ? r >> 3 : r >> 2) & 3))) * PIECE; };
+    const unsigned kt_put = vt + piece(lr, lq), kt_get = vt + piece(li, G);
     auto compute = [&](int t, Tile<HD>& T) {
         const int key0 = (cs.lo_tile + (t - cs.S)) * KT;
-        const unsigned ok = bits0;
+        const unsigned ok = bits;
         const bool full = ok == 15u && key0 >= flo && key0 + KT - 1 <= fhi;
         // codes past the head dim are 0, since inf x 0 is NaN
         if (groups * kGroup != HD) {
@@ -267,6 +293,19 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, 1) fa_fp4_decode_kernel(
 #pragma unroll
                 for (int w = 0; w < W; ++w) T.k[b][w] &= mine[w * NL / W];
         }
+        // Keys to the lanes that want them, the codes by LDS and the scales from lane to lane
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int u = 0; u < NL; ++u) words_write<W / NL>(kt_put + (b * NL + u) * KB, T.k[b] + u * (W / NL));
+        uint32_t kw[NB][W], ks[NB][NL];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int u = 0; u < NL; ++u) {
+                words_read<W / NL>(kw[b] + u * (W / NL), kt_get + (b * NL + u) * KB);
+                ks[b][u] = (uint32_t)__builtin_amdgcn_ds_bpermute((4 * li + G) * 4, (int)T.ks[b][u]);
+            }
         // S^T = K . Q^T
         f32x4 x[NR][NB];
 #pragma unroll
@@ -275,13 +314,13 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, 1) fa_fp4_decode_kernel(
             for (int rt = 0; rt < NR; ++rt) x[rt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                const u32x4 op = fp4_widen8<DT>(T.k[b][w], fp4_scale(T.ks[b][w * NL / W]));
+                const u32x4 op = fp4_widen8<DT>(kw[b][w], fp4_scale(ks[b][w * NL / W]));
 #pragma unroll
                 for (int rt = 0; rt < NR; ++rt) x[rt][b] = mfma16x16x32<DT>(op, qreg[rt][w], x[rt][b]);
             }
         }
         ask_k(T);
-        const unsigned bits2 = bits_of();
+        bits = bits_of();
         if (a.softcap > 0.f) {
 #pragma unroll
             for (int rt = 0; rt < NR; ++rt)
@@ -345,14 +384,14 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, 1) fa_fp4_decode_kernel(
         for (int k2 = 0; k2 < NB / 2; ++k2) {
 #pragma unroll
             for (int bb = 0; bb < 2; ++bb) {
-                const int b = 2 * k2 + bb, r = 16 * bb + li, j = key0 + 16 * b + li;
+                const int b = 2 * k2 + bb, r = 16 * bb + lr, j = key0 + 16 * b + lr;
                 // values that no row sees must not meet the products, where 0 x NaN is NaN
                 const bool seen = full || ((ok >> b & 1) && j >= cs.q.lo && j < cs.q.hi);
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
                     u32x4 y = fp4_widen8<DT>(T.v[b][w], fp4_scale(T.vs[b][w * NL / W]));
                     if (!full && !seen) y = u32x4{0u, 0u, 0u, 0u};
-                    row_write(vt + r * ROW + (C::slot(li, C::channel(G, w) / 8) << 4), y);
+                    row_write(vt + r * ROW + (C::slot(lr, C::channel(lq, w) / 8) << 4), y);
                 }
             }
             if (k2 == NB / 2 - 1) ask_v(T);
@@ -367,20 +406,16 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, 1) fa_fp4_decode_kernel(
                 }
             }
         }
-        bits0 = bits1;
-        bits1 = bits2;
     };
 
-    Tile<HD> A, B;
+    Tile<HD> T;
     ask_ids(t0);
-    ask_k(A);
-    bits0 = bits_of();
-    ask_v(A);
-    ask_k(B);
-    bits1 = bits_of();
-    ask_v(B);
+    ask_k(T);
+    bits = bits_of();
+    ask_v(T);
     int qat = t0, send = t0;
-    auto step = [&](int t, Tile<HD>& T) {
+#pragma unroll 1
+    for (int t = t0; t < t1; ++t) {
         if (t == qat) {
             begin_seg(t);
             send = min(cs.S + cs.n, t1);
@@ -390,35 +425,33 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, 1) fa_fp4_decode_kernel(
             end_seg();
             qat = send;
         }
-    };
-#pragma unroll 1
-    for (int t = t0; t < t1; t += 2) {
-        step(t, A);
-        if (t + 1 < t1) step(t + 1, B);
     }
 }
 
 template <int DT, int HD>
-void launch_n(const QuantFwdArgs& a, int nr, int grid, hipStream_t stream) {
+void launch_n(const QuantFwdArgs& a, int nr, int cus, hipStream_t stream) {
     const dim3 nt(Cfg4<HD>::NWAVE * 64);
+    const int grid = cus * groups_of_cu(HD, nr);
     if (nr == 1) hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 1>), dim3(grid), nt, 0, stream, a);
     else hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 2>), dim3(grid), nt, 0, stream, a);
-    launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE>(a, nr, grid, stream);
+    launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE, Cfg4<HD>::HS>(a, nr, grid, stream);
 }
 
 template <int HD>
-void launch_d(const QuantFwdArgs& a, int nr, int grid, hipStream_t stream) {
-    if (a.bf16) launch_n<DT_BF16, HD>(a, nr, grid, stream);
-    else launch_n<DT_FP16, HD>(a, nr, grid, stream);
+void launch_d(const QuantFwdArgs& a, int nr, int cus, hipStream_t stream) {
+    if (a.bf16) launch_n<DT_BF16, HD>(a, nr, cus, stream);
+    else launch_n<DT_FP16, HD>(a, nr, cus, stream);
 }
 
 }  // namespace
 
-// kd: kernel head dim; nr: 16-row tiles (1 or 2)
-hipError_t launch_fp4_decode(const QuantFwdArgs& a, int, int kd, int nr, int grid, hipStream_t stream) {
-    if (kd == 64) launch_d<64>(a, nr, grid, stream);
-    else if (kd == 128) launch_d<128>(a, nr, grid, stream);
-    else launch_d<256>(a, nr, grid, stream);
+int fp4_decode_workers(int kd, int nr, int cus) { return cus * groups_of_cu(kd, nr) * Cfg4<128>::NWAVE; }
+
+// kd: kernel head dim; nr: 16-row tiles (1 or 2); cus: compute units
+hipError_t launch_fp4_decode(const QuantFwdArgs& a, int, int kd, int nr, int cus, hipStream_t stream) {
+    if (kd == 64) launch_d<64>(a, nr, cus, stream);
+    else if (kd == 128) launch_d<128>(a, nr, cus, stream);
+    else launch_d<256>(a, nr, cus, stream);
     return hipGetLastError();
 }
 

@@ -10,12 +10,15 @@
 
 namespace fa {
 hipError_t launch_page_table(const PageTableArgs& a, hipStream_t stream);
+int quant_decode_workers(int kd, int grid);
 hipError_t launch_quant_append(QuantAppendArgs a, int dtype, int ct, hipStream_t stream);
 hipError_t launch_quant_decode(const QuantFwdArgs& a, int ct, int kd, int nr, int grid, hipStream_t stream);
 hipError_t launch_quant_prefill(const QuantFwdArgs& a, int ct, int kd, int rows, int grid, hipStream_t stream);
 }  // namespace fa
 
 namespace {
+
+int workers(int kd, int, int cus) { return fa::quant_decode_workers(kd, cus); }
 
 fa_status_t check_table(const fa_page_table_params* p) {
     FA_CHECK(p != nullptr, "params must not be null");
@@ -81,14 +84,14 @@ fa_status_t fa_quant_fwd_workspace_size(const fa_quant_fwd_params* p, size_t* by
     if (!bytes) return fail(FA_EINVAL, "bytes must not be null");
     fa_status_t st = check_fwd(p, Codes::Eight);
     if (st != FA_OK) return st;
-    *bytes = p->seqlen_q > 0 ? make_plan(p).total : 0;
+    *bytes = p->seqlen_q > 0 ? make_plan(p, workers).total : 0;
     return FA_OK;
 }
 
 fa_status_t fa_quant_fwd(const fa_quant_fwd_params* p, void* stream) {
     fa_status_t st = check_fwd(p, Codes::Eight);
     if (st != FA_OK) return st;
-    return attend(p, stream, fa::launch_quant_decode, fa::launch_quant_prefill);
+    return attend(p, stream, workers, fa::launch_quant_decode, fa::launch_quant_prefill);
 }
 
 }  // extern "C"

@@ -10,7 +10,11 @@ namespace fa {
 
 namespace {
 
-__device__ __forceinline__ int heads_per_group(const QuantFwdArgs& a) { return a.Hk % 4 == 0 ? 4 : a.Hk % 2 == 0 ? 2 : 1; }
+// kv heads whose tiles neighbouring waves take: a key's rows of them lie side by side
+template <int MOST>
+__device__ __forceinline__ int heads_per_group(const QuantFwdArgs& a) {
+    return MOST == 8 && a.Hk % 8 == 0 ? 8 : a.Hk % 4 == 0 ? 4 : a.Hk % 2 == 0 ? 2 : 1;
+}
 
 struct Seg {
     int S, n;      // first tile of the list, tiles
@@ -54,15 +58,15 @@ __device__ __forceinline__ float max4(float v) {
 // maximum, and meet in LDS. A row is empty where its weights sum to 0, which says so
 // for NaN as well: such partials have no part in the maximum (fmaxf).
 constexpr int MT = 512;
-// KT: keys of a tile, NWAVE: waves of a workgroup of the kernel that left them.
-template <int DT, int HD, int KT, int NWAVE>
+// KT: keys of a tile, NWAVE: waves of a workgroup of the kernel that left them, HS: heads of a group at most.
+template <int DT, int HD, int KT, int NWAVE, int HS>
 __global__ void __launch_bounds__(MT) fa_quant_merge_kernel(QuantFwdArgs a, int grid, int nr) {
     __shared__ __attribute__((aligned(16))) float s_acc[MT][8];
     __shared__ float s_gm[MT], s_gs[MT];
     constexpr int COLS = HD / 32, CH = 4;  // 8-column chunks of a workgroup
     const int sig = blockIdx.x / COLS, part = blockIdx.x % COLS;
     const int b = (int)((uint32_t)sig / (uint32_t)a.Hk), hk = sig - b * a.Hk;
-    const int hs = heads_per_group(a), hg = hk / hs, hsel = hk - hg * hs;
+    const int hs = heads_per_group<HS>(a), hg = hk / hs, hsel = hk - hg * hs;
     const QuantSeq q = quant_seq(a, b);
     const int T = a.sched[a.B], S0 = a.sched[b];
     const int row0 = blockIdx.y * 16, rows = min(q.sq * a.g - row0, 16);
@@ -135,9 +139,9 @@ __global__ void __launch_bounds__(MT) fa_quant_merge_kernel(QuantFwdArgs a, int 
     if (d0 == 0) a.lse[lse_at(a, b, h, i)] = sum == 0.f ? INFINITY : m + fast_log2(sum) * kLn2;
 }
 
-template <int DT, int HD, int KT, int NWAVE>
+template <int DT, int HD, int KT, int NWAVE, int HS>
 void launch_list_merge(const QuantFwdArgs& a, int nr, int grid, hipStream_t stream) {
-    hipLaunchKernelGGL((fa_quant_merge_kernel<DT, HD, KT, NWAVE>), dim3(a.B * a.Hk * (HD / 32), nr), dim3(MT), 0, stream, a, grid, nr);
+    hipLaunchKernelGGL((fa_quant_merge_kernel<DT, HD, KT, NWAVE, HS>), dim3(a.B * a.Hk * (HD / 32), nr), dim3(MT), 0, stream, a, grid, nr);
 }
 
 }  // namespace

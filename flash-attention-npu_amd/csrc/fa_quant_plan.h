@@ -12,7 +12,6 @@
 
 namespace fa {
 int64_t quant_decode_batch(int kd, int Hk, int64_t capacity);
-int quant_decode_workers(int kd, int grid);
 int quant_prefill_rows(int kd, bool many);
 int compute_units();
 }  // namespace fa
@@ -129,7 +128,7 @@ struct Plan {
     int g;
     int dec_rows;    // sequences of at most so many packed rows run on the decode kernel
     bool prefill;    // some may have more
-    int nr, grid;    // decode: 16-row tiles, workgroups
+    int nr, grid;    // decode: 16-row tiles, compute units
     int pf_rows, pf_grid;
     bool cut;        // prefill: the items are cut over the workgroups
     size_t off_lse, off_o, off_pcut, off_plse, off_po, total;
@@ -137,7 +136,10 @@ struct Plan {
 
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-inline Plan make_plan(const fa_quant_fwd_params* p) {
+// The waves that share the list of tiles, by the kernel head dim, 16-row tiles and compute units
+using Workers = int (*)(int kd, int nr, int cus);
+
+inline Plan make_plan(const fa_quant_fwd_params* p, Workers workers) {
     Plan pl{};
     pl.kd = kernel_headdim(p->headdim);
     pl.nb = (int)std::min<int64_t>(p->batch, batch_of_launch(p));
@@ -155,7 +157,7 @@ inline Plan make_plan(const fa_quant_fwd_params* p) {
     pl.grid = cus;
     size_t off = 0;
     if (pl.dec_rows) {
-        const size_t parts = (size_t)fa::quant_decode_workers(pl.kd, pl.grid) * 2 * 16 * pl.nr;
+        const size_t parts = (size_t)workers(pl.kd, pl.nr, pl.grid) * 2 * 16 * pl.nr;
         pl.off_lse = off = align256(sizeof(int) * (nb + 1));
         pl.off_o = off = align256(off + sizeof(float) * parts);
         off = align256(off + sizeof(float) * parts * pl.kd);
@@ -229,10 +231,10 @@ using LaunchDecode = hipError_t (*)(const fa::QuantFwdArgs& a, int ct, int kd, i
 using LaunchPrefill = hipError_t (*)(const fa::QuantFwdArgs& a, int ct, int kd, int rows, int grid, hipStream_t stream);
 
 // A checked attention call
-inline fa_status_t attend(const fa_quant_fwd_params* p, void* stream, LaunchDecode decode, LaunchPrefill prefill) {
+inline fa_status_t attend(const fa_quant_fwd_params* p, void* stream, Workers workers, LaunchDecode decode, LaunchPrefill prefill) {
     const int64_t rows = p->cu_seqlens_q ? (int64_t)p->total_q : (int64_t)p->batch * p->seqlen_q;
     if (rows == 0 || p->seqlen_q == 0) return FA_OK;
-    const Plan pl = make_plan(p);
+    const Plan pl = make_plan(p, workers);
     if (pl.total > 0) {
         if (!p->workspace || p->workspace_bytes < pl.total)
             return fail(FA_EWORKSPACE, "workspace of %zu bytes required, %zu given", pl.total, p->workspace ? p->workspace_bytes : (size_t)0);

@@ -38,7 +38,7 @@ namespace fa {
 fa_status_t report_error(fa_status_t st, const char*) { return st; }
 int compute_units() { return 256; }
 int64_t quant_decode_batch(int, int, int64_t) { return 1 << 20; }
-int quant_decode_workers(int kd, int grid) { return grid * (kd == 256 ? 4 : 8); }
+int fp4_decode_workers(int kd, int nr, int cus) { return 4 * cus * (kd == 256 || nr == 2 ? 2 : 3); }
 int quant_prefill_rows(int kd, bool many) { return many && kd < 256 ? 256 : 128; }
 static void check_cache(int hd, int page, int Hk) {
     CHECK(hd >= 32 && hd <= 256 && hd % 32 == 0 && page >= 16 && page % 16 == 0 && Hk >= 1 && Hk <= 65535, "cache %d %d %d", hd, page, Hk);
