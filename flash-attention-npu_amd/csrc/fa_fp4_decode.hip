@@ -12,13 +12,15 @@
 // time, since O^T = V^T.P^T wants the keys of a channel side by side: written by rows, read by transpose
 // reads. Nothing waits for another wave.
 //
-// Weights are kept in units that make a row's largest 2^14 in fp16, so that a weight has all
-// its bits down to 2^-28 of that, and 2^-20 in bf16, whose values reach to 2^128: the sum of 2^20 of
-// them stays in fp32. In bf16, whose 8 bits would be most of the result's error, a weight is the
-// sum of two bf16 numbers and meets V twice; the products have the time, since what bounds
-// a step is memory.
+// Weights and values meet as fp16, in bf16 calls too, whose 8 bits for a weight would be most of the
+// result's error: fp16 holds the values of scales from 2^-23 to 2^13 exactly. Weights are kept in units
+// that make a row's largest 2^14, so that one has all its bits down to 2^-28 of that. A bf16 call whose
+// values leave that range goes on in bf16, a weight as the sum of two numbers, in units that make the
+// largest 2^-20: the sum of 2^20 values of 2^127 stays in fp32.
 #include "fa_fp4.h"
 #include "fa_quant_list.h"
+
+#include <type_traits>
 
 namespace fa {
 
@@ -88,8 +90,9 @@ template <int DT, int HD, int NR>
 __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, groups_of_cu(HD, NR)) fa_fp4_decode_kernel(QuantFwdArgs a) {
     using C = Cfg4<HD>;
     constexpr int NWAVE = C::NWAVE, NT = NWAVE * 64, KT = C::KT, NB = C::NB, W = C::W, NL = C::NL, DBLK = C::DBLK, ROW = C::ROW, TILES = C::TILES;
-    constexpr bool SPLIT = DT == DT_BF16;
-    constexpr float kTop = DT == DT_BF16 ? -20.f : 14.f;  // log2 of the largest weight
+    constexpr float kTop = 14.f, kTopWide = -20.f;  // log2 of the largest weight
+    // bf16 calls go by fp16 while they can, but for those whose registers hold the products' code once only
+    constexpr bool WIDE = DT == DT_BF16, BOTH = WIDE && (NR == 1 || HD == 64);
     __shared__ __attribute__((aligned(1024))) char s_v[NWAVE][32 * ROW];
     __shared__ int s_pref[kQuantMaxB + 1];
 
@@ -215,13 +218,17 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, groups_of_cu(HD, NR)) fa
     int qi[NR];
     f32x4 oacc[NR][DBLK];
     float m_run[NR], l_run[NR];
+    bool wide = WIDE && !BOTH;  // values out of the range of fp16 have come up
     int rows = 0;
     int flo = 0, fhi = 0;      // keys that every row sees
     const float scale2 = a.softcap > 0.f ? a.scale / a.softcap : a.scale * kLog2e;
+    // what scores are multiplied by in the exponent, where that leaves their order
+    const float late = a.softcap > 0.f || !(scale2 > 0.f) ? 1.f : scale2;
     auto begin_seg = [&](int t) {
         const QuantFwdArgs& A = anew();
         cs = seg_of(A, s_pref, t, hs, hsel, KT);
         rows = cs.q.sq * A.g;
+        wide = WIDE && !BOTH;
         flo = key_lo(cs.q.sk - 1, A.wl, 0);
         fhi = min(key_hi(cs.q.sk - cs.q.sq, A.wr, 0), cs.q.sk - 1);
 #pragma unroll
@@ -251,7 +258,7 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, groups_of_cu(HD, NR)) fa
             const float l = wave_sum16x4(l_run[rt]);
             const bool some = l != 0.f;  // NaN: some
             const float inv = some ? 1.f / l : 0.f;
-            const float lse = some ? (m_run[rt] - kTop + fast_log2(l)) * kLn2 : INFINITY;
+            const float lse = some ? (m_run[rt] - (wide ? kTopWide : kTop) + fast_log2(l)) * kLn2 : INFINITY;
             if (r >= rows) continue;
             if (whole) {
                 const int h = cs.hk * A.g + r % A.g;
@@ -328,7 +335,7 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, groups_of_cu(HD, NR)) fa
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[rt][b][e] = a.softcap * kLog2e * fast_tanh(x[rt][b][e] * scale2);
-        } else {
+        } else if (!(scale2 > 0.f)) {
 #pragma unroll
             for (int rt = 0; rt < NR; ++rt)
 #pragma unroll
@@ -348,63 +355,105 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, groups_of_cu(HD, NR)) fa
                     }
             }
         }
-        // weights, the running maximum's 2^kTop
-        u32x4 pk[NR][NB / 2], pl[NR][NB / 2];
-        float up[NR];
+        // values that no row sees must not meet the products, where 0 x NaN is NaN
+        if (!full) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const int j = key0 + 16 * b + lr;
+                const bool seen = (ok >> b & 1) && j >= cs.q.lo && j < cs.q.hi;
+#pragma unroll
+                for (int w = 0; w < W; ++w) T.v[b][w] = seen ? T.v[b][w] : 0u;
+#pragma unroll
+                for (int u = 0; u < NL; ++u) T.vs[b][u] = seen ? T.vs[b][u] : 127u;
+            }
+        }
+        if constexpr (BOTH) {
+            uint32_t out = 0;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int u = 0; u < NL; ++u) out = max(out, T.vs[b][u] - 104u);
+            if (!wide && __ballot(out > 140u - 104u)) {
+                wide = true;
+#pragma unroll
+                for (int rt = 0; rt < NR; ++rt) {
+                    l_run[rt] *= 0x1p-34f;  // 2^(kTopWide - kTop)
+#pragma unroll
+                    for (int db = 0; db < DBLK; ++db) oacc[rt][db] *= 0x1p-34f;
+                }
+            }
+        }
+        // the running maximum
+        float up[NR], base[NR];
         bool moved = false;
 #pragma unroll
         for (int rt = 0; rt < NR; ++rt) {
             float mx = -INFINITY;
 #pragma unroll
             for (int b = 0; b < NB; ++b) mx = fmaxf(mx, fmaxf(fmaxf(x[rt][b][0], x[rt][b][1]), fmaxf(x[rt][b][2], x[rt][b][3])));
-            mx = fmaxf(m_run[rt], max4(mx));
+            mx = fmaxf(m_run[rt], max4(mx) * late);
             moved |= mx > m_run[rt];
             const float u = mx == -INFINITY ? 0.f : mx;
             up[rt] = fast_exp2(m_run[rt] - u);
+            base[rt] = u - (wide ? kTopWide : kTop);
             m_run[rt] = mx;
-            l_run[rt] *= up[rt];
-#pragma unroll
-            for (int k2 = 0; k2 < NB / 2; ++k2) {
-                f32x8 w;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] = fast_exp2(x[rt][2 * k2 + (e >> 2)][e & 3] - (u - kTop));
-                l_run[rt] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-                pk[rt][k2] = pack8<DT>(w);
-                if constexpr (SPLIT) pl[rt][k2] = pack8<DT>(w - widen8<DT>(pk[rt][k2]));
-            }
         }
         if (__ballot(moved)) {
 #pragma unroll
-            for (int rt = 0; rt < NR; ++rt)
+            for (int rt = 0; rt < NR; ++rt) {
+                l_run[rt] *= up[rt];
 #pragma unroll
                 for (int db = 0; db < DBLK; ++db) oacc[rt][db] *= up[rt];
-        }
-        // O^T += V^T . P^T, 32 keys at a time
-#pragma unroll
-        for (int k2 = 0; k2 < NB / 2; ++k2) {
-#pragma unroll
-            for (int bb = 0; bb < 2; ++bb) {
-                const int b = 2 * k2 + bb, r = 16 * bb + lr, j = key0 + 16 * b + lr;
-                // values that no row sees must not meet the products, where 0 x NaN is NaN
-                const bool seen = full || ((ok >> b & 1) && j >= cs.q.lo && j < cs.q.hi);
-#pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    u32x4 y = fp4_widen8<DT>(T.v[b][w], fp4_scale(T.vs[b][w * NL / W]));
-                    if (!full && !seen) y = u32x4{0u, 0u, 0u, 0u};
-                    row_write(vt + r * ROW + (C::slot(lr, C::channel(lq, w) / 8) << 4), y);
-                }
             }
-            if (k2 == NB / 2 - 1) ask_v(T);
+        }
+        // weights, and O^T += V^T . P^T, 32 keys at a time, on operands of type OT
+        auto values = [&](auto tag) {
+            constexpr int OT = decltype(tag)::value;
+            constexpr bool TWO = OT == DT_BF16;
 #pragma unroll
-            for (int db = 0; db < DBLK; ++db) {
-                const unsigned p = vt + tr_row * ROW + (C::slot(tr_row, 2 * db + ((li & 3) >> 1)) << 4) + (li & 1) * 8;
-                const u32x4 op = tr_read(p, p + 16 * ROW);
+            for (int k2 = 0; k2 < NB / 2; ++k2) {
+                u32x4 pk[NR], pl[NR];
 #pragma unroll
                 for (int rt = 0; rt < NR; ++rt) {
-                    oacc[rt][db] = mfma16x16x32<DT>(op, pk[rt][k2], oacc[rt][db]);
-                    if constexpr (SPLIT) oacc[rt][db] = mfma16x16x32<DT>(op, pl[rt][k2], oacc[rt][db]);
+                    f32x8 w;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = fast_exp2(__builtin_fmaf(x[rt][2 * k2 + (e >> 2)][e & 3], late, -base[rt]));
+                    l_run[rt] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+                    pk[rt] = pack8<OT>(w);
+                    if constexpr (TWO) {
+                        pl[rt] = pack8<OT>(w - widen8<OT>(pk[rt]));
+                        if constexpr (BOTH) fence();  // the rare path is not to take registers of the other
+                    }
+                }
+#pragma unroll
+                for (int bb = 0; bb < 2; ++bb) {
+                    const int b = 2 * k2 + bb, r = 16 * bb + lr;
+#pragma unroll
+                    for (int w = 0; w < W; ++w)
+                        row_write(vt + r * ROW + (C::slot(lr, C::channel(lq, w) / 8) << 4), fp4_widen8<OT>(T.v[b][w], fp4_scale(T.vs[b][w * NL / W])));
+                    if constexpr (TWO && BOTH) fence();
+                }
+                if (k2 == NB / 2 - 1) ask_v(T);
+#pragma unroll
+                for (int db = 0; db < DBLK; ++db) {
+                    const unsigned p = vt + tr_row * ROW + (C::slot(tr_row, 2 * db + ((li & 3) >> 1)) << 4) + (li & 1) * 8;
+                    const u32x4 op = tr_read(p, p + 16 * ROW);
+#pragma unroll
+                    for (int rt = 0; rt < NR; ++rt) {
+                        oacc[rt][db] = mfma16x16x32<OT>(op, pk[rt], oacc[rt][db]);
+                        if constexpr (TWO) oacc[rt][db] = mfma16x16x32<OT>(op, pl[rt], oacc[rt][db]);
+                    }
+                    if constexpr (TWO && BOTH) fence();
                 }
             }
+        };
+        if constexpr (!WIDE) {
+            values(std::integral_constant<int, DT_FP16>{});
+        } else if constexpr (!BOTH) {
+            values(std::integral_constant<int, DT_BF16>{});
+        } else {
+            if (wide) values(std::integral_constant<int, DT_BF16>{});
+            else values(std::integral_constant<int, DT_FP16>{});
         }
     };
 
@@ -434,7 +483,9 @@ void launch_n(const QuantFwdArgs& a, int nr, int cus, hipStream_t stream) {
     const int grid = cus * groups_of_cu(HD, nr);
     if (nr == 1) hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 1>), dim3(grid), nt, 0, stream, a);
     else hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 2>), dim3(grid), nt, 0, stream, a);
-    launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE, Cfg4<HD>::HS>(a, nr, grid, stream);
+    // Many segments fill the chip with small workgroups, few want more threads for the pieces of each
+    if ((int64_t)a.B * a.Hk * (HD / 32) >= 4 * cus) launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE, Cfg4<HD>::HS, 256>(a, nr, grid, stream);
+    else launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE, Cfg4<HD>::HS>(a, nr, grid, stream);
 }
 
 template <int HD>

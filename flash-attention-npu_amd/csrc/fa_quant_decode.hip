@@ -535,7 +535,7 @@ void launch_d(const QuantFwdArgs& a, int ct, int nr, int grid, hipStream_t strea
 // merge has fewer than 2^32 threads (kd: kernel head dim)
 int64_t quant_decode_batch(int kd, int Hk, int64_t capacity) {
     const int64_t hgs = Hk % 4 == 0 ? Hk / 4 : Hk % 2 == 0 ? Hk / 2 : Hk, kt = kd == 64 ? Cfg<64>::KT : Cfg<128>::KT;
-    return std::min(0x7fffffffll / (hgs * (capacity / kt + 2)), 0xffffffffll / MT / ((int64_t)Hk * (kd / 32)));
+    return std::min(0x7fffffffll / (hgs * (capacity / kt + 2)), 0xffffffffll / kMergeThreads / ((int64_t)Hk * (kd / 32)));
 }
 
 int quant_decode_workers(int kd, int grid) { return grid * (kd == 256 ? Cfg<256>::NWAVE : Cfg<128>::NWAVE); }

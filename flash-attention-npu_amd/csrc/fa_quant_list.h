@@ -57,9 +57,9 @@ __device__ __forceinline__ float max4(float v) {
 // workgroup; groups of threads fold a share of the partials each, with a running
 // maximum, and meet in LDS. A row is empty where its weights sum to 0, which says so
 // for NaN as well: such partials have no part in the maximum (fmaxf).
-constexpr int MT = 512;
-// KT: keys of a tile, NWAVE: waves of a workgroup of the kernel that left them, HS: heads of a group at most.
-template <int DT, int HD, int KT, int NWAVE, int HS>
+// KT: keys of a tile, NWAVE: waves of a workgroup of the kernel that left them, HS: heads of a group at most,
+// MT: threads of a workgroup.
+template <int DT, int HD, int KT, int NWAVE, int HS, int MT>
 __global__ void __launch_bounds__(MT) fa_quant_merge_kernel(QuantFwdArgs a, int grid, int nr) {
     __shared__ __attribute__((aligned(16))) float s_acc[MT][8];
     __shared__ float s_gm[MT], s_gs[MT];
@@ -139,9 +139,10 @@ __global__ void __launch_bounds__(MT) fa_quant_merge_kernel(QuantFwdArgs a, int 
     if (d0 == 0) a.lse[lse_at(a, b, h, i)] = sum == 0.f ? INFINITY : m + fast_log2(sum) * kLn2;
 }
 
-template <int DT, int HD, int KT, int NWAVE, int HS>
+constexpr int kMergeThreads = 512;
+template <int DT, int HD, int KT, int NWAVE, int HS, int MT = kMergeThreads>
 void launch_list_merge(const QuantFwdArgs& a, int nr, int grid, hipStream_t stream) {
-    hipLaunchKernelGGL((fa_quant_merge_kernel<DT, HD, KT, NWAVE, HS>), dim3(a.B * a.Hk * (HD / 32), nr), dim3(MT), 0, stream, a, grid, nr);
+    hipLaunchKernelGGL((fa_quant_merge_kernel<DT, HD, KT, NWAVE, HS, MT>), dim3(a.B * a.Hk * (HD / 32), nr), dim3(MT), 0, stream, a, grid, nr);
 }
 
 }  // namespace
