@@ -14,6 +14,38 @@ namespace {
 
 constexpr int kMostRows = 32;  // rows of a workgroup
 
+// The largest |x| of a group, 8 values in each of four neighbouring lanes, by its bits: below the
+// sign they are in the order of the values, inf and NaN on top.
+__device__ __forceinline__ uint32_t group_most(u32x4 x) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 m = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[e] & 0x7fff7fffu));
+    uint32_t most = max((uint32_t)m[0], (uint32_t)m[1]);
+    most = max(most, (uint32_t)__builtin_amdgcn_mov_dpp((int)most, 0xb1, 0xf, 0xf, true));  // lane ^ 1
+    return max(most, (uint32_t)__builtin_amdgcn_mov_dpp((int)most, 0x4e, 0xf, 0xf, true));  // lane ^ 2
+}
+
+// Eight codes of x / s
+template <int DT>
+__device__ __forceinline__ uint32_t codes8(u32x4 x, float s) {
+    const uint32_t x0 = x[0], x1 = x[1], x2 = x[2], x3 = x[3];  // (a bit cast of a vector's element takes the first)
+    uint32_t r = 0;
+    if constexpr (DT == DT_FP16) {
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, x0), s, 0);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, x1), s, 1);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, x2), s, 2);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, x3), s, 3);
+    } else {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, x0), s, 0);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, x1), s, 1);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, x2), s, 2);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, x3), s, 3);
+    }
+    return r;
+}
+
 // Four lanes hold a group, 8 channels each. Rows of a workgroup: their places first, then all
 // their groups of k and v.
 template <int DT>
@@ -35,45 +67,54 @@ __global__ void __launch_bounds__(256) fa_fp4_append_kernel(QuantAppendArgs a, i
         }
     }
     __syncthreads();
-    for (uint32_t id = threadIdx.x; id < (uint32_t)n * per_row.d; id += 256) {
-        const int r = (int)udiv(per_row, id);
-        const uint32_t in = id - (uint32_t)r * per_row.d, h = udiv(a.chunks, in), c = in - h * a.chunks.d;
-        if (s_at[0][r] == -1) continue;  // all four lanes
-        u32x4 x[2];
+    // Two of a lane's pieces at a time, k and v of each: four loads are under way together.
+    const uint32_t all = (uint32_t)n * per_row.d;
+    for (uint32_t id0 = threadIdx.x; id0 < all; id0 += 512) {
+        u32x4 x[2][2];
+        int r[2], h[2], c[2];
+        bool ok[2];
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv)
-            x[kv] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.x[kv]) + (r0 + r) * a.x_si[kv] + (int64_t)h * a.x_sh[kv] + c * 8);
+        for (int u = 0; u < 2; ++u) {
+            const uint32_t id = id0 + 256 * u;
+            ok[u] = id < all;
+            r[u] = ok[u] ? (int)udiv(per_row, id) : 0;
+            const uint32_t in = ok[u] ? id - (uint32_t)r[u] * per_row.d : 0;
+            h[u] = (int)udiv(a.chunks, in);
+            c[u] = (int)(in - (uint32_t)h[u] * a.chunks.d);
+            ok[u] = ok[u] && s_at[0][r[u]] != -1;  // alike in the four lanes of a group
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-            // the largest |x| by its bits, which are in the order of the values, inf and NaN on top
-            uint32_t most = 0;
-            bool odd = false;
+            for (int kv = 0; kv < 2; ++kv)
+                x[u][kv] = ok[u] ? *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.x[kv]) + (r0 + r[u]) * a.x_si[kv] +
+                                                                   (int64_t)h[u] * a.x_sh[kv] + c[u] * 8)
+                                 : u32x4{0u, 0u, 0u, 0u};
+        }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) most = max(most, x[kv][e >> 1] >> (16 * (e & 1)) & 0x7fffu);
-            most = max(most, (uint32_t)__shfl_xor((int)most, 1));
-            most = max(most, (uint32_t)__shfl_xor((int)most, 2));
-            odd = most >= kInf;
-            const bool nan = most > kInf;
-            most = min(most, kInf - 1);
-            // most = m 2^e with 1 <= m < 2: s = 2^(e - 2), 2^(e - 1) where m > 1.5
-            const uint32_t u = __builtin_bit_cast(uint32_t, f16_to_32<DT>((uint16_t)most));
-            const int e = min(max((int)(u >> 23) - 127 - 2 + ((u & 0x7fffffu) > 0x400000u ? 1 : 0), -100), kMost);
-            const float inv = exp2i(-e);
-            uint32_t code = 0;
-            float y[8];
+        for (int u = 0; u < 2; ++u) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                uint32_t b = x[kv][i >> 1] >> (16 * (i & 1)) & 0xffffu;
-                if (odd && (b & 0x7fffu) >= kInf) b = (b & 0x8000u) | (kInf - 1);
-                y[i] = f16_to_32<DT>((uint16_t)b) * inv;
+            for (int kv = 0; kv < 2; ++kv) {
+                u32x4& y = x[u][kv];
+                uint32_t most = group_most(y);
+                const bool nan = most > kInf;
+                if (__ballot(most >= kInf)) {
+                    // inf, and NaN of whatever, as the largest finite value
+                    if (most >= kInf) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if ((y[e >> 1] >> (16 * (e & 1)) & 0x7fffu) >= kInf)
+                                y[e >> 1] = (y[e >> 1] & ~(0x7fffu << (16 * (e & 1)))) | (kInf - 1) << (16 * (e & 1));
+                        most = kInf - 1;
+                    }
+                }
+                // most = m 2^e with 1 <= m < 2: s = 2^(e - 2), 2^(e - 1) where m > 1.5
+                const uint32_t b = __builtin_bit_cast(uint32_t, f16_to_32<DT>((uint16_t)most));
+                const int e = min(max((int)(b >> 23) - 127 - 2 + ((b & 0x7fffffu) > 0x400000u ? 1 : 0), -100), kMost);
+                const uint32_t code = codes8<DT>(y, exp2i(e));
+                if (ok[u]) {
+                    *reinterpret_cast<uint32_t*>(a.c[kv] + s_at[kv][r[u]] + (int64_t)h[u] * a.c_sh[kv] + c[u] * 4) = code;
+                    if (c[u] % 4 == 0)
+                        reinterpret_cast<uint8_t*>(a.s[kv])[s_at[2 + kv][r[u]] + (int64_t)h[u] * a.s_sh[kv] + c[u] / 4] = nan ? 255 : (uint8_t)(e + 127);
+                }
             }
-            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[0], y[1], 1.f, 0);
-            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[2], y[3], 1.f, 1);
-            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[4], y[5], 1.f, 2);
-            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[6], y[7], 1.f, 3);
-            *reinterpret_cast<uint32_t*>(a.c[kv] + s_at[kv][r] + (int64_t)h * a.c_sh[kv] + c * 4) = code;
-            if (c % 4 == 0)
-                reinterpret_cast<uint8_t*>(a.s[kv])[s_at[2 + kv][r] + (int64_t)h * a.s_sh[kv] + c / 4] = nan ? 255 : (uint8_t)(e + 127);
         }
     }
 }

@@ -14,6 +14,21 @@ namespace {
 constexpr int kMostRows = 32;  // rows of a workgroup
 enum : int { DT_F32 = 2 };
 
+// Eight codes under their scale, in fp32 (0 of a row that is not there: the codes and the scale are 0)
+template <int CT>
+__device__ __forceinline__ f32x8 values8(u32x2 w, float s) {
+    f32x8 y;
+    if constexpr (CT == CT_FP4) {
+        const auto p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s, 1),
+                   p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s, 3);
+        y[0] = p0[0], y[1] = p0[1], y[2] = p1[0], y[3] = p1[1], y[4] = p2[0], y[5] = p2[1], y[6] = p3[0], y[7] = p3[1];
+    } else {
+        const u32x2 lo = widen4<CT>(w[0]), hi = widen4<CT>(w[1]);  // exact in fp16
+        y = widen8<DT_FP16>(u32x4{lo[0], lo[1], hi[0], hi[1]}) * s;
+    }
+    return y;
+}
+
 // A thread makes 8 channels of a row and head, of k and of v.
 template <int OT, int CT>
 __global__ void __launch_bounds__(256) fa_quant_read_kernel(QuantReadArgs a, int rows_per_group) {
@@ -49,50 +64,51 @@ __global__ void __launch_bounds__(256) fa_quant_read_kernel(QuantReadArgs a, int
         }
     }
     __syncthreads();
-    for (uint32_t id = threadIdx.x; id < (uint32_t)n * a.per_row.d; id += 256) {
-        const int r = (int)udiv(a.per_row, id);
-        const uint32_t in = id - (uint32_t)r * a.per_row.d, h = udiv(a.chunks, in), c = in - h * a.chunks.d;
-        const bool ok = s_at[0][r] != -1;
-        const int64_t to = ((r0 + r) * (int64_t)a.per_row.d + in) * 8;
+    // Two of a lane's pieces at a time, k and v of each: eight loads are under way together.
+    const uint32_t all = (uint32_t)n * a.per_row.d;
+    for (uint32_t id0 = threadIdx.x; id0 < all; id0 += 512) {
+        u32x2 w[2][2];
+        float s[2][2];
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-            f32x8 y = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            u32x4 o = {0u, 0u, 0u, 0u};
-            if (ok) {
-                const uint8_t* codes = a.c[kv] + s_at[kv][r] + (int64_t)h * a.c_sh[kv];
-                const int64_t sat = s_at[2 + kv][r] + (int64_t)h * a.s_sh[kv];
-                if constexpr (CT == CT_FP4) {
-                    const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + c * 4);
-                    const float s = fp4_scale(static_cast<const uint8_t*>(a.s[kv])[sat + c / 4]);
-                    if constexpr (OT == DT_F32) {
+        for (int u = 0; u < 2; ++u) {
+            const uint32_t id = id0 + 256 * u;
+            const int r = id < all ? (int)udiv(a.per_row, id) : 0;
+            const uint32_t in = id < all ? id - (uint32_t)r * a.per_row.d : 0, h = udiv(a.chunks, in), c = in - h * a.chunks.d;
+            const bool ok = id < all && s_at[0][r] != -1;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            typedef float f32x2 __attribute__((ext_vector_type(2)));
-                            f32x2 p;
-                            if (e == 0) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0);
-                            else if (e == 1) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
-                            else if (e == 2) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2);
-                            else p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
-                            y[2 * e] = p[0];
-                            y[2 * e + 1] = p[1];
-                        }
+            for (int kv = 0; kv < 2; ++kv) {
+                w[u][kv] = u32x2{0u, 0u};
+                s[u][kv] = 0.f;
+                if (ok) {
+                    const uint8_t* codes = a.c[kv] + s_at[kv][r] + (int64_t)h * a.c_sh[kv];
+                    const int64_t sat = s_at[2 + kv][r] + (int64_t)h * a.s_sh[kv];
+                    if constexpr (CT == CT_FP4) {
+                        w[u][kv][0] = *reinterpret_cast<const uint32_t*>(codes + c * 4);
+                        s[u][kv] = fp4_scale(static_cast<const uint8_t*>(a.s[kv])[sat + c / 4]);
                     } else {
-                        o = fp4_widen8<OT>(w, s);
+                        w[u][kv] = *reinterpret_cast<const u32x2*>(codes + c * 8);
+                        s[u][kv] = static_cast<const float*>(a.s[kv])[sat];
                     }
-                } else {
-                    const u32x2 w = *reinterpret_cast<const u32x2*>(codes + c * 8);
-                    const float s = static_cast<const float*>(a.s[kv])[sat];
-                    const u32x2 lo = widen4<CT>(w[0]), hi = widen4<CT>(w[1]);  // exact in fp16
-                    y = widen8<DT_FP16>(u32x4{lo[0], lo[1], hi[0], hi[1]}) * s;
-                    if constexpr (OT != DT_F32) o = pack8<OT>(y);
                 }
             }
-            if constexpr (OT == DT_F32) {
-                float* t = static_cast<float*>(a.o[kv]) + to;
-                *reinterpret_cast<f32x4*>(t) = f32x4{y[0], y[1], y[2], y[3]};
-                *reinterpret_cast<f32x4*>(t + 4) = f32x4{y[4], y[5], y[6], y[7]};
-            } else {
-                *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.o[kv]) + to) = o;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const uint32_t id = id0 + 256 * u;
+            if (id >= all) break;
+            const int64_t to = (r0 * (int64_t)a.per_row.d + id) * 8;
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+                if constexpr (OT == DT_F32) {
+                    const f32x8 y = values8<CT>(w[u][kv], s[u][kv]);
+                    float* t = static_cast<float*>(a.o[kv]) + to;
+                    *reinterpret_cast<f32x4*>(t) = f32x4{y[0], y[1], y[2], y[3]};
+                    *reinterpret_cast<f32x4*>(t + 4) = f32x4{y[4], y[5], y[6], y[7]};
+                } else {
+                    u32x4* t = reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.o[kv]) + to);
+                    if constexpr (CT == CT_FP4) *t = fp4_widen8<OT>(w[u][kv][0], s[u][kv]);
+                    else *t = pack8<OT>(values8<CT>(w[u][kv], s[u][kv]));
+                }
             }
         }
     }
