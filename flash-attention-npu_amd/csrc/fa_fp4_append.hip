@@ -126,7 +126,7 @@ hipError_t launch_fp4_append(QuantAppendArgs a, int dtype, hipStream_t stream) {
     a.chunks = udiv_make((uint32_t)a.hd / 8);
     const UDiv per_row = udiv_make((uint32_t)a.Hk * (uint32_t)(a.hd / 8));
     // several passes of a workgroup where there are workgroups enough for that
-    const int rows = (int)std::min<int64_t>(std::max<int64_t>(a.total_new / 2048, 1), kMostRows);
+    const int rows = (int)std::min<int64_t>(std::max<int64_t>(a.total_new / 4096, 1), kMostRows);
     const int64_t groups = (a.total_new + rows - 1) / rows, most = 1 << 24;  // 2^32 threads of a launch
     for (int64_t g = 0; g < groups; g += most - 1) {
         a.row0 = g * rows;

@@ -125,7 +125,7 @@ void launch_read_t(const QuantReadArgs& a, int ct, int rows, dim3 grid, hipStrea
 }  // namespace
 
 hipError_t launch_quant_read(QuantReadArgs a, int dtype, int ct, hipStream_t stream) {
-    const int rows = (int)std::min<int64_t>(std::max<int64_t>(a.total / 2048, 1), kMostRows);
+    const int rows = (int)std::min<int64_t>(std::max<int64_t>(a.total / 4096, 1), kMostRows);
     const int64_t groups = (a.total + rows - 1) / rows, most = (1 << 24) - 1;  // less than 2^32 threads of a launch
     for (int64_t g = 0; g < groups; g += most) {
         a.row0 = g * rows;

@@ -87,5 +87,11 @@ def apply_rotary_emb(q, k, rotary_cos, rotary_sin, positions: Optional[torch.Ten
     inplace turns q and k themselves, without new memory; neither may hold a row twice, nor share memory with the other.
     Gradients of q and k are turned back, which takes no saved rows; the tables get none."""
     offsets = maybe_contiguous(seqlen_offsets) if isinstance(seqlen_offsets, torch.Tensor) else None
-    return ApplyRotaryEmb.apply(q, k, rotary_cos, rotary_sin, positions, offsets, 0 if offsets is not None else int(seqlen_offsets),
-                                maybe_contiguous(cu_seqlens), bool(rotary_interleaved), bool(inplace))
+    where = (positions, offsets, 0 if offsets is not None else int(seqlen_offsets), maybe_contiguous(cu_seqlens), bool(rotary_interleaved))
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return ApplyRotaryEmb.apply(q, k, rotary_cos, rotary_sin, *where, bool(inplace))
+    if inplace:
+        _rotary_in_place(q, k, rotary_cos, rotary_sin, *where, False)
+        return (q, k) if k is not None else q
+    turned_q, turned_k = _rotary(q, k, rotary_cos, rotary_sin, *where, False)
+    return (turned_q, turned_k) if k is not None else turned_q
