@@ -112,6 +112,7 @@ fa_status_t fa_rotary_table(const fa_rotary_table_params* p, void* stream) {
             const double keep = std::fmin(std::fmax((turns - p->low) / (p->high - p->low), 0.0), 1.0);
             f *= keep + (1.0 - keep) / p->factor;
         }
+        FA_CHECK(std::isfinite(f), "angle %d of base, factor and original_length is not finite", i);
         a.turns[i] = f / kTwoPi;
     }
     const hipError_t e = fa::launch_rotary_table(a, p->dtype, static_cast<hipStream_t>(stream));

@@ -112,7 +112,7 @@ TABLE = dict(dtype=2, rotary_dim=64, scaling=0, base=1e4, factor=1.0, attention_
     (dict(dtype=3), "fp32, fp16 or bf16"), (dict(rotary_dim=8), "multiple of 16"), (dict(rotary_dim=272), "multiple of 16"), (dict(rotary_dim=-16), "multiple of 16"),
     (dict(num_positions=-1), "negative"), (dict(base=-1.0), "base"), (dict(base=float("inf")), "base"), (dict(factor=float("nan")), "factor"), (dict(scaling=4), "scaling"),
     (dict(scaling=-1), "scaling"), (dict(scaling=3), "original_length"), (dict(scaling=3, original_length=8.0), "low"), (dict(cos=None), "required"),
-    (dict(sin=PTR + 8), "aligned"), (dict(attention_factor=float("nan")), "attention_factor")])
+    (dict(scaling=1, factor=5e-324, base=1e-300), "not finite"), (dict(sin=PTR + 8), "aligned"), (dict(attention_factor=float("nan")), "attention_factor")])
 def test_table_refuses(more, says):
     assert capi.rotary_table(**dict(TABLE, **more)) == capi.FA_EINVAL and says in capi.last_error(), capi.last_error()
 

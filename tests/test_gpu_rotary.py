@@ -242,6 +242,78 @@ def test_gradients_of_one_and_broadcast():
         fa.apply_rotary_emb(q.clone().requires_grad_(), None, cos, sin, inplace=True)  # a leaf
 
 
+def test_second_gradients():
+    """The gradient of a gradient: the rotation again, of q and k and of one alone."""
+    print("case rotate second gradients", flush=True)
+    g = torch.Generator().manual_seed(14)
+    cos, sin = tables(8, 32, torch.float32)
+    place = torch.arange(8).expand(2, 8)
+    for both in (True, False):
+        x, dx, w = (torch.randn(2, 8, 3, 32, generator=g).to(torch.bfloat16).to(DEV) for _ in range(3))
+        x.requires_grad_()
+        dx.requires_grad_()
+        out = fa.apply_rotary_emb(x, x * 2 if both else None, cos, sin)
+        (first,) = torch.autograd.grad(out[0] if both else out, x, dx, create_graph=True)
+        check(first, dx.detach().cpu(), cos, sin, place, True, torch.bfloat16, -1.0)
+        (second,) = torch.autograd.grad(first, dx, w)
+        check(second, w.cpu(), cos, sin, place, True, torch.bfloat16)
+
+
+def test_in_place_on_parts_of_a_projection():
+    """q and k out of one projection, turned where they lie: right gradients, or a refusal by autograd."""
+    print("case rotate projection", flush=True)
+    g = torch.Generator().manual_seed(15)
+    cos, sin = tables(8, 32, torch.float32)
+    place = torch.arange(8).expand(2, 8)
+    leaf = torch.randn(2, 8, 6, 32, generator=g).to(torch.bfloat16).to(DEV).requires_grad_()
+    d = torch.randn(2, 8, 6, 32, generator=g).to(torch.bfloat16)
+    try:
+        qkv = leaf * 1.0
+        q, k = fa.apply_rotary_emb(qkv[:, :, :3], qkv[:, :, 3:5], cos, sin, inplace=True)
+        (grad,) = torch.autograd.grad((q, k), leaf, (d[:, :, :3].to(DEV), d[:, :, 3:5].to(DEV)))
+    except RuntimeError as e:
+        assert "view" in str(e)
+    else:
+        check(grad[:, :, :5], d[:, :, :5], cos, sin, place, True, torch.bfloat16, -1.0)
+    qkv = leaf.detach().clone()
+    q, k = fa.apply_rotary_emb(qkv[:, :, :3], qkv[:, :, 3:5], cos, sin, inplace=True)
+    check(qkv[:, :, :5], leaf.detach().cpu()[:, :, :5], cos, sin, place, True, torch.bfloat16)
+    assert torch.equal(qkv[:, :, 5], leaf[:, :, 5]) and q.data_ptr() == qkv.data_ptr()
+
+
+def test_captured_backward():
+    """Forward and backward in one graph, leaves and gradients in place, replayed with other values."""
+    print("case rotate captured backward", flush=True)
+    g = torch.Generator().manual_seed(16)
+    cos, sin = tables(8, 32, torch.float32)
+    place = torch.arange(8)
+    q, k = (torch.zeros(8, h, 32, dtype=torch.bfloat16, device=DEV, requires_grad=True) for h in (4, 2))
+    dq, dk = (torch.zeros_like(t) for t in (q, k))
+
+    def step():
+        a, b = fa.apply_rotary_emb(q, k, cos, sin)
+        return a, b, *torch.autograd.grad((a, b), (q, k), (dq, dk))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a, b, ga, gb = step()
+    for _ in range(3):
+        vals = [torch.randn(t.shape, generator=g).to(t.dtype) for t in (q, k, dq, dk)]
+        with torch.no_grad():
+            for t, v in zip((q, k, dq, dk), vals):
+                t.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, v, sign in zip((a, b, ga, gb), vals, (1.0, 1.0, -1.0, -1.0)):
+            check(got, v, cos, sin, place, True, torch.bfloat16, sign)
+
+
 def test_layouts():
     """Rows that 16-byte loads cannot take are copied, or refused in place; heads first; rows repeated."""
     print("case rotate layouts", flush=True)
@@ -318,6 +390,7 @@ def test_refusals():
     for bad in (dict(rotary_dim=24), dict(rotary_dim=0), dict(rotary_dim=272), dict(base=0.0), dict(base=math.nan), dict(scaling="other"),
                 dict(scaling="linear", factor=0.0), dict(scaling="by_parts", factor=2.0), dict(scaling="by_parts", original_length=5, low=2.0, high=2.0),
                 dict(dtype=torch.float64), dict(positions=mk(4, dt=f32)), dict(positions=mk(2, 2, dt=i64)), dict(positions=pos.cpu()),
-                dict(attention_factor=math.inf)):
+                dict(attention_factor=math.inf),
+                dict(scaling="linear", factor=5e-324, base=1e-300)):
         with pytest.raises(RuntimeError):
             fa.rotary_cos_sin(**dict(dict(positions=pos, rotary_dim=32), **bad))
