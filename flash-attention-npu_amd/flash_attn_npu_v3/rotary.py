@@ -42,44 +42,20 @@ def rotary_cos_sin(positions, rotary_dim, base=10000.0, scaling=None, factor=1.0
                   float(original_length), float(low), float(high), float(attention_factor), dtype)
 
 
-class ApplyRotaryEmb(torch.autograd.Function):
+class ApplyRotaryEmbInPlace(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, seqlen_offsets, seqlen_offset, cu_seqlens, interleaved, conjugate, inplace):
-        where = (positions, seqlen_offsets, seqlen_offset, cu_seqlens, interleaved, conjugate)
+    def forward(ctx, q, k, cos, sin, positions, seqlen_offsets, seqlen_offset, cu_seqlens, interleaved):
+        _rotary_in_place(q, k, cos, sin, positions, seqlen_offsets, seqlen_offset, cu_seqlens, interleaved, False)
         ctx.save_for_backward(cos, sin, positions, seqlen_offsets, cu_seqlens)
-        ctx.seqlen_offset, ctx.interleaved, ctx.conjugate = seqlen_offset, interleaved, conjugate
-        if inplace:
-            _rotary_in_place(q, k, cos, sin, *where)
-            ctx.mark_dirty(*(x for x in (q, k) if x is not None))
-            return (q, k) if k is not None else q
-        q, turned = _rotary(q, k, cos, sin, *where)
-        return (q, turned) if k is not None else q
+        ctx.seqlen_offset, ctx.interleaved = seqlen_offset, interleaved
+        ctx.mark_dirty(*(x for x in (q, k) if x is not None))
+        return (q, k) if k is not None else q
 
     @staticmethod
     def backward(ctx, dq, dk=None):
-        # the turn back, which has a gradient of its own
         cos, sin, positions, seqlen_offsets, cu_seqlens = ctx.saved_tensors
-        need_q, need_k = ctx.needs_input_grad[:2]
-        rest = (cos, sin, positions, seqlen_offsets, ctx.seqlen_offset, cu_seqlens, ctx.interleaved, not ctx.conjugate)
-        if need_q and need_k:
-            dq, dk = _turn(dq, dk, *rest)
-        elif need_q:
-            dq, dk = _turn(dq, None, *rest), None
-        elif need_k:
-            dq, dk = None, _turn(dk, None, *rest)
-        else:
-            dq = dk = None
-        return (dq, dk) + (None,) * 9
-
-
-def _turn(q, k, cos, sin, *where, inplace=False):
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return ApplyRotaryEmb.apply(q, k, cos, sin, *where, inplace)
-    if inplace:
-        _rotary_in_place(q, k, cos, sin, *where)
-        return (q, k) if k is not None else q
-    turned_q, turned_k = _rotary(q, k, cos, sin, *where)
-    return (turned_q, turned_k) if k is not None else turned_q
+        dq, turned = _rotary(dq, dk, cos, sin, positions, seqlen_offsets, ctx.seqlen_offset, cu_seqlens, ctx.interleaved, True)
+        return (dq, turned if dk is not None else None) + (None,) * 7
 
 
 def apply_rotary_emb(q, k, rotary_cos, rotary_sin, positions: Optional[torch.Tensor] = None, seqlen_offsets=0,
@@ -99,5 +75,11 @@ def apply_rotary_emb(q, k, rotary_cos, rotary_sin, positions: Optional[torch.Ten
     inplace turns q and k themselves, without new memory; neither may hold a row twice, nor share memory with the other.
     Gradients of q and k are turned back, which takes no saved rows; the tables get none."""
     offsets = maybe_contiguous(seqlen_offsets) if isinstance(seqlen_offsets, torch.Tensor) else None
-    return _turn(q, k, rotary_cos, rotary_sin, positions, offsets, 0 if offsets is not None else int(seqlen_offsets),
-                 maybe_contiguous(cu_seqlens), bool(rotary_interleaved), False, inplace=bool(inplace))
+    where = (positions, offsets, 0 if offsets is not None else int(seqlen_offsets), maybe_contiguous(cu_seqlens), bool(rotary_interleaved))
+    if inplace:
+        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+            return ApplyRotaryEmbInPlace.apply(q, k, rotary_cos, rotary_sin, *where)
+        _rotary_in_place(q, k, rotary_cos, rotary_sin, *where, False)
+        return (q, k) if k is not None else q
+    turned_q, turned_k = _rotary(q, k, rotary_cos, rotary_sin, *where, False)
+    return (turned_q, turned_k) if k is not None else turned_q
