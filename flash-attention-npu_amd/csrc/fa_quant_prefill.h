@@ -99,6 +99,18 @@ __device__ __forceinline__ void dma_fp4(unsigned lds, uint64_t k, uint64_t v, ui
         "global_load_lds_ubyte %4, off offset:2304" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(k), "v"(v), "v"(ks), "v"(vs)
         : "memory", "m0");
 }
+// The same from scalar bases and offsets of 32 bits
+__device__ __forceinline__ void dma_fp4(unsigned lds, uint64_t k, uint64_t v, uint64_t ks, uint64_t vs, unsigned kin, unsigned vin, unsigned ksin,
+                                        unsigned vsin) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 3\n\t"
+        "global_load_lds_dwordx4 %5, %1\n\t"
+        "global_load_lds_dwordx4 %6, %2 offset:1024\n\t"
+        "global_load_lds_ubyte %7, %3 offset:2048\n\t"
+        "global_load_lds_ubyte %8, %4 offset:2304" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "s"(k), "s"(v), "s"(ks), "s"(vs), "v"(kin),
+        "v"(vin), "v"(ksin), "v"(vsin)
+        : "memory", "m0");
+}
 // the dword at an LDS address
 __device__ __forceinline__ uint32_t word_read(unsigned a) {
     return *(const __attribute__((address_space(3))) uint32_t*)(size_t)a;
@@ -294,9 +306,11 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
             have_a = have_b;
             have_b = have >> (tg * NB);
             part_b = base + t * BN < k_lo || base + (t + 1) * BN > k_hi || !full || (have_b & kTileBlocks) != kTileBlocks;
-            if constexpr (FOUR) {
+            if constexpr (FOUR && HD > 64) {
+                dma_fp4(raw + (t & 1) * (NW * O::RAW), from(ko, 0), from(vo, 0), from(kso, 0), from(vso, 0), kin, vin, ksin, vsin);
+            } else if constexpr (FOUR) {
                 // at head dim 64 a wave's rows lie in two blocks
-                auto mine = [&](int64_t o) { return HD == 64 && lane >= 32 ? from(o, 1) : from(o, 0); };
+                auto mine = [&](int64_t o) { return lane >= 32 ? from(o, 1) : from(o, 0); };
                 dma_fp4(raw + (t & 1) * (NW * O::RAW), mine(ko) + kin, mine(vo) + vin, mine(kso) + ksin, mine(vso) + vsin);
             } else {
                 dma16_kkvv(raw + (t & 1) * (NW * O::RAW), from(ko, 0), from(ko, 1), from(vo, 0), from(vo, 1), kin, vin);
