@@ -110,14 +110,14 @@ fa_status_t fa_fp4_fwd_workspace_size(const fa_quant_fwd_params* p, size_t* byte
     if (!bytes) return fail(FA_EINVAL, "bytes must not be null");
     const fa_status_t st = check_fwd(p, Codes::Four);
     if (st != FA_OK) return st;
-    *bytes = p->seqlen_q > 0 ? make_plan(p, fa::fp4_decode_workers).total : 0;
+    *bytes = p->seqlen_q > 0 ? make_plan(p, fa::fp4_decode_workers, true).total : 0;
     return FA_OK;
 }
 
 fa_status_t fa_fp4_fwd(const fa_quant_fwd_params* p, void* stream) {
     const fa_status_t st = check_fwd(p, Codes::Four);
     if (st != FA_OK) return st;
-    return attend(p, stream, fa::fp4_decode_workers, fa::launch_fp4_decode, fa::launch_fp4_prefill);
+    return attend(p, stream, fa::fp4_decode_workers, fa::launch_fp4_decode, fa::launch_fp4_prefill, true);
 }
 
 }  // extern "C"

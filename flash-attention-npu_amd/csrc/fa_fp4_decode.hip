@@ -85,8 +85,9 @@ __device__ __forceinline__ void words_read(uint32_t* to, unsigned a) {
 }
 
 // DT: type of q and out; HD: kernel head dim (the cache's may be smaller: lanes past it
-// hold the row's first codes and meet zeros of q); NR: 16-row tiles of packed rows.
-template <int DT, int HD, int NR>
+// hold the row's first codes and meet zeros of q); NR: 16-row tiles of packed rows; BLK: sequences of
+// more rows are there in blocks (fa_quant_list.h).
+template <int DT, int HD, int NR, bool BLK>
 __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, groups_of_cu(HD, NR)) fa_fp4_decode_kernel(QuantFwdArgs a) {
     using C = Cfg4<HD>;
     constexpr int NWAVE = C::NWAVE, NT = NWAVE * 64, KT = C::KT, NB = C::NB, W = C::W, NL = C::NL, DBLK = C::DBLK, ROW = C::ROW, TILES = C::TILES;
@@ -94,7 +95,7 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, groups_of_cu(HD, NR)) fa
     // bf16 calls go by fp16 while they can, but for those whose registers hold the products' code once only
     constexpr bool WIDE = DT == DT_BF16, BOTH = WIDE && (NR == 1 || HD == 64);
     __shared__ __attribute__((aligned(1024))) char s_v[NWAVE][32 * ROW];
-    __shared__ int s_pref[kQuantMaxB + 1];
+    __shared__ int s_pref[kQuantMaxB + 1], s_blk[BLK ? kQuantMaxB + 1 : 1];
 
     auto anew = []() -> const QuantFwdArgs& {  // as in fa_quant_decode.hip
         auto p = __builtin_amdgcn_kernarg_segment_ptr();
@@ -107,20 +108,48 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, groups_of_cu(HD, NR)) fa
     const int hs = heads_per_group<Cfg4<HD>::HS>(a), hgs = a.Hk / hs;
 
     // ---- the list of tiles ----------------------------------------------------------
-    for (int b = tid; b < a.B; b += NT) {
-        const QuantSeq s = quant_seq(a, b);
-        s_pref[b + 1] = s.hi > s.lo && s.sq * a.g <= a.dec_rows ? hgs * ((s.hi + KT - 1) / KT - s.lo / KT) : 0;
+    const int hsel = wave % hs;
+    int n = a.B;  // its entries
+    if constexpr (BLK) {
+        static_assert(NR * 16 == kBlockRows, "");
+        __shared__ int64_t s_sum[NWAVE];
+        const bool all = blocks_take<NT>(a, s_sum);
+        for (int b = tid; b < a.B; b += NT) {
+            const QuantSeq s = quant_seq(a, b);
+            s_blk[b + 1] = all || s.sq * a.g <= a.dec_rows ? blocks_of(a, s) : 0;
+        }
+        __syncthreads();
+        if (wave == 0) prefix_sums(s_blk, a.B);
+        __syncthreads();
+        n = min(s_blk[a.B], a.blocks);  // (a.blocks is enough for prefixes of rows)
+        for (int e = tid; e < n; e += NT) {
+            Seg s;
+            s.b = place_of(s_blk, a.B, e);
+            s.q = quant_seq(a, s.b);
+            cut_to_block(a, s, e - s_blk[s.b]);
+            s_pref[e + 1] = s.q.hi > s.q.lo ? hgs * ((s.q.hi + KT - 1) / KT - s.q.lo / KT) : 0;
+        }
+        if (blockIdx.x == 0)
+            for (int b = tid; b <= a.B; b += NT) a.block_pref[b] = s_blk[b];
+    } else {
+        for (int b = tid; b < a.B; b += NT) {
+            const QuantSeq s = quant_seq(a, b);
+            s_pref[b + 1] = s.hi > s.lo && s.sq * a.g <= a.dec_rows ? hgs * ((s.hi + KT - 1) / KT - s.lo / KT) : 0;
+        }
     }
     __syncthreads();
-    if (wave == 0) prefix_sums(s_pref, a.B);
+    if (wave == 0) prefix_sums(s_pref, n);
     __syncthreads();
     if (blockIdx.x == 0)
-        for (int b = tid; b <= a.B; b += NT) a.sched[b] = s_pref[b];
+        for (int b = tid; b <= n; b += NT) a.sched[b] = s_pref[b];
+    auto seg_at = [&](const QuantFwdArgs& A, int t) {
+        if constexpr (BLK) return block_seg_of(A, s_blk, s_pref, n, t, hs, hsel, KT);
+        else return seg_of(A, s_pref, t, hs, hsel, KT);
+    };
 
-    const int hsel = wave % hs;
     const int gw = (wave / hs) * gridDim.x + blockIdx.x;  // wave-major, as in fa_decode.hip
     const int64_t wid = (int64_t)gw * hs + hsel;
-    const Split sp = split_list(s_pref[a.B], gridDim.x * (NWAVE / hs));
+    const Split sp = split_list(s_pref[n], gridDim.x * (NWAVE / hs));
     const int t0 = __builtin_amdgcn_readfirstlane(sp.first(gw)), t1 = __builtin_amdgcn_readfirstlane(sp.first(gw + 1));
     if (t0 >= t1) return;  // no barrier follows: the waves go on alone
 
@@ -135,7 +164,7 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, groups_of_cu(HD, NR)) fa
         id = -1;
         inp = kvh = 0;
         if (t < t1) {
-            const Seg s = seg_of(A, s_pref, t, hs, hsel, KT);
+            const Seg s = seg_at(A, t);
             const int key = (s.lo_tile + (t - s.S)) * KT + (lane % NB) * 16;
             kvh = s.hk;
             if (key < s.q.hi && key + 16 > s.q.lo) {
@@ -226,17 +255,18 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, groups_of_cu(HD, NR)) fa
     const float late = a.softcap > 0.f || !(scale2 > 0.f) ? 1.f : scale2;
     auto begin_seg = [&](int t) {
         const QuantFwdArgs& A = anew();
-        cs = seg_of(A, s_pref, t, hs, hsel, KT);
-        rows = cs.q.sq * A.g;
+        cs = seg_at(A, t);
+        rows = cs.rows;
         wide = WIDE && !BOTH;
-        flo = key_lo(cs.q.sk - 1, A.wl, 0);
-        fhi = min(key_hi(cs.q.sk - cs.q.sq, A.wr, 0), cs.q.sk - 1);
+        const int diag = cs.q.sk - cs.q.sq;
+        flo = key_lo(BLK ? (cs.row0 + rows - 1) / A.g + diag : cs.q.sk - 1, A.wl, 0);
+        fhi = min(key_hi(BLK ? cs.row0 / A.g + diag : diag, A.wr, 0), cs.q.sk - 1);
 #pragma unroll
         for (int rt = 0; rt < NR; ++rt) {
             const int r = rt * 16 + li;
             const bool ok = r < rows;
-            qi[rt] = ok ? r / A.g : 0;
-            const int h = cs.hk * A.g + (ok ? r % A.g : 0);
+            qi[rt] = ok ? (cs.row0 + r) / A.g : 0;
+            const int h = cs.hk * A.g + (ok ? (cs.row0 + r) % A.g : 0);
             const uint16_t* q = static_cast<const uint16_t*>(A.q) + q_row(A, cs.b, qi[rt], A.q_sb, A.q_si) + (int64_t)h * A.q_sh;
 #pragma unroll
             for (int w = 0; w < W; ++w) {
@@ -261,7 +291,7 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, groups_of_cu(HD, NR)) fa
             const float lse = some ? (m_run[rt] - (wide ? kTopWide : kTop) + fast_log2(l)) * kLn2 : INFINITY;
             if (r >= rows) continue;
             if (whole) {
-                const int h = cs.hk * A.g + r % A.g;
+                const int h = cs.hk * A.g + (cs.row0 + r) % A.g;
                 uint16_t* o = static_cast<uint16_t*>(A.out) + q_row(A, cs.b, qi[rt], A.o_sb, A.o_si) + (int64_t)h * A.o_sh;
 #pragma unroll
                 for (int db = 0; db < DBLK; ++db) {
@@ -481,8 +511,13 @@ template <int DT, int HD>
 void launch_n(const QuantFwdArgs& a, int nr, int cus, hipStream_t stream) {
     const dim3 nt(Cfg4<HD>::NWAVE * 64);
     const int grid = cus * groups_of_cu(HD, nr);
-    if (nr == 1) hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 1>), dim3(grid), nt, 0, stream, a);
-    else hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 2>), dim3(grid), nt, 0, stream, a);
+    if (a.blocks) {
+        hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 2, true>), dim3(grid), nt, 0, stream, a);
+        launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE, Cfg4<HD>::HS, 256, true>(a, nr, grid, stream);
+        return;
+    }
+    if (nr == 1) hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 1, false>), dim3(grid), nt, 0, stream, a);
+    else hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 2, false>), dim3(grid), nt, 0, stream, a);
     // Many segments fill the chip with small workgroups, few want more threads for the pieces of each
     if ((int64_t)a.B * a.Hk * (HD / 32) >= 4 * cus) launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE, Cfg4<HD>::HS, 256>(a, nr, grid, stream);
     else launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE, Cfg4<HD>::HS>(a, nr, grid, stream);

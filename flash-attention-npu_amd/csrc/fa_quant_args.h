@@ -12,6 +12,11 @@ enum : int { CT_E4M3 = 3, CT_INT8 = 4, CT_FP4 = 5 };
 
 constexpr int kQuantMaxB = 2048;  // sequences of an attention launch, and entries of a list that is cut: they live in LDS
 
+// Packed rows of a block of the 4-bit decode kernel; most that a call of blocks may have: (block, kv head) pairs, and
+// those times 64 keys (fa_quant_list.h)
+constexpr int kBlockRows = 32, kBlockSegs = 512, kBlockUnits = 16384;
+static_assert(kBlockSegs <= kQuantMaxB, "blocks live in the list of sequences");
+
 struct PageTableArgs {
     int* table;
     int64_t t_stride;
@@ -77,6 +82,8 @@ struct QuantFwdArgs {
     int wl, wr;                    // normalised window, -1 = unbounded, causal => wr = 0
     int bf16;                      // q and out: 0 = fp16, 1 = bf16
     int dec_rows;                  // sequences of at most as many packed rows take the decode kernel
+    int blocks;                    // 4-bit codes: blocks of 32 packed rows that its list may have, 0: one for a sequence
+    int* block_pref;               // [0..B]: block prefix, with `blocks`
     // scratch of the decode kernel
     int* sched;                    // [0..B]: tile prefix
     float* part_lse;               // [worker][2][16 * row tiles]

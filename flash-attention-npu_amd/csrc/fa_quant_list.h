@@ -20,7 +20,8 @@ struct Seg {
     int S, n;      // first tile of the list, tiles
     int b, hk;
     int lo_tile;
-    QuantSeq q;
+    QuantSeq q;    // of a block of rows: lo and hi are the block's
+    int row0, rows;  // packed rows
 };
 
 __device__ __forceinline__ Seg seg_of(const QuantFwdArgs& a, const int* s_pref, int t, int hs, int h, int KT) {
@@ -38,6 +39,73 @@ __device__ __forceinline__ Seg seg_of(const QuantFwdArgs& a, const int* s_pref, 
     const int hg = (int)((uint32_t)(t - s_pref[bl]) / (uint32_t)max(s.n, 1));
     s.hk = hg * hs + h;
     s.S = s_pref[bl] + hg * s.n;
+    s.row0 = 0;
+    s.rows = s.q.sq * a.g;
+    return s;
+}
+
+// the last i of [0, n) with s[i] <= x
+template <typename T>
+__device__ __forceinline__ int place_of(const T* s, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Longer sequences, in blocks of kBlockRows packed rows that read their keys each for itself. A tile costs the decode
+// kernel twice what its rows cost the prefill kernel, but that one begins 40 us later: it executes 2700
+// instructions before its first product, and fetches each line of them for the first time. Prompts of 64, 128, 256 and
+// 512 tokens of 32 heads onto 8 take 25, 32, 38 and 54 us in place of 61, 68, 66 and 74, one of 1024 96 in place
+// of 85; 256 tokens that end 4000 keys 67 in place of 73, 16000 keys 163 in place of 110; 8 prompts of 256 tokens, of which each wave has several blocks,
+// 89 in place of 36. The number of blocks is the host's to bound (kBlockSegs); the keys every
+// workgroup of both kernels counts, alike (kBlockUnits). A call whose
+// blocks are not taken after all costs 7 us more.
+__device__ __forceinline__ int blocks_of(const QuantFwdArgs& a, const QuantSeq& q) { return (q.sq * a.g + kBlockRows - 1) / kBlockRows; }
+
+// by a whole workgroup of NT threads
+template <int NT>
+__device__ __forceinline__ bool blocks_take(const QuantFwdArgs& a, int64_t* s_sum) {
+    int64_t units = 0;
+    for (int b = threadIdx.x; b < a.B; b += NT) {
+        const QuantSeq q = quant_seq(a, b);
+        units += (int64_t)a.Hk * blocks_of(a, q) * max((q.hi - q.lo) / 64, 1);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) units += (int64_t)__shfl_xor((long long)units, o);
+    if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = units;
+    __syncthreads();
+    units = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) units += s_sum[w];
+    __syncthreads();
+    return units <= kBlockUnits;
+}
+
+// Block i of sequence b: q's keys become those that its rows see.
+__device__ __forceinline__ void cut_to_block(const QuantFwdArgs& a, Seg& s, int i) {
+    s.row0 = i * kBlockRows;
+    s.rows = min(s.q.sq * a.g - s.row0, kBlockRows);
+    const int diag = s.q.sk - s.q.sq;
+    s.q.lo = max(0, key_lo(s.row0 / a.g + diag, a.wl, 0));
+    s.q.hi = max(s.q.lo, min(s.q.sk, key_hi((s.row0 + s.rows - 1) / a.g + diag, a.wr, 0) + 1));
+}
+
+// Segment of tile t of the list of blocks: s_blk blocks before each sequence, s_pref tiles before each of n blocks
+__device__ __forceinline__ Seg block_seg_of(const QuantFwdArgs& a, const int* s_blk, const int* s_pref, int n, int t, int hs, int h, int KT) {
+    const int e = place_of(s_pref, n, t);
+    Seg s;
+    s.b = place_of(s_blk, a.B, e);
+    s.q = quant_seq(a, s.b);
+    cut_to_block(a, s, e - s_blk[s.b]);
+    s.lo_tile = s.q.lo / KT;
+    s.n = (s.q.hi + KT - 1) / KT - s.lo_tile;
+    const int hg = (int)((uint32_t)(t - s_pref[e]) / (uint32_t)max(s.n, 1));
+    s.hk = hg * hs + h;
+    s.S = s_pref[e] + hg * s.n;
     return s;
 }
 
@@ -58,19 +126,32 @@ __device__ __forceinline__ float max4(float v) {
 // maximum, and meet in LDS. A row is empty where its weights sum to 0, which says so
 // for NaN as well: such partials have no part in the maximum (fmaxf).
 // KT: keys of a tile, NWAVE: waves of a workgroup of the kernel that left them, HS: heads of a group at most,
-// MT: threads of a workgroup.
-template <int DT, int HD, int KT, int NWAVE, int HS, int MT>
+// MT: threads of a workgroup, BLK: the list is of blocks.
+template <int DT, int HD, int KT, int NWAVE, int HS, int MT, bool BLK>
 __global__ void __launch_bounds__(MT) fa_quant_merge_kernel(QuantFwdArgs a, int grid, int nr) {
     __shared__ __attribute__((aligned(16))) float s_acc[MT][8];
     __shared__ float s_gm[MT], s_gs[MT];
     constexpr int COLS = HD / 32, CH = 4;  // 8-column chunks of a workgroup
     const int sig = blockIdx.x / COLS, part = blockIdx.x % COLS;
-    const int b = (int)((uint32_t)sig / (uint32_t)a.Hk), hk = sig - b * a.Hk;
+    const int e = (int)((uint32_t)sig / (uint32_t)a.Hk), hk = sig - e * a.Hk;  // sequence, or block
     const int hs = heads_per_group<HS>(a), hg = hk / hs, hsel = hk - hg * hs;
-    const QuantSeq q = quant_seq(a, b);
-    const int T = a.sched[a.B], S0 = a.sched[b];
-    const int row0 = blockIdx.y * 16, rows = min(q.sq * a.g - row0, 16);
-    if (rows <= 0 || q.sq * a.g > a.dec_rows) return;
+    int b = e, last = a.B, first = 0;  // first: the block's first row
+    QuantSeq q;
+    if constexpr (BLK) {
+        last = min(a.block_pref[a.B], a.blocks);
+        if (e >= last) return;
+        Seg s;
+        b = place_of(a.block_pref, a.B, e);
+        s.q = quant_seq(a, b);
+        cut_to_block(a, s, e - a.block_pref[b]);
+        q = s.q;
+        first = s.row0;
+    } else {
+        q = quant_seq(a, b);
+    }
+    const int T = a.sched[last], S0 = a.sched[e];
+    const int row0 = blockIdx.y * 16, rows = min(q.sq * a.g - first - row0, 16);
+    if (rows <= 0 || (!BLK && q.sq * a.g > a.dec_rows)) return;
     const int per = q.hi > q.lo ? (q.hi + KT - 1) / KT - q.lo / KT : 0, S = S0 + hg * per;
     const Split sp = split_list(T, grid * (NWAVE / hs));
     int wf = 0, n = 0;
@@ -131,7 +212,7 @@ __global__ void __launch_bounds__(MT) fa_quant_merge_kernel(QuantFwdArgs a, int 
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     acc0 *= inv;
     acc1 *= inv;
-    const int r = row0 + rr, i = r / a.g, h = hk * a.g + r % a.g;
+    const int r = first + row0 + rr, i = r / a.g, h = hk * a.g + r % a.g;
     uint16_t* o = static_cast<uint16_t*>(a.out) + q_row(a, b, i, a.o_sb, a.o_si) + (int64_t)h * a.o_sh;
     if (d0 < a.hd)
         *reinterpret_cast<u32x4*>(o + d0) = u32x4{pack2<DT>(acc0[0], acc0[1]), pack2<DT>(acc0[2], acc0[3]),
@@ -140,9 +221,9 @@ __global__ void __launch_bounds__(MT) fa_quant_merge_kernel(QuantFwdArgs a, int 
 }
 
 constexpr int kMergeThreads = 512;
-template <int DT, int HD, int KT, int NWAVE, int HS, int MT = kMergeThreads>
+template <int DT, int HD, int KT, int NWAVE, int HS, int MT = kMergeThreads, bool BLK = false>
 void launch_list_merge(const QuantFwdArgs& a, int nr, int grid, hipStream_t stream) {
-    hipLaunchKernelGGL((fa_quant_merge_kernel<DT, HD, KT, NWAVE, HS, MT>), dim3(a.B * a.Hk * (HD / 32), nr), dim3(MT), 0, stream, a, grid, nr);
+    hipLaunchKernelGGL((fa_quant_merge_kernel<DT, HD, KT, NWAVE, HS, MT, BLK>), dim3((BLK ? a.blocks : a.B) * a.Hk * (HD / 32), nr), dim3(MT), 0, stream, a, grid, nr);
 }
 
 }  // namespace

@@ -131,6 +131,8 @@ struct Plan {
     int nr, grid;    // decode: 16-row tiles, compute units
     int pf_rows, pf_grid;
     bool cut;        // prefill: the items are cut over the workgroups
+    int blocks;      // 4-bit codes: blocks of rows that the decode kernel's list may have
+    size_t off_blk;
     size_t off_lse, off_o, off_pcut, off_plse, off_po, total;
 };
 
@@ -139,7 +141,8 @@ inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 // The waves that share the list of tiles, by the kernel head dim, 16-row tiles and compute units
 using Workers = int (*)(int kd, int nr, int cus);
 
-inline Plan make_plan(const fa_quant_fwd_params* p, Workers workers) {
+// in_blocks: the decode kernel takes longer sequences in blocks of their rows (fa_quant_list.h)
+inline Plan make_plan(const fa_quant_fwd_params* p, Workers workers, bool in_blocks = false) {
     Plan pl{};
     pl.kd = kernel_headdim(p->headdim);
     pl.nb = (int)std::min<int64_t>(p->batch, batch_of_launch(p));
@@ -152,13 +155,22 @@ inline Plan make_plan(const fa_quant_fwd_params* p, Workers workers) {
     // are single tokens; 64 sequences of 2 to 7 tokens of 8 heads take 353 us in place of 403.
     pl.dec_rows = !pl.prefill ? (int)rows : p->cu_seqlens_q ? 16 : 0;
     pl.nr = pl.dec_rows <= 16 ? 1 : 2;
+    if (pl.prefill && in_blocks) {
+        const int64_t most = p->cu_seqlens_q ? (int64_t)p->total_q * pl.g / fa::kBlockRows + pl.nb
+                                             : pl.nb * ((rows + fa::kBlockRows - 1) / fa::kBlockRows);
+        if (most * p->nheads_k <= fa::kBlockSegs) {
+            pl.blocks = (int)most;
+            pl.nr = 2;
+        }
+    }
     const int cus = fa::compute_units();
     const size_t nb = pl.nb;
     pl.grid = cus;
     size_t off = 0;
-    if (pl.dec_rows) {
+    if (pl.dec_rows || pl.blocks) {
         const size_t parts = (size_t)workers(pl.kd, pl.nr, pl.grid) * 2 * 16 * pl.nr;
-        pl.off_lse = off = align256(sizeof(int) * (nb + 1));
+        pl.off_blk = sizeof(int) * (std::max(nb, (size_t)pl.blocks) + 1);
+        pl.off_lse = off = align256(pl.off_blk + (pl.blocks ? sizeof(int) * (nb + 1) : 0));
         pl.off_o = off = align256(off + sizeof(float) * parts);
         off = align256(off + sizeof(float) * parts * pl.kd);
     }
@@ -231,10 +243,11 @@ using LaunchDecode = hipError_t (*)(const fa::QuantFwdArgs& a, int ct, int kd, i
 using LaunchPrefill = hipError_t (*)(const fa::QuantFwdArgs& a, int ct, int kd, int rows, int grid, hipStream_t stream);
 
 // A checked attention call
-inline fa_status_t attend(const fa_quant_fwd_params* p, void* stream, Workers workers, LaunchDecode decode, LaunchPrefill prefill) {
+inline fa_status_t attend(const fa_quant_fwd_params* p, void* stream, Workers workers, LaunchDecode decode, LaunchPrefill prefill,
+                          bool in_blocks = false) {
     const int64_t rows = p->cu_seqlens_q ? (int64_t)p->total_q : (int64_t)p->batch * p->seqlen_q;
     if (rows == 0 || p->seqlen_q == 0) return FA_OK;
-    const Plan pl = make_plan(p, workers);
+    const Plan pl = make_plan(p, workers, in_blocks);
     if (pl.total > 0) {
         if (!p->workspace || p->workspace_bytes < pl.total)
             return fail(FA_EWORKSPACE, "workspace of %zu bytes required, %zu given", pl.total, p->workspace ? p->workspace_bytes : (size_t)0);
@@ -292,8 +305,10 @@ inline fa_status_t attend(const fa_quant_fwd_params* p, void* stream, Workers wo
     a.wr = p->is_causal ? 0 : window_bound(p->window_size_right);
     a.bf16 = p->dtype == FA_DTYPE_BF16;
     a.dec_rows = pl.dec_rows;
+    a.blocks = pl.blocks;
     char* ws = static_cast<char*>(p->workspace);
     a.sched = reinterpret_cast<int*>(ws);
+    a.block_pref = reinterpret_cast<int*>(ws + pl.off_blk);
     a.part_lse = reinterpret_cast<float*>(ws + pl.off_lse);
     a.part_o = reinterpret_cast<float*>(ws + pl.off_o);
     a.cut = pl.cut;
@@ -316,7 +331,7 @@ inline fa_status_t attend(const fa_quant_fwd_params* p, void* stream, Workers wo
         }
         if (a.batch_idx) c.batch_idx = a.batch_idx + b0;
         hipError_t e = hipSuccess;
-        if (pl.dec_rows) e = decode(c, p->cache_dtype, pl.kd, pl.nr, pl.grid, static_cast<hipStream_t>(stream));
+        if (pl.dec_rows || pl.blocks) e = decode(c, p->cache_dtype, pl.kd, pl.nr, pl.grid, static_cast<hipStream_t>(stream));
         if (e == hipSuccess && pl.prefill) e = prefill(c, p->cache_dtype, pl.kd, pl.pf_rows, pl.pf_grid, static_cast<hipStream_t>(stream));
         if (e != hipSuccess) return fail(FA_EHIP, "attention launch failed: %s", hipGetErrorString(e));
     }

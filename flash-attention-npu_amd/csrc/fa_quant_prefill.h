@@ -37,6 +37,7 @@
 #include "fa_fp4.h"
 #include "fa_pipe.h"
 #include "fa_quant_items.h"
+#include "fa_quant_list.h"
 
 #include <type_traits>
 
@@ -136,6 +137,12 @@ __global__ void __launch_bounds__(NT, 1) fa_quant_prefill_kernel(QuantFwdArgs a)
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, hi = lane >> 5;
+    if constexpr (FOUR) {
+        if (a.blocks && blocks_take<NT>(a, s_line)) {  // the decode kernel has them all
+            if (a.cut && tid == 0) reinterpret_cast<CutItem*>(a.pf_cut)[blockIdx.x] = CutItem{0, 0, 0, 0};
+            return;
+        }
+    }
     build_list<BM, BN, NW>(a, s_pref, s_line);
 
     const unsigned lds0 = lds_addr(s_t);
