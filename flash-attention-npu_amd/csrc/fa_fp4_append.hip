@@ -4,6 +4,11 @@
 // two s with max |x| <= 6 s, its codes are x / s (exact) rounded by the hardware's
 // conversion, to the nearest with ties to the even code. Scales that are powers of two
 // are what the format holds, and a token's own scales leave earlier tokens alone.
+//
+// What bounds it: memory; a row is read once, a quarter of its bytes written. 41 000 rows of
+// 8 heads x 128, bf16, take 55 us (3.9 TB/s; 42 at the rate of a copy); 64 rows 3.6, a launch.
+// Two pieces of a row are in flight per thread, so that the second's loads lie under the first's maximum
+// (one: 65 us for what 58 took, with fp32 conversions in place of the 16-bit pairs').
 #include "fa_fp4.h"
 
 #include <algorithm>
@@ -125,7 +130,8 @@ hipError_t launch_fp4_append(QuantAppendArgs a, int dtype, hipStream_t stream) {
     a.page = udiv_make((uint32_t)a.page_size);
     a.chunks = udiv_make((uint32_t)a.hd / 8);
     const UDiv per_row = udiv_make((uint32_t)a.Hk * (uint32_t)(a.hd / 8));
-    // several passes of a workgroup where there are workgroups enough for that
+    // Several rows to a workgroup, which looks up their places once, where there are workgroups enough for that:
+    // 41 000 rows take 54.9 us at 1/4096 of them each, 58.1 at 1/1024, 57.5 at 1/2048, 53.9 at 1/8192
     const int rows = (int)std::min<int64_t>(std::max<int64_t>(a.total_new / 4096, 1), kMostRows);
     const int64_t groups = (a.total_new + rows - 1) / rows, most = 1 << 24;  // 2^32 threads of a launch
     for (int64_t g = 0; g < groups; g += most - 1) {

@@ -16,7 +16,18 @@
 // result's error: fp16 holds the values of scales from 2^-23 to 2^13 exactly. Weights are kept in units
 // that make a row's largest 2^14, so that one has all its bits down to 2^-28 of that. A bf16 call whose
 // values leave that range goes on in bf16, a weight as the sum of two numbers, in units that make the
-// largest 2^-20: the sum of 2^20 values of 2^127 stays in fp32.
+// largest 2^-20: the sum of 2^20 values of 2^127 stays in fp32. (bf16 weights of one part took the same time, at
+// 1.35 times the error.)
+//
+// What bounds it: reads, and for short calls the start. 64 paged sequences of 512 to 32768 keys, H64/8
+// D128 bf16, 427 MB: 95 us (4.5 TB/s; of 64 x 32768 keys 5.0), and 9 for the merge; the data path of the loads is busy 74 % of
+// the time, vector instructions take a third, products 11 %, and waves wait for a third of it. One sequence of 777 keys: 12
+// and 4.6 us, of which the list, page ids, first keys and q, one after another, have 8; 4 tokens over a window of
+// 4096, 8 sequences, fp16: 21 and 7. D64 3.7, D256 4.4, 32 packed rows 3.3 TB/s, where
+// registers hold fewer loads in flight.
+// Lanes that load 16 apart, as the products want them, keep the data path of the loads busy 83 % of the time and
+// cost more than the exchange through LDS; loads marked non-temporal made 127 us of 106, as
+// a 128-byte line holds two heads' rows.
 #include "fa_fp4.h"
 #include "fa_quant_list.h"
 
@@ -47,7 +58,8 @@ struct Cfg4 {
     }
 };
 
-// Workgroups of a compute unit, a wave of each on a SIMD: as many as the registers hold.
+// Workgroups of a compute unit, a wave of each on a SIMD: as many as the registers hold. (Three at
+// head dim 128, with a third fewer registers each: 126 us where two took 123.)
 __host__ __device__ constexpr int groups_of_cu(int hd, int nr) { return hd == 256 ? 1 : 2; }
 
 // A tile's codes and scales, as a lane loads them
@@ -518,7 +530,9 @@ void launch_n(const QuantFwdArgs& a, int nr, int cus, hipStream_t stream) {
     }
     if (nr == 1) hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 1, false>), dim3(grid), nt, 0, stream, a);
     else hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 2, false>), dim3(grid), nt, 0, stream, a);
-    // Many segments fill the chip with small workgroups, few want more threads for the pieces of each
+    // Many segments fill the chip with small workgroups, few want more threads for the pieces of each:
+    // 64 sequences of 8 heads of D128 take 9.0 us with 256 threads and 12.8 with 512, 8 sequences 7.2 with 512 and
+    // 9.6 with 256. Blocks have few pieces each: 512 tokens of 32 heads 54 us in all with 256, 61 with 512.
     if ((int64_t)a.B * a.Hk * (HD / 32) >= 4 * cus) launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE, Cfg4<HD>::HS, 256>(a, nr, grid, stream);
     else launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE, Cfg4<HD>::HS>(a, nr, grid, stream);
 }

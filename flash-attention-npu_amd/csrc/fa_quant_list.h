@@ -56,15 +56,17 @@ __device__ __forceinline__ int place_of(const T* s, int n, int x) {
     return lo;
 }
 
-// Longer sequences, in blocks of kBlockRows packed rows that read their keys each for itself. A tile costs the decode
-// kernel twice what its rows cost the prefill kernel, but that one begins 40 us later: it executes 2700
-// instructions before its first product, and fetches each line of them for the first time. Prompts of 64, 128, 256 and
-// 512 tokens of 32 heads onto 8 take 25, 32, 38 and 54 us in place of 61, 68, 66 and 74, one of 1024 96 in place
-// of 85; 256 tokens that end 4000 keys 67 in place of 73, 16000 keys 163 in place of 110; 8 prompts of 256 tokens, of which each wave has several blocks,
-// 89 in place of 36. The number of blocks is the host's to bound (kBlockSegs); the keys every
-// workgroup of both kernels counts, alike (kBlockUnits). A call whose
-// blocks are not taken after all costs 7 us more.
-__device__ __forceinline__ int blocks_of(const QuantFwdArgs& a, const QuantSeq& q) { return (q.sq * a.g + kBlockRows - 1) / kBlockRows; }
+// Longer sequences, in blocks of kBlockRows packed rows that read their keys each for itself. A tile costs the
+// decode kernel twice what its rows cost the prefill kernel, but that one begins 40 us later: it executes 2700
+// instructions before its first product, and fetches each line of them for the first time. Prompts of 64, 128,
+// 256 and 512 tokens of 32 heads onto 8 take 25, 32, 38 and 54 us in place of 61, 68, 66 and 74, one of 1024
+// 96 in place of 85; 256 tokens that end 4000 keys 67 in place of 73, 16000 keys 163 in place of 110; 8
+// prompts of 256 tokens, of which each wave has several blocks, 89 in place of 36. The number of blocks is the
+// host's to bound (kBlockSegs); the keys every workgroup of both kernels counts, alike (kBlockUnits). A call
+// whose blocks are not taken after all costs 7 us more.
+__device__ __forceinline__ int blocks_of(const QuantFwdArgs& a, const QuantSeq& q) {
+    return (q.sq * a.g + kBlockRows - 1) / kBlockRows;
+}
 
 // by a whole workgroup of NT threads
 template <int NT>
@@ -95,7 +97,8 @@ __device__ __forceinline__ void cut_to_block(const QuantFwdArgs& a, Seg& s, int 
 }
 
 // Segment of tile t of the list of blocks: s_blk blocks before each sequence, s_pref tiles before each of n blocks
-__device__ __forceinline__ Seg block_seg_of(const QuantFwdArgs& a, const int* s_blk, const int* s_pref, int n, int t, int hs, int h, int KT) {
+__device__ __forceinline__ Seg block_seg_of(const QuantFwdArgs& a, const int* s_blk, const int* s_pref, int n, int t, int hs, int h,
+                                            int KT) {
     const int e = place_of(s_pref, n, t);
     Seg s;
     s.b = place_of(s_blk, a.B, e);

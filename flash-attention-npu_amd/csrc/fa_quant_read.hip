@@ -1,7 +1,9 @@
 // fa_quant_read.hip -- rows of a quantised cache as values of 16 or 32 bits: fa_quant_read.
 //
 // One pass: codes and scales in, values out, which are most of what moves (2 bytes
-// for 0.53 of a 4-bit cache).
+// for 0.53 of a 4-bit cache), and the rate of writes is what bounds it: 41 000 rows of 8 heads x 128 from
+// a 4-bit cache to bf16 take 36 us (5.9 TB/s), 64 rows 3.5; 13 contexts of 5 heads x 96, 128 MB in all, 25 us
+// from the last cache level and 35 from memory. Values are rounded once, from 32 bits.
 #include "fa_fp4.h"
 #include "fa_quant_read_args.h"
 
@@ -125,6 +127,8 @@ void launch_read_t(const QuantReadArgs& a, int ct, int rows, dim3 grid, hipStrea
 }  // namespace
 
 hipError_t launch_quant_read(QuantReadArgs a, int dtype, int ct, hipStream_t stream) {
+    // as in fa_fp4_append.hip: 41 000 rows take 36.0 us, 40.8 at 1/1024, 38.2 at 1/2048, 35.0 at 1/8192; the
+    // 13 contexts 24.8, 23.8, 26.1 and 26.2
     const int rows = (int)std::min<int64_t>(std::max<int64_t>(a.total / 4096, 1), kMostRows);
     const int64_t groups = (a.total + rows - 1) / rows, most = (1 << 24) - 1;  // less than 2^32 threads of a launch
     for (int64_t g = 0; g < groups; g += most) {
