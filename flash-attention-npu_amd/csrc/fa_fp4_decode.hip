@@ -125,11 +125,8 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, groups_of_cu(HD, NR)) fa
     if constexpr (BLK) {
         static_assert(NR * 16 == kBlockRows, "");
         __shared__ int64_t s_sum[NWAVE];
-        const bool all = blocks_take<NT>(a, s_sum);
-        for (int b = tid; b < a.B; b += NT) {
-            const QuantSeq s = quant_seq(a, b);
-            s_blk[b + 1] = all || s.sq * a.g <= a.dec_rows ? blocks_of(a, s) : 0;
-        }
+        const bool all = blocks_take<NT>(a, s_sum);  // or none
+        for (int b = tid; b < a.B; b += NT) s_blk[b + 1] = all ? blocks_of(a, quant_seq(a, b)) : 0;
         __syncthreads();
         if (wave == 0) prefix_sums(s_blk, a.B);
         __syncthreads();
@@ -144,6 +141,11 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, groups_of_cu(HD, NR)) fa
         if (blockIdx.x == 0)
             for (int b = tid; b <= a.B; b += NT) a.block_pref[b] = s_blk[b];
     } else {
+        __shared__ int64_t s_sum[NWAVE];
+        if (a.blocks && blocks_take<NT>(a, s_sum)) {  // nothing is left, nor for the merge
+            if (blockIdx.x == 0 && tid == 0) a.sched[a.B] = -1;
+            return;
+        }
         for (int b = tid; b < a.B; b += NT) {
             const QuantSeq s = quant_seq(a, b);
             s_pref[b + 1] = s.hi > s.lo && s.sq * a.g <= a.dec_rows ? hgs * ((s.hi + KT - 1) / KT - s.lo / KT) : 0;
@@ -525,8 +527,9 @@ void launch_n(const QuantFwdArgs& a, int nr, int cus, hipStream_t stream) {
     const int grid = cus * groups_of_cu(HD, nr);
     if (a.blocks) {
         hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 2, true>), dim3(grid), nt, 0, stream, a);
-        launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE, Cfg4<HD>::HS, 256, true>(a, nr, grid, stream);
-        return;
+        launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE, Cfg4<HD>::HS, 256, true>(a, 2, grid, stream);
+        if (a.dec_rows == 0) return;
+        nr = 1;  // short sequences of a call whose blocks are not taken
     }
     if (nr == 1) hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 1, false>), dim3(grid), nt, 0, stream, a);
     else hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 2, false>), dim3(grid), nt, 0, stream, a);

@@ -155,12 +155,14 @@ inline Plan make_plan(const fa_quant_fwd_params* p, Workers workers, bool in_blo
     // are single tokens; 64 sequences of 2 to 7 tokens of 8 heads take 353 us in place of 403.
     pl.dec_rows = !pl.prefill ? (int)rows : p->cu_seqlens_q ? 16 : 0;
     pl.nr = pl.dec_rows <= 16 ? 1 : 2;
-    if (pl.prefill && in_blocks) {
+    // (ragged: where most sequences are at their next token, their kernel is meant, and blocks are seldom taken)
+    if (pl.prefill && in_blocks && (!p->cu_seqlens_q || (int64_t)p->total_q * pl.g >= (int64_t)fa::kBlockRows * p->batch)) {
         const int64_t most = p->cu_seqlens_q ? (int64_t)p->total_q * pl.g / fa::kBlockRows + pl.nb
                                              : pl.nb * ((rows + fa::kBlockRows - 1) / fa::kBlockRows);
         if (most * p->nheads_k <= fa::kBlockSegs) {
             pl.blocks = (int)most;
             pl.nr = 2;
+            if (p->batch == 1) pl.dec_rows = 0;  // its only sequence is hardly shorter than a block: no launch for that
         }
     }
     const int cus = fa::compute_units();

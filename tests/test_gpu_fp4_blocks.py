@@ -106,3 +106,20 @@ def test_the_number_of_blocks(B, sq, H, Hk):
                                                     return_softmax_lse=True)
     for b in list(range(min(B, 9))) + [B - 1]:
         check_attend4(out[b], lse[b], q[b], *c.rows(b, torch.float16), torch.float16, causal=True)
+
+
+@pytest.mark.parametrize("rows,keys,behind", [([64, 1, 70, 3], [9000, 12000, 4000, 16000], 0), ([1], [30000], 40), ([3], [9], 40), ([40, 4], [20000, 20000], 0),
+                                              ([5, 5, 0], [300, 40000, 7], 60)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_few_rows_beside_long_keys(D, rows, keys, behind):
+    """Single tokens beside prompts whose keys are too many for blocks; padded calls of fewer rows than they are sized for."""
+    print(f"case fp4 few rows beside long keys {D} {rows}", flush=True)
+    g = torch.Generator().manual_seed(55)
+    c = Cache4(g, keys, 2, D, 128)
+    q = torch.randn(sum(rows), 8, D, generator=g).to(torch.bfloat16)
+    cu = torch.tensor([sum(rows[:i]) for i in range(len(rows) + 1)], **I32)
+    tail = torch.full((behind, 8, D), float("nan"), dtype=q.dtype)
+    out, lse = fa.flash_attn_with_quantized_kvcache(torch.cat([q, tail]).to(DEV), *c.args(DEV), torch.tensor(c.lens, **I32),
+                                                    page_table=c.table.to(DEV), cu_seqlens_q=cu, max_seqlen_q=max(*rows, 16), causal=True,
+                                                    return_softmax_lse=True)
+    check(c, q, rows, torch.bfloat16, out, lse, causal=True)
