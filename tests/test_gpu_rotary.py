@@ -394,3 +394,21 @@ def test_refusals():
                 dict(scaling="linear", factor=5e-324, base=1e-300)):
         with pytest.raises(RuntimeError):
             fa.rotary_cos_sin(**dict(dict(positions=pos, rotary_dim=32), **bad))
+
+
+def test_memory_given_twice_is_not_turned_in_place():
+    """Rows that share memory by any strides, and one tensor as q and as k, are refused; what lies between other rows is not."""
+    x = torch.randn(4096, device=DEV).to(torch.bfloat16)
+    cos, sin = fa.rotary_cos_sin(torch.arange(8, device=DEV), 32, dtype=torch.bfloat16)
+    for size, stride in (((1, 4, 2, 64), (0, 64, 64, 1)), ((1, 4, 2, 64), (0, 128, 56, 1)), ((2, 3, 2, 64), (256, 128, 64, 1))):
+        with pytest.raises(RuntimeError, match="repeat rows"):
+            fa.apply_rotary_emb(torch.as_strided(x, size, stride), None, cos, sin, inplace=True)
+    q = torch.as_strided(x, (1, 4, 2, 64), (0, 128, 64, 1))
+    with pytest.raises(RuntimeError, match="same memory"):
+        fa.apply_rotary_emb(q, q, cos, sin, inplace=True)
+    both = x[:1536].view(1, 4, 6, 64)
+    want = [t.clone() for t in fa.apply_rotary_emb(both[:, :, :4], both[:, :, 4:5], cos, sin)] + [both[:, :, 5:].clone()]
+    fa.apply_rotary_emb(both[:, :, :4], both[:, :, 4:5], cos, sin, inplace=True)  # heads of one projection
+    for got, t in zip((both[:, :, :4], both[:, :, 4:5], both[:, :, 5:]), want):
+        assert torch.equal(got, t)
+    fa.apply_rotary_emb(both.transpose(1, 2), None, cos, sin, inplace=True)  # (heads first)
