@@ -1197,6 +1197,22 @@ void rotary_(Tensor& q, const OptT& k, const Tensor& cos, const Tensor& sin, con
     rotary_into(q, k, q, k, cos, sin, positions, seqlen_offsets, seqlen_offset, cu_seqlens, interleaved, conjugate);
 }
 
+// What autograd saved of a tensor holds for its version only, so what is turned in place gets another one, as
+// with torch's own operations in place.
+void rotary_version_(Tensor& q, const OptT& k, const Tensor& cos, const Tensor& sin, const OptT& positions, const OptT& offsets,
+                     int64_t offset, const OptT& cu, bool interleaved, bool conjugate) {
+    using Op = void(Tensor&, const OptT&, const Tensor&, const Tensor&, const OptT&, const OptT&, int64_t, const OptT&, bool, bool);
+    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fa_mi355x::rotary_", "").typed<Op>();
+    const bool plain = q.is_inference() || (k.has_value() && k->is_inference());
+    TORCH_CHECK(!plain || c10::InferenceMode::is_enabled(), "an inference tensor is turned in place in inference_mode only");
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        op.call(q, k, cos, sin, positions, offsets, offset, cu, interleaved, conjugate);
+    }
+    q.unsafeGetTensorImpl()->bump_version();
+    if (k.has_value()) k->unsafeGetTensorImpl()->bump_version();
+}
+
 }  // namespace
 
 TORCH_LIBRARY(fa_mi355x, m) {
@@ -1279,3 +1295,5 @@ TORCH_LIBRARY_IMPL(fa_mi355x, CUDA, m) {
 }
 
 TORCH_LIBRARY_IMPL(fa_mi355x, Autograd, m) { m.impl("rotary", &rotary_autograd); }
+
+TORCH_LIBRARY_IMPL(fa_mi355x, ADInplaceOrView, m) { m.impl("rotary_", &rotary_version_); }
