@@ -15,11 +15,16 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
+#include <array>
 #include <cmath>
+#include <memory>
+#include <mutex>
 #include <optional>
 #include <utility>
 #include <vector>
@@ -1197,17 +1202,86 @@ void rotary_(Tensor& q, const OptT& k, const Tensor& cos, const Tensor& sin, con
     rotary_into(q, k, q, k, cos, sin, positions, seqlen_offsets, seqlen_offset, cu_seqlens, interleaved, conjugate);
 }
 
+using InPlace = void(Tensor&, const OptT&, const Tensor&, const Tensor&, const OptT&, const OptT&, int64_t, const OptT&, bool, bool);
+const c10::TypedOperatorHandle<InPlace>& in_place_op() {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fa_mi355x::rotary_", "").typed<InPlace>();
+    return op;
+}
+
+// The gradient of what was turned in place: of one tensor, or of q and k in one call.
+struct RotaryInPlaceBackward : public torch::autograd::Node {
+    std::array<torch::autograd::SavedVariable, 5> saved;  // cos, sin, positions, offsets, cu
+    int64_t offset;
+    bool interleaved, conjugate;
+
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& d) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        const auto given = [&](int i) {
+            const Tensor t = saved[i].unpack();
+            return t.defined() ? OptT(t) : OptT();
+        };
+        torch::autograd::variable_list to(d.size());
+        std::vector<size_t> have;
+        for (size_t i = 0; i < d.size(); ++i)
+            if (d[i].defined()) have.push_back(i);
+        if (have.empty()) return to;
+        auto [a, b] = RotaryGrad::call(d[have[0]], have.size() > 1 ? OptT(d[have[1]]) : OptT(), saved[0].unpack(), saved[1].unpack(), given(2),
+                                       given(3), offset, given(4), interleaved, !conjugate);
+        to[have[0]] = a;
+        if (have.size() > 1) to[have[1]] = b;
+        return to;
+    }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (auto& s : saved) s.reset_data();
+    }
+    std::string name() const override { return "RotaryInPlaceBackward"; }
+};
+
+// In place with gradients. What autograd refuses (a leaf, the pieces of a split, tables that cannot be kept) is refused before
+// anything is turned. History is written after, so that other refusals leave none. A part of a tensor has
+// its history in that tensor, which takes one with one result: q and k then have a node each.
+void rotary_autograd_(Tensor& q, const OptT& k, const Tensor& cos, const Tensor& sin, const OptT& positions, const OptT& offsets,
+                      int64_t offset, const OptT& cu, bool interleaved, bool conjugate) {
+    using namespace torch::autograd;
+    const auto needs = [](const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); };
+    std::vector<Tensor> turned;
+    for (const OptT& t : {OptT(q), k}) {
+        if (!t.has_value()) continue;
+        check_inplace(*t, needs(*t));
+        if (needs(*t)) turned.push_back(*t);
+    }
+    const bool parts = std::any_of(turned.begin(), turned.end(), [](const Tensor& t) { return t.is_view(); });
+    std::vector<std::pair<std::shared_ptr<RotaryInPlaceBackward>, variable_list>> history;
+    for (const Tensor& t : turned) {
+        if (history.empty() || parts) {
+            auto node = std::shared_ptr<RotaryInPlaceBackward>(new RotaryInPlaceBackward(), deleteNode);
+            const OptT given[] = {cos, sin, positions, offsets, cu};
+            for (int i = 0; i < 5; ++i) node->saved[i] = SavedVariable(given[i].value_or(Tensor()), false);
+            node->offset = offset;
+            node->interleaved = interleaved;
+            node->conjugate = conjugate;
+            history.emplace_back(std::move(node), variable_list());
+        }
+        history.back().first->add_next_edge(impl::gradient_edge(t));
+        history.back().second.push_back(t);
+    }
+    {
+        at::AutoDispatchBelowAutograd below;
+        in_place_op().call(q, k, cos, sin, positions, offsets, offset, cu, interleaved, conjugate);
+    }
+    for (auto& [node, of] : history) rebase_history(of, node);
+}
+
 // What autograd saved of a tensor holds for its version only, so what is turned in place gets another one, as
 // with torch's own operations in place.
 void rotary_version_(Tensor& q, const OptT& k, const Tensor& cos, const Tensor& sin, const OptT& positions, const OptT& offsets,
                      int64_t offset, const OptT& cu, bool interleaved, bool conjugate) {
-    using Op = void(Tensor&, const OptT&, const Tensor&, const Tensor&, const OptT&, const OptT&, int64_t, const OptT&, bool, bool);
-    static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fa_mi355x::rotary_", "").typed<Op>();
     const bool plain = q.is_inference() || (k.has_value() && k->is_inference());
     TORCH_CHECK(!plain || c10::InferenceMode::is_enabled(), "an inference tensor is turned in place in inference_mode only");
     {
         at::AutoDispatchBelowADInplaceOrView below;
-        op.call(q, k, cos, sin, positions, offsets, offset, cu, interleaved, conjugate);
+        in_place_op().call(q, k, cos, sin, positions, offsets, offset, cu, interleaved, conjugate);
     }
     q.unsafeGetTensorImpl()->bump_version();
     if (k.has_value()) k->unsafeGetTensorImpl()->bump_version();
@@ -1294,6 +1368,9 @@ TORCH_LIBRARY_IMPL(fa_mi355x, CUDA, m) {
     m.impl("rotary_", &rotary_);
 }
 
-TORCH_LIBRARY_IMPL(fa_mi355x, Autograd, m) { m.impl("rotary", &rotary_autograd); }
+TORCH_LIBRARY_IMPL(fa_mi355x, Autograd, m) {
+    m.impl("rotary", &rotary_autograd);
+    m.impl("rotary_", &rotary_autograd_);
+}
 
 TORCH_LIBRARY_IMPL(fa_mi355x, ADInplaceOrView, m) { m.impl("rotary_", &rotary_version_); }

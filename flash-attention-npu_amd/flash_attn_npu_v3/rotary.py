@@ -42,22 +42,6 @@ def rotary_cos_sin(positions, rotary_dim, base=10000.0, scaling=None, factor=1.0
                   float(original_length), float(low), float(high), float(attention_factor), dtype)
 
 
-class ApplyRotaryEmbInPlace(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, seqlen_offsets, seqlen_offset, cu_seqlens, interleaved):
-        _rotary_in_place(q, k, cos, sin, positions, seqlen_offsets, seqlen_offset, cu_seqlens, interleaved, False)
-        ctx.save_for_backward(cos, sin, positions, seqlen_offsets, cu_seqlens)
-        ctx.seqlen_offset, ctx.interleaved = seqlen_offset, interleaved
-        ctx.mark_dirty(*(x for x in (q, k) if x is not None))
-        return (q, k) if k is not None else q
-
-    @staticmethod
-    def backward(ctx, dq, dk=None):
-        cos, sin, positions, seqlen_offsets, cu_seqlens = ctx.saved_tensors
-        dq, turned = _rotary(dq, dk, cos, sin, positions, seqlen_offsets, ctx.seqlen_offset, cu_seqlens, ctx.interleaved, True)
-        return (dq, turned if dk is not None else None) + (None,) * 7
-
-
 def apply_rotary_emb(q, k, rotary_cos, rotary_sin, positions: Optional[torch.Tensor] = None, seqlen_offsets=0,
                      cu_seqlens: Optional[torch.Tensor] = None, rotary_interleaved=True, inplace=False):
     """Turn the first rotary_dim channels of q and k (or of q alone, k None) by their positions; returns (q, k), or q.
@@ -72,13 +56,12 @@ def apply_rotary_emb(q, k, rotary_cos, rotary_sin, positions: Optional[torch.Ten
     of cu_seqlens (batch_size + 1,) int32, or one. Rows that belong to no sequence stay as they are. Positions outside
     the tables take their first or last row.
 
-    inplace turns q and k themselves, without new memory; neither may hold a row twice, nor share memory with the other.
+    inplace turns q and k themselves, without new memory; neither may hold a row twice, nor share memory with the other. What
+    autograd does not let be changed (a leaf that requires a gradient, the pieces of a split) is refused and stays as it was.
     Gradients of q and k are turned back, which takes no saved rows; the tables get none."""
     offsets = maybe_contiguous(seqlen_offsets) if isinstance(seqlen_offsets, torch.Tensor) else None
     where = (positions, offsets, 0 if offsets is not None else int(seqlen_offsets), maybe_contiguous(cu_seqlens), bool(rotary_interleaved))
     if inplace:
-        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-            return ApplyRotaryEmbInPlace.apply(q, k, rotary_cos, rotary_sin, *where)
         _rotary_in_place(q, k, rotary_cos, rotary_sin, *where, False)
         return (q, k) if k is not None else q
     turned_q, turned_k = _rotary(q, k, rotary_cos, rotary_sin, *where, False)

@@ -1,0 +1,134 @@
+"""apply_rotary_emb in place beside autograd: gradients, and refusals that leave the rows as they were."""
+import pytest
+import torch
+
+import flash_attn_npu_v3 as fa
+from oracle import fa_rotary_oracle as ro
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+B, S, D, RD = 2, 8, 64, 32
+
+
+def tables():
+    cos, sin = ro.table(range(S), RD)
+    return cos.float().to(DEV), sin.float().to(DEV)
+
+
+def rows(g, heads, **kw):
+    return torch.randn(B, S, heads, D, generator=g).to(torch.bfloat16).to(DEV).requires_grad_(kw.get("requires_grad", False))
+
+
+def back(d, cos, sin):
+    """The gradient: turned back by the operator out of place, which test_gpu_rotary.py holds against the formula."""
+    return torch.ops.fa_mi355x.rotary(d.contiguous(), None, cos, sin, None, None, 0, None, True, True)[0]
+
+
+@pytest.mark.parametrize("parts", [False, True])
+@pytest.mark.parametrize("need", ["both", "q", "k"])
+def test_gradients(parts, need):
+    """Of q and k, each a tensor of its own or a part of one projection: the bits of the operator turned back."""
+    print(f"case in place gradients {parts} {need}", flush=True)
+    g = torch.Generator().manual_seed(1)
+    cos, sin = tables()
+    d = rows(g, 6)
+    x = rows(g, 6, requires_grad=need == "both" or parts)
+    y = rows(g, 6, requires_grad=need == "both")
+    if parts:
+        both = x * 1
+        q, k = both[:, :, :4], both[:, :, 4:5]
+        q, k = (q, k) if need == "both" else (q, y[:, :, 4:5].detach().clone()) if need == "q" else (y[:, :, :4].detach().clone(), k)
+    else:
+        q, k = ((t * 1).detach().requires_grad_(n) * 1 for t, n in ((x[:, :, :4], need != "k"), (x[:, :, 4:5], need != "q")))
+    plain = [t.detach().clone() for t in (q, k)]
+    leaves = None if parts else [t.grad_fn.next_functions[0][0].variable if t.requires_grad else None for t in (q, k)]
+    a, b = fa.apply_rotary_emb(q, k, cos, sin, inplace=True)
+    assert a is q and b is k
+    want = fa.apply_rotary_emb(*plain, cos, sin)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    if not parts:
+        outs = [(t, leaf, dd) for t, leaf, dd in zip((q, k), leaves, (d[:, :, :4], d[:, :, 4:5])) if leaf is not None]
+        got = torch.autograd.grad([o[0] for o in outs], [o[1] for o in outs], [o[2] for o in outs])
+        for gr, o in zip(got, outs):
+            assert torch.equal(gr, back(o[2], cos, sin))
+        return
+    # the projection's own gradient, and the parts'
+    ref = d.clone()
+    if need != "k":
+        ref[:, :, :4] = back(d[:, :, :4], cos, sin)
+    if need != "q":
+        ref[:, :, 4:5] = back(d[:, :, 4:5], cos, sin)
+    (whole,) = torch.autograd.grad(both, x, d, retain_graph=True)
+    assert torch.equal(whole, ref)
+    turned = [(t, s) for t, s, n in ((q, slice(0, 4), need != "k"), (k, slice(4, 5), need != "q")) if n]
+    (of_parts,) = torch.autograd.grad([t for t, _ in turned], x, [d[:, :, s] for _, s in turned])
+    for _, s in turned:
+        assert torch.equal(of_parts[:, :, s], ref[:, :, s])
+
+
+def test_twice_and_second_gradients():
+    print("case in place twice", flush=True)
+    g = torch.Generator().manual_seed(2)
+    cos, sin = tables()
+    x, d, w = rows(g, 3, requires_grad=True), rows(g, 3, requires_grad=True), rows(g, 3)
+    q = x * 1
+    fa.apply_rotary_emb(q, None, cos, sin, inplace=True)
+    fa.apply_rotary_emb(q, None, cos, sin, inplace=True)
+    (first,) = torch.autograd.grad(q, x, d, create_graph=True)
+    assert torch.equal(first, back(back(d.detach(), cos, sin), cos, sin))
+    (second,) = torch.autograd.grad(first, d, w)
+    once = fa.apply_rotary_emb(w, None, cos, sin)
+    assert torch.equal(second, fa.apply_rotary_emb(once, None, cos, sin))
+
+
+def test_refusals_leave_the_rows():
+    """What autograd does not let be changed is refused with its rows as they were, and an argument that is refused leaves
+    no history."""
+    print("case in place refusals", flush=True)
+    g = torch.Generator().manual_seed(3)
+    cos, sin = tables()
+    leaf = rows(g, 4, requires_grad=True)
+    pieces = (rows(g, 4, requires_grad=True) * 1).split(2, 2)
+    for q, k in ((leaf, None), (leaf[:, :, 1:], None), (pieces[0], None), (pieces[0], pieces[1]), (rows(g, 4, requires_grad=True) * 1, leaf)):
+        given = [t for t in (q, k) if t is not None]
+        before = [(t.detach().clone(), t._version, t.grad_fn) for t in given]
+        with pytest.raises(RuntimeError):
+            fa.apply_rotary_emb(q, k, cos, sin, inplace=True)
+        for t, (bits, version, fn) in zip(given, before):
+            assert torch.equal(t, bits) and t._version == version and t.grad_fn is fn
+    q = rows(g, 4, requires_grad=True) * 1
+    bits, fn = q.detach().clone(), q.grad_fn
+    for bad in (dict(rotary_cos=cos[:, :12], rotary_sin=sin[:, :12]), dict(positions=torch.zeros(B, S + 1, dtype=torch.int64, device=DEV)), dict(k=q)):
+        with pytest.raises(RuntimeError):
+            fa.apply_rotary_emb(**dict(dict(q=q, k=None, rotary_cos=cos, rotary_sin=sin, inplace=True), **bad))
+        assert torch.equal(q, bits) and q.grad_fn is fn
+
+
+def test_saved_rows_are_missed():
+    """The case that gave wrong gradients: a factor turned after it was saved."""
+    print("case in place saved", flush=True)
+    g = torch.Generator().manual_seed(4)
+    cos, sin = tables()
+    x, w = rows(g, 4), rows(g, 4, requires_grad=True)
+    y = (x * w).sum()
+    fa.apply_rotary_emb(x, None, cos, sin, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_compiled():
+    """A step with the rotation in place, traced: eager results."""
+    print("case in place compiled", flush=True)
+    g = torch.Generator().manual_seed(5)
+    cos, sin = tables()
+    x, d = rows(g, 4, requires_grad=True), rows(g, 4)
+
+    def step(x):
+        q = x * 2
+        fa.apply_rotary_emb(q, None, cos, sin, inplace=True)
+        return q * 0.5
+
+    want = step(x)
+    (grad,) = torch.autograd.grad(want, x, d)
+    got = torch.compile(step, backend="aot_eager")(x)
+    assert torch.equal(got, want) and torch.equal(torch.autograd.grad(got, x, d)[0], grad)

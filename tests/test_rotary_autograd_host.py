@@ -58,3 +58,65 @@ def test_inference_tensors_stay_in_inference():
         fa.apply_rotary_emb(q, None, cos, sin, inplace=True)
     with pytest.raises(RuntimeError, match="(?i)inference"):
         fa.apply_rotary_emb(q, None, cos, sin, inplace=True)
+
+
+def refused_in_place():
+    """Rows that autograd does not let be changed, by what makes them so."""
+    leaf = rows(requires_grad=True)
+    yield "a leaf", leaf, None
+    yield "a part of a leaf", leaf[:, :, 1:], None
+    yield "pieces of one call", (rows(requires_grad=True) * 1).split(2, 2)[0], None
+    yield "pieces of one call, as k", rows(requires_grad=True) * 1, (rows(requires_grad=True) * 1).unbind(0)[0][None].expand(2, 5, 4, 64)
+    yield "k a leaf", rows(requires_grad=True) * 1, leaf
+    with torch.no_grad():
+        part = leaf[:, :, 1:]
+    yield "a part taken without gradients", part, None
+
+
+@pytest.mark.parametrize("direct", [False, True])
+def test_refused_before_anything_is_turned(direct):
+    cos, sin = tables()
+    for why, q, k in refused_in_place():
+        given = [t for t in (q, k) if t is not None]
+        before = [(t._version, t.grad_fn) for t in given]
+        with pytest.raises(RuntimeError):
+            if direct:
+                ops.rotary_(q, k, cos, sin, None, None, 0, None, True, False)
+            else:
+                fa.apply_rotary_emb(q, k, cos, sin, inplace=True)
+        assert [t._version for t in given] == [b[0] for b in before], why
+        assert all(t.grad_fn is b[1] for t, b in zip(given, before)), why
+    with torch.inference_mode():
+        cos, sin = tables()
+    q = rows(requires_grad=True) * 1
+    before = q._version
+    with pytest.raises(RuntimeError, match="(?i)inference tensors"):  # they cannot be kept for the backward pass
+        fa.apply_rotary_emb(q, None, cos, sin, inplace=True)
+    assert q._version == before
+
+
+def test_history_in_place():
+    """Whoever needs a gradient gets the turn's history, and nothing else does."""
+    cos, sin = tables()
+    for need_q, need_k in ((True, True), (True, False), (False, True), (False, False)):
+        x, y = rows(requires_grad=need_q), rows(2, requires_grad=need_k)
+        q, k = x * 1, y * 1
+        a, b = fa.apply_rotary_emb(q, k, cos, sin, inplace=True)
+        assert a is q and b is k and (q.requires_grad, k.requires_grad) == (need_q, need_k)
+        if need_q or need_k:
+            (a.sum() + b.sum()).backward()
+        assert (x.grad is not None, y.grad is not None) == (need_q, need_k)
+    q = rows(requires_grad=True) * 1
+    with torch.no_grad():
+        fa.apply_rotary_emb(q, None, cos, sin, inplace=True)
+    assert "Mul" in type(q.grad_fn).__name__
+
+
+def test_tables_changed_before_the_backward_pass():
+    cos, sin = tables()
+    for inplace in (False, True):
+        q = rows(requires_grad=True) * 1
+        out = fa.apply_rotary_emb(q, None, cos, sin, inplace=inplace)
+        cos.zero_()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
