@@ -1126,6 +1126,14 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& q, const OptT& k, const Tensor& 
     return {qo, ko.has_value() ? *ko : none};
 }
 
+// Forward-mode derivatives are refused, as flash_attn_func refuses them: a dual tensor does not require a gradient, and
+// its tangent would be left behind.
+void refuse_tangents(const Tensor& q, const OptT& k, const Tensor& cos, const Tensor& sin) {
+    const auto dual = [](const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); };
+    TORCH_CHECK_NOT_IMPLEMENTED(!dual(q) && !(k.has_value() && dual(*k)) && !dual(cos) && !dual(sin),
+                                "apply_rotary_emb has no forward-mode derivative");
+}
+
 // The rotation with its gradient, the turn back. Here and not in Python, which the autograd engine's thread
 // would wait for: 37 packed sequences forward and backward, whose kernels take 40 us, 85 us there and 70 here.
 class RotaryGrad : public torch::autograd::Function<RotaryGrad> {
@@ -1169,6 +1177,7 @@ public:
 
 std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const OptT& k, const Tensor& cos, const Tensor& sin, const OptT& positions,
                                            const OptT& offsets, int64_t offset, const OptT& cu, bool interleaved, bool conjugate) {
+    refuse_tangents(q, k, cos, sin);
     if (at::GradMode::is_enabled() && (q.requires_grad() || (k.has_value() && k->requires_grad()))) {
         auto r = RotaryGrad::apply(q, k, cos, sin, positions, offsets, offset, cu, interleaved, conjugate);
         return {r[0], r[1]};
@@ -1244,6 +1253,7 @@ struct RotaryInPlaceBackward : public torch::autograd::Node {
 void rotary_autograd_(Tensor& q, const OptT& k, const Tensor& cos, const Tensor& sin, const OptT& positions, const OptT& offsets,
                       int64_t offset, const OptT& cu, bool interleaved, bool conjugate) {
     using namespace torch::autograd;
+    refuse_tangents(q, k, cos, sin);
     const auto needs = [](const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); };
     std::vector<Tensor> turned;
     for (const OptT& t : {OptT(q), k}) {

@@ -58,7 +58,7 @@ def apply_rotary_emb(q, k, rotary_cos, rotary_sin, positions: Optional[torch.Ten
 
     inplace turns q and k themselves, without new memory; neither may hold a row twice, nor share memory with the other. What
     autograd does not let be changed (a leaf that requires a gradient, the pieces of a split) is refused and stays as it was.
-    Gradients of q and k are turned back, which takes no saved rows; the tables get none."""
+    Gradients of q and k are turned back, which takes no saved rows; the tables get none. Forward-mode derivatives are refused."""
     offsets = maybe_contiguous(seqlen_offsets) if isinstance(seqlen_offsets, torch.Tensor) else None
     where = (positions, offsets, 0 if offsets is not None else int(seqlen_offsets), maybe_contiguous(cu_seqlens), bool(rotary_interleaved))
     if inplace:

@@ -120,3 +120,28 @@ def test_tables_changed_before_the_backward_pass():
         cos.zero_()
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             out.sum().backward()
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+def test_no_forward_mode(inplace):
+    """Tangents of rows or of tables are refused, not dropped; the rows then are as they were."""
+    fw = torch.autograd.forward_ad
+    for of in ("q", "k", "cos", "sin"):
+        for needs in (False, True):
+            with fw.dual_level():
+                cos, sin = tables()
+                args = dict(q=rows(), k=rows(2), cos=cos, sin=sin)
+                plain = args[of].clone()
+                args[of] = fw.make_dual(plain.requires_grad_() * 1 if needs and of in "qk" else plain, torch.empty_like(plain))
+                before = [t._version for t in args.values()]
+                with pytest.raises(RuntimeError, match="forward"):
+                    fa.apply_rotary_emb(*args.values(), inplace=inplace)
+                assert [t._version for t in args.values()] == before
+    cos, sin = tables()
+    with pytest.raises(RuntimeError, match="forward"):
+        torch.func.jvp(lambda q: fa.apply_rotary_emb(q, None, cos, sin, inplace=inplace), (rows(),), (rows(),))
+    with fw.dual_level(), torch.no_grad():
+        q = fw.make_dual(rows(), rows())
+        with pytest.raises(RuntimeError, match="forward"):
+            ops.rotary_(q, None, cos, sin, None, None, 0, None, True, False)
+        fa.apply_rotary_emb(rows(), None, cos, sin, inplace=inplace)  # none of its own
