@@ -8,6 +8,7 @@
 
 #include "fa_checks.h"
 #include "fa_rotary_args.h"
+#include "fa_rotary_rows.h"
 
 namespace fa {
 hipError_t launch_rotary_table(const RotaryTableArgs& a, int dtype, hipStream_t stream);
@@ -82,6 +83,14 @@ fa_status_t check_rotary(const fa_rotary_params* p) {
                                    p->k_out_batch_stride % 8 == 0 && p->k_out_row_stride % 8 == 0 && p->k_out_head_stride % 8 == 0)),
              "strides of q, k and their results must be multiples of 8 elements");
     FA_CHECK(p->cos_row_stride % 8 == 0 && p->sin_row_stride % 8 == 0, "row strides of cos and sin must be multiples of 8 elements");
+    if (in_place) {
+        const int64_t B = p->cu_seqlens ? 1 : p->batch, S = p->cu_seqlens ? p->total : p->seqlen;
+        const fa::RotaryRows q{{B, S, p->nheads}, {p->q_batch_stride, p->q_row_stride, p->q_head_stride}, p->headdim};
+        const fa::RotaryRows k{{B, S, p->nheads_k}, {p->k_batch_stride, p->k_row_stride, p->k_head_stride}, p->headdim};
+        FA_CHECK(fa::rows_once(q) && fa::rows_once(k), "q and k turned in place must not repeat rows");
+        FA_CHECK(!p->nheads_k || fa::rows_apart(q, k, ((int64_t)(uintptr_t)p->k - (int64_t)(uintptr_t)p->q) / 2),
+                 "q and k turned in place must not hold the same memory");
+    }
     return FA_OK;
 }
 

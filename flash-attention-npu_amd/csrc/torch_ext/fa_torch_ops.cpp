@@ -1192,22 +1192,9 @@ void rotary_(Tensor& q, const OptT& k, const Tensor& cos, const Tensor& sin, con
     check_rotary(q, k, cos, sin);
     auto check = [](const Tensor& t, const char* name) {
         TORCH_CHECK(rows_of_16(t), name, " turned in place must have contiguous last dimension, strides of 8 elements and 16-byte alignment");
-        // Rows that share memory would be turned more than once: each stride has to pass what the smaller ones reach.
-        std::vector<std::pair<int64_t, int64_t>> steps;
-        for (int64_t i = 0; i < t.dim(); ++i)
-            if (t.size(i) > 1) steps.emplace_back(t.stride(i), t.size(i));
-        std::sort(steps.begin(), steps.end());
-        int64_t reach = 0;
-        for (const auto& [stride, size] : steps) {
-            TORCH_CHECK(t.numel() == 0 || stride > reach, name, " turned in place must not repeat rows");
-            reach += stride * (size - 1);
-        }
     };
     check(q, "q");
-    if (k.has_value()) {
-        check(*k, "k");
-        TORCH_CHECK(q.numel() == 0 || k->numel() == 0 || q.data_ptr() != k->data_ptr(), "q and k turned in place must not be the same memory");
-    }
+    if (k.has_value()) check(*k, "k");
     rotary_into(q, k, q, k, cos, sin, positions, seqlen_offsets, seqlen_offset, cu_seqlens, interleaved, conjugate);
 }
 

@@ -529,7 +529,8 @@ typedef struct fa_rotary_params {
 } fa_rotary_params;
 
 /* x1' = x1 cos - x2 sin, x2' = x2 cos + x1 sin of each pair; channels past rotary_dim
- * and rows that belong to no sequence stay. Positions outside [0, seqlen_ro) take the nearest row. */
+ * and rows that belong to no sequence stay. Positions outside [0, seqlen_ro) take the nearest row. Results are q and k
+ * themselves, which then may hold no memory twice or in common, or memory that no input lies in. */
 fa_status_t fa_rotary(const fa_rotary_params* p, void* stream);
 
 /* Thread-local message describing the last non-FA_OK status on this thread. */

@@ -132,3 +132,28 @@ def test_compiled():
     (grad,) = torch.autograd.grad(want, x, d)
     got = torch.compile(step, backend="aot_eager")(x)
     assert torch.equal(got, want) and torch.equal(torch.autograd.grad(got, x, d)[0], grad)
+
+
+def test_memory_in_common():
+    """q and k of one projection, side by side or alternating by heads, are turned; a head that both hold is refused."""
+    print("case in place common memory", flush=True)
+    g = torch.Generator().manual_seed(6)
+    cos, sin = tables()
+    base = rows(g, 9)
+    alternate = base.view(B, S, 3, 3, D)
+    for q, k in ((base[:, :, 2:6], base[:, :, :2]), (alternate[:, :, :, 0], alternate[:, :, :, 1]), (base[:, :4, :4], base[:, 4:, 3:5]),
+                 (base[:, ::2, :4], base[:, 1::2, 3:5]), (base[0, :, :4][None], base[1, :, 3:5][None])):
+        want = [t.clone() for t in fa.apply_rotary_emb(q, k, cos, sin)]
+        rest = base.clone()
+        fa.apply_rotary_emb(q, k, cos, sin, inplace=True)
+        assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+        q.zero_(), k.zero_()
+        turned = base != rest  # zeros where q and k are; the rest as it was
+        assert (base[turned] == 0).all() and turned.sum() <= q.numel() + k.numel()
+        base.copy_(rest)
+    before = base.clone()
+    for q, k in ((base[:, :, :4], base[:, :, 3:5]), (base[:, :, 3:5], base[:, :, :4]), (base[:, :, :4], base[:, :, :4]),
+                 (alternate[:, :, :, 0], base[:, :, 3:4]), (base[0, :, :4][None], base[0, :, 2:3][None])):
+        with pytest.raises(RuntimeError, match="same memory"):
+            fa.apply_rotary_emb(q, k, cos, sin, inplace=True)
+    assert torch.equal(base, before)
