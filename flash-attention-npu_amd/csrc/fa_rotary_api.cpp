@@ -2,6 +2,7 @@
 // Checks and launches only: no device memory is read, allocated or waited for.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -167,7 +168,8 @@ fa_status_t fa_rotary(const fa_rotary_params* p, void* stream) {
     a.p_sb = p->positions_batch_stride;
     a.p_si = p->positions_row_stride;
     a.offsets = p->seqlen_offsets;
-    a.offset = p->seqlen_offset;
+    // a row is less than 2^31 behind its sequence's first, and so are the tables' rows: farther offsets all lead outside
+    a.offset = std::clamp<int64_t>(p->seqlen_offset, -(1ll << 31), 1ll << 31);
     a.cu = p->cu_seqlens;
     a.B = p->batch;
     a.seqlen = fa::udiv_make((uint32_t)(p->cu_seqlens ? 1 : p->seqlen));

@@ -157,3 +157,14 @@ def test_memory_in_common():
         with pytest.raises(RuntimeError, match="same memory"):
             fa.apply_rotary_emb(q, k, cos, sin, inplace=True)
     assert torch.equal(base, before)
+
+
+def test_farthest_offsets():
+    """Rows whose place in the tables passes 64 bits take the nearest row like others outside."""
+    print("case rotate farthest offsets", flush=True)
+    g = torch.Generator().manual_seed(7)
+    cos, sin = tables()
+    q = rows(g, 2)
+    for offset, row in ((2 ** 63 - 1, S - 1), (2 ** 63 - 4, S - 1), (-2 ** 63, 0), (2 ** 31, S - 1), (-2 ** 31, 0)):
+        at = torch.full((B, S), row, dtype=torch.int32, device=DEV)
+        assert torch.equal(fa.apply_rotary_emb(q, None, cos, sin, seqlen_offsets=offset), fa.apply_rotary_emb(q, None, cos, sin, positions=at)), offset
