@@ -123,7 +123,7 @@ fa_status_t fa_rotary_table(const fa_rotary_table_params* p, void* stream) {
             f *= keep + (1.0 - keep) / p->factor;
         }
         FA_CHECK(std::isfinite(f), "angle %d of base, factor and original_length is not finite", i);
-        a.turns[i] = f / kTwoPi;
+        a.turns[i] = 4.0 * (f / kTwoPi);
     }
     const hipError_t e = fa::launch_rotary_table(a, p->dtype, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail(FA_EHIP, "rotary table launch failed: %s", hipGetErrorString(e));

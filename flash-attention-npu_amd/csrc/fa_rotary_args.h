@@ -17,7 +17,7 @@ struct RotaryTableArgs {
     float factor;                // of cosines and sines
     void* cos;
     void* sin;
-    double turns[kMaxAngles];    // whole turns that angle i takes for a position
+    double turns[kMaxAngles];    // quarter turns that angle i takes for a position
 };
 
 // x[0] is q, x[1] k (heads 0: there is none). A row is (batch, position) or, ragged,

@@ -35,7 +35,8 @@ def rotary_cos_sin(positions, rotary_dim, base=10000.0, scaling=None, factor=1.0
       "by_parts"  f_i (g + (1 - g) / factor), where g goes from 0 to 1 while the turns that f_i makes over
                   original_length tokens, original_length * f_i / 2 pi, go from low to high
 
-    Angles are formed in 64 bits, so far positions keep all bits of the result."""
+    Angles are formed in 64 bits, so that of position p is off by less than p * f_i * 2 ** -50; its cosine and sine are good to
+    2 ** -22 of their value."""
     if scaling not in _SCALING:
         raise RuntimeError(f"scaling must be None, 'linear', 'ntk' or 'by_parts', got {scaling!r}")
     return _table(maybe_contiguous(positions), int(rotary_dim), float(base), _SCALING[scaling], float(factor),
