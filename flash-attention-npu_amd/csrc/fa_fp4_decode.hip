@@ -42,7 +42,6 @@ namespace {
 template <int HD>
 struct Cfg4 {
     static constexpr int NWAVE = 4;                  // waves of a workgroup
-    static constexpr int HS = 4;                     // heads of a group at most
     static constexpr int KT = 64, NB = KT / 16;      // keys of a tile, blocks of 16
     static constexpr int W = HD / 32;                // words of 8 codes that a lane has of a row
     static constexpr int NL = HD == 256 ? 2 : 1;     // loads of them, each under one scale
@@ -119,7 +118,7 @@ __global__ void __launch_bounds__(Cfg4<HD>::NWAVE * 64, groups_of_cu(HD, NR)) fa
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, G = lane >> 4;   // row (column) and quarter of a product's operand
     const int lr = lane >> 2, lq = lane & 3;   // row and quarter that a lane loads of 16 keys: four lanes a row
-    const int hs = heads_per_group<Cfg4<HD>::HS>(a), hgs = a.Hk / hs;
+    const int hs = heads_per_group(a), hgs = a.Hk / hs;
 
     // ---- the list of tiles ----------------------------------------------------------
     const int hsel = wave % hs;
@@ -529,7 +528,7 @@ void launch_n(const QuantFwdArgs& a, int nr, int cus, hipStream_t stream) {
     const int grid = cus * groups_of_cu(HD, nr);
     if (a.blocks) {
         hipLaunchKernelGGL((fa_fp4_decode_kernel<DT, HD, 2, true>), dim3(grid), nt, 0, stream, a);
-        launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE, Cfg4<HD>::HS, 256, true>(a, 2, grid, stream);
+        launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE, 256, true>(a, 2, grid, stream);
         if (a.dec_rows == 0) return;
         nr = 1;  // short sequences of a call whose blocks are not taken
     }
@@ -538,8 +537,8 @@ void launch_n(const QuantFwdArgs& a, int nr, int cus, hipStream_t stream) {
     // Many segments fill the chip with small workgroups, few want more threads for the pieces of each:
     // 64 sequences of 8 heads of D128 take 9.0 us with 256 threads and 12.8 with 512, 8 sequences 7.2 with 512 and
     // 9.6 with 256. Blocks have few pieces each: 512 tokens of 32 heads 54 us in all with 256, 61 with 512.
-    if ((int64_t)a.B * a.Hk * (HD / 32) >= 4 * cus) launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE, Cfg4<HD>::HS, 256>(a, nr, grid, stream);
-    else launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE, Cfg4<HD>::HS>(a, nr, grid, stream);
+    if ((int64_t)a.B * a.Hk * (HD / 32) >= 4 * cus) launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE, 256>(a, nr, grid, stream);
+    else launch_list_merge<DT, HD, Cfg4<HD>::KT, Cfg4<HD>::NWAVE>(a, nr, grid, stream);
 }
 
 template <int HD>

@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(Cfg<HD>::NWAVE * 64, 1) fa_quant_decode_kernel
     };
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, G = lane >> 4;
-    const int hs = heads_per_group<4>(a), hgs = a.Hk / hs;
+    const int hs = heads_per_group(a), hgs = a.Hk / hs;
 
     // ---- the list of tiles ----------------------------------------------------------
     for (int b = tid; b < a.B; b += NT) {
@@ -515,7 +515,7 @@ void launch_n(const QuantFwdArgs& a, int nr, int grid, hipStream_t stream) {
     const dim3 nt(Cfg<HD>::NWAVE * 64);
     if (nr == 1) hipLaunchKernelGGL((fa_quant_decode_kernel<DT, CT, HD, 1>), dim3(grid), nt, 0, stream, a);
     else hipLaunchKernelGGL((fa_quant_decode_kernel<DT, CT, HD, 2>), dim3(grid), nt, 0, stream, a);
-    launch_list_merge<DT, HD, Cfg<HD>::KT, Cfg<HD>::NWAVE, 4>(a, nr, grid, stream);
+    launch_list_merge<DT, HD, Cfg<HD>::KT, Cfg<HD>::NWAVE>(a, nr, grid, stream);
 }
 
 template <int HD>

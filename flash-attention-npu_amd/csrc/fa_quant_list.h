@@ -11,10 +11,7 @@ namespace fa {
 namespace {
 
 // kv heads whose tiles neighbouring waves take: a key's rows of them lie side by side
-template <int MOST>
-__device__ __forceinline__ int heads_per_group(const QuantFwdArgs& a) {
-    return MOST == 8 && a.Hk % 8 == 0 ? 8 : a.Hk % 4 == 0 ? 4 : a.Hk % 2 == 0 ? 2 : 1;
-}
+__device__ __forceinline__ int heads_per_group(const QuantFwdArgs& a) { return a.Hk % 4 == 0 ? 4 : a.Hk % 2 == 0 ? 2 : 1; }
 
 struct Seg {
     int S, n;      // first tile of the list, tiles
@@ -128,16 +125,15 @@ __device__ __forceinline__ float max4(float v) {
 // workgroup; groups of threads fold a share of the partials each, with a running
 // maximum, and meet in LDS. A row is empty where its weights sum to 0, which says so
 // for NaN as well: such partials have no part in the maximum (fmaxf).
-// KT: keys of a tile, NWAVE: waves of a workgroup of the kernel that left them, HS: heads of a group at most,
-// MT: threads of a workgroup, BLK: the list is of blocks.
-template <int DT, int HD, int KT, int NWAVE, int HS, int MT, bool BLK>
+// KT: keys of a tile, NWAVE: waves of a workgroup of the kernel that left them, MT: threads of a workgroup, BLK: the list is of blocks.
+template <int DT, int HD, int KT, int NWAVE, int MT, bool BLK>
 __global__ void __launch_bounds__(MT) fa_quant_merge_kernel(QuantFwdArgs a, int grid, int nr) {
     __shared__ __attribute__((aligned(16))) float s_acc[MT][8];
     __shared__ float s_gm[MT], s_gs[MT];
     constexpr int COLS = HD / 32, CH = 4;  // 8-column chunks of a workgroup
     const int sig = blockIdx.x / COLS, part = blockIdx.x % COLS;
     const int e = (int)((uint32_t)sig / (uint32_t)a.Hk), hk = sig - e * a.Hk;  // sequence, or block
-    const int hs = heads_per_group<HS>(a), hg = hk / hs, hsel = hk - hg * hs;
+    const int hs = heads_per_group(a), hg = hk / hs, hsel = hk - hg * hs;
     int b = e, last = a.B, first = 0;  // first: the block's first row
     QuantSeq q;
     if constexpr (BLK) {
@@ -224,9 +220,9 @@ __global__ void __launch_bounds__(MT) fa_quant_merge_kernel(QuantFwdArgs a, int 
 }
 
 constexpr int kMergeThreads = 512;
-template <int DT, int HD, int KT, int NWAVE, int HS, int MT = kMergeThreads, bool BLK = false>
+template <int DT, int HD, int KT, int NWAVE, int MT = kMergeThreads, bool BLK = false>
 void launch_list_merge(const QuantFwdArgs& a, int nr, int grid, hipStream_t stream) {
-    hipLaunchKernelGGL((fa_quant_merge_kernel<DT, HD, KT, NWAVE, HS, MT, BLK>), dim3((BLK ? a.blocks : a.B) * a.Hk * (HD / 32), nr), dim3(MT), 0, stream, a, grid, nr);
+    hipLaunchKernelGGL((fa_quant_merge_kernel<DT, HD, KT, NWAVE, MT, BLK>), dim3((BLK ? a.blocks : a.B) * a.Hk * (HD / 32), nr), dim3(MT), 0, stream, a, grid, nr);
 }
 
 }  // namespace
