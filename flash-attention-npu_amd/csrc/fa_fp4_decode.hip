@@ -25,8 +25,8 @@
 // D128 bf16, 427 MB: 95 us (4.5 TB/s; of 64 x 32768 keys 5.0), and 9 for the merge; the data path of the loads is busy 74 % of
 // the time, vector instructions take a third, products 11 %, and waves wait for a third of it. One sequence of 777 keys: 12
 // and 4.6 us, of which the list, page ids, first keys and q, one after another, have 8; 4 tokens over a window of
-// 4096, 8 sequences, fp16: 21 and 7. D64 3.7, D256 4.4, 32 packed rows 3.3 TB/s, where
-// registers hold fewer loads in flight.
+// 4096, 8 sequences, fp16: 21 and 7. Long sequences of D64 3.85, D256 4.4 TB/s,
+// of 32 packed rows 3.25 (fp16 3.7), where registers hold fewer loads in flight.
 // Lanes that load 16 apart, as the products want them, keep the data path of the loads busy 83 % of the time and
 // cost more than the exchange through LDS; loads marked non-temporal made 127 us of 106, as
 // a 128-byte line holds two heads' rows.

@@ -56,11 +56,13 @@ __device__ __forceinline__ int place_of(const T* s, int n, int x) {
 // Longer sequences, in blocks of kBlockRows packed rows that read their keys each for itself. A tile costs the
 // decode kernel twice what its rows cost the prefill kernel, but that one begins 40 us later: it executes 2700
 // instructions before its first product, and fetches each line of them for the first time. Prompts of 64, 128,
-// 256 and 512 tokens of 32 heads onto 8 take 25, 32, 38 and 54 us in place of 61, 68, 66 and 74, one of 1024
+// 256 and 512 tokens of 32 heads onto 8 take 30, 30, 35 and 43 us in place of 53, 56, 59 and 68, one of 1024, if it were let,
 // 96 in place of 85; 256 tokens that end 4000 keys 67 in place of 73, 16000 keys 163 in place of 110; 8
 // prompts of 256 tokens, of which each wave has several blocks, 89 in place of 36. The number of blocks is the
 // host's to bound (kBlockSegs); the keys every workgroup of both kernels counts, alike (kBlockUnits). A call
-// whose blocks are not taken after all costs 3 to 10 us more.
+// whose blocks are not taken after all costs 3 to 10 us more. At head dims 64, 128 and 256, with 32, 64 and 8 heads
+// onto 8 and 16 onto 1, 64 to 1024 tokens behind none to 16000 keys, calls with the rule take 0.69, 0.73 and 0.78 of what they
+// take without on average, 1.11 at worst (D256, 64 heads onto 8, 128 tokens after 4000 keys: 125 for 113).
 __device__ __forceinline__ int blocks_of(const QuantFwdArgs& a, const QuantSeq& q) {
     return (q.sq * a.g + kBlockRows - 1) / kBlockRows;
 }

@@ -17,7 +17,8 @@
 //     rows of q's type hold it with its scale, and nothing below is left of scales. A thread's 32 codes
 //     of a row are one group, whose scale byte comes beside them. Weights are then of q's type too: in bf16
 //     each is off by up to half a step of 2^-8, as in the 16-bit kernels (the result's error is 1.35
-//     times that of exact weights; a second part of them would be half of all products again).
+//     times that of exact weights; a second part of them would be half of all products again, and fp16 weights,
+//     which the decode kernel has while V's scales lie in fp16's range, a second copy of each unit for those that do not).
 //   * K's scale multiplies the scores of its 16 keys. V's goes into the weights'
 //     exponent (fa_quant.h), so that the weight comes out whole; the row's sum takes it
 //     back once for a block. The running maximum is lazy: it moves only where a

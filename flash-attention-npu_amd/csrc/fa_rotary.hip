@@ -3,9 +3,10 @@
 //
 // Tables: the angle of position p and pair i is p f_i. In 32 bits an angle of 10^5
 // keeps no more than 7 bits behind the point, so the product is taken in 64, in quarter
-// turns, and only what is left of one (|r| <= 1/2) goes through a sine and cosine in 32 bits. Whole quarters change places and signs, so that a value near 0 is the sine of a small rest, whose bits
-// are all there (of whole turns, the cosine of 52174 would have 6). The f_i, whatever their scaling, are the host's and
-// come as arguments.
+// turns, and only what is left of one (|r| <= 1/2) goes through a sine and cosine in 32
+// bits. Whole quarters change places and signs, so that a value near 0 is the sine of a
+// small rest, whose bits are all there (of whole turns, the cosine of 52174 would have 6).
+// The f_i, whatever their scaling, are the host's and come as arguments.
 // 131072 positions of 64 pairs in fp32, 67 MB, take 13.8 us (4.9 TB/s of writes), 64 positions
 // 2.8. Four angles a thread make whole 16-byte stores.
 //
