@@ -1156,8 +1156,7 @@ public:
         ctx->saved_data["conjugate"] = conjugate;
         ctx->save_for_backward({cos, sin, positions.value_or(Tensor()), offsets.value_or(Tensor()), cu.value_or(Tensor())});
         auto [qo, ko] = call(q, k, cos, sin, positions, offsets, offset, cu, interleaved, conjugate);
-        if (!k.has_value()) ctx->mark_non_differentiable({ko});
-        return {qo, ko};
+        return k.has_value() ? torch::autograd::variable_list{qo, ko} : torch::autograd::variable_list{qo};
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list d) {
         const auto saved = ctx->get_saved_variables();
@@ -1180,7 +1179,7 @@ std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const OptT& k, const
     refuse_tangents(q, k, cos, sin);
     if (at::GradMode::is_enabled() && (q.requires_grad() || (k.has_value() && k->requires_grad()))) {
         auto r = RotaryGrad::apply(q, k, cos, sin, positions, offsets, offset, cu, interleaved, conjugate);
-        return {r[0], r[1]};
+        return {r[0], k.has_value() ? r[1] : at::empty({0}, q.options())};
     }
     at::AutoDispatchBelowADInplaceOrView below;
     return RotaryGrad::call(q, k, cos, sin, positions, offsets, offset, cu, interleaved, conjugate);

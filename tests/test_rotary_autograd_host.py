@@ -145,3 +145,17 @@ def test_no_forward_mode(inplace):
         with pytest.raises(RuntimeError, match="forward"):
             ops.rotary_(q, None, cos, sin, None, None, 0, None, True, False)
         fa.apply_rotary_emb(rows(), None, cos, sin, inplace=inplace)  # none of its own
+
+
+@pytest.mark.parametrize("with_k", [False, True])
+@pytest.mark.parametrize("inplace", [False])
+def test_compiled_autograd(inplace, with_k):
+    """The backward pass traced by torch's compiled autograd."""
+    import torch._dynamo.compiled_autograd as compiled
+
+    cos, sin = tables()
+    x, y = rows(requires_grad=True), rows(2, requires_grad=True) if with_k else None
+    out = fa.apply_rotary_emb(x * 1, y * 1 if with_k else None, cos, sin, inplace=inplace)
+    with compiled._enable(lambda gm: torch.compile(gm, backend="eager")):
+        (out[0].sum() + out[1].sum() if with_k else out.sum()).backward()
+    assert x.grad.shape == x.shape and (y is None or y.grad.shape == y.shape)
