@@ -18,6 +18,7 @@
 #include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/dynamo/compiled_autograd.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -1231,6 +1232,20 @@ struct RotaryInPlaceBackward : public torch::autograd::Node {
         for (auto& s : saved) s.reset_data();
     }
     std::string name() const override { return "RotaryInPlaceBackward"; }
+    // (compiled autograd)
+    void compiled_args(torch::dynamo::autograd::CompiledNodeArgs& args) const override {
+        for (const auto& s : saved) args.collect(s, false);
+        args.collect(offset);
+        args.collect(interleaved);
+        args.collect(conjugate);
+    }
+    torch::autograd::variable_list apply_with_saved(const torch::autograd::variable_list& d,
+                                                    torch::dynamo::autograd::SwapSavedVariables& swap) override {
+        for (auto& s : saved) swap.before(s);
+        auto to = apply(torch::autograd::variable_list(d));
+        for (auto& s : saved) swap.after(s);
+        return to;
+    }
 };
 
 // In place with gradients. What autograd refuses (a leaf, the pieces of a split, tables that cannot be kept) is refused before

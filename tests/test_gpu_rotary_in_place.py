@@ -116,16 +116,16 @@ def test_saved_rows_are_missed():
         y.backward()
 
 
-def test_compiled():
-    """A step with the rotation in place, traced: eager results."""
-    print("case in place compiled", flush=True)
+@pytest.mark.parametrize("inplace", [False, True])
+def test_compiled(inplace):
+    """A step with the rotation, traced: eager results."""
+    print(f"case in place compiled {inplace}", flush=True)
     g = torch.Generator().manual_seed(5)
     cos, sin = tables()
     x, d = rows(g, 4, requires_grad=True), rows(g, 4)
 
     def step(x):
-        q = x * 2
-        fa.apply_rotary_emb(q, None, cos, sin, inplace=True)
+        q = fa.apply_rotary_emb(x * 2, None, cos, sin, inplace=inplace)
         return q * 0.5
 
     want = step(x)
@@ -168,3 +168,32 @@ def test_farthest_offsets():
     for offset, row in ((2 ** 63 - 1, S - 1), (2 ** 63 - 4, S - 1), (-2 ** 63, 0), (2 ** 31, S - 1), (-2 ** 31, 0)):
         at = torch.full((B, S), row, dtype=torch.int32, device=DEV)
         assert torch.equal(fa.apply_rotary_emb(q, None, cos, sin, seqlen_offsets=offset), fa.apply_rotary_emb(q, None, cos, sin, positions=at)), offset
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+def test_traced_and_transformed_backward(inplace):
+    """Compiled autograd and torch.func.grad (in place; out of place it is refused): the eager gradient."""
+    print(f"case in place traced backward {inplace}", flush=True)
+    import torch._dynamo.compiled_autograd as compiled
+
+    g = torch.Generator().manual_seed(8)
+    cos, sin = tables()
+    d = rows(g, 5)
+    pos = torch.randint(0, S, (B, S), generator=g).to(DEV)
+
+    def loss(x):
+        both = x * 1
+        q, k = fa.apply_rotary_emb(both[:, :, :4], both[:, :, 4:], cos, sin, positions=pos, inplace=inplace)
+        return (q * d[:, :, :4]).sum() + (k * d[:, :, 4:]).sum()
+
+    x = rows(g, 5, requires_grad=True)
+    (want,) = torch.autograd.grad(loss(x), x)
+    value = loss(x)
+    with compiled._enable(lambda gm: torch.compile(gm, backend="eager")):
+        value.backward()
+    assert torch.equal(x.grad, want)
+    if inplace:
+        assert torch.equal(torch.func.grad(loss)(x.detach()), want)
+    else:
+        with pytest.raises(RuntimeError, match="functorch"):
+            torch.func.grad(loss)(x.detach())

@@ -148,7 +148,7 @@ def test_no_forward_mode(inplace):
 
 
 @pytest.mark.parametrize("with_k", [False, True])
-@pytest.mark.parametrize("inplace", [False])
+@pytest.mark.parametrize("inplace", [False, True])
 def test_compiled_autograd(inplace, with_k):
     """The backward pass traced by torch's compiled autograd."""
     import torch._dynamo.compiled_autograd as compiled
