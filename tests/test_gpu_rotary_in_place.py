@@ -197,3 +197,53 @@ def test_traced_and_transformed_backward(inplace):
     else:
         with pytest.raises(RuntimeError, match="functorch"):
             torch.func.grad(loss)(x.detach())
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_captured(grad):
+    """A step that turns parts of a projection in place, captured and replayed with other values; on a stream of its own before."""
+    print(f"case in place captured {grad}", flush=True)
+    g = torch.Generator().manual_seed(9)
+    cos, sin = tables()
+    x, d = rows(g, 6, requires_grad=grad), rows(g, 6)
+    pos = torch.zeros(B, S, dtype=torch.int64, device=DEV)
+
+    def step():
+        both = x * 1
+        fa.apply_rotary_emb(both[:, :, :4], both[:, :, 4:5], cos, sin, positions=pos, inplace=True)
+        return (both, *torch.autograd.grad(both, x, d)) if grad else (both,)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            early = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(early, step()):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for _ in range(3):
+        with torch.no_grad():
+            for t in (x, d):
+                t.copy_(torch.randn(t.shape, generator=g).to(t.dtype))
+        pos.copy_(torch.randint(0, S, pos.shape, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, step()):
+            assert torch.equal(a, b)
+
+
+def test_no_rows_and_one():
+    print("case in place sizes", flush=True)
+    cos, sin = tables()
+    for shape in ((0, 4, 3, D), (2, 0, 3, D), (0, 3, D), (1, 1, 1, D), (1, 1, D)):
+        x = torch.ones(shape, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+        q, k = x * 1, x.detach()[..., :1, :].clone()
+        before = q.detach().clone(), k.clone()
+        a, b = fa.apply_rotary_emb(q, k, cos, sin, inplace=True)
+        want = fa.apply_rotary_emb(*before, cos, sin)
+        assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+        (gr,) = torch.autograd.grad(a, x, torch.ones_like(a))
+        assert gr.shape == x.shape
