@@ -211,7 +211,8 @@ def test_captured(grad):
     def step():
         both = x * 1
         fa.apply_rotary_emb(both[:, :, :4], both[:, :, 4:5], cos, sin, positions=pos, inplace=True)
-        return (both, *torch.autograd.grad(both, x, d)) if grad else (both,)
+        # (no step's history may outlive it: a backward pass of the same leaf cannot be captured beside one)
+        return (both.detach(), *torch.autograd.grad(both, x, d)) if grad else (both,)
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
